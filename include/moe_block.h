@@ -419,6 +419,67 @@ moe_status moe_route_forward(moe_ctx *ctx, int layer, const float *x_dev,
                              int32_t *ids_dev, float *wts_dev, float *out_dev,
                              uint32_t flags, void *stream);
 
+/* ---- around the expert products ------------------------------------------ */
+
+/* For experts that a caller multiplies with products of its own, or trains:
+ * the tokens' rows to expert order and back.  inv is moe_group's pair ->
+ * grouped row map ([T*k], -1: the pair was dropped and has no row); row types
+ * are MOE_GGML_F32, MOE_GGML_F16 or MOE_GGML_BF16, in and out independent;
+ * any H; buffers must not overlap.  Sums are f32, in slot order; a result is
+ * rounded once, to its type.  An entry of inv outside [0, n_rows) is taken as
+ * dropped.  A valid inv names no row twice (moe_group's does not).  These
+ * calls allocate nothing and share no scratch: they may overlap on streams
+ * and threads and be captured, and leave the caller's current device as it was. */
+
+/* rows[inv[t*k+s]] = x[t].  x [T][H], rows [n_rows][H]; rows that no pair
+ * names are left as they were.  (ggml's mul_mat_id gathers the same rows on
+ * the fly; here they are the operator's result.) */
+moe_status moe_dispatch(moe_ctx *ctx, const void *x_dev, int x_type, const int32_t *inv_dev, int T, int k, int H,
+                        int n_rows, void *rows_dev, int rows_type, void *stream);
+
+/* Its gradient: dx[t] = sum_s drows[inv[t*k+s]] (0 for a token without rows). */
+moe_status moe_dispatch_grad(moe_ctx *ctx, const void *drows_dev, int drows_type, int n_rows, const int32_t *inv_dev,
+                             int T, int k, int H, void *dx_dev, int dx_type, void *stream);
+
+/* out[t] = sum_s wts[t*k+s] * rows[inv[t*k+s]] (0 for a token without rows). */
+moe_status moe_combine(moe_ctx *ctx, const void *rows_dev, int rows_type, int n_rows, const float *wts_dev,
+                       const int32_t *inv_dev, int T, int k, int H, void *out_dev, int out_type, void *stream);
+
+/* Its gradient: drows[inv[p]] = wts[p] * dout[t] (drows has rows' type and
+ * size; rows that no pair names are left as they were) and dwts[p] =
+ * <dout[t], rows[inv[p]]> (0 for a dropped pair). */
+moe_status moe_combine_grad(moe_ctx *ctx, const void *dout_dev, int dout_type, const void *rows_dev, int rows_type,
+                            int n_rows, const float *wts_dev, const int32_t *inv_dev, int T, int k, int H,
+                            void *drows_dev, float *dwts_dev, void *stream);
+
+/* Rows in 8 bits: scale[r] = amax_k |x[r][k]| / 127 (f32), q[r][k] = x[r][k] /
+ * scale[r] to the nearest whole number, ties to even, in [-127, 127]; a row
+ * of zeros, or whose scale rounds to 0, has codes 0.  A row with a NaN or an
+ * infinity has a NaN scale and codes 0, so that every product of it is NaN.
+ * Any K and alignment.  Also how weights are quantised, a scale for each
+ * channel. */
+moe_status moe_quantize_i8(moe_ctx *ctx, const void *x_dev, int x_type, int M, int K, int8_t *q_dev, float *scale_dev,
+                           void *stream);
+
+/* moe_matmul_i8 flags: out is silu(gate) * up of the channels [0, N/2) and
+ * [N/2, N), [M][N/2]; clamp > 1e-6 bounds gate from above and up on both
+ * sides first, as moe_layer_desc.clamp does. */
+#define MOE_MM_SWIGLU (1u << 0)
+
+/* Products of 8-bit rows with 8-bit weights, a scale for each row and channel:
+ *   out[r][n] = (sum_k q[src(r)][k] * w[e(r)][n][k]) * q_scale[src(r)] * w_scale[e(r)][n]
+ * q [n_src][K], w [E][N][K], w_scale [E][N], out [M][N] of out_type.
+ * offsets NULL: one matrix (E = 1).  Else rows [offsets[e], offsets[e+1])
+ * are expert e's (moe_group's offsets; E <= 1024) and the rows from offsets[E]
+ * on are left as they were.  perm NULL: src(r) = r, k = 1; else
+ * src(r) = perm[r] / k (moe_group's perm: the row's token), and a row whose
+ * perm is outside [0, n_src*k) is computed from zeros.
+ * The sum is exact in 32 bits: K <= 131071, else MOE_ERR_UNSUPPORTED.  Any N,
+ * K and alignment; K % 16 == 0 with 16-byte aligned q and w is the fast path. */
+moe_status moe_matmul_i8(moe_ctx *ctx, const int8_t *q_dev, const float *q_scale_dev, int n_src, const int8_t *w_dev,
+                         const float *w_scale_dev, int E, const int32_t *offsets_dev, const int32_t *perm_dev, int k,
+                         int M, int N, int K, uint32_t flags, float clamp, void *out_dev, int out_type, void *stream);
+
 /* ---- hipGraph of a decode step ------------------------------------------- */
 
 /* Capture n_layers consecutive moe_forward calls (layer ids layers[i],

@@ -8,6 +8,7 @@
 #include "../../include/moe_block.h"
 
 #include "device_common.h"
+#include "expert_kernels.h"
 #include "gguf_reader.h"
 #include "grouped_plan.h"
 #include "kernels_decode.h"
@@ -81,10 +82,10 @@ struct work_bufs {
 // Kernel classes timed by the profiler (moe_prof_*), in the order of
 // kernel_names[].
 enum { K_ROUTE = 0, K_GROUP, K_GU_DECODE, K_DOWN_DECODE, K_GU_GROUPED, K_DOWN_GROUPED,
-       K_COMBINE, K_COUNT };
+       K_COMBINE, K_DISPATCH, K_COMBINE_ROWS, K_COMBINE_GRAD, K_QUANT_I8, K_MM_I8, K_COUNT };
 static const char *const kernel_names[K_COUNT] = {
     "route", "group", "gate_up_decode", "down_decode", "gate_up_grouped",
-    "down_grouped", "combine"};
+    "down_grouped", "combine", "dispatch", "combine_rows", "combine_grad", "quantize_i8", "matmul_i8"};
 
 struct prof_state {
   bool on = false;
@@ -1315,5 +1316,6 @@ extern "C" moe_status moe_debug_last_h(moe_ctx *c, float *h, size_t cap, size_t 
   return MOE_OK;
 }
 
+#include "expert_ops.h"
 #include "moe_server.h"
 #include "graph_split.h"

@@ -29,6 +29,7 @@ MOE_ERR_FORMAT = -8
 
 MOE_FWD_PER_SLOT = 1
 MOE_FWD_NO_SHARED = 2
+MOE_MM_SWIGLU = 1
 
 ROUTE_SOFTMAX, ROUTE_SIGMOID, ROUTE_SQRT_SOFTPLUS = 0, 1, 2
 T_GATE, T_UP, T_DOWN = 0, 1, 2
@@ -47,6 +48,7 @@ EXPORTS = (
     "moe_gguf_read_layer", "moe_layer_upload_gguf",
     "moe_server_open", "moe_server_close", "moe_server_last_error", "moe_server_handle", "moe_server_listen",
     "moe_server_serve", "moe_router_logits", "moe_node_claimed", "moe_split_parse", "moe_split_compute",
+    "moe_dispatch", "moe_dispatch_grad", "moe_combine", "moe_combine_grad", "moe_quantize_i8", "moe_matmul_i8",
 )
 
 # graph nodes of the ggml backend's split (include/moe_block.h, moe_node)
@@ -245,6 +247,20 @@ def load_library(path: str | None = None):
     L.moe_split_compute.argtypes = [_vp, ctypes.POINTER(ctypes.POINTER(MoeNode)), ctypes.c_int]
     L.moe_router_logits.restype = st
     L.moe_router_logits.argtypes = [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]
+    ci = ctypes.c_int
+    L.moe_dispatch.restype = st
+    L.moe_dispatch.argtypes = [_vp, _vp, ci, _vp, ci, ci, ci, ci, _vp, ci, _vp]
+    L.moe_dispatch_grad.restype = st
+    L.moe_dispatch_grad.argtypes = [_vp, _vp, ci, ci, _vp, ci, ci, ci, _vp, ci, _vp]
+    L.moe_combine.restype = st
+    L.moe_combine.argtypes = [_vp, _vp, ci, ci, _vp, _vp, ci, ci, ci, _vp, ci, _vp]
+    L.moe_combine_grad.restype = st
+    L.moe_combine_grad.argtypes = [_vp, _vp, ci, _vp, ci, ci, _vp, _vp, ci, ci, ci, _vp, _vp, _vp]
+    L.moe_quantize_i8.restype = st
+    L.moe_quantize_i8.argtypes = [_vp, _vp, ci, ci, ci, _vp, _vp, _vp]
+    L.moe_matmul_i8.restype = st
+    L.moe_matmul_i8.argtypes = [_vp, _vp, _vp, ci, _vp, _vp, ci, _vp, _vp, ci, ci, ci, ci, ctypes.c_uint32,
+                                ctypes.c_float, _vp, ci, _vp]
     if path is None:
         _lib = L
     return L
@@ -335,6 +351,55 @@ def check_tensor(t, name: str, dtype: str, shape=None, device: bool = True):
         raise ValueError(f"{name}: on {t.device}, expected a ROCm device tensor")
 
 
+_row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled at the first use
+
+
+def _row_type(t, name: str) -> int:
+    """The ggml type of a row operand (float32, float16 or bfloat16)."""
+    if not _row_types:
+        import torch
+        _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
+    v = _row_types.get(getattr(t, "dtype", None))
+    if v is None:
+        if not hasattr(t, "data_ptr"):
+            raise ValueError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+        raise ValueError(f"{name}: dtype {t.dtype}, expected torch.float32, torch.float16 or torch.bfloat16")
+    return v
+
+
+def check_rows(name: str, t, rows=None, cols=None) -> int:
+    """t: a contiguous 2-d row operand of [rows, cols] (None: any, at least
+    one) of a row type; its ggml type."""
+    ty = _row_type(t, name)
+    sh = t.shape
+    if len(sh) != 2 or (rows is not None and sh[0] != rows) or (cols is not None and sh[1] != cols):
+        raise ValueError(f"{name}: shape {tuple(sh)}, expected {(rows, cols)}")
+    if sh[0] == 0 or sh[1] == 0:
+        raise ValueError(f"{name}: empty")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    return ty
+
+
+def check_pairs(inv, T: int) -> int:
+    """k of a pair map inv, int32 [T * k] (or [T, k]) for T tokens."""
+    check_tensor(inv, "inv", "int32", device=False)
+    n = inv.numel()
+    if n == 0 or n % T or (inv.dim() == 2 and inv.shape[0] != T) or inv.dim() > 2:
+        raise ValueError(f"inv: shape {tuple(inv.shape)}, expected (T * k,) or (T, k) with T = {T}")
+    if n // T > 64:
+        raise ValueError(f"inv: k = {n // T}, at most 64")
+    return n // T
+
+
+def check_apart(*named):
+    """No two of the (tensor, name) buffers overlap in memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), n) for t, n in named)
+    for (_, end, n), (lo, _, m) in zip(spans, spans[1:]):
+        if lo < end:
+            raise ValueError(f"{n} and {m} overlap")
+
+
 def check_forward_args(desc, x, ids, wts, out, flags: int = 0):
     """moe_forward's tensors: x float32 [T, H]; ids int32 / wts float32
     [T, k]; out float32 [T, H], or [T, k, H] with MOE_FWD_PER_SLOT.  desc:
@@ -387,6 +452,15 @@ def _stream(stream) -> int | None:
     return _current_stream() if stream is None else int(stream)
 
 
+def _device_stream(device: int) -> int:
+    """The handle of torch's current stream of one device, whichever is current."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None or not torch.cuda.is_initialized():
+        return int(torch.cuda.current_stream(device).cuda_stream)
+    return int(raw(device))
+
+
 class Graph:
     def __init__(self, ctx: "MoeBlock", handle: int, keep):
         self._ctx, self._h, self._keep = ctx, handle, keep
@@ -416,6 +490,7 @@ class MoeBlock:
         if st != MOE_OK:
             raise MoeError(st, f"moe_ctx_create: {self.lib.moe_status_str(st).decode()}")
         self.h = h.value
+        self.device = int(device)
         self.descs: dict[int, LayerDesc] = {}
 
     # -- lifecycle --------------------------------------------------------
@@ -547,6 +622,115 @@ class MoeBlock:
         self._check(self.lib.moe_route_forward(self.h, layer, _ptr(x), _ptr(logits), _ptr(bias), T, mode,
                                                int(norm), scale, _ptr(ids), _ptr(wts), _ptr(out), flags,
                                                _stream(stream)), "moe_route_forward")
+
+    # -- around the expert products (torch device tensors) ------------------------
+    def _launch(self, entry, stream, tensors, args):
+        """entry(ctx, *args, stream) on this context's device: its current
+        stream unless one is given."""
+        for t, name in tensors:
+            d = t.device
+            if d.type != "cuda" or d.index != self.device:
+                raise ValueError(f"{name}: on {d}, expected this context's ROCm device (cuda:{self.device})")
+        st = getattr(self.lib, entry)(self.h, *args, _device_stream(self.device) if stream is None else int(stream))
+        if st != MOE_OK:
+            self._check(st, entry)
+
+    def dispatch(self, x, inv, rows, stream=None):
+        """rows[inv[t*k+s]] = x[t]: tokens' rows [T, H] to expert order
+        [n_rows, H]; inv from group(); rows no pair names stay as they were."""
+        xt = check_rows("x", x)
+        T, H = x.shape
+        rt = check_rows("rows", rows, None, H)
+        k = check_pairs(inv, T)
+        check_apart((x, "x"), (rows, "rows"), (inv, "inv"))
+        self._launch("moe_dispatch", stream, ((x, "x"), (inv, "inv"), (rows, "rows")),
+                     (x.data_ptr(), xt, inv.data_ptr(), T, k, H, rows.shape[0], rows.data_ptr(), rt))
+
+    def dispatch_grad(self, drows, inv, dx, stream=None):
+        """dx[t] = sum over s of drows[inv[t*k+s]]."""
+        xt = check_rows("dx", dx)
+        T, H = dx.shape
+        rt = check_rows("drows", drows, None, H)
+        k = check_pairs(inv, T)
+        check_apart((drows, "drows"), (dx, "dx"), (inv, "inv"))
+        self._launch("moe_dispatch_grad", stream, ((drows, "drows"), (inv, "inv"), (dx, "dx")),
+                     (drows.data_ptr(), rt, drows.shape[0], inv.data_ptr(), T, k, H, dx.data_ptr(), xt))
+
+    def combine(self, rows, wts, inv, out, stream=None):
+        """out[t] = sum over s of wts[t, s] * rows[inv[t*k+s]]: expert rows
+        [n_rows, H] back in token order [T, H], weighted."""
+        ot = check_rows("out", out)
+        T, H = out.shape
+        rt = check_rows("rows", rows, None, H)
+        k = check_pairs(inv, T)
+        check_tensor(wts, "wts", "float32", (T, k), device=False)
+        check_apart((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out"))
+        self._launch("moe_combine", stream, ((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out")),
+                     (rows.data_ptr(), rt, rows.shape[0], wts.data_ptr(), inv.data_ptr(), T, k, H, out.data_ptr(), ot))
+
+    def combine_grad(self, dout, rows, wts, inv, drows, dwts, stream=None):
+        """combine's gradient: drows[inv[t*k+s]] = wts[t, s] * dout[t] and
+        dwts[t, s] = <dout[t], rows[inv[t*k+s]]> (0 for a dropped pair)."""
+        dt = check_rows("dout", dout)
+        T, H = dout.shape
+        rt = check_rows("rows", rows, None, H)
+        if check_rows("drows", drows, rows.shape[0], H) != rt:
+            raise ValueError(f"drows: dtype {drows.dtype}, expected rows' {rows.dtype}")
+        k = check_pairs(inv, T)
+        check_tensor(wts, "wts", "float32", (T, k), device=False)
+        check_tensor(dwts, "dwts", "float32", (T, k), device=False)
+        ts = ((dout, "dout"), (rows, "rows"), (wts, "wts"), (inv, "inv"), (drows, "drows"), (dwts, "dwts"))
+        check_apart(*ts)
+        self._launch("moe_combine_grad", stream, ts,
+                     (dout.data_ptr(), dt, rows.data_ptr(), rt, rows.shape[0], wts.data_ptr(), inv.data_ptr(), T, k, H,
+                      drows.data_ptr(), dwts.data_ptr()))
+
+    def quantize_i8(self, x, q, scale, stream=None):
+        """Rows x [M, K] in 8 bits: scale [M] = amax / 127, q [M, K] int8 = x /
+        scale to the nearest whole number."""
+        xt = check_rows("x", x)
+        M, K = x.shape
+        check_tensor(q, "q", "int8", (M, K), device=False)
+        check_tensor(scale, "scale", "float32", (M,), device=False)
+        ts = ((x, "x"), (q, "q"), (scale, "scale"))
+        check_apart(*ts)
+        self._launch("moe_quantize_i8", stream, ts,
+                     (x.data_ptr(), xt, M, K, q.data_ptr(), scale.data_ptr()))
+
+    def matmul_i8(self, q, scale, w, w_scale, out, offsets=None, perm=None, k: int = 1, swiglu: bool = False,
+                  clamp: float = 0.0, stream=None):
+        """out[r, n] = (sum of q[src, i] * w[e, n, i]) * scale[src] * w_scale[e, n].
+        Dense: w [N, K], out [M, N] for q [M, K].  Grouped: w [E, N, K], rows
+        offsets[e] .. offsets[e+1] are expert e's (offsets [E + 1] and perm from
+        group(): row r's codes are those of token perm[r] // k; without perm, of
+        row r).  swiglu: the channels are N/2 of gate and N/2 of up, and out
+        [M, N/2] is silu(gate) * up, clamped as LayerDesc.clamp says."""
+        check_tensor(q, "q", "int8", (None, None), device=False)
+        n_src, K = q.shape
+        grouped = offsets is not None
+        check_tensor(w, "w", "int8", (None, None, K) if grouped else (None, K), device=False)
+        E, N = (w.shape[0], w.shape[1]) if grouped else (1, w.shape[0])
+        check_tensor(scale, "scale", "float32", (n_src,), device=False)
+        check_tensor(w_scale, "w_scale", "float32", (E, N) if grouped else (N,), device=False)
+        if swiglu and N % 2:
+            raise ValueError(f"w: {N} channels are not gate and up of one width")
+        ot = check_rows("out", out, None, N // 2 if swiglu else N)
+        M = out.shape[0]
+        ts = [(q, "q"), (scale, "scale"), (w, "w"), (w_scale, "w_scale"), (out, "out")]
+        if grouped:
+            check_tensor(offsets, "offsets", "int32", (E + 1,), device=False)
+            ts.append((offsets, "offsets"))
+        if perm is not None:
+            check_tensor(perm, "perm", "int32", (M,), device=False)
+            ts.append((perm, "perm"))
+        elif k != 1 or n_src != M:
+            raise ValueError(f"out: {M} rows for {n_src} rows of q without perm (k = {k})")
+        for t, name in ts:
+            if t is not out:
+                check_apart((t, name), (out, "out"))
+        self._launch("moe_matmul_i8", stream, ts,
+                     (q.data_ptr(), scale.data_ptr(), n_src, w.data_ptr(), w_scale.data_ptr(), E, _ptr(offsets),
+                      _ptr(perm), int(k), M, N, K, MOE_MM_SWIGLU if swiglu else 0, float(clamp), out.data_ptr(), ot))
 
     def split_compute(self, nodes):
         """Compute a parsed split (moe_split_compute) into its MUL node's host data."""
