@@ -17,7 +17,7 @@ struct i8_mm {
   const float *ws;
   const int32_t *offsets, *perm;
   void *out;
-  int n_src, E, k, M, N, K, swiglu;
+  int n_src, E, k, M, N, K, swiglu, out_type;
   float clamp;
 };
 
@@ -28,5 +28,5 @@ void launch_combine_rows(const void *rows, int rows_type, int n_rows, const floa
                          int H, void *out, int out_type, hipStream_t st);  // wts NULL: unit weights
 void launch_combine_grad(const void *dout, int dout_type, const void *rows, int rows_type, int n_rows, const float *wts,
                          const int32_t *inv, int T, int k, int H, void *drows, float *dwts, hipStream_t st);
-void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, hipStream_t st);
-bool launch_matmul_i8(const i8_mm &a, int out_type, int n_cu, hipStream_t st);  // false: more rows than a grid takes
+void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st);
+bool launch_matmul_i8(const i8_mm &a, int n_cu, hipStream_t st);  // false: more rows than a grid takes

@@ -6,6 +6,7 @@
 #include "kernels_dispatch.h"
 #include "kernels_i8.h"
 
+
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 // f(T{}) for the element type t.
@@ -66,10 +67,29 @@ void launch_combine_grad(const void *dout, int dout_type, const void *rows, int 
   });
 }
 
-void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, hipStream_t st) {
+template <typename T, int WPR, int VPT>
+static void launch_quantize(const T *x, int M, int K, int8_t *q, float *scale, hipStream_t st) {
+  constexpr int rows = WPR < 4 ? 4 / WPR : 1;
+  hipLaunchKernelGGL((k_quantize_i8<T, WPR, VPT>), dim3(ceil_div(M, rows)), dim3(WPR < 4 ? 256 : 64 * WPR), 0, st, x, M, K,
+                     q, scale);
+}
+
+// One vector a thread where the rows are too few to fill the chip (a row is
+// then spread as wide as it goes), else as many rows at once as registers allow.
+void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st) {
   with_type(x_type, [&](auto t) {
     typedef decltype(t) T;
-    hipLaunchKernelGGL((k_quantize_i8_any<T>), dim3(M), dim3(256), 0, st, (const T *)x, K, q, scale);
+    const T *p = (const T *)x;
+    const bool few = M < 2 * n_cu;
+    if (K <= 512) launch_quantize<T, 1, 1>(p, M, K, q, scale, st);
+    else if (K <= 1024 && !few) launch_quantize<T, 1, 2>(p, M, K, q, scale, st);
+    else if (K <= 2048 && few) launch_quantize<T, 4, 1>(p, M, K, q, scale, st);
+    else if (K <= 2048) launch_quantize<T, 1, 4>(p, M, K, q, scale, st);
+    else if (K <= 8192 && few) launch_quantize<T, 16, 1>(p, M, K, q, scale, st);
+    else if (K <= 4096) launch_quantize<T, 4, 2>(p, M, K, q, scale, st);
+    else if (K <= 8192) launch_quantize<T, 4, 4>(p, M, K, q, scale, st);
+    else if (K <= 32768) launch_quantize<T, 16, 4>(p, M, K, q, scale, st);
+    else hipLaunchKernelGGL((k_quantize_i8_long<T>), dim3(M), dim3(256), 0, st, p, K, q, scale);
   });
 }
 
@@ -78,12 +98,30 @@ static long i8_tiles(const i8_mm &a, int BM) {
   return a.offsets ? a.M / BM + (a.M < a.E ? a.M : a.E) : ((long)a.M + BM - 1) / BM;
 }
 
-bool launch_matmul_i8(const i8_mm &a, int out_type, int n_cu, hipStream_t st) {
+template <int BM, int BN, int WM, int WN, int WK, int NBUF, int MF, int OCC>
+static bool launch_tiles(const i8_mm &a, hipStream_t st) {
+  const int nt = ceil_div(a.N, BN);
+  const long n = nt * i8_tiles(a, BM);
+  if (n > 0x7fffffff) return false;
+  hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF, MF, OCC>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
+                     (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF, MF>()), st, a, nt);
+  return true;
+}
+
+bool launch_matmul_i8(const i8_mm &a, int n_cu, hipStream_t st) {
+  const bool aligned = a.K % 16 == 0 && ((uintptr_t)a.q | (uintptr_t)a.w) % 16 == 0;
+  const bool offsets32 = (uint64_t)a.n_src * a.K < MOE_I8_OOB && (uint64_t)a.N * a.K < MOE_I8_OOB;
+  if (aligned && offsets32) {
+    const long rows = a.offsets ? (a.M + a.E - 1) / a.E : a.M;  // a matrix's, on average
+    const long matrices = a.offsets ? (a.M < a.E ? a.M : a.E) : 1;
+    if (rows <= 16 && matrices * ceil_div(a.N, 128) < n_cu) return launch_tiles<16, 32, 1, 1, 8, 3, 16, 1>(a, st);
+    if (rows <= 64) return launch_tiles<64, 128, 2, 2, 1, 3, 32, 1>(a, st);
+    if (i8_tiles(a, 256) * ceil_div(a.N, 256) < n_cu) return launch_tiles<128, 128, 2, 2, 1, 2, 32, 1>(a, st);
+    return launch_tiles<256, 256, 2, 4, 1, 2, 16, 1>(a, st);
+  }
   const int nt = a.swiglu ? ceil_div(a.N / 2, 32) : ceil_div(a.N, 64);
   const long mt = i8_tiles(a, 64);
   if (mt > 65535) return false;
-  with_type(out_type, [&](auto t) {
-    hipLaunchKernelGGL((k_mm_i8_any<decltype(t)>), dim3(nt, (unsigned)mt), dim3(256), 0, st, a);
-  });
+  hipLaunchKernelGGL(k_mm_i8_any, dim3(nt, (unsigned)mt), dim3(256), 0, st, a);
   return true;
 }
