@@ -26,12 +26,30 @@ static size_t type_bytes(int t) { return t == MOE_GGML_F32 ? 4 : t == MOE_GGML_F
 // p holds elements of size b (b = 0: an unknown type).
 static bool is_array(const void *p, size_t b) { return p && b && (uintptr_t)p % b == 0; }
 
+// A buffer of a call: what is written may overlap nothing else.
+struct call_buf {
+  const void *p;
+  size_t bytes;
+  bool written;
+};
+static bool overlap(std::initializer_list<call_buf> bufs) {
+  for (const call_buf &a : bufs)
+    for (const call_buf &b : bufs)
+      if (&a != &b && a.written && a.p && b.p && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes &&
+          (uintptr_t)b.p < (uintptr_t)a.p + a.bytes)
+        return true;
+  return false;
+}
+
 extern "C" moe_status moe_dispatch(moe_ctx *c, const void *x, int x_type, const int32_t *inv, int T, int k, int H,
                                    int n_rows, void *rows, int rows_type, void *stream) {
   if (!c) return MOE_ERR_INVALID_ARG;
   if (!is_array(x, type_bytes(x_type)) || !is_array(rows, type_bytes(rows_type)) || !is_array(inv, 4) || T <= 0 ||
       k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_dispatch: bad arguments");
+  if (overlap({{x, (size_t)T * H * type_bytes(x_type), false}, {inv, (size_t)T * k * 4, false},
+               {rows, (size_t)n_rows * H * type_bytes(rows_type), true}}))
+    return fail(c, MOE_ERR_INVALID_ARG, "moe_dispatch: rows overlaps another buffer");
   device_scope ds(c->device);
   HIPC(c, ds.err);
   {
@@ -47,6 +65,9 @@ static moe_status combine_rows(moe_ctx *c, const char *who, const void *rows, in
   if (!is_array(rows, type_bytes(rows_type)) || !is_array(out, type_bytes(out_type)) || !is_array(inv, 4) ||
       (wts && !is_array(wts, 4)) || T <= 0 || k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "%s: bad arguments", who);
+  if (overlap({{rows, (size_t)n_rows * H * type_bytes(rows_type), false}, {wts, (size_t)T * k * 4, false},
+               {inv, (size_t)T * k * 4, false}, {out, (size_t)T * H * type_bytes(out_type), true}}))
+    return fail(c, MOE_ERR_INVALID_ARG, "%s: the output overlaps another buffer", who);
   device_scope ds(c->device);
   HIPC(c, ds.err);
   {
@@ -77,8 +98,12 @@ extern "C" moe_status moe_combine_grad(moe_ctx *c, const void *dout, int dout_ty
   if (!c) return MOE_ERR_INVALID_ARG;
   const size_t rb = type_bytes(rows_type);
   if (!is_array(dout, type_bytes(dout_type)) || !is_array(rows, rb) || !is_array(drows, rb) || !is_array(wts, 4) ||
-      !is_array(inv, 4) || !is_array(dwts, 4) || drows == rows || T <= 0 || k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
+      !is_array(inv, 4) || !is_array(dwts, 4) || T <= 0 || k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_combine_grad: bad arguments");
+  const size_t nr = (size_t)n_rows * H * rb, np = (size_t)T * k * 4;
+  if (overlap({{dout, (size_t)T * H * type_bytes(dout_type), false}, {rows, nr, false}, {wts, np, false}, {inv, np, false},
+               {drows, nr, true}, {dwts, np, true}}))
+    return fail(c, MOE_ERR_INVALID_ARG, "moe_combine_grad: an output overlaps another buffer");
   device_scope ds(c->device);
   HIPC(c, ds.err);
   {
@@ -94,6 +119,8 @@ extern "C" moe_status moe_quantize_i8(moe_ctx *c, const void *x, int x_type, int
   if (!c) return MOE_ERR_INVALID_ARG;
   if (!is_array(x, type_bytes(x_type)) || !q || !is_array(scale, 4) || M <= 0 || K <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_quantize_i8: bad arguments");
+  if (overlap({{x, (size_t)M * K * type_bytes(x_type), false}, {q, (size_t)M * K, true}, {scale, (size_t)M * 4, true}}))
+    return fail(c, MOE_ERR_INVALID_ARG, "moe_quantize_i8: an output overlaps another buffer");
   device_scope ds(c->device);
   HIPC(c, ds.err);
   {
@@ -114,6 +141,11 @@ extern "C" moe_status moe_matmul_i8(moe_ctx *c, const int8_t *q, const float *q_
       E <= 0 || E > MOE_GROUP_MAX_E || (!offsets && E != 1) || k <= 0 || (!perm && (k != 1 || n_src < M)) || M <= 0 ||
       N <= 0 || K <= 0 || (swiglu && N % 2) || !(clamp >= 0.0f))
     return fail(c, MOE_ERR_INVALID_ARG, "moe_matmul_i8: bad arguments");
+  const size_t n_out = (size_t)M * (swiglu ? N / 2 : N) * type_bytes(out_type);
+  if (overlap({{q, (size_t)n_src * K, false}, {q_scale, (size_t)n_src * 4, false}, {w, (size_t)E * N * K, false},
+               {w_scale, (size_t)E * N * 4, false}, {offsets, ((size_t)E + 1) * 4, false}, {perm, (size_t)M * 4, false},
+               {out, n_out, true}}))
+    return fail(c, MOE_ERR_INVALID_ARG, "moe_matmul_i8: out overlaps another buffer");
   if (K > MOE_I8_MAX_K)
     return fail(c, MOE_ERR_UNSUPPORTED, "moe_matmul_i8: K = %d: sums of more than %d products can pass 32 bits", K,
                 MOE_I8_MAX_K);

@@ -351,14 +351,22 @@ def check_tensor(t, name: str, dtype: str, shape=None, device: bool = True):
         raise ValueError(f"{name}: on {t.device}, expected a ROCm device tensor")
 
 
-_row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled at the first use
+_row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled by the first context
+_f32 = _i32 = _i8 = _raw_stream = None
+
+
+def _know_torch():
+    global _f32, _i32, _i8, _raw_stream
+    if not _row_types:
+        import torch
+        _f32, _i32, _i8 = torch.float32, torch.int32, torch.int8
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
 
 
 def _row_type(t, name: str) -> int:
     """The ggml type of a row operand (float32, float16 or bfloat16)."""
-    if not _row_types:
-        import torch
-        _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
+    _know_torch()
     v = _row_types.get(getattr(t, "dtype", None))
     if v is None:
         if not hasattr(t, "data_ptr"):
@@ -392,12 +400,8 @@ def check_pairs(inv, T: int) -> int:
     return n // T
 
 
-def check_apart(*named):
-    """No two of the (tensor, name) buffers overlap in memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), n) for t, n in named)
-    for (_, end, n), (lo, _, m) in zip(spans, spans[1:]):
-        if lo < end:
-            raise ValueError(f"{n} and {m} overlap")
+# What a check that compares without naming may raise for an argument that is no such tensor
+_NOT_FINE = (AttributeError, KeyError, TypeError, ValueError)
 
 
 def check_forward_args(desc, x, ids, wts, out, flags: int = 0):
@@ -454,11 +458,10 @@ def _stream(stream) -> int | None:
 
 def _device_stream(device: int) -> int:
     """The handle of torch's current stream of one device, whichever is current."""
+    if _raw_stream is not None:
+        return _raw_stream(device)
     import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is None or not torch.cuda.is_initialized():
-        return int(torch.cuda.current_stream(device).cuda_stream)
-    return int(raw(device))
+    return int(torch.cuda.current_stream(device).cuda_stream)
 
 
 class Graph:
@@ -491,6 +494,7 @@ class MoeBlock:
             raise MoeError(st, f"moe_ctx_create: {self.lib.moe_status_str(st).decode()}")
         self.h = h.value
         self.device = int(device)
+        _know_torch()
         self.descs: dict[int, LayerDesc] = {}
 
     # -- lifecycle --------------------------------------------------------
@@ -624,78 +628,136 @@ class MoeBlock:
                                                _stream(stream)), "moe_route_forward")
 
     # -- around the expert products (torch device tensors) ------------------------
-    def _launch(self, entry, stream, tensors, args):
-        """entry(ctx, *args, stream) on this context's device: its current
-        stream unless one is given."""
-        for t, name in tensors:
-            d = t.device
-            if d.type != "cuda" or d.index != self.device:
-                raise ValueError(f"{name}: on {d}, expected this context's ROCm device (cuda:{self.device})")
-        st = getattr(self.lib, entry)(self.h, *args, _device_stream(self.device) if stream is None else int(stream))
-        if st != MOE_OK:
-            self._check(st, entry)
+    # Each call first compares its tensors with what it needs (a fifth of the
+    # cost of the checks that name what is wrong, which run only then: the
+    # smallest calls take a few microseconds on the device).  Buffers that
+    # overlap are refused by the library.
+    def _on_device(self, *named):
+        for t, name in named:
+            if t is not None and t.get_device() != self.device:
+                raise ValueError(f"{name}: on {t.device}, expected this context's ROCm device (cuda:{self.device})")
 
     def dispatch(self, x, inv, rows, stream=None):
         """rows[inv[t*k+s]] = x[t]: tokens' rows [T, H] to expert order
         [n_rows, H]; inv from group(); rows no pair names stay as they were."""
-        xt = check_rows("x", x)
-        T, H = x.shape
-        rt = check_rows("rows", rows, None, H)
-        k = check_pairs(inv, T)
-        check_apart((x, "x"), (rows, "rows"), (inv, "inv"))
-        self._launch("moe_dispatch", stream, ((x, "x"), (inv, "inv"), (rows, "rows")),
-                     (x.data_ptr(), xt, inv.data_ptr(), T, k, H, rows.shape[0], rows.data_ptr(), rt))
+        try:
+            xt, rt = _row_types[x.dtype], _row_types[rows.dtype]
+            (T, H), (R, Hr), n, d = x.shape, rows.shape, inv.numel(), self.device
+            k = n // T
+            fine = (inv.dtype is _i32 and H == Hr and inv.dim() == 1 and R and 0 < k <= 64 and k * T == n and H
+                    and x.is_contiguous() and rows.is_contiguous() and inv.is_contiguous()
+                    and x.get_device() == d == rows.get_device() == inv.get_device())
+        except (*_NOT_FINE, ZeroDivisionError):
+            fine = False
+        if not fine:
+            xt = check_rows("x", x)
+            T, H = x.shape
+            rt = check_rows("rows", rows, None, H)
+            k, R = check_pairs(inv, T), rows.shape[0]
+            self._on_device((x, "x"), (inv, "inv"), (rows, "rows"))
+        st = self.lib.moe_dispatch(self.h, x.data_ptr(), xt, inv.data_ptr(), T, k, H, R, rows.data_ptr(), rt,
+                                   _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_dispatch")
 
     def dispatch_grad(self, drows, inv, dx, stream=None):
         """dx[t] = sum over s of drows[inv[t*k+s]]."""
-        xt = check_rows("dx", dx)
-        T, H = dx.shape
-        rt = check_rows("drows", drows, None, H)
-        k = check_pairs(inv, T)
-        check_apart((drows, "drows"), (dx, "dx"), (inv, "inv"))
-        self._launch("moe_dispatch_grad", stream, ((drows, "drows"), (inv, "inv"), (dx, "dx")),
-                     (drows.data_ptr(), rt, drows.shape[0], inv.data_ptr(), T, k, H, dx.data_ptr(), xt))
+        try:
+            xt, rt = _row_types[dx.dtype], _row_types[drows.dtype]
+            (T, H), (R, Hr), n, d = dx.shape, drows.shape, inv.numel(), self.device
+            k = n // T
+            fine = (inv.dtype is _i32 and H == Hr and inv.dim() == 1 and R and 0 < k <= 64 and k * T == n and H
+                    and dx.is_contiguous() and drows.is_contiguous() and inv.is_contiguous()
+                    and dx.get_device() == d == drows.get_device() == inv.get_device())
+        except (*_NOT_FINE, ZeroDivisionError):
+            fine = False
+        if not fine:
+            xt = check_rows("dx", dx)
+            T, H = dx.shape
+            rt = check_rows("drows", drows, None, H)
+            k, R = check_pairs(inv, T), drows.shape[0]
+            self._on_device((drows, "drows"), (inv, "inv"), (dx, "dx"))
+        st = self.lib.moe_dispatch_grad(self.h, drows.data_ptr(), rt, R, inv.data_ptr(), T, k, H, dx.data_ptr(), xt,
+                                        _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_dispatch_grad")
 
     def combine(self, rows, wts, inv, out, stream=None):
         """out[t] = sum over s of wts[t, s] * rows[inv[t*k+s]]: expert rows
         [n_rows, H] back in token order [T, H], weighted."""
-        ot = check_rows("out", out)
-        T, H = out.shape
-        rt = check_rows("rows", rows, None, H)
-        k = check_pairs(inv, T)
-        check_tensor(wts, "wts", "float32", (T, k), device=False)
-        check_apart((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out"))
-        self._launch("moe_combine", stream, ((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out")),
-                     (rows.data_ptr(), rt, rows.shape[0], wts.data_ptr(), inv.data_ptr(), T, k, H, out.data_ptr(), ot))
+        try:
+            ot, rt = _row_types[out.dtype], _row_types[rows.dtype]
+            (T, H), (R, Hr), (Tw, k), d = out.shape, rows.shape, wts.shape, self.device
+            fine = (inv.dtype is _i32 and wts.dtype is _f32 and H == Hr and Tw == T and inv.dim() == 1
+                    and inv.numel() == k * T and T and H and R and 0 < k <= 64 and out.is_contiguous()
+                    and rows.is_contiguous() and wts.is_contiguous() and inv.is_contiguous()
+                    and out.get_device() == d == rows.get_device() == wts.get_device() == inv.get_device())
+        except _NOT_FINE:
+            fine = False
+        if not fine:
+            ot = check_rows("out", out)
+            T, H = out.shape
+            rt = check_rows("rows", rows, None, H)
+            k, R = check_pairs(inv, T), rows.shape[0]
+            check_tensor(wts, "wts", "float32", (T, k), device=False)
+            self._on_device((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out"))
+        st = self.lib.moe_combine(self.h, rows.data_ptr(), rt, R, wts.data_ptr(), inv.data_ptr(), T, k, H, out.data_ptr(),
+                                  ot, _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_combine")
 
     def combine_grad(self, dout, rows, wts, inv, drows, dwts, stream=None):
         """combine's gradient: drows[inv[t*k+s]] = wts[t, s] * dout[t] and
         dwts[t, s] = <dout[t], rows[inv[t*k+s]]> (0 for a dropped pair)."""
-        dt = check_rows("dout", dout)
-        T, H = dout.shape
-        rt = check_rows("rows", rows, None, H)
-        if check_rows("drows", drows, rows.shape[0], H) != rt:
-            raise ValueError(f"drows: dtype {drows.dtype}, expected rows' {rows.dtype}")
-        k = check_pairs(inv, T)
-        check_tensor(wts, "wts", "float32", (T, k), device=False)
-        check_tensor(dwts, "dwts", "float32", (T, k), device=False)
-        ts = ((dout, "dout"), (rows, "rows"), (wts, "wts"), (inv, "inv"), (drows, "drows"), (dwts, "dwts"))
-        check_apart(*ts)
-        self._launch("moe_combine_grad", stream, ts,
-                     (dout.data_ptr(), dt, rows.data_ptr(), rt, rows.shape[0], wts.data_ptr(), inv.data_ptr(), T, k, H,
-                      drows.data_ptr(), dwts.data_ptr()))
+        try:
+            dt, rt = _row_types[dout.dtype], _row_types[rows.dtype]
+            (T, H), (R, Hr), (Tw, k), d = dout.shape, rows.shape, wts.shape, self.device
+            fine = (inv.dtype is _i32 and wts.dtype is _f32 and dwts.dtype is _f32 and drows.dtype is rows.dtype
+                    and drows.shape == rows.shape and dwts.shape == wts.shape and H == Hr and Tw == T and inv.dim() == 1
+                    and inv.numel() == k * T and T and H and R and 0 < k <= 64 and dout.is_contiguous()
+                    and rows.is_contiguous() and wts.is_contiguous() and inv.is_contiguous() and drows.is_contiguous()
+                    and dwts.is_contiguous() and dout.get_device() == d == rows.get_device() == wts.get_device()
+                    and inv.get_device() == d == drows.get_device() == dwts.get_device())
+        except _NOT_FINE:
+            fine = False
+        if not fine:
+            dt = check_rows("dout", dout)
+            T, H = dout.shape
+            rt = check_rows("rows", rows, None, H)
+            R = rows.shape[0]
+            if check_rows("drows", drows, R, H) != rt:
+                raise ValueError(f"drows: dtype {drows.dtype}, expected rows' {rows.dtype}")
+            k = check_pairs(inv, T)
+            check_tensor(wts, "wts", "float32", (T, k), device=False)
+            check_tensor(dwts, "dwts", "float32", (T, k), device=False)
+            self._on_device((dout, "dout"), (rows, "rows"), (wts, "wts"), (inv, "inv"), (drows, "drows"), (dwts, "dwts"))
+        st = self.lib.moe_combine_grad(self.h, dout.data_ptr(), dt, rows.data_ptr(), rt, R, wts.data_ptr(), inv.data_ptr(),
+                                       T, k, H, drows.data_ptr(), dwts.data_ptr(),
+                                       _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_combine_grad")
 
     def quantize_i8(self, x, q, scale, stream=None):
         """Rows x [M, K] in 8 bits: scale [M] = amax / 127, q [M, K] int8 = x /
         scale to the nearest whole number."""
-        xt = check_rows("x", x)
-        M, K = x.shape
-        check_tensor(q, "q", "int8", (M, K), device=False)
-        check_tensor(scale, "scale", "float32", (M,), device=False)
-        ts = ((x, "x"), (q, "q"), (scale, "scale"))
-        check_apart(*ts)
-        self._launch("moe_quantize_i8", stream, ts,
-                     (x.data_ptr(), xt, M, K, q.data_ptr(), scale.data_ptr()))
+        try:
+            xt = _row_types[x.dtype]
+            (M, K), d = x.shape, self.device
+            fine = (q.dtype is _i8 and scale.dtype is _f32 and q.shape == (M, K) and scale.shape == (M,) and M and K
+                    and x.is_contiguous() and q.is_contiguous() and scale.is_contiguous()
+                    and x.get_device() == d == q.get_device() == scale.get_device())
+        except _NOT_FINE:
+            fine = False
+        if not fine:
+            xt = check_rows("x", x)
+            M, K = x.shape
+            check_tensor(q, "q", "int8", (M, K), device=False)
+            check_tensor(scale, "scale", "float32", (M,), device=False)
+            self._on_device((x, "x"), (q, "q"), (scale, "scale"))
+        st = self.lib.moe_quantize_i8(self.h, x.data_ptr(), xt, M, K, q.data_ptr(), scale.data_ptr(),
+                                      _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_quantize_i8")
 
     def matmul_i8(self, q, scale, w, w_scale, out, offsets=None, perm=None, k: int = 1, swiglu: bool = False,
                   clamp: float = 0.0, stream=None):
@@ -705,32 +767,55 @@ class MoeBlock:
         group(): row r's codes are those of token perm[r] // k; without perm, of
         row r).  swiglu: the channels are N/2 of gate and N/2 of up, and out
         [M, N/2] is silu(gate) * up, clamped as LayerDesc.clamp says."""
-        check_tensor(q, "q", "int8", (None, None), device=False)
-        n_src, K = q.shape
-        grouped = offsets is not None
-        check_tensor(w, "w", "int8", (None, None, K) if grouped else (None, K), device=False)
-        E, N = (w.shape[0], w.shape[1]) if grouped else (1, w.shape[0])
-        check_tensor(scale, "scale", "float32", (n_src,), device=False)
-        check_tensor(w_scale, "w_scale", "float32", (E, N) if grouped else (N,), device=False)
-        if swiglu and N % 2:
-            raise ValueError(f"w: {N} channels are not gate and up of one width")
-        ot = check_rows("out", out, None, N // 2 if swiglu else N)
-        M = out.shape[0]
-        ts = [(q, "q"), (scale, "scale"), (w, "w"), (w_scale, "w_scale"), (out, "out")]
-        if grouped:
-            check_tensor(offsets, "offsets", "int32", (E + 1,), device=False)
-            ts.append((offsets, "offsets"))
-        if perm is not None:
-            check_tensor(perm, "perm", "int32", (M,), device=False)
-            ts.append((perm, "perm"))
-        elif k != 1 or n_src != M:
-            raise ValueError(f"out: {M} rows for {n_src} rows of q without perm (k = {k})")
-        for t, name in ts:
-            if t is not out:
-                check_apart((t, name), (out, "out"))
-        self._launch("moe_matmul_i8", stream, ts,
-                     (q.data_ptr(), scale.data_ptr(), n_src, w.data_ptr(), w_scale.data_ptr(), E, _ptr(offsets),
-                      _ptr(perm), int(k), M, N, K, MOE_MM_SWIGLU if swiglu else 0, float(clamp), out.data_ptr(), ot))
+        try:
+            ot = _row_types[out.dtype]
+            (S, K), (M, No), d, E = q.shape, out.shape, self.device, 1
+            if offsets is None:
+                N = w.shape[0]
+                fine = w.shape == (N, K) and w_scale.shape == (N,)
+            else:
+                E, N = w_scale.shape
+                fine = (w.shape == (E, N, K) and offsets.dtype is _i32 and offsets.shape == (E + 1,)
+                        and offsets.is_contiguous() and offsets.get_device() == d)
+            if perm is None:
+                fine = fine and k == 1 and S == M
+            else:
+                fine = fine and perm.dtype is _i32 and perm.shape == (M,) and perm.is_contiguous() and perm.get_device() == d
+            fine = (fine and q.dtype is _i8 and w.dtype is _i8 and scale.dtype is _f32 and w_scale.dtype is _f32
+                    and scale.shape == (S,) and No == (N // 2 if swiglu else N) and not (swiglu and N % 2) and M and N and K
+                    and q.is_contiguous() and w.is_contiguous() and scale.is_contiguous() and w_scale.is_contiguous()
+                    and out.is_contiguous() and q.get_device() == d == w.get_device() == scale.get_device()
+                    and w_scale.get_device() == d == out.get_device())
+        except _NOT_FINE:
+            fine = False
+        if not fine:
+            grouped = offsets is not None
+            check_tensor(q, "q", "int8", (None, None), device=False)
+            S, K = q.shape
+            check_tensor(w, "w", "int8", (None, None, K) if grouped else (None, K), device=False)
+            E, N = (w.shape[0], w.shape[1]) if grouped else (1, w.shape[0])
+            check_tensor(scale, "scale", "float32", (S,), device=False)
+            check_tensor(w_scale, "w_scale", "float32", (E, N) if grouped else (N,), device=False)
+            if swiglu and N % 2:
+                raise ValueError(f"w: {N} channels are not gate and up of one width")
+            ot = check_rows("out", out, None, N // 2 if swiglu else N)
+            M = out.shape[0]
+            if S * K * N * E == 0:
+                raise ValueError(f"w: shape {tuple(w.shape)} for q of {tuple(q.shape)}: empty")
+            if grouped:
+                check_tensor(offsets, "offsets", "int32", (E + 1,), device=False)
+            if perm is not None:
+                check_tensor(perm, "perm", "int32", (M,), device=False)
+            elif k != 1 or S != M:
+                raise ValueError(f"out: {M} rows for {S} rows of q without perm (k = {k})")
+            self._on_device((q, "q"), (scale, "scale"), (w, "w"), (w_scale, "w_scale"), (out, "out"),
+                            (offsets, "offsets"), (perm, "perm"))
+        st = self.lib.moe_matmul_i8(self.h, q.data_ptr(), scale.data_ptr(), S, w.data_ptr(), w_scale.data_ptr(), E,
+                                    None if offsets is None else offsets.data_ptr(),
+                                    None if perm is None else perm.data_ptr(), k, M, N, K, 1 if swiglu else 0, clamp,
+                                    out.data_ptr(), ot, _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_matmul_i8")
 
     def split_compute(self, nodes):
         """Compute a parsed split (moe_split_compute) into its MUL node's host data."""

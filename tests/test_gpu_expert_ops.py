@@ -561,6 +561,27 @@ def test_refusals_of_the_library(blk):
     assert (buf == 0).all()
 
 
+def test_overlapping_buffers_are_refused(blk):
+    say("overlapping buffers")
+    H, T, k = 32, 4, 2
+    a = torch.zeros((20, H), device=DEV)
+    inv, wts = torch.zeros(T * k, dtype=torch.int32, device=DEV), torch.zeros((T, k), device=DEV)
+    z8 = torch.zeros((20, H), dtype=torch.int8, device=DEV)
+    for call in (lambda: blk.dispatch(a[:T], inv, a[T - 1:12]),
+                 lambda: blk.dispatch_grad(a[:8], inv, a[7:7 + T]),
+                 lambda: blk.combine(a[:8], wts, inv, a[4:4 + T]),
+                 lambda: blk.combine(a[:8], wts, inv, a[8:8 + T]) or blk.combine(a[:8], a[8, :8].view(T, k), inv, a[8:12]),
+                 lambda: blk.combine_grad(a[:T], a[4:12], wts, inv, a[4:12], torch.zeros_like(wts)),
+                 lambda: blk.combine_grad(a[:T], a[4:12], wts, inv, torch.zeros_like(a[:8]), wts),
+                 lambda: blk.quantize_i8(a[:T], z8[:T], a[3, :T]),
+                 lambda: blk.quantize_i8(a[:T], a[:1].view(torch.int8).view(T, H), torch.zeros(T, device=DEV)),
+                 lambda: blk.matmul_i8(z8[:T], wts[:, 0].contiguous(), z8[4:8], a[0, :4], a[0, :16].view(T, 4))):
+        with pytest.raises(mb.MoeError, match="overlaps") as ei:
+            call()
+        assert ei.value.status == mb.MOE_ERR_INVALID_ARG
+    torch.cuda.synchronize()
+
+
 def test_profiler_counts_the_operators(blk):
     say("profiler")
     blk.prof_enable(True)
