@@ -21,6 +21,18 @@ static void with_type(int t, F f) {
 template <typename A, typename B>
 constexpr int vec_of() { return sizeof(A) == 4 && sizeof(B) == 4 ? 4 : 8; }
 
+// Rows of more than this go past the caches (non-temporal): they displace what
+// the next kernels could find in the 256 MiB cache, and the plain form spends its
+// bandwidth on writing back what it displaced.  Measured with H = 7168, us
+// plain / non-temporal: dispatch of 59 MB 11.6 / 12.4, 117 MB 28.4 / 24.7, 470 MB
+// 108 / 95; combine 59 MB 11.9 / 12.5, 117 MB 29.0 / 25.8, 470 MB 110 / 98;
+// combine_grad (read and written) 59 MB 12.1 / 13.3, 117 MB 27.6 / 25.2, 940 MB 207 / 195.
+static constexpr size_t MOE_STREAM_BYTES = (size_t)96 << 20;
+
+// Pairs below which 4 waves share one of combine_grad's (H = 7168, bf16, us with 1
+// wave / 4: 128 pairs 6.0 / 3.7, 512 7.7 / 5.4, 1024 8.8 / 8.4, 2048 12.1 / 13.3).
+static constexpr long MOE_FEW_PAIRS = 1024;
+
 // Workgroups a token of nv vectors: enough for the chip, no more than have work.
 static int row_splits(int T, int nv) {
   const int most = ceil_div(nv, 256), want = ceil_div(2048, T);
@@ -34,7 +46,8 @@ void launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k
       typedef decltype(ti) TI;
       typedef decltype(to) TO;
       constexpr int V = vec_of<TI, TO>();
-      hipLaunchKernelGGL((k_dispatch<TI, TO, V>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
+      const bool nt = (size_t)T * k * H * sizeof(TO) > MOE_STREAM_BYTES;
+      hipLaunchKernelGGL((nt ? k_dispatch<TI, TO, V, true> : k_dispatch<TI, TO, V, false>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
                          (const TI *)x, inv, k, H, n_rows, (TO *)rows);
     });
   });
@@ -47,7 +60,8 @@ void launch_combine_rows(const void *rows, int rows_type, int n_rows, const floa
       typedef decltype(ti) TI;
       typedef decltype(to) TO;
       constexpr int V = vec_of<TI, TO>();
-      hipLaunchKernelGGL((k_combine_rows<TI, TO, V>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
+      const bool nt = (size_t)T * k * H * sizeof(TI) > MOE_STREAM_BYTES;
+      hipLaunchKernelGGL((nt ? k_combine_rows<TI, TO, V, true> : k_combine_rows<TI, TO, V, false>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
                          (const TI *)rows, wts, inv, k, H, n_rows, (TO *)out);
     });
   });
@@ -61,7 +75,10 @@ void launch_combine_grad(const void *dout, int dout_type, const void *rows, int 
       typedef decltype(td) TD;
       typedef decltype(tr) TR;
       constexpr int V = vec_of<TD, TR>();
-      hipLaunchKernelGGL((k_combine_grad<TD, TR, V>), dim3((unsigned)((P + 3) / 4)), dim3(256), 0, st, (const TD *)dout,
+      const bool nt = 2 * (size_t)P * H * sizeof(TR) > MOE_STREAM_BYTES, few = P < MOE_FEW_PAIRS && H >= 256 * V;
+      hipLaunchKernelGGL((few ? k_combine_grad<TD, TR, V, 4, false> : nt ? k_combine_grad<TD, TR, V, 1, true>
+                                                                         : k_combine_grad<TD, TR, V, 1, false>),
+                         dim3((unsigned)(few ? (P + 1) / 2 : (P + 7) / 8)), dim3(512), 0, st, (const TD *)dout,
                          (const TR *)rows, wts, inv, P, k, H, n_rows, (TR *)drows, dwts);
     });
   });
