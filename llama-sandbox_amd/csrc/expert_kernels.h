@@ -19,6 +19,7 @@ struct i8_mm {
   void *out;
   int n_src, E, k, M, N, K, swiglu, out_type;
   float clamp;
+  int stream = 0;  // set by the launch: a weight that one tile alone reads goes past the caches
 };
 
 // element types: moe_block.h's MOE_GGML_F32 / F16 / BF16

@@ -6,6 +6,8 @@
 #include "kernels_dispatch.h"
 #include "kernels_i8.h"
 
+#include <cmath>
+
 
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
@@ -115,26 +117,77 @@ static long i8_tiles(const i8_mm &a, int BM) {
   return a.offsets ? a.M / BM + (a.M < a.E ? a.M : a.E) : ((long)a.M + BM - 1) / BM;
 }
 
-template <int BM, int BN, int WM, int WN, int WK, int NBUF, int MF, int OCC>
+template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 static bool launch_tiles(const i8_mm &a, hipStream_t st) {
   const int nt = ceil_div(a.N, BN);
-  const long n = nt * i8_tiles(a, BM);
+  const long n = i8_tiles(a, BM) * nt;
   if (n > 0x7fffffff) return false;
-  hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF, MF, OCC>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
-                     (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF, MF>()), st, a, nt);
+  hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
+                     (i8_lds_bytes<BM, BN, WK, NBUF>()), st, a, nt);
   return true;
 }
 
-bool launch_matmul_i8(const i8_mm &a, int n_cu, hipStream_t st) {
+// The tile shapes, and what they cost.  A call of `rounds` tiles one after the other
+// on a CU takes about
+//   call + rounds * (tile + K / 128 * (k + k_share * tiles that share the CU))  us,
+// fitted (errors of 4 to 14%) to 52 products of 1 to 8192 rows, K = 7168, 2048, 768
+// and N = 7168, 4096, 2048.  The least of these is on average 0.6% slower than the
+// fastest shape measured there, at most 7%; over 46 grouped calls of 4 to 32764 rows
+// 1.2%, at most 29% (a skewed call).  Some of them, us with each shape's neighbours:
+//   16 rows x 7168 x 7168: 16x16 13.9, 32x32 15.2, 64x32 18.3;   64: 64x32 20.2, 32x32 28, 128x32 25
+//   512: 64x128 48, 128x64 71, 256x128 53;   1024: 256x128 57, 64x128 94, 256x256 101
+//   4096: 256x256 206, 256x128 230, 64x128 325 (the same rows over 64 wide tiles a round: 2050 TOP/s)
+struct i8_shape {
+  int BM, BN, lds;
+  float call, tile, k, k_share;
+  bool (*launch)(const i8_mm &, hipStream_t);
+};
+template <int BM, int BN, int WM, int WN, int WK, int NBUF>
+static constexpr i8_shape shape_of(float call, float tile, float k, float k_share) {
+  return {BM, BN, i8_lds_bytes<BM, BN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
+}
+static const i8_shape i8_shapes[] = {
+    shape_of<16, 16, 1, 1, 4, 4>(1.90f, 1.93f, 0.056f, 0.026f),
+    shape_of<32, 32, 1, 1, 4, 4>(1.84f, 3.95f, 0.152f, 0.0f),
+    shape_of<64, 32, 1, 1, 4, 3>(1.69f, 4.97f, 0.203f, 0.0f),
+    shape_of<128, 32, 2, 1, 2, 3>(1.42f, 4.16f, 0.332f, 0.0f),
+    shape_of<128, 64, 2, 1, 2, 3>(1.38f, 6.34f, 0.485f, 0.0f),
+    shape_of<32, 128, 1, 4, 1, 3>(1.63f, 3.05f, 0.415f, 0.096f),
+    shape_of<64, 128, 1, 4, 1, 3>(1.55f, 3.82f, 0.424f, 0.160f),
+    shape_of<256, 128, 4, 2, 1, 3>(0.0f, 6.16f, 0.782f, 0.0f),
+    shape_of<256, 256, 4, 2, 1, 2>(0.0f, 7.31f, 1.454f, 0.0f),
+};
+
+static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
+  const i8_shape *best = nullptr;
+  float least = 0.0f;
+  // experts: as many as can have rows, of the same number each
+  const float matrices = a.offsets ? (float)(a.M < a.E ? a.M : a.E) : 1.0f, rows = a.M / matrices;
+  for (const i8_shape &s : i8_shapes) {
+    const float row_tiles = !a.offsets ? (float)ceil_div(a.M, s.BM) : rows <= s.BM ? 1.0f : rows / s.BM + 0.5f;
+    const float tiles = matrices * row_tiles * (float)ceil_div(a.N, s.BN);
+    const int fit = (160 << 10) / s.lds, occ = fit < 4 ? fit : 4;
+    const float each = tiles / (float)(n_cu * occ), per_cu = ceilf(tiles / (float)n_cu);
+    const float rounds = each <= 3.0f ? ceilf(each) : each + 0.5f;
+    const float cost = s.call + rounds * (s.tile + a.K / 128.0f * (s.k + s.k_share * (per_cu < occ ? per_cu : occ)));
+    if (!best || cost < least) {
+      best = &s;
+      least = cost;
+    }
+  }
+  return *best;
+}
+
+bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
+  i8_mm a = args;
+  // the tiles: 16-byte loads at 32-bit offsets (a smaller row count is a uniform matter of the operands)
   const bool aligned = a.K % 16 == 0 && ((uintptr_t)a.q | (uintptr_t)a.w) % 16 == 0;
   const bool offsets32 = (uint64_t)a.n_src * a.K < MOE_I8_OOB && (uint64_t)a.N * a.K < MOE_I8_OOB;
   if (aligned && offsets32) {
-    const long rows = a.offsets ? (a.M + a.E - 1) / a.E : a.M;  // a matrix's, on average
-    const long matrices = a.offsets ? (a.M < a.E ? a.M : a.E) : 1;
-    if (rows <= 16 && matrices * ceil_div(a.N, 128) < n_cu) return launch_tiles<16, 32, 1, 1, 8, 3, 16, 1>(a, st);
-    if (rows <= 64) return launch_tiles<64, 128, 2, 2, 1, 3, 32, 1>(a, st);
-    if (i8_tiles(a, 256) * ceil_div(a.N, 256) < n_cu) return launch_tiles<128, 128, 2, 2, 1, 2, 32, 1>(a, st);
-    return launch_tiles<256, 256, 2, 4, 1, 2, 16, 1>(a, st);
+    // weights of more than the caches hold from call to call, each read by one tile: past the caches.  Measured:
+    // 939 MB against 16 rows 164 us with plain loads, 146 without (5.75 and 6.5 TB/s)
+    a.stream = (size_t)a.N * a.K * (a.M < a.E ? a.M : a.E) > MOE_STREAM_BYTES;
+    return choose_shape(a, n_cu).launch(a, st);
   }
   const int nt = a.swiglu ? ceil_div(a.N / 2, 32) : ceil_div(a.N, 64);
   const long mt = i8_tiles(a, 64);

@@ -12,6 +12,8 @@
 #include "../../include/moe_block.h"
 #include "kernels_dispatch.h"
 
+#include <type_traits>
+
 
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -156,51 +158,69 @@ __global__ __launch_bounds__(256) void k_quantize_i8_long(const T *__restrict__ 
 
 // ---- products --------------------------------------------------------------------
 
-// The rows of one tile: expert e (-1: none left), rows [r0, r0 + n).
+// The rows of one tile: expert e (-1: none left), rows [r0, r0 + n); only: the expert has no others.
 struct i8_tile {
-  int e, r0, n;
+  int e, r0, n, only;
 };
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);  // row_bcast15: the last lane of rows 0 and 2 to rows 1 and 3
+  v = dpp_add<0x143, 0xC>(v);  // row_bcast31: lane 31 to rows 2 and 3
+  return v;
+}
+
 // Tile `item` of the grouped rows cut into tiles of at most BM: expert e has
-// ceil(c_e / BM) of them, in expert order.  Every wave finds it for itself,
-// 64 experts at a time (E <= 1024: all offsets are asked for at once), with a
-// scan over the lanes.  Offsets are held to [0, M].
+// ceil(c_e / BM) of them, in expert order.  Every wave finds it for itself: lane
+// l counts the tiles of E / 64 experts side by side (all offsets are asked for
+// at once), a scan over the lanes finds the lane that holds the item.  Offsets are
+// held to [0, M].  PER: experts a lane, at least E / 64.
+template <int PER>
+__device__ __forceinline__ i8_tile i8_search(const i8_mm &a, int item, int BM) {
+  const int lane = threadIdx.x & 63;
+  int o[PER + 1];
+#pragma unroll
+  for (int i = 0; i <= PER; i++) o[i] = a.offsets[min(PER * lane + i, a.E)];  // (past the end: equal, no rows)
+  int c[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i <= PER; i++) o[i] = min(max(o[i], 0), a.M);
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    c[i] = o[i + 1] > o[i] ? (o[i + 1] - o[i] + BM - 1) / BM : 0;
+    sum += c[i];
+  }
+  int at = wave_scan(sum) - sum;
+  const uint64_t here = __ballot(at <= item && item < at + sum);
+  if (!here) return {-1, 0, 0, 0};
+  i8_tile t = {-1, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    if (at <= item && item < at + c[i]) {
+      const int r0 = o[i] + (item - at) * BM;
+      t = {PER * lane + i, r0, o[i + 1] - r0 < BM ? o[i + 1] - r0 : BM, c[i] == 1};
+    }
+    at += c[i];
+  }
+  const int owner = __ffsll((unsigned long long)here) - 1;
+  return {__builtin_amdgcn_readlane(t.e, owner), __builtin_amdgcn_readlane(t.r0, owner), __builtin_amdgcn_readlane(t.n, owner),
+          __builtin_amdgcn_readlane(t.only, owner)};
+}
 __device__ __forceinline__ i8_tile i8_find_tile(const i8_mm &a, int item, int BM) {
   if (!a.offsets) {
     const int r0 = item * BM;
-    return {r0 < a.M ? 0 : -1, r0, a.M - r0 < BM ? a.M - r0 : BM};
+    return {r0 < a.M ? 0 : -1, r0, a.M - r0 < BM ? a.M - r0 : BM, a.M <= BM};
   }
-  const int lane = threadIdx.x & 63;
-  int lo[16], hi[16];
-#pragma unroll
-  for (int j = 0; j < 16; j++)
-    if (64 * j < a.E) {
-      const int e = min(64 * j + lane, a.E - 1);
-      lo[j] = a.offsets[e];
-      hi[j] = a.offsets[e + 1];
-    }
-  int first = 0;
-#pragma unroll
-  for (int j = 0; j < 16; j++)
-    if (64 * j < a.E) {
-      const int l = min(max(lo[j], 0), a.M), h = min(max(hi[j], 0), a.M);
-      const int c = 64 * j + lane < a.E && h > l ? (h - l + BM - 1) / BM : 0;
-      int sum = c;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(sum, o);
-        if (lane >= o) sum += u;
-      }
-      const int at = first + sum - c;
-      const uint64_t here = __ballot(at <= item && item < at + c);
-      if (here) {
-        const int r0 = l + (item - at) * BM, n = h - r0 < BM ? h - r0 : BM;
-        const int owner = __ffsll((unsigned long long)here) - 1;
-        return {64 * j + owner, __builtin_amdgcn_readlane(r0, owner), __builtin_amdgcn_readlane(n, owner)};
-      }
-      first += __builtin_amdgcn_readlane(sum, 63);
-    }
-  return {-1, 0, 0};
+  if (a.E <= 64) return i8_search<1>(a, item, BM);
+  if (a.E <= 256) return i8_search<4>(a, item, BM);
+  return i8_search<16>(a, item, BM);
 }
 
 // Source row of grouped row r (-1 where perm points outside).
@@ -305,39 +325,17 @@ __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
 // ---- staged tiles -------------------------------------------------------------------
 //
 // K % 16 == 0 and 16-byte aligned rows.  A workgroup multiplies BM rows with BN
-// channels; both go to LDS by direct loads, 128 bytes of K a row, NBUF stages
-// around.  A 1 KiB load is 8 rows; the 16-byte chunk c of row r lies at c ^ (r & 7),
-// so the 16 or 32 rows that an MFMA operand reads at one chunk fall on all banks.
-// Waves: WM x WN over the tile, and WK over K (wave k takes every WK-th 128
-// bytes; the sums meet in LDS after the loop).
-// MF x MF MFMA with the rows as A and the channels as B: a D lane holds one
-// channel (gate and up of one column are in one lane: the wave's channel tiles
-// alternate) and 4 consecutive rows an element quad.
+// channels; both go to LDS by direct loads, 128 bytes of K a row and block,
+// NBUF stages around.  A 1 KiB load is 8 rows; the 16-byte chunk c of row r lies
+// at c ^ (r & 7), so that the 16 rows that an MFMA operand reads at one chunk fall
+// on all banks.  Waves: WM x WN over the tile, and WK over K (a stage is WK blocks
+// of 128 bytes, wave k takes block k; the sums meet in LDS after the loop).
+// 16x16x64 MFMA, channels as A and rows as B: D lane l holds row l % 16 of its
+// row tile and channels 4 (l / 16) + i of its channel tile.
 #define MOE_I8_OOB 0xffffff00u  // a lane offset past any buffer: the load returns 0
 #define MOE_I8_RSRC 0x00020000  // raw buffer, 32-bit dwords, no swizzle
 
-template <int MF>
-struct i8_frag;
-template <>
-struct i8_frag<16> {
-  typedef v4i acc_t;
-  static constexpr int KC = 4, NACC = 4;  // 16-byte chunks of K an MFMA takes; values a lane holds
-  static __device__ __forceinline__ acc_t mfma(v4i a, v4i b, acc_t c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int i) { return 4 * (lane >> 4) + i; }
-};
-template <>
-struct i8_frag<32> {
-  typedef v16i acc_t;
-  static constexpr int KC = 2, NACC = 16;
-  static __device__ __forceinline__ acc_t mfma(v4i a, v4i b, acc_t c) {
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ int row(int lane, int i) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
-};
-
-// Waits for vmcnt <= n only (gfx9 encoding), then for every wave's LDS reads.
+// Waits for vmcnt <= n only (gfx9 encoding), then for this wave's LDS reads, then for every wave.
 template <int N>
 __device__ __forceinline__ void i8_wait_barrier() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70 | 0xF00);
@@ -346,188 +344,233 @@ __device__ __forceinline__ void i8_wait_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// 64 lanes' 16 bytes at base + vo + so into the 1 KiB at buf.
-__device__ __forceinline__ void i8_dma(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so) {
+// 64 lanes' 16 bytes at base + vo + so into the 1 KiB at buf.  once: read by no other workgroup (non-temporal).
+__device__ __forceinline__ void i8_dma(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so, bool once) {
   typedef __attribute__((address_space(3))) void *lds_t;
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, MOE_I8_RSRC);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 0);
+  if (once) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 2);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 0);
 }
 
-// This wave's share of the N_LOAD 1 KiB loads of `span` bytes of K, from k0 on, of
-// R rows a 128-byte block: loads wave, wave + NW, ...  vo: lane offsets at K 0.
-// Lanes past K, and every lane of a stage past the end, are out of range: they
-// read 0, and the waits can count on the loads.
+// Load i of this wave's share (loads wave, wave + NW, ...) of the N_LOAD 1 KiB loads
+// of a stage from K byte k0 on, R rows a block of 128 bytes.  vo: lane offsets at
+// K 0.  Lanes past K, and every lane of a stage past the end, are out of range:
+// they read 0, and the waits can count on the loads.
 template <int R, int N_LOAD, int NW>
-__device__ __forceinline__ void i8_stage(const int8_t *base, uint32_t bytes, const uint32_t (&vo)[(N_LOAD + NW - 1) / NW],
-                                         v4i *buf, int wave, int k0, int span, int k_lane, int K) {
-  constexpr int N = (N_LOAD + NW - 1) / NW;
-  if (k0 + span <= K) {
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      if (N_LOAD % NW == 0 || wave + NW * i < N_LOAD) i8_dma(base, bytes, buf + (wave + NW * i) * 64, vo[i], k0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      if (N_LOAD % NW == 0 || wave + NW * i < N_LOAD) {
-        const int u = wave + NW * i;
-        i8_dma(base, bytes, buf + u * 64, k0 + 8 * u / R * 128 + k_lane < K ? vo[i] : MOE_I8_OOB, k0 < K ? k0 : 0);
-      }
-  }
+__device__ __forceinline__ void i8_load(int i, const int8_t *base, uint32_t bytes, uint32_t vo, v4i *buf, int wave, int k0,
+                                        int k_lane, int K, bool once) {
+  const int u = wave + NW * i;
+  if (N_LOAD % NW == 0 || u < N_LOAD)  // uniform over the wave
+    i8_dma(base, bytes, buf + u * 64, k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB, k0 < K ? k0 : 0, once);
 }
 
-// Floats from a row to the next in a wave's region of LDS on the way out.
-template <int TN>
-constexpr int i8_out_stride() { return TN + 4; }
-
-// The stages; then, over them, the sums of the waves along K and each wave's rows on their way out; the rows' scales.
-template <int BM, int BN, int WM, int WN, int WK, int NBUF, int MF>
+// The stages; then, over them, the sums of the waves along K; the rows' scales.
+template <int BM, int BN, int WK, int NBUF>
 constexpr int i8_lds_bytes() {
-  const int ring = NBUF * (BM + BN) * WK * 128, part = (WK - 1) * BM * BN * 4 + WM * WN * MF * i8_out_stride<BN / WN>() * 4;
+  const int ring = NBUF * (BM + BN) * WK * 128, part = (WK - 1) * BM * BN * 4;
   return (ring > part ? ring : part) + 4 * BM;
 }
 
-template <int BM, int BN, int WM, int WN, int WK, int NBUF, int MF, int OCC>
-__global__ __launch_bounds__(64 * WM * WN * WK, OCC) void k_mm_i8(i8_mm a, int nt) {
-  typedef i8_frag<MF> F;
-  constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, MI = TM / MF, NI = TN / MF;
-  constexpr int STAGE = (BM + BN) * WK * 8;                     // 16-byte chunks of a stage
-  constexpr int XI = BM * WK / 8, WI = BN * WK / 8;             // 1 KiB loads of a stage
+// Row `row` (0..15) of a wave's channel tile j is this column of its output
+// columns.  SwiGLU: gate and up tiles alternate (one tile alone holds 8 rows of
+// each).  The 4 rows that a lane holds of two output tiles are 8 columns side by
+// side, and the lane stores them at once; a last tile without a partner is in order.
+template <int NI>
+__device__ __forceinline__ int i8_column(int swiglu, int j, int row) {
+  if (swiglu && NI == 1) return row % 8;
+  const int o = swiglu ? j / 2 : j, outs = swiglu ? NI / 2 : NI;
+  return outs % 2 && o == outs - 1 ? o * 16 + row : o / 2 * 32 + 8 * (row / 4) + 4 * (o & 1) + row % 4;
+}
+template <int NI>
+__device__ __forceinline__ bool i8_is_up(int j, int row) { return NI == 1 ? row >= 8 : j & 1; }
+
+template <int V>
+__device__ __forceinline__ void i8_store_v(const i8_mm &a, size_t at, int left, const float (&f)[V]) {
+  if (a.out_type == MOE_GGML_F32) store_v<float, V>(reinterpret_cast<float *>(a.out) + at, left, f);
+  else if (a.out_type == MOE_GGML_F16) store_v<_Float16, V>(reinterpret_cast<_Float16 *>(a.out) + at, left, f);
+  else store_v<bf16_t, V>(reinterpret_cast<bf16_t *>(a.out) + at, left, f);
+}
+
+template <int BM, int BN, int WM, int WN, int WK, int NBUF>
+__global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
+  constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
+  constexpr int STAGE = (BM + BN) * WK * 8;          // 16-byte chunks of a stage
+  constexpr int XI = BM * WK / 8, WI = BN * WK / 8;  // 1 KiB loads of a stage
   constexpr int NX = (XI + NW - 1) / NW, NWI = (WI + NW - 1) / NW;
-  constexpr int CNT = XI / NW + WI / NW;                        // of every wave, at least
+  constexpr int CX = XI / NW, CNT = CX + WI / NW;    // loads of every wave, at least
   // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
-  static_assert(NI % 2 == 0, "gate and up of a column are channel tiles of one wave");
   extern __shared__ v4i lds[];
-  float *sxs = reinterpret_cast<float *>(lds + i8_lds_bytes<BM, BN, WM, WN, WK, NBUF, MF>() / 16) - BM;  // the rows' scales
+  float *sxs = reinterpret_cast<float *>(lds + i8_lds_bytes<BM, BN, WK, NBUF>() / 16) - BM;  // the rows' scales
+  static_assert(NI > 1 || MI == 1, "one channel tile: one row tile");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
-  const int nb = blockIdx.x % nt;
   const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
   if (t.e < 0) return;
   const int half = a.N / 2, n_end = a.swiglu ? half : a.N;
-  // output column of channel row j of the tile, and its weight row
-  auto column = [&](int j) {
-    const int jj = j % TN;
-    return a.swiglu ? nb * (BN / 2) + j / TN * (TN / 2) + jj / (2 * MF) * MF + jj % MF : nb * BN + j;
-  };
-  auto weight_row = [&](int j) { return a.swiglu && (j % TN / MF & 1) ? half + column(j) : column(j); };
+  const int cols = a.swiglu ? TN / 2 : TN, c0 = blockIdx.x % nt * WN * cols;  // a wave's output columns; the workgroup's first
 
-  // lane offsets of this wave's loads: row of the 8, chunk swizzled by it
+  // lane offsets of this wave's loads at K 0: row lr of the load's 8, chunk swizzled by it
   const int lr = lane >> 3, lc = (lane & 7) ^ lr;
   uint32_t vx[NX], vw[NWI];
-  for (int i = tid; i < BM; i += 64 * NW) {
-    const int s = i < t.n ? i8_src(a, t.r0 + i) : -1;
-    sxs[i] = s >= 0 ? a.qs[s] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < NWI; i++) {
+    const int rr = 8 * (wave + NW * i), j = rr % BN + lr, jt = j % TN / 16;
+    const int c = c0 + j / TN * cols + i8_column<NI>(a.swiglu, jt, j % 16), w = a.swiglu && i8_is_up<NI>(jt, j % 16) ? half + c : c;
+    vw[i] = c < n_end ? (uint32_t)w * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_I8_OOB;
   }
+  const int8_t *wbase = a.w + (size_t)t.e * a.N * a.K;
+  const uint32_t xbytes = (uint32_t)a.n_src * (uint32_t)a.K, wbytes = (uint32_t)a.N * (uint32_t)a.K;
+  const int stages = (a.K + 128 * WK - 1) / (128 * WK);
+  const bool once = a.stream && t.only;
+  // loads l of this wave's of stage s, into buffer b: the rows' WK blocks of BM x 128 bytes, then the channels'
+  auto load_x = [&](int l, int s, int b) __attribute__((always_inline)) {
+    i8_load<BM, XI, NW>(l, a.q, xbytes, vx[l], lds + b * STAGE, wave, s * 128 * WK, lc * 16, a.K, false);
+  };
+  auto load_w = [&](int l, int s, int b) __attribute__((always_inline)) {
+    i8_load<BN, WI, NW>(l, wbase, wbytes, vw[l], lds + b * STAGE + BM * WK * 8, wave, s * 128 * WK, lc * 16, a.K, once);
+  };
+  // the weights go out before the rows are known (a load and a division away)
+#pragma unroll
+  for (int s = 0; s < NBUF; s++)
+#pragma unroll
+    for (int l = 0; l < NWI; l++) load_w(l, s, s);
+  const int srow = tid < BM && tid < t.n ? i8_src(a, t.r0 + tid) : -1;
+  static_assert(64 * NW >= BM, "a thread for each row's scale");
 #pragma unroll
   for (int i = 0; i < NX; i++) {
     const int rr = 8 * (wave + NW * i), row = rr % BM + lr, s = row < t.n ? i8_src(a, t.r0 + row) : -1;
     vx[i] = s >= 0 ? (uint32_t)s * (uint32_t)a.K + rr / BM * 128 + lc * 16 : MOE_I8_OOB;
   }
+  const float srow_scale = srow >= 0 ? a.qs[srow] : 0.0f;
 #pragma unroll
-  for (int i = 0; i < NWI; i++) {
-    const int rr = 8 * (wave + NW * i), j = rr % BN + lr;
-    vw[i] = column(j) < n_end ? (uint32_t)weight_row(j) * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_I8_OOB;
-  }
-  const int8_t *wbase = a.w + (size_t)t.e * a.N * a.K;
-  const uint32_t xbytes = (uint32_t)a.n_src * (uint32_t)a.K, wbytes = (uint32_t)a.N * (uint32_t)a.K;
-  const int stages = (a.K + 128 * WK - 1) / (128 * WK);
-  typename F::acc_t acc[MI][NI];
+  for (int s = 0; s < NBUF; s++)
 #pragma unroll
-  for (int i = 0; i < MI; i++)
+    for (int l = 0; l < NX; l++) load_x(l, s, s);
+  if (tid < BM) sxs[tid] = srow_scale;
+
+  v4i acc[NI][MI];
 #pragma unroll
-    for (int j = 0; j < NI; j++) acc[i][j] = typename F::acc_t{};
-  const int fr = lane % MF, fg = lane / MF;  // this lane's row of an operand, and which chunk of the MFMA's
-  // stage s into buffer b: the rows' WK blocks of BM x 128 bytes, then the channels'
-  auto issue = [&](int s, int b) __attribute__((always_inline)) {
-    const int k0 = s * 128 * WK;
-    i8_stage<BM, XI, NW>(a.q, xbytes, vx, lds + b * STAGE, wave, k0, 128 * WK, lc * 16, a.K);
-    i8_stage<BN, WI, NW>(wbase, wbytes, vw, lds + b * STAGE + BM * WK * 8, wave, k0, 128 * WK, lc * 16, a.K);
+  for (int j = 0; j < NI; j++)
+#pragma unroll
+    for (int i = 0; i < MI; i++) acc[j][i] = v4i{0, 0, 0, 0};
+  const int fr = lane & 15, fg = lane >> 4;  // this lane's row of an operand, and its chunk of 4
+  // Two MFMA steps a stage, 64 bytes of K each; their operands alternate between two sets of
+  // registers, a step ahead of the MFMAs (over the stages' border too).
+  v4i A[2][NI], B[2][MI];
+  // the operands of step kk of the stage in buffer b, in MI parts
+  auto read = [&](int i, int set, int b, int kk) __attribute__((always_inline)) {
+    const v4i *xb = lds + b * STAGE + (wk * BM + wm * TM + fr) * 8;
+    const v4i *wb = lds + b * STAGE + (BM * WK + wk * BN + wn * TN + fr) * 8;
+    const int c = (kk * 4 + fg) ^ (fr & 7);
+    B[set][i] = xb[i * 128 + c];
+#pragma unroll
+    for (int j = 0; j < NI; j++)
+      if (j * MI / NI == i) A[set][j] = wb[j * 128 + c];
   };
+  i8_wait_barrier<(NBUF - 1) * CX>();
 #pragma unroll
-  for (int s = 0; s < NBUF - 1; s++) issue(s, s);
+  for (int i = 0; i < MI; i++) read(i, 0, 0, 0);
   int cur = 0;
 #pragma unroll 1
   for (int s = 0; s < stages; s++) {
-    i8_wait_barrier<(NBUF - 2) * CNT>();
-    issue(s + NBUF - 1, cur == 0 ? NBUF - 1 : cur - 1);
-    const v4i *xb = lds + cur * STAGE + (wk * BM + wm * TM + fr) * 8;
-    const v4i *wb = lds + cur * STAGE + (BM * WK + wk * BN + wn * TN + fr) * 8;
+    const int next = cur + 1 == NBUF ? 0 : cur + 1;
 #pragma unroll
-    for (int kk = 0; kk < 8 / F::KC; kk++) {
-      const int c = (kk * F::KC + fg) ^ (fr & 7);
-      v4i A[MI], B[NI];
+    for (int kk = 0; kk < 2; kk++) {
+      // Before a stage's last step: the next stage has landed, and every wave
+      // holds the rest of this one in registers, so its buffer is free.  (The
+      // first NBUF stages' weights were all asked for before their rows.)
+      if (kk == 1) {
+        if (NBUF > 2 && s < NBUF - 2) i8_wait_barrier<(NBUF - 2) * CX>();
+        else i8_wait_barrier<(NBUF - 2) * CNT>();
+      }
 #pragma unroll
-      for (int i = 0; i < MI; i++) A[i] = xb[i * MF * 8 + c];
+      for (int i = 0; i < MI; i++) {
+        read(i, kk ^ 1, kk ? next : cur, kk ^ 1);
 #pragma unroll
-      for (int j = 0; j < NI; j++) B[j] = wb[j * MF * 8 + c];
+        for (int j = 0; j < NI; j++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[kk][j], B[kk][i], acc[j][i], 0, 0, 0);
+        // spread between the MFMAs: a wave that waits to issue a load issues nothing else
+        if (kk == 1) {
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+          for (int l = 0; l < NWI; l++)
+            if (l * MI / NWI == i) load_w(l, s + NBUF, cur);
 #pragma unroll
-        for (int j = 0; j < NI; j++) acc[i][j] = F::mfma(A[i], B[j], acc[i][j]);
+          for (int l = 0; l < NX; l++)
+            if (l * MI / NX == i) load_x(l, s + NBUF, cur);
+        }
+      }
     }
-    cur = cur + 1 == NBUF ? 0 : cur + 1;
+    cur = next;
   }
   if constexpr (WK > 1) {
     i8_wait_barrier<0>();  // the last loads, out of range as they are, have landed: the stages are free
-    typename F::acc_t *part = reinterpret_cast<typename F::acc_t *>(lds);
-    const int tile = (wm * WN + wn) * MI * NI;
+    v4i *part = lds + ((wm * WN + wn) * MI * NI) * 64 + lane;
     if (wk > 0) {
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+      for (int j = 0; j < NI; j++)
 #pragma unroll
-        for (int j = 0; j < NI; j++) part[((wk - 1) * WM * WN * MI * NI + tile + i * NI + j) * 64 + lane] = acc[i][j];
+        for (int i = 0; i < MI; i++) part[((wk - 1) * WM * WN * MI * NI + j * MI + i) * 64] = acc[j][i];
     }
     i8_wait_barrier<0>();
     if (wk > 0) return;
     for (int q = 0; q < WK - 1; q++)
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+      for (int j = 0; j < NI; j++)
 #pragma unroll
-        for (int j = 0; j < NI; j++) acc[i][j] += part[(q * WM * WN * MI * NI + tile + i * NI + j) * 64 + lane];
+        for (int i = 0; i < MI; i++) acc[j][i] += part[(q * WM * WN * MI * NI + j * MI + i) * 64];
   } else {
-    i8_wait_barrier<0>();
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // no load into LDS outlives the workgroup
   }
-  // through LDS a block of MF rows at a time, in a region of the wave's own: a
-  // D lane holds one channel, a store wants a row's channels side by side
-  float *reg = reinterpret_cast<float *>(lds + (WK > 1 ? (WK - 1) * BM * BN / 4 : 0)) + (wm * WN + wn) * MF * i8_out_stride<TN>();
+
   const float *ws = a.ws + (size_t)t.e * a.N;
-  float sw[NI];
+  const int cw = c0 + wn * cols;  // this wave's first column
+  auto scale_of = [&](int j, int v) __attribute__((always_inline)) {  // channel scale of value v of tile j
+    const int row = 4 * fg + v, c = cw + i8_column<NI>(a.swiglu, j, row), w = a.swiglu && i8_is_up<NI>(j, row) ? half + c : c;
+    return c < n_end ? ws[w] : 0.0f;
+  };
+  // V columns side by side of output tiles o on, of every row tile
+  auto out = [&](auto width, int o) __attribute__((always_inline)) {
+    constexpr int V = decltype(width)::value;
+    const int c = cw + i8_column<NI>(a.swiglu, a.swiglu ? 2 * o : o, 4 * fg);
+    float s0[V], s1[V];
 #pragma unroll
-  for (int j = 0; j < NI; j++) {
-    const int jr = wn * TN + j * MF + fr;
-    sw[j] = column(jr) < n_end ? ws[weight_row(jr)] : 0.0f;
-  }
-  const int wide = a.swiglu ? TN / 2 : TN, c0 = column(wn * TN);  // the wave's columns, and the first
-  const int left = n_end - c0 < wide ? n_end - c0 : wide;
-#pragma unroll
-  for (int i = 0; i < MI; i++) {
-    const int m0 = wm * TM + i * MF;
-    if (m0 >= t.n) break;
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int v = 0; v < F::NACC; v++) {
-      const float sx = sxs[m0 + F::row(lane, v)];
-      float *to = reg + F::row(lane, v) * i8_out_stride<TN>() + fr;
-      if (!a.swiglu) {
-#pragma unroll
-        for (int j = 0; j < NI; j++) to[j * MF] = (float)acc[i][j][v] * sx * sw[j];
-      } else if constexpr (NI > 1) {
-#pragma unroll
-        for (int j = 0; j < NI; j += 2)
-          to[j / 2 * MF] = i8_swiglu((float)acc[i][j][v] * sx * sw[j], (float)acc[i][j + 1][v] * sx * sw[j + 1], a.clamp);
+    for (int v = 0; v < V; v++) {
+      if (!a.swiglu) s0[v] = scale_of((o + v / 4) % NI, v % 4);
+      else {
+        s0[v] = scale_of(2 * (o + v / 4) % NI, v % 4);
+        s1[v] = scale_of((2 * (o + v / 4) + 1) % NI, v % 4);
       }
     }
-    asm volatile("" ::: "memory");
-    const int rows = t.n - m0 < MF ? t.n - m0 : MF, per = wide / 4;
-    for (int u = lane; u < rows * per; u += 64) {
-      const int r = u / per, c = u % per * 4;
-      const float *from = reg + r * i8_out_stride<TN>() + c;
-      const float f[4] = {from[0], from[1], from[2], from[3]};
-      const size_t at = (size_t)(t.r0 + m0 + r) * n_end + c0 + c;
-      if (c >= left) continue;
-      if (a.out_type == MOE_GGML_F32) store_v<float, 4>(reinterpret_cast<float *>(a.out) + at, left - c, f);
-      else if (a.out_type == MOE_GGML_F16) store_v<_Float16, 4>(reinterpret_cast<_Float16 *>(a.out) + at, left - c, f);
-      else store_v<bf16_t, 4>(reinterpret_cast<bf16_t *>(a.out) + at, left - c, f);
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+      const int m = wm * TM + i * 16 + fr;
+      const float sx = m < t.n ? sxs[m] : 0.0f;
+      float f[V];
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        if (!a.swiglu) f[v] = (float)acc[(o + v / 4) % NI][i][v % 4] * sx * s0[v];
+        else
+          f[v] = i8_swiglu((float)acc[2 * (o + v / 4) % NI][i][v % 4] * sx * s0[v],
+                           (float)acc[(2 * (o + v / 4) + 1) % NI][i][v % 4] * sx * s1[v], a.clamp);
+      }
+      if (m < t.n && c < n_end) i8_store_v<V>(a, (size_t)(t.r0 + m) * n_end + c, n_end - c, f);
     }
+  };
+  if (a.swiglu && NI == 1) {  // lanes 0-31 hold gate, 32-63 up
+    const int c = cw + 4 * fg;
+    float f[4];
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+      const float y = (float)acc[0][0][v] * sxs[wm * TM + fr] * scale_of(0, v);
+      f[v] = i8_swiglu(y, __shfl_xor(y, 32), a.clamp);
+    }
+    if (fg < 2 && wm * TM + fr < t.n && c < n_end) i8_store_v<4>(a, (size_t)(t.r0 + wm * TM + fr) * n_end + c, n_end - c, f);
+  } else if (a.swiglu) {
+#pragma unroll
+    for (int o = 0; o + 1 < NI / 2; o += 2) out(std::integral_constant<int, 8>{}, o);
+    if (NI / 2 % 2) out(std::integral_constant<int, 4>{}, NI / 2 - 1);
+  } else {
+#pragma unroll
+    for (int o = 0; o + 1 < NI; o += 2) out(std::integral_constant<int, 8>{}, o);
+    if (NI % 2) out(std::integral_constant<int, 4>{}, NI - 1);
   }
 }
