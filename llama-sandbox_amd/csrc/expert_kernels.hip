@@ -123,7 +123,7 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
   const long n = i8_tiles(a, BM) * nt;
   if (n > 0x7fffffff) return false;
   hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
-                     (i8_lds_bytes<BM, BN, WK, NBUF>()), st, a, nt);
+                     (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>()), st, a, nt);
   return true;
 }
 
@@ -144,7 +144,7 @@ struct i8_shape {
 };
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 static constexpr i8_shape shape_of(float call, float tile, float k, float k_share) {
-  return {BM, BN, i8_lds_bytes<BM, BN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
+  return {BM, BN, i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
 }
 static const i8_shape i8_shapes[] = {
     shape_of<16, 16, 1, 1, 4, 4>(1.90f, 1.93f, 0.056f, 0.026f),

@@ -364,11 +364,15 @@ __device__ __forceinline__ void i8_load(int i, const int8_t *base, uint32_t byte
     i8_dma(base, bytes, buf + u * 64, k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB, k0 < K ? k0 : 0, once);
 }
 
-// The stages; then, over them, the sums of the waves along K; the rows' scales.
-template <int BM, int BN, int WK, int NBUF>
+// A wave's rows on their way out: 16 rows of up to TN floats, and 16 bytes between them.
+template <int TN>
+constexpr int i8_out_bytes() { return 16 * (TN * 4 + 16); }
+
+// The stages; then, over them, the sums of the waves along K and the rows on their way out; the rows' scales.
+template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 constexpr int i8_lds_bytes() {
-  const int ring = NBUF * (BM + BN) * WK * 128, part = (WK - 1) * BM * BN * 4;
-  return (ring > part ? ring : part) + 4 * BM;
+  const int ring = NBUF * (BM + BN) * WK * 128, after = (WK - 1) * BM * BN * 4 + WM * WN * i8_out_bytes<BN / WN>();
+  return (ring > after ? ring : after) + 4 * BM;
 }
 
 // Row `row` (0..15) of a wave's channel tile j is this column of its output
@@ -384,11 +388,49 @@ __device__ __forceinline__ int i8_column(int swiglu, int j, int row) {
 template <int NI>
 __device__ __forceinline__ bool i8_is_up(int j, int row) { return NI == 1 ? row >= 8 : j & 1; }
 
-template <int V>
-__device__ __forceinline__ void i8_store_v(const i8_mm &a, size_t at, int left, const float (&f)[V]) {
-  if (a.out_type == MOE_GGML_F32) store_v<float, V>(reinterpret_cast<float *>(a.out) + at, left, f);
-  else if (a.out_type == MOE_GGML_F16) store_v<_Float16, V>(reinterpret_cast<_Float16 *>(a.out) + at, left, f);
-  else store_v<bf16_t, V>(reinterpret_cast<bf16_t *>(a.out) + at, left, f);
+// 16 rows x COLS columns of T that a wave holds (`value`: the V columns from 8 p + lane's
+// on of this lane's row) to out's rows r0 on, columns c0 on; `rows` and `left` of them
+// exist.  Through LDS: a lane's columns are one row's, and neighbouring lanes hold
+// other rows; stored from there, a quad of lanes would touch 4 rows (256 KiB a tile of
+// f32 took 20 thousand cycles, the K loop of K = 768 as many).
+template <typename T, int COLS, int V, typename F>
+__device__ __forceinline__ void i8_rows_out(T *out, int8_t *reg, int lane, size_t r0, int rows, int pitch, int c0, int left,
+                                            F value) {
+  constexpr int ES = sizeof(T), ROW = COLS * ES + 16, PIECES = COLS * ES / 16;  // bytes to the next row; 16-byte pieces of one
+  typedef T quad_t __attribute__((ext_vector_type(4)));
+  typedef T piece_t __attribute__((ext_vector_type(16 / ES)));
+  const int fr = lane & 15, fg = lane >> 4;
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int p = 0; p < (COLS + 4 * V - 1) / (4 * V); p++) {
+    float f[V];
+    value(p, f);
+    if (COLS < 4 * V && fg >= COLS / V) continue;  // (one tile of 8 gate and 8 up rows: two lane groups hold them)
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      quad_t w;
+#pragma unroll
+      for (int v = 0; v < 4; v++) w[v] = (T)f[q + v];
+      *reinterpret_cast<quad_t *>(reg + fr * ROW + (p * 4 * V + fg * V + q) * ES) = w;
+    }
+  }
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int u0 = 0; u0 < 16 * PIECES; u0 += 64) {
+    const int u = u0 + lane, r = u / PIECES, c = u % PIECES * (16 / ES);
+    if (16 * PIECES % 64 && u >= 16 * PIECES) break;
+    if (r >= rows || c >= left) continue;
+    const piece_t w = *reinterpret_cast<const piece_t *>(reg + r * ROW + c * ES);
+    T *to = out + (r0 + r) * (size_t)pitch + c0 + c;
+    typedef T any_t __attribute__((ext_vector_type(16 / ES), aligned(ES)));
+    if (c + 16 / ES <= left) {
+      *reinterpret_cast<any_t *>(to) = w;
+    } else {
+#pragma unroll
+      for (int v = 0; v < 16 / ES; v++)
+        if (c + v < left) to[v] = w[v];
+    }
+  }
 }
 
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
@@ -400,8 +442,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   constexpr int CX = XI / NW, CNT = CX + WI / NW;    // loads of every wave, at least
   // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
   extern __shared__ v4i lds[];
-  float *sxs = reinterpret_cast<float *>(lds + i8_lds_bytes<BM, BN, WK, NBUF>() / 16) - BM;  // the rows' scales
-  static_assert(NI > 1 || MI == 1, "one channel tile: one row tile");
+  float *sxs = reinterpret_cast<float *>(lds + i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>() / 16) - BM;  // the rows' scales
+  static_assert(NI == 1 || NI % 4 == 0 || NI == 2, "output tiles in pairs, or one");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
   const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
@@ -518,59 +560,59 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
 #pragma unroll
         for (int i = 0; i < MI; i++) acc[j][i] += part[(q * WM * WN * MI * NI + j * MI + i) * 64];
   } else {
-    __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // no load into LDS outlives the workgroup
+    i8_wait_barrier<0>();
   }
 
+  int8_t *reg = reinterpret_cast<int8_t *>(lds) + (WK - 1) * BM * BN * 4 + (wm * WN + wn) * i8_out_bytes<TN>();
   const float *ws = a.ws + (size_t)t.e * a.N;
   const int cw = c0 + wn * cols;  // this wave's first column
   auto scale_of = [&](int j, int v) __attribute__((always_inline)) {  // channel scale of value v of tile j
     const int row = 4 * fg + v, c = cw + i8_column<NI>(a.swiglu, j, row), w = a.swiglu && i8_is_up<NI>(j, row) ? half + c : c;
     return c < n_end ? ws[w] : 0.0f;
   };
-  // V columns side by side of output tiles o on, of every row tile
-  auto out = [&](auto width, int o) __attribute__((always_inline)) {
-    constexpr int V = decltype(width)::value;
-    const int c = cw + i8_column<NI>(a.swiglu, a.swiglu ? 2 * o : o, 4 * fg);
-    float s0[V], s1[V];
+  float sw[NI][4];
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-      if (!a.swiglu) s0[v] = scale_of((o + v / 4) % NI, v % 4);
-      else {
-        s0[v] = scale_of(2 * (o + v / 4) % NI, v % 4);
-        s1[v] = scale_of((2 * (o + v / 4) + 1) % NI, v % 4);
-      }
-    }
+  for (int j = 0; j < NI; j++)
 #pragma unroll
-    for (int i = 0; i < MI; i++) {
-      const int m = wm * TM + i * 16 + fr;
-      const float sx = m < t.n ? sxs[m] : 0.0f;
-      float f[V];
+    for (int v = 0; v < 4; v++) sw[j][v] = scale_of(j, v);
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        if (!a.swiglu) f[v] = (float)acc[(o + v / 4) % NI][i][v % 4] * sx * s0[v];
-        else
-          f[v] = i8_swiglu((float)acc[2 * (o + v / 4) % NI][i][v % 4] * sx * s0[v],
-                           (float)acc[(2 * (o + v / 4) + 1) % NI][i][v % 4] * sx * s1[v], a.clamp);
-      }
-      if (m < t.n && c < n_end) i8_store_v<V>(a, (size_t)(t.r0 + m) * n_end + c, n_end - c, f);
-    }
-  };
-  if (a.swiglu && NI == 1) {  // lanes 0-31 hold gate, 32-63 up
-    const int c = cw + 4 * fg;
-    float f[4];
+  for (int i = 0; i < MI; i++) {
+    const int m0 = wm * TM + i * 16, rows = t.n - m0 < 16 ? t.n - m0 : 16;
+    if (rows <= 0) break;
+    const float sx = sxs[m0 + fr];
+    auto plain = [&](auto width) __attribute__((always_inline)) {
+      constexpr int V = decltype(width)::value;
+      return [&](int p, float(&f)[V]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int v = 0; v < 4; v++) {
-      const float y = (float)acc[0][0][v] * sxs[wm * TM + fr] * scale_of(0, v);
-      f[v] = i8_swiglu(y, __shfl_xor(y, 32), a.clamp);
-    }
-    if (fg < 2 && wm * TM + fr < t.n && c < n_end) i8_store_v<4>(a, (size_t)(t.r0 + wm * TM + fr) * n_end + c, n_end - c, f);
-  } else if (a.swiglu) {
+        for (int v = 0; v < V; v++) f[v] = (float)acc[p * V / 4 + v / 4][i][v % 4] * sx * sw[p * V / 4 + v / 4][v % 4];
+      };
+    };
+    auto gated = [&](auto width) __attribute__((always_inline)) {
+      constexpr int V = decltype(width)::value;
+      return [&](int p, float(&f)[V]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int o = 0; o + 1 < NI / 2; o += 2) out(std::integral_constant<int, 8>{}, o);
-    if (NI / 2 % 2) out(std::integral_constant<int, 4>{}, NI / 2 - 1);
-  } else {
-#pragma unroll
-    for (int o = 0; o + 1 < NI; o += 2) out(std::integral_constant<int, 8>{}, o);
-    if (NI % 2) out(std::integral_constant<int, 4>{}, NI - 1);
+        for (int v = 0; v < V; v++) {
+          if constexpr (NI == 1) {  // lanes 0-31 hold gate, 32-63 up
+            const float y = (float)acc[0][i][v] * sx * sw[0][v];
+            f[v] = i8_swiglu(y, __shfl_xor(y, 32), a.clamp);
+          } else {
+            const int j = 2 * (p * V / 4 + v / 4);
+            f[v] = i8_swiglu((float)acc[j][i][v % 4] * sx * sw[j][v % 4], (float)acc[j + 1][i][v % 4] * sx * sw[j + 1][v % 4], a.clamp);
+          }
+        }
+      };
+    };
+    auto to = [&](auto zero) __attribute__((always_inline)) {
+      typedef decltype(zero) T;
+      T *o = reinterpret_cast<T *>(a.out);
+      constexpr int VP = NI % 2 ? 4 : 8, VG = NI < 4 ? 4 : 8;  // columns side by side in a lane
+      if (!a.swiglu)
+        i8_rows_out<T, TN, VP>(o, reg, lane, t.r0 + m0, rows, n_end, cw, n_end - cw, plain(std::integral_constant<int, VP>{}));
+      else
+        i8_rows_out<T, TN / 2, VG>(o, reg, lane, t.r0 + m0, rows, n_end, cw, n_end - cw, gated(std::integral_constant<int, VG>{}));
+    };
+    if (a.out_type == MOE_GGML_F32) to(float{});
+    else if (a.out_type == MOE_GGML_F16) to((_Float16)0.0f);
+    else to((bf16_t)0.0f);
   }
 }
