@@ -364,15 +364,16 @@ __device__ __forceinline__ void i8_load(int i, const int8_t *base, uint32_t byte
     i8_dma(base, bytes, buf + u * 64, k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB, k0 < K ? k0 : 0, once);
 }
 
-// A wave's rows on their way out: 16 rows of up to TN floats, and 16 bytes between them.
-template <int TN>
-constexpr int i8_out_bytes() { return 16 * (TN * 4 + 16); }
+// A wave's rows on their way out: 16 rows of up to 128 bytes, and 16 between them.
+#define MOE_I8_OUT 128
+#define MOE_I8_OUT_BYTES (16 * (MOE_I8_OUT + 16))
 
-// The stages; then, over them, the sums of the waves along K and the rows on their way out; the rows' scales.
+// The stages; over them, after the loop, the sums of the waves along K and the rows on their way
+// out; the rows' and channels' scales.
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 constexpr int i8_lds_bytes() {
-  const int ring = NBUF * (BM + BN) * WK * 128, after = (WK - 1) * BM * BN * 4 + WM * WN * i8_out_bytes<BN / WN>();
-  return (ring > after ? ring : after) + 4 * BM;
+  const int ring = NBUF * (BM + BN) * WK * 128, after = (WK - 1) * BM * BN * 4 + WM * WN * MOE_I8_OUT_BYTES;
+  return (ring > after ? ring : after) + 4 * (BM + BN);
 }
 
 // Row `row` (0..15) of a wave's channel tile j is this column of its output
@@ -388,47 +389,52 @@ __device__ __forceinline__ int i8_column(int swiglu, int j, int row) {
 template <int NI>
 __device__ __forceinline__ bool i8_is_up(int j, int row) { return NI == 1 ? row >= 8 : j & 1; }
 
-// 16 rows x COLS columns of T that a wave holds (`value`: the V columns from 8 p + lane's
-// on of this lane's row) to out's rows r0 on, columns c0 on; `rows` and `left` of them
-// exist.  Through LDS: a lane's columns are one row's, and neighbouring lanes hold
-// other rows; stored from there, a quad of lanes would touch 4 rows (256 KiB a tile of
-// f32 took 20 thousand cycles, the K loop of K = 768 as many).
+// 16 rows x COLS columns of T that a wave holds (`value`: part p's V columns of this
+// lane, from column 4 V p + V (lane / 16) of its row lane % 16 on) to out's rows r0
+// on, columns c0 on; `rows` and `left` of them exist.  Through LDS, 128 bytes of a row
+// at a time: a lane's columns are one row's, and neighbouring lanes hold other rows;
+// stored from there, a quad of lanes touches 4 rows (256 KiB of f32 took 20 thousand
+// cycles that way, 15 so).
 template <typename T, int COLS, int V, typename F>
 __device__ __forceinline__ void i8_rows_out(T *out, int8_t *reg, int lane, size_t r0, int rows, int pitch, int c0, int left,
                                             F value) {
-  constexpr int ES = sizeof(T), ROW = COLS * ES + 16, PIECES = COLS * ES / 16;  // bytes to the next row; 16-byte pieces of one
+  constexpr int ES = sizeof(T), RUN = COLS * ES < MOE_I8_OUT ? COLS : MOE_I8_OUT / ES;  // columns at a time
+  constexpr int ROW = RUN * ES + 16, PIECES = RUN * ES / 16, PARTS = RUN < 4 * V ? 1 : RUN / (4 * V);
   typedef T quad_t __attribute__((ext_vector_type(4)));
   typedef T piece_t __attribute__((ext_vector_type(16 / ES)));
+  typedef T any_t __attribute__((ext_vector_type(16 / ES), aligned(ES)));
   const int fr = lane & 15, fg = lane >> 4;
-  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int p = 0; p < (COLS + 4 * V - 1) / (4 * V); p++) {
-    float f[V];
-    value(p, f);
-    if (COLS < 4 * V && fg >= COLS / V) continue;  // (one tile of 8 gate and 8 up rows: two lane groups hold them)
+  for (int n = 0; n < COLS / RUN; n++) {
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int q = 0; q < V; q += 4) {
-      quad_t w;
+    for (int p = 0; p < PARTS; p++) {
+      float f[V];
+      value(n * PARTS + p, f);
+      if (RUN < 4 * V && fg >= RUN / V) continue;  // (one tile of 8 gate and 8 up rows: two lane groups hold them)
 #pragma unroll
-      for (int v = 0; v < 4; v++) w[v] = (T)f[q + v];
-      *reinterpret_cast<quad_t *>(reg + fr * ROW + (p * 4 * V + fg * V + q) * ES) = w;
+      for (int q = 0; q < V; q += 4) {
+        quad_t w;
+#pragma unroll
+        for (int v = 0; v < 4; v++) w[v] = (T)f[q + v];
+        *reinterpret_cast<quad_t *>(reg + fr * ROW + (p * 4 * V + fg * V + q) * ES) = w;
+      }
     }
-  }
-  asm volatile("" ::: "memory");
+    asm volatile("" ::: "memory");
 #pragma unroll
-  for (int u0 = 0; u0 < 16 * PIECES; u0 += 64) {
-    const int u = u0 + lane, r = u / PIECES, c = u % PIECES * (16 / ES);
-    if (16 * PIECES % 64 && u >= 16 * PIECES) break;
-    if (r >= rows || c >= left) continue;
-    const piece_t w = *reinterpret_cast<const piece_t *>(reg + r * ROW + c * ES);
-    T *to = out + (r0 + r) * (size_t)pitch + c0 + c;
-    typedef T any_t __attribute__((ext_vector_type(16 / ES), aligned(ES)));
-    if (c + 16 / ES <= left) {
-      *reinterpret_cast<any_t *>(to) = w;
-    } else {
+    for (int u0 = 0; u0 < 16 * PIECES; u0 += 64) {
+      const int u = u0 + lane, r = u / PIECES, c = n * RUN + u % PIECES * (16 / ES);
+      if (16 * PIECES % 64 && u >= 16 * PIECES) break;
+      if (r >= rows || c >= left) continue;
+      const piece_t w = *reinterpret_cast<const piece_t *>(reg + r * ROW + u % PIECES * 16);
+      T *to = out + (r0 + r) * (size_t)pitch + c0 + c;
+      if (c + 16 / ES <= left) {
+        *reinterpret_cast<any_t *>(to) = w;
+      } else {
 #pragma unroll
-      for (int v = 0; v < 16 / ES; v++)
-        if (c + v < left) to[v] = w[v];
+        for (int v = 0; v < 16 / ES; v++)
+          if (c + v < left) to[v] = w[v];
+      }
     }
   }
 }
@@ -442,28 +448,34 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   constexpr int CX = XI / NW, CNT = CX + WI / NW;    // loads of every wave, at least
   // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
   extern __shared__ v4i lds[];
-  float *sxs = reinterpret_cast<float *>(lds + i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>() / 16) - BM;  // the rows' scales
+  constexpr int LDS = i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>();
+  float *scales = reinterpret_cast<float *>(lds + LDS / 16) - (BM + BN);  // rows, channels
   static_assert(NI == 1 || NI % 4 == 0 || NI == 2, "output tiles in pairs, or one");
+  static_assert(64 * NW >= BM && 64 * NW >= BN, "a thread for each scale");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
+  const int half = a.N / 2, n_end = a.swiglu ? half : a.N, cols = a.swiglu ? TN / 2 : TN;  // a wave's output columns
+  const uint32_t xbytes = (uint32_t)a.n_src * (uint32_t)a.K, wbytes = (uint32_t)a.N * (uint32_t)a.K;
+  const int stages = (a.K + 128 * WK - 1) / (128 * WK);
+
   const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
   if (t.e < 0) return;
-  const int half = a.N / 2, n_end = a.swiglu ? half : a.N;
-  const int cols = a.swiglu ? TN / 2 : TN, c0 = blockIdx.x % nt * WN * cols;  // a wave's output columns; the workgroup's first
-
+  const int c0 = blockIdx.x % nt * WN * cols;  // the workgroup's first column
+  const int8_t *wbase = a.w + (size_t)t.e * a.N * a.K;
+  const bool once = a.stream && t.only;
+  // weight row of channel row j of the tile; past the end where its column does not exist
+  auto channel = [&](int j) __attribute__((always_inline)) {
+    const int jt = j % TN / 16, c = c0 + j / TN * cols + i8_column<NI>(a.swiglu, jt, j % 16);
+    return c < n_end ? (a.swiglu && i8_is_up<NI>(jt, j % 16) ? half + c : c) : a.N;
+  };
   // lane offsets of this wave's loads at K 0: row lr of the load's 8, chunk swizzled by it
   const int lr = lane >> 3, lc = (lane & 7) ^ lr;
   uint32_t vx[NX], vw[NWI];
 #pragma unroll
   for (int i = 0; i < NWI; i++) {
-    const int rr = 8 * (wave + NW * i), j = rr % BN + lr, jt = j % TN / 16;
-    const int c = c0 + j / TN * cols + i8_column<NI>(a.swiglu, jt, j % 16), w = a.swiglu && i8_is_up<NI>(jt, j % 16) ? half + c : c;
-    vw[i] = c < n_end ? (uint32_t)w * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_I8_OOB;
+    const int rr = 8 * (wave + NW * i), w = channel(rr % BN + lr);
+    vw[i] = w < a.N ? (uint32_t)w * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_I8_OOB;
   }
-  const int8_t *wbase = a.w + (size_t)t.e * a.N * a.K;
-  const uint32_t xbytes = (uint32_t)a.n_src * (uint32_t)a.K, wbytes = (uint32_t)a.N * (uint32_t)a.K;
-  const int stages = (a.K + 128 * WK - 1) / (128 * WK);
-  const bool once = a.stream && t.only;
   // loads l of this wave's of stage s, into buffer b: the rows' WK blocks of BM x 128 bytes, then the channels'
   auto load_x = [&](int l, int s, int b) __attribute__((always_inline)) {
     i8_load<BM, XI, NW>(l, a.q, xbytes, vx[l], lds + b * STAGE, wave, s * 128 * WK, lc * 16, a.K, false);
@@ -476,25 +488,22 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   for (int s = 0; s < NBUF; s++)
 #pragma unroll
     for (int l = 0; l < NWI; l++) load_w(l, s, s);
-  const int srow = tid < BM && tid < t.n ? i8_src(a, t.r0 + tid) : -1;
-  static_assert(64 * NW >= BM, "a thread for each row's scale");
+  const int srow = tid < BM && tid < t.n ? i8_src(a, t.r0 + tid) : -1, schannel = tid < BN ? channel(tid) : a.N;
 #pragma unroll
   for (int i = 0; i < NX; i++) {
     const int rr = 8 * (wave + NW * i), row = rr % BM + lr, s = row < t.n ? i8_src(a, t.r0 + row) : -1;
     vx[i] = s >= 0 ? (uint32_t)s * (uint32_t)a.K + rr / BM * 128 + lc * 16 : MOE_I8_OOB;
   }
-  const float srow_scale = srow >= 0 ? a.qs[srow] : 0.0f;
+  const float row_scale = srow >= 0 ? a.qs[srow] : 0.0f;
+  const float channel_scale = schannel < a.N ? a.ws[(size_t)t.e * a.N + schannel] : 0.0f;
 #pragma unroll
   for (int s = 0; s < NBUF; s++)
 #pragma unroll
     for (int l = 0; l < NX; l++) load_x(l, s, s);
-  if (tid < BM) sxs[tid] = srow_scale;
+  if (tid < BM) scales[tid] = row_scale;
+  if (tid < BN) scales[BM + tid] = channel_scale;
 
   v4i acc[NI][MI];
-#pragma unroll
-  for (int j = 0; j < NI; j++)
-#pragma unroll
-    for (int i = 0; i < MI; i++) acc[j][i] = v4i{0, 0, 0, 0};
   const int fr = lane & 15, fg = lane >> 4;  // this lane's row of an operand, and its chunk of 4
   // Two MFMA steps a stage, 64 bytes of K each; their operands alternate between two sets of
   // registers, a step ahead of the MFMAs (over the stages' border too).
@@ -512,6 +521,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   i8_wait_barrier<(NBUF - 1) * CX>();
 #pragma unroll
   for (int i = 0; i < MI; i++) read(i, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < NI; j++)
+#pragma unroll
+    for (int i = 0; i < MI; i++) acc[j][i] = v4i{0, 0, 0, 0};
   int cur = 0;
 #pragma unroll 1
   for (int s = 0; s < stages; s++) {
@@ -563,28 +576,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
     i8_wait_barrier<0>();
   }
 
-  int8_t *reg = reinterpret_cast<int8_t *>(lds) + (WK - 1) * BM * BN * 4 + (wm * WN + wn) * i8_out_bytes<TN>();
-  const float *ws = a.ws + (size_t)t.e * a.N;
+  int8_t *reg = reinterpret_cast<int8_t *>(lds) + (WK - 1) * BM * BN * 4 + (wm * WN + wn) * MOE_I8_OUT_BYTES;
   const int cw = c0 + wn * cols;  // this wave's first column
-  auto scale_of = [&](int j, int v) __attribute__((always_inline)) {  // channel scale of value v of tile j
-    const int row = 4 * fg + v, c = cw + i8_column<NI>(a.swiglu, j, row), w = a.swiglu && i8_is_up<NI>(j, row) ? half + c : c;
-    return c < n_end ? ws[w] : 0.0f;
-  };
-  float sw[NI][4];
-#pragma unroll
-  for (int j = 0; j < NI; j++)
-#pragma unroll
-    for (int v = 0; v < 4; v++) sw[j][v] = scale_of(j, v);
+  const float *sr = scales + wm * TM + fr, *sc = scales + BM + wn * TN + 4 * fg;
+  // value v of channel tile j of row tile i, scaled; its 4 channels' scales lie side by side
+  auto value = [&](int i, int j, int v, float sx) __attribute__((always_inline)) { return (float)acc[j][i][v] * sx * sc[j * 16 + v]; };
 #pragma unroll
   for (int i = 0; i < MI; i++) {
     const int m0 = wm * TM + i * 16, rows = t.n - m0 < 16 ? t.n - m0 : 16;
     if (rows <= 0) break;
-    const float sx = sxs[m0 + fr];
+    const float sx = sr[i * 16];
     auto plain = [&](auto width) __attribute__((always_inline)) {
       constexpr int V = decltype(width)::value;
       return [&](int p, float(&f)[V]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int v = 0; v < V; v++) f[v] = (float)acc[p * V / 4 + v / 4][i][v % 4] * sx * sw[p * V / 4 + v / 4][v % 4];
+        for (int v = 0; v < V; v++) f[v] = value(i, p * V / 4 + v / 4, v % 4, sx);
       };
     };
     auto gated = [&](auto width) __attribute__((always_inline)) {
@@ -593,11 +599,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
 #pragma unroll
         for (int v = 0; v < V; v++) {
           if constexpr (NI == 1) {  // lanes 0-31 hold gate, 32-63 up
-            const float y = (float)acc[0][i][v] * sx * sw[0][v];
+            const float y = value(i, 0, v, sx);
             f[v] = i8_swiglu(y, __shfl_xor(y, 32), a.clamp);
           } else {
             const int j = 2 * (p * V / 4 + v / 4);
-            f[v] = i8_swiglu((float)acc[j][i][v % 4] * sx * sw[j][v % 4], (float)acc[j + 1][i][v % 4] * sx * sw[j + 1][v % 4], a.clamp);
+            f[v] = i8_swiglu(value(i, j, v % 4, sx), value(i, j + 1, v % 4, sx), a.clamp);
           }
         }
       };
