@@ -59,13 +59,44 @@ __device__ __forceinline__ int i8_code_in(const i8_row &w, float x) {
   return w.inv > 0.0f ? i8_code(x * w.pre, w.s, w.inv) : 0;
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = dpp_max<0xB1>(v);   // quad_perm [1,0,3,2]
+  v = dpp_max<0x4E>(v);   // quad_perm [2,3,0,1]
+  v = dpp_max<0x141>(v);  // row_half_mirror
+  v = dpp_max<0x140>(v);  // row_mirror: every lane holds its row of 16's
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+  return max(max(a, b), max(c, d));
+}
+
+// Largest |x| of a vector as it was loaded, as the bits of a float: bits without the
+// sign grow with the value, NaN above infinity above every finite one.
+template <typename T, int V>
+__device__ __forceinline__ uint32_t abs_bits(const raw_v<T, V> &r) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t u = (uint32_t)__shfl_xor((int)v, o);
-    v = u > v ? u : v;
+    for (int i = 0; i < V; i++) {
+      const float e = r.v[i];  // (a bit cast of the vector's element itself reads element 0)
+      m = max(m, __builtin_bit_cast(uint32_t, e) & 0x7fffffffu);
+    }
+    return m;
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 p = {0, 0};
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const T e0 = r.v[i], e1 = r.v[i + 1];
+      const u16x2 w = {(uint16_t)(__builtin_bit_cast(uint16_t, e0) & 0x7fff), (uint16_t)(__builtin_bit_cast(uint16_t, e1) & 0x7fff)};
+      p = __builtin_elementwise_max(p, w);
+    }
+    const uint16_t h = p.x > p.y ? p.x : p.y;
+    return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(T, h));
   }
-  return v;
 }
 
 // A row's codes in one pass: WPR waves hold it in registers, VPT vectors of 8 a
@@ -73,7 +104,8 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
 // Memory bound (2 to 4 bytes in, 1 out) only while the codes are cheap: a
 // quotient x * inv is within 1.6e-5 of x / s, so it decides all but those next
 // to a tie, and the exact comparison runs only for waves that hold one (about
-// one vector in ten).
+// one vector in ten).  x * inv + 1.5 * 2^23 is rounded to a whole number, ties to
+// even, with the code in its low byte.
 template <typename T, int WPR, int VPT>
 __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void k_quantize_i8(const T *__restrict__ x, int M, int K,
                                                                           int8_t *__restrict__ q, float *__restrict__ scale) {
@@ -82,18 +114,15 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void k_quantize_i8(const 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, in_row = tid % (64 * WPR);
   const long row = (long)blockIdx.x * RPW + wave / WPR;
   const T *xr = x + (row < M ? row : 0) * K;
-  float f[VPT][8];
-  uint32_t m = 0;
+  raw_v<T, 8> r[VPT];
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
     const int c = (in_row + v * 64 * WPR) * 8;
-    load_v<T, 8>(xr + c, row < M ? K - c : 0, f[v]);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint32_t b = __builtin_bit_cast(uint32_t, f[v][i]) & 0x7fffffffu;
-      m = b > m ? b : m;
-    }
+    r[v].load(xr + c, row < M ? K - c : 0);
   }
+  uint32_t m = 0;
+#pragma unroll
+  for (int v = 0; v < VPT; v++) m = max(m, abs_bits(r[v]));
   m = wave_max_u(m);
   if constexpr (WPR > 1) {
     if (lane == 0) part[wave] = m;
@@ -107,29 +136,30 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void k_quantize_i8(const 
   for (int v = 0; v < VPT; v++) {
     const int c = (in_row + v * 64 * WPR) * 8;
     if (c >= K) break;
-    int8_t code[8];
-    bool near = w.pre != 1.0f;
+    uint32_t code[8];
+    float far = w.pre != 1.0f ? 1.0f : 0.0f;  // the largest distance of a quotient from its whole number
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float t = f[v][i] * w.inv, r = __builtin_rintf(t);
-      near |= fabsf(t - r) > 0.4999f;
-      code[i] = (int8_t)(int)r;
+      const float t = (float)r[v].v[i] * w.inv, u = t + 0x1.8p23f;
+      far = fmaxf(far, fabsf(t - (u - 0x1.8p23f)));
+      code[i] = __builtin_bit_cast(uint32_t, u);
     }
-    if (__any(near)) {
+    if (__any(far > 0.4999f)) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) code[i] = (int8_t)i8_code_in(w, f[v][i]);
+      for (int i = 0; i < 8; i++) code[i] = (uint32_t)i8_code_in(w, (float)r[v].v[i]);
     }
-    typedef int8_t c8 __attribute__((ext_vector_type(8), aligned(1)));
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(1)));
     int8_t *to = q + row * K + c;
     if (c + 8 <= K) {
-      c8 o;
+      u32x2 o;
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[i] = code[i];
-      *reinterpret_cast<c8 *>(to) = o;
+      for (int h = 0; h < 2; h++)
+        o[h] = (code[4 * h] & 255) | (code[4 * h + 1] & 255) << 8 | (code[4 * h + 2] & 255) << 16 | code[4 * h + 3] << 24;
+      *reinterpret_cast<u32x2 *>(to) = o;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (c + i < K) to[i] = code[i];
+        if (c + i < K) to[i] = (int8_t)code[i];
     }
   }
   if (in_row == 0) scale[row] = w.scale;
@@ -261,14 +291,17 @@ __device__ __forceinline__ v4i i8_bytes(const int8_t *row, int k, int K) {
   return v;
 }
 
-// Any K and alignment: tiles of 64 rows x 64 channels, 64 bytes of K a step
-// through registers into LDS.  Wave (wm, wn) multiplies 32 rows with two
-// 16-channel tiles, wn*16 of each half of the 64 (SwiGLU: the halves are gate
-// and up, so a lane holds both of its channels).
-// 16x16x64 MFMA, weights as A, rows as B: lane l holds K bytes [16 (l/16), +16)
+// Any K and alignment: tiles of 64 rows x 64 channels, 128 bytes of K a step
+// through registers (unaligned 16-byte loads, a step ahead) into LDS.  Wave (wm, wn)
+// multiplies 32 rows with two 16-channel tiles, wn*16 of each half of the 64
+// (SwiGLU: the halves are gate and up, so a lane holds both of its channels).
+// 16x16x64 MFMA, channels as A, rows as B: lane l holds K bytes [16 (l/16), +16)
 // of A row (B column) l % 16; D lane l holds column l % 16, rows 4 (l/16) + i.
+// Bound by the loads' latency where the tiles are few, by the small tile's traffic
+// where they are many: K = 1765 against K = 1776 on the staged tiles, 4096 channels:
+// 1 row 12.6 and 4.7 us, 300 rows 22 and 12.7, 4096 rows 134 and 39.
 __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
-  __shared__ v4i xs[64][5], wsh[64][5];  // 4 chunks of 16 bytes a row, and one of padding
+  __shared__ v4i xs[64][9], wsh[64][9];  // 8 chunks of 16 bytes a row, and one of padding
   const i8_tile t = i8_find_tile(a, blockIdx.y, 64);
   if (t.e < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
@@ -282,23 +315,39 @@ __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
   const int8_t *xr = a.q + (size_t)max(src, 0) * a.K;
   const int8_t *wr = a.w + ((size_t)t.e * a.N + (wc < n_end ? wrow : 0)) * a.K;
   v4i acc[2][2] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
+  v4i xv[2], wv[2];
+  auto fetch = [&](int k0) __attribute__((always_inline)) {
     const v4i z = {0, 0, 0, 0};
-    const v4i xv = src >= 0 ? i8_bytes(xr, k0 + 16 * ch, a.K) : z, wv = wc < n_end ? i8_bytes(wr, k0 + 16 * ch, a.K) : z;
-    __syncthreads();
-    xs[row][ch] = xv;
-    wsh[row][ch] = wv;
-    __syncthreads();
-    v4i A[2], B[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      A[j] = wsh[32 * j + 16 * wn + (lane & 15)][lane >> 4];
-      B[j] = xs[32 * wm + 16 * j + (lane & 15)][lane >> 4];
+    for (int i = 0; i < 2; i++) {
+      const int k = k0 + 16 * (ch + 4 * i);
+      xv[i] = src >= 0 ? i8_bytes(xr, k, a.K) : z;
+      wv[i] = wc < n_end ? i8_bytes(wr, k, a.K) : z;
     }
+  };
+  fetch(0);
+  for (int k0 = 0; k0 < a.K; k0 += 128) {
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 2; i++) {
+      xs[row][ch + 4 * i] = xv[i];
+      wsh[row][ch + 4 * i] = wv[i];
+    }
+    __syncthreads();
+    if (k0 + 128 < a.K) fetch(k0 + 128);
 #pragma unroll
-      for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[i], B[j], acc[i][j], 0, 0, 0);
+    for (int kk = 0; kk < 2; kk++) {
+      v4i A[2], B[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        A[j] = wsh[32 * j + 16 * wn + (lane & 15)][4 * kk + (lane >> 4)];
+        B[j] = xs[32 * wm + 16 * j + (lane & 15)][4 * kk + (lane >> 4)];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[i], B[j], acc[i][j], 0, 0, 0);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 2; j++) {
