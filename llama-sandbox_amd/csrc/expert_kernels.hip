@@ -130,13 +130,19 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
 // The tile shapes, and what they cost.  A call of `rounds` tiles one after the other
 // on a CU takes about
 //   call + rounds * (tile + K / 128 * (k + k_share * tiles that share the CU))  us,
-// fitted (errors of 4 to 14%) to 52 products of 1 to 8192 rows, K = 7168, 2048, 768
-// and N = 7168, 4096, 2048.  The least of these is on average 0.6% slower than the
-// fastest shape measured there, at most 7%; over 46 grouped calls of 4 to 32764 rows
-// 1.2%, at most 29% (a skewed call).  Some of them, us with each shape's neighbours:
-//   16 rows x 7168 x 7168: 16x16 13.9, 32x32 15.2, 64x32 18.3;   64: 64x32 20.2, 32x32 28, 128x32 25
-//   512: 64x128 48, 128x64 71, 256x128 53;   1024: 256x128 57, 64x128 94, 256x256 101
-//   4096: 256x256 206, 256x128 230, 64x128 325 (the same rows over 64 wide tiles a round: 2050 TOP/s)
+// fitted to 83 dense products of 1 to 8192 rows, K and N from 640 to 7168, on each of
+// 25 shapes.  The shape of the least cost is on average 0.6% slower than the
+// fastest of the 25 there (at most 12%), and 2.8% (24%) over 72 grouped calls of 4 to
+// 32764 rows, where the rows of each expert are not known here.
+//   rows x 7168 x 7168, us:  16x16  32x32  64x32  64x64  128x64  64x128  128x128  256x128  256x256
+//                      16:    15.7   14.0   15.8   18.7    22.5    29.2     31.4     41.9     83
+//                      64:    35.9   23.6   17.0   21.8    23.6    31.6     33.5     45.1     87
+//                     256:     118     71     49   38.3    27.3    31.9     37.3     52.9     99
+//                     512:     231    136     84   64.2    51.3    40.7     37.2     51.7     96
+//                    1024:     453    265    162    121      93      82       71     55.9     98
+//                    4096:    1788   1036    619    461     331     283      247      215    199
+// 128x128 stands twice: 3 stages for one workgroup a CU, 2 for two.  Eight waves a
+// workgroup in all but the smallest: with 4 the same tiles took up to a third longer.
 struct i8_shape {
   int BM, BN, lds;
   float call, tile, k, k_share;
@@ -147,15 +153,17 @@ static constexpr i8_shape shape_of(float call, float tile, float k, float k_shar
   return {BM, BN, i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
 }
 static const i8_shape i8_shapes[] = {
-    shape_of<16, 16, 1, 1, 4, 4>(1.90f, 1.93f, 0.056f, 0.026f),
-    shape_of<32, 32, 1, 1, 4, 4>(1.84f, 3.95f, 0.152f, 0.0f),
-    shape_of<64, 32, 1, 1, 4, 3>(1.69f, 4.97f, 0.203f, 0.0f),
-    shape_of<128, 32, 2, 1, 2, 3>(1.42f, 4.16f, 0.332f, 0.0f),
-    shape_of<128, 64, 2, 1, 2, 3>(1.38f, 6.34f, 0.485f, 0.0f),
-    shape_of<32, 128, 1, 4, 1, 3>(1.63f, 3.05f, 0.415f, 0.096f),
-    shape_of<64, 128, 1, 4, 1, 3>(1.55f, 3.82f, 0.424f, 0.160f),
-    shape_of<256, 128, 4, 2, 1, 3>(0.0f, 6.16f, 0.782f, 0.0f),
-    shape_of<256, 256, 4, 2, 1, 2>(0.0f, 7.31f, 1.454f, 0.0f),
+    shape_of<16, 16, 1, 1, 4, 4>(2.11f, 1.81f, 0.031f, 0.039f),
+    shape_of<32, 32, 2, 1, 4, 4>(1.81f, 2.36f, 0.112f, 0.0f),
+    shape_of<64, 32, 4, 1, 2, 4>(1.68f, 2.27f, 0.165f, 0.0f),
+    shape_of<64, 64, 2, 2, 2, 3>(1.30f, 2.77f, 0.225f, 0.0f),
+    shape_of<128, 64, 4, 2, 1, 4>(1.27f, 2.80f, 0.350f, 0.0f),
+    shape_of<64, 128, 2, 4, 1, 3>(1.57f, 2.41f, 0.134f, 0.253f),
+    shape_of<128, 128, 4, 2, 1, 3>(0.0f, 4.09f, 0.504f, 0.0f),
+    shape_of<128, 128, 2, 4, 1, 2>(0.0f, 2.95f, 0.509f, 0.264f),
+    shape_of<128, 256, 2, 4, 1, 3>(0.0f, 5.61f, 0.810f, 0.0f),
+    shape_of<256, 128, 4, 2, 1, 3>(0.0f, 5.59f, 0.779f, 0.0f),
+    shape_of<256, 256, 4, 2, 1, 2>(0.0f, 5.95f, 1.544f, 0.0f),
 };
 
 static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
