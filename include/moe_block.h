@@ -427,9 +427,11 @@ moe_status moe_route_forward(moe_ctx *ctx, int layer, const float *x_dev,
  * are MOE_GGML_F32, MOE_GGML_F16 or MOE_GGML_BF16, in and out independent;
  * any H; buffers must not overlap.  Sums are f32, in slot order; a result is
  * rounded once, to its type.  An entry of inv outside [0, n_rows) is taken as
- * dropped.  A valid inv names no row twice (moe_group's does not).  These
- * calls allocate nothing and share no scratch: they may overlap on streams
- * and threads and be captured, and leave the caller's current device as it was. */
+ * dropped.  A valid inv names no row twice (moe_group's does not).  k <= 64,
+ * H <= 2^30; more tokens than a launch takes (2^24, or 2^26 pairs in
+ * moe_combine_grad): MOE_ERR_UNSUPPORTED.  These calls, and the 8-bit ones
+ * below, allocate nothing and share no scratch: they may overlap on several
+ * streams and be captured, and leave the caller's current device as it was. */
 
 /* rows[inv[t*k+s]] = x[t].  x [T][H], rows [n_rows][H]; rows that no pair
  * names are left as they were.  (ggml's mul_mat_id gathers the same rows on
@@ -456,8 +458,8 @@ moe_status moe_combine_grad(moe_ctx *ctx, const void *dout_dev, int dout_type, c
  * scale[r] to the nearest whole number, ties to even, in [-127, 127]; a row
  * of zeros, or whose scale rounds to 0, has codes 0.  A row with a NaN or an
  * infinity has a NaN scale and codes 0, so that every product of it is NaN.
- * Any K and alignment.  Also how weights are quantised, a scale for each
- * channel. */
+ * Any K and alignment, M < 2^22.  Also how weights are quantised, a scale for
+ * each channel. */
 moe_status moe_quantize_i8(moe_ctx *ctx, const void *x_dev, int x_type, int M, int K, int8_t *q_dev, float *scale_dev,
                            void *stream);
 
@@ -474,8 +476,9 @@ moe_status moe_quantize_i8(moe_ctx *ctx, const void *x_dev, int x_type, int M, i
  * on are left as they were.  perm NULL: src(r) = r, k = 1; else
  * src(r) = perm[r] / k (moe_group's perm: the row's token), and a row whose
  * perm is outside [0, n_src*k) is computed from zeros.
- * The sum is exact in 32 bits: K <= 131071, else MOE_ERR_UNSUPPORTED.  Any N,
- * K and alignment; K % 16 == 0 with 16-byte aligned q and w is the fast path. */
+ * The sum is exact in 32 bits: K <= 131071, else MOE_ERR_UNSUPPORTED (as are
+ * more rows than a launch takes: 2^22).  Any N, K and alignment; the fast path
+ * takes K % 16 == 0, 16-byte aligned q and w, and q and each w[e] below 4 GiB. */
 moe_status moe_matmul_i8(moe_ctx *ctx, const int8_t *q_dev, const float *q_scale_dev, int n_src, const int8_t *w_dev,
                          const float *w_scale_dev, int E, const int32_t *offsets_dev, const int32_t *perm_dev, int k,
                          int M, int N, int K, uint32_t flags, float clamp, void *out_dev, int out_type, void *stream);

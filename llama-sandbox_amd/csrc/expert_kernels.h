@@ -1,5 +1,6 @@
 // expert_kernels.h -- launches of expert_kernels.hip, for expert_ops.h.  Arguments are
-// checked there; a launch error is left for hipGetLastError.
+// checked there; false: more rows than a grid takes; a launch error is left for
+// hipGetLastError.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -23,11 +24,11 @@ struct i8_mm {
 };
 
 // element types: moe_block.h's MOE_GGML_F32 / F16 / BF16
-void launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k, int H, int n_rows, void *rows,
+bool launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k, int H, int n_rows, void *rows,
                      int rows_type, hipStream_t st);
-void launch_combine_rows(const void *rows, int rows_type, int n_rows, const float *wts, const int32_t *inv, int T, int k,
+bool launch_combine_rows(const void *rows, int rows_type, int n_rows, const float *wts, const int32_t *inv, int T, int k,
                          int H, void *out, int out_type, hipStream_t st);  // wts NULL: unit weights
-void launch_combine_grad(const void *dout, int dout_type, const void *rows, int rows_type, int n_rows, const float *wts,
+bool launch_combine_grad(const void *dout, int dout_type, const void *rows, int rows_type, int n_rows, const float *wts,
                          const int32_t *inv, int T, int k, int H, void *drows, float *dwts, hipStream_t st);
-void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st);
-bool launch_matmul_i8(const i8_mm &a, int n_cu, hipStream_t st);  // false: more rows than a grid takes
+bool launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st);
+bool launch_matmul_i8(const i8_mm &a, int n_cu, hipStream_t st);

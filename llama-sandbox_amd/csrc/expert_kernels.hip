@@ -11,6 +11,9 @@
 
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
+// A grid's x dimension holds fewer than 2^32 threads.
+static bool fits(long blocks, int threads) { return blocks * threads < (1L << 32); }
+
 // f(T{}) for the element type t.
 template <typename F>
 static void with_type(int t, F f) {
@@ -41,8 +44,9 @@ static int row_splits(int T, int nv) {
   return most < want ? most : want;
 }
 
-void launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k, int H, int n_rows, void *rows,
+bool launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k, int H, int n_rows, void *rows,
                      int rows_type, hipStream_t st) {
+  if (!fits(T, 256)) return false;
   with_type(x_type, [&](auto ti) {
     with_type(rows_type, [&](auto to) {
       typedef decltype(ti) TI;
@@ -53,10 +57,12 @@ void launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k
                          (const TI *)x, inv, k, H, n_rows, (TO *)rows);
     });
   });
+  return true;
 }
 
-void launch_combine_rows(const void *rows, int rows_type, int n_rows, const float *wts, const int32_t *inv, int T, int k,
+bool launch_combine_rows(const void *rows, int rows_type, int n_rows, const float *wts, const int32_t *inv, int T, int k,
                          int H, void *out, int out_type, hipStream_t st) {
+  if (!fits(T, 256)) return false;
   with_type(rows_type, [&](auto ti) {
     with_type(out_type, [&](auto to) {
       typedef decltype(ti) TI;
@@ -67,11 +73,13 @@ void launch_combine_rows(const void *rows, int rows_type, int n_rows, const floa
                          (const TI *)rows, wts, inv, k, H, n_rows, (TO *)out);
     });
   });
+  return true;
 }
 
-void launch_combine_grad(const void *dout, int dout_type, const void *rows, int rows_type, int n_rows, const float *wts,
+bool launch_combine_grad(const void *dout, int dout_type, const void *rows, int rows_type, int n_rows, const float *wts,
                          const int32_t *inv, int T, int k, int H, void *drows, float *dwts, hipStream_t st) {
   const long P = (long)T * k;
+  if (!fits((P + 7) / 8, 512)) return false;
   with_type(dout_type, [&](auto td) {
     with_type(rows_type, [&](auto tr) {
       typedef decltype(td) TD;
@@ -84,6 +92,7 @@ void launch_combine_grad(const void *dout, int dout_type, const void *rows, int 
                          (const TR *)rows, wts, inv, P, k, H, n_rows, (TR *)drows, dwts);
     });
   });
+  return true;
 }
 
 template <typename T, int WPR, int VPT>
@@ -95,7 +104,8 @@ static void launch_quantize(const T *x, int M, int K, int8_t *q, float *scale, h
 
 // One vector a thread where the rows are too few to fill the chip (a row is
 // then spread as wide as it goes), else as many rows at once as registers allow.
-void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st) {
+bool launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, float *scale, int n_cu, hipStream_t st) {
+  if (!fits(M, K > 8192 ? 1024 : 256)) return false;
   with_type(x_type, [&](auto t) {
     typedef decltype(t) T;
     const T *p = (const T *)x;
@@ -110,6 +120,7 @@ void launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, floa
     else if (K <= 32768) launch_quantize<T, 16, 4>(p, M, K, q, scale, st);
     else hipLaunchKernelGGL((k_quantize_i8_long<T>), dim3(M), dim3(256), 0, st, p, K, q, scale);
   });
+  return true;
 }
 
 // Tiles of at most BM rows that M rows of E experts can make.
@@ -121,7 +132,7 @@ template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 static bool launch_tiles(const i8_mm &a, hipStream_t st) {
   const int nt = ceil_div(a.N, BN);
   const long n = i8_tiles(a, BM) * nt;
-  if (n > 0x7fffffff) return false;
+  if (!fits(n, 64 * WM * WN * WK)) return false;
   hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
                      (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>()), st, a, nt);
   return true;
@@ -199,7 +210,7 @@ bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
   }
   const int nt = a.swiglu ? ceil_div(a.N / 2, 32) : ceil_div(a.N, 64);
   const long mt = i8_tiles(a, 64);
-  if (mt > 65535) return false;
+  if (mt > 65535 || !fits(nt, 256)) return false;
   hipLaunchKernelGGL(k_mm_i8_any, dim3(nt, (unsigned)mt), dim3(256), 0, st, a);
   return true;
 }

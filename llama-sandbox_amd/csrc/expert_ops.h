@@ -21,6 +21,8 @@ struct device_scope {
   }
 };
 
+#define MOE_ROW_MAX (1 << 30)  // elements of a row: indexes within one stay in 32 bits
+
 static size_t type_bytes(int t) { return t == MOE_GGML_F32 ? 4 : t == MOE_GGML_F16 || t == MOE_GGML_BF16 ? 2 : 0; }
 
 // p holds elements of size b (b = 0: an unknown type).
@@ -45,7 +47,7 @@ extern "C" moe_status moe_dispatch(moe_ctx *c, const void *x, int x_type, const 
                                    int n_rows, void *rows, int rows_type, void *stream) {
   if (!c) return MOE_ERR_INVALID_ARG;
   if (!is_array(x, type_bytes(x_type)) || !is_array(rows, type_bytes(rows_type)) || !is_array(inv, 4) || T <= 0 ||
-      k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
+      k <= 0 || k > 64 || H <= 0 || H > MOE_ROW_MAX || n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_dispatch: bad arguments");
   if (overlap({{x, (size_t)T * H * type_bytes(x_type), false}, {inv, (size_t)T * k * 4, false},
                {rows, (size_t)n_rows * H * type_bytes(rows_type), true}}))
@@ -54,7 +56,8 @@ extern "C" moe_status moe_dispatch(moe_ctx *c, const void *x, int x_type, const 
   HIPC(c, ds.err);
   {
     prof_scope ps(c, K_DISPATCH, (hipStream_t)stream, true);
-    launch_dispatch(x, x_type, inv, T, k, H, n_rows, rows, rows_type, (hipStream_t)stream);
+    if (!launch_dispatch(x, x_type, inv, T, k, H, n_rows, rows, rows_type, (hipStream_t)stream))
+      return fail(c, MOE_ERR_UNSUPPORTED, "moe_dispatch: T = %d tokens", T);
   }
   HIPC(c, hipGetLastError());
   return MOE_OK;
@@ -63,7 +66,8 @@ extern "C" moe_status moe_dispatch(moe_ctx *c, const void *x, int x_type, const 
 static moe_status combine_rows(moe_ctx *c, const char *who, const void *rows, int rows_type, int n_rows, const float *wts,
                                const int32_t *inv, int T, int k, int H, void *out, int out_type, hipStream_t st) {
   if (!is_array(rows, type_bytes(rows_type)) || !is_array(out, type_bytes(out_type)) || !is_array(inv, 4) ||
-      (wts && !is_array(wts, 4)) || T <= 0 || k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
+      (wts && !is_array(wts, 4)) || T <= 0 || k <= 0 || k > 64 || H <= 0 || H > MOE_ROW_MAX ||
+      n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "%s: bad arguments", who);
   if (overlap({{rows, (size_t)n_rows * H * type_bytes(rows_type), false}, {wts, (size_t)T * k * 4, false},
                {inv, (size_t)T * k * 4, false}, {out, (size_t)T * H * type_bytes(out_type), true}}))
@@ -72,7 +76,8 @@ static moe_status combine_rows(moe_ctx *c, const char *who, const void *rows, in
   HIPC(c, ds.err);
   {
     prof_scope ps(c, K_COMBINE_ROWS, st, true);
-    launch_combine_rows(rows, rows_type, n_rows, wts, inv, T, k, H, out, out_type, st);
+    if (!launch_combine_rows(rows, rows_type, n_rows, wts, inv, T, k, H, out, out_type, st))
+      return fail(c, MOE_ERR_UNSUPPORTED, "%s: T = %d tokens", who, T);
   }
   HIPC(c, hipGetLastError());
   return MOE_OK;
@@ -98,7 +103,8 @@ extern "C" moe_status moe_combine_grad(moe_ctx *c, const void *dout, int dout_ty
   if (!c) return MOE_ERR_INVALID_ARG;
   const size_t rb = type_bytes(rows_type);
   if (!is_array(dout, type_bytes(dout_type)) || !is_array(rows, rb) || !is_array(drows, rb) || !is_array(wts, 4) ||
-      !is_array(inv, 4) || !is_array(dwts, 4) || T <= 0 || k <= 0 || k > 64 || H <= 0 || n_rows <= 0)
+      !is_array(inv, 4) || !is_array(dwts, 4) || T <= 0 || k <= 0 || k > 64 || H <= 0 || H > MOE_ROW_MAX ||
+      n_rows <= 0)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_combine_grad: bad arguments");
   const size_t nr = (size_t)n_rows * H * rb, np = (size_t)T * k * 4;
   if (overlap({{dout, (size_t)T * H * type_bytes(dout_type), false}, {rows, nr, false}, {wts, np, false}, {inv, np, false},
@@ -108,7 +114,8 @@ extern "C" moe_status moe_combine_grad(moe_ctx *c, const void *dout, int dout_ty
   HIPC(c, ds.err);
   {
     prof_scope ps(c, K_COMBINE_GRAD, (hipStream_t)stream, true);
-    launch_combine_grad(dout, dout_type, rows, rows_type, n_rows, wts, inv, T, k, H, drows, dwts, (hipStream_t)stream);
+    if (!launch_combine_grad(dout, dout_type, rows, rows_type, n_rows, wts, inv, T, k, H, drows, dwts, (hipStream_t)stream))
+      return fail(c, MOE_ERR_UNSUPPORTED, "moe_combine_grad: T = %d tokens of %d slots", T, k);
   }
   HIPC(c, hipGetLastError());
   return MOE_OK;
@@ -117,7 +124,7 @@ extern "C" moe_status moe_combine_grad(moe_ctx *c, const void *dout, int dout_ty
 extern "C" moe_status moe_quantize_i8(moe_ctx *c, const void *x, int x_type, int M, int K, int8_t *q, float *scale,
                                       void *stream) {
   if (!c) return MOE_ERR_INVALID_ARG;
-  if (!is_array(x, type_bytes(x_type)) || !q || !is_array(scale, 4) || M <= 0 || K <= 0)
+  if (!is_array(x, type_bytes(x_type)) || !q || !is_array(scale, 4) || M <= 0 || K <= 0 || K > MOE_ROW_MAX)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_quantize_i8: bad arguments");
   if (overlap({{x, (size_t)M * K * type_bytes(x_type), false}, {q, (size_t)M * K, true}, {scale, (size_t)M * 4, true}}))
     return fail(c, MOE_ERR_INVALID_ARG, "moe_quantize_i8: an output overlaps another buffer");
@@ -125,7 +132,8 @@ extern "C" moe_status moe_quantize_i8(moe_ctx *c, const void *x, int x_type, int
   HIPC(c, ds.err);
   {
     prof_scope ps(c, K_QUANT_I8, (hipStream_t)stream, true);
-    launch_quantize_i8(x, x_type, M, K, q, scale, c->n_cu, (hipStream_t)stream);
+    if (!launch_quantize_i8(x, x_type, M, K, q, scale, c->n_cu, (hipStream_t)stream))
+      return fail(c, MOE_ERR_UNSUPPORTED, "moe_quantize_i8: M = %d rows", M);
   }
   HIPC(c, hipGetLastError());
   return MOE_OK;
@@ -139,7 +147,7 @@ extern "C" moe_status moe_matmul_i8(moe_ctx *c, const int8_t *q, const float *q_
   if (!q || !is_array(q_scale, 4) || !w || !is_array(w_scale, 4) || (offsets && !is_array(offsets, 4)) ||
       (perm && !is_array(perm, 4)) || !is_array(out, type_bytes(out_type)) || (flags & ~MOE_MM_SWIGLU) || n_src <= 0 ||
       E <= 0 || E > MOE_GROUP_MAX_E || (!offsets && E != 1) || k <= 0 || (!perm && (k != 1 || n_src < M)) || M <= 0 ||
-      N <= 0 || K <= 0 || (swiglu && N % 2) || !(clamp >= 0.0f))
+      N <= 0 || N > MOE_ROW_MAX || K <= 0 || (swiglu && N % 2) || !(clamp >= 0.0f))
     return fail(c, MOE_ERR_INVALID_ARG, "moe_matmul_i8: bad arguments");
   const size_t n_out = (size_t)M * (swiglu ? N / 2 : N) * type_bytes(out_type);
   if (overlap({{q, (size_t)n_src * K, false}, {q_scale, (size_t)n_src * 4, false}, {w, (size_t)E * N * K, false},

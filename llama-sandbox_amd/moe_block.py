@@ -812,7 +812,7 @@ class MoeBlock:
                             (offsets, "offsets"), (perm, "perm"))
         st = self.lib.moe_matmul_i8(self.h, q.data_ptr(), scale.data_ptr(), S, w.data_ptr(), w_scale.data_ptr(), E,
                                     None if offsets is None else offsets.data_ptr(),
-                                    None if perm is None else perm.data_ptr(), k, M, N, K, 1 if swiglu else 0, clamp,
+                                    None if perm is None else perm.data_ptr(), int(k), M, N, K, 1 if swiglu else 0, clamp,
                                     out.data_ptr(), ot, _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_matmul_i8")

@@ -350,6 +350,91 @@ def test_row_map_entries_outside_the_sources_are_zero_rows(blk):
         check_product(got[[r]], q[t], s[t], w[r // 4], ws[r // 4], False, 0.0, torch.float32)
 
 
+@pytest.mark.parametrize("K, sw", [(192, False), (192, True), (77, False)])
+def test_dense_product_through_a_row_map(blk, K, sw):
+    """One matrix, rows taken through perm (the same source more than once)."""
+    say("dense product through a row map", K, sw)
+    rng = np.random.default_rng(21)
+    S, M, N = 9, 150, 72
+    perm = rng.integers(0, S * 3, M).astype(np.int32)
+    q, w, s, ws = codes(rng, (S, K)), codes(rng, (N, K)), scales(rng, S, K), scales(rng, N, K)
+    got = torch.full((M, N // 2 if sw else N), float("nan"), device=DEV)
+    blk.matmul_i8(dev(q), dev(s), dev(w), dev(ws), got, perm=dev(perm), k=3, swiglu=sw)
+    at = torch.from_numpy(perm.astype(np.int64) // 3)
+    check_product(got, q[at], s[at], w, ws, sw, 0.0, torch.float32)
+
+
+def test_offsets_past_32_bits(blk):
+    """Buffers of more than 4 GiB: the rows at their ends."""
+    say("offsets past 32 bits: rows")
+    H, R = 4096, 600_000  # 4.9 GB of bf16
+    T, k = 4, 2
+    inv = np.array([R - 1, 0, 3, R // 2, -1, R - 2, 524_288, 524_289], np.int32)  # 524288 * H * 2 is 2^32
+    rng = np.random.default_rng(22)
+    x, wts = floats(rng, (T, H), "bf16"), floats(rng, (T, k), "f32")
+    rows = torch.zeros((R, H), dtype=torch.bfloat16, device=DEV)
+    blk.dispatch(dev(x), dev(inv), rows)
+    at = [R - 1, 0, 3, R // 2, R - 2, 524_288, 524_289]
+    assert torch.equal(rows[at].cpu(), x[[0, 0, 1, 1, 2, 3, 3]])
+    out, dx = torch.empty((T, H), device=DEV), torch.empty((T, H), dtype=torch.bfloat16, device=DEV)
+    blk.combine(rows, dev(wts), dev(inv), out)
+    there = torch.from_numpy(inv.reshape(T, k) >= 0)
+    w = torch.where(there, wts, torch.zeros(()))
+    want = x.double() * w.double().sum(1, keepdim=True)
+    close(out, want, (k + 1) * U * x.double().abs() * w.double().abs().sum(1, keepdim=True))
+    blk.dispatch_grad(rows, dev(inv), dx)
+    assert torch.equal(dx.cpu(), (x.float() * there.sum(1, keepdim=True)).to(torch.bfloat16))
+    drows, dwts = torch.zeros_like(rows), torch.empty((T, k), device=DEV)
+    blk.combine_grad(dev(x), rows, dev(wts), dev(inv), drows, dwts)
+    flat = torch.from_numpy(inv.astype(np.int64))
+    pair = torch.nonzero(flat >= 0).view(-1)
+    v = x[pair // k].double() * wts.view(-1)[pair, None].double()
+    close(drows[flat[pair].to(DEV)], v, ref.rounded(U * v.abs(), v, torch.bfloat16))
+    del rows, drows
+    torch.cuda.empty_cache()
+    say("offsets past 32 bits: products")
+    for S, K, E, N in ((300_000, 16384, 2, 40), (70, 16384, 70, 4096)):  # 4.9 GB of codes; 4.7 GB of weights
+        q = torch.zeros((S, K), dtype=torch.int8, device=DEV)
+        w = torch.zeros((E, N, K), dtype=torch.int8, device=DEV)
+        M = 70
+        src = np.linspace(0, S - 1, M).astype(np.int32)
+        src[-1] = S - 1
+        qc, wc = codes(rng, (M, K)), codes(rng, (2, N, K))
+        q[torch.from_numpy(src.astype(np.int64)).to(DEV)] = dev(qc)
+        w[0], w[E - 1] = dev(wc[0]), dev(wc[1])
+        s, ws = scales(rng, S, K), scales(rng, (E, N), K)
+        offsets = np.full(E + 1, 30, np.int32)
+        offsets[0], offsets[E] = 0, M
+        got = torch.full((M, N), float("nan"), device=DEV)
+        blk.matmul_i8(q, dev(s), w, dev(ws), got, offsets=dev(offsets), perm=dev(src))
+        st = s[torch.from_numpy(src.astype(np.int64))]
+        check_product(got[:30], qc[:30], st[:30], wc[0], ws[0], False, 0.0, torch.float32)
+        check_product(got[30:], qc[30:], st[30:], wc[1], ws[E - 1], False, 0.0, torch.float32)
+        del q, w
+        torch.cuda.empty_cache()
+
+
+def test_rows_at_odd_addresses(blk):
+    say("dispatch and combine at odd addresses")
+    rng = np.random.default_rng(23)
+    T, k, H = 5, 3, 520
+    inv = np.arange(T * k, dtype=np.int32)[::-1].copy()
+    for kind in ("bf16", "f32"):
+        put = lambda t, o: torch.cat([torch.zeros(o, dtype=t.dtype), t.view(-1)]).to(DEV)[o:].view(t.shape)  # noqa: E731
+        x, wts = floats(rng, (T, H), kind), floats(rng, (T, k), "f32")
+        rows = put(torch.zeros((T * k, H), dtype=TYPES[kind]), 3)
+        blk.dispatch(put(x, 1), dev(inv), rows)
+        assert torch.equal(rows.cpu()[torch.from_numpy(inv.astype(np.int64))], x.repeat_interleave(k, 0))
+        out = put(torch.zeros((T, H)), 1)
+        blk.combine(rows, put(wts, 1), dev(inv), out)
+        want, mag = ref.combine(rows.cpu(), wts, inv, T, k)
+        close(out, want, (k + 1) * U * mag)
+        drows, dwts = put(torch.zeros((T * k, H), dtype=TYPES[kind]), 1), put(torch.zeros((T, k)), 1)
+        blk.combine_grad(put(x, 3), rows, put(wts, 1), dev(inv), drows, dwts)
+        v = x.repeat_interleave(k, 0).double() * wts.view(-1, 1).double()
+        close(drows[torch.from_numpy(inv.astype(np.int64)).to(DEV)], v, ref.rounded(U * v.abs(), v, TYPES[kind]))
+
+
 def test_offsets_are_held_to_the_rows(blk):
     """Offsets that leave [0, M] or fall are cut, not followed: the rows inside are right, nothing else is written."""
     say("offsets held to the rows")
@@ -548,6 +633,7 @@ def test_refusals_of_the_library(blk):
         lib.moe_combine(h, p, F32, 1, None, p, 1, 1, 4, p, F32, None),
         lib.moe_combine_grad(h, p, F32, p, F32, 1, p, p, 1, 1, 4, p, p, None),  # drows is rows
         lib.moe_quantize_i8(h, p, F32, 0, 4, p, p, None),
+        lib.moe_quantize_i8(h, p, F32, 1, 2 ** 30 + 1, p, p, None),
         lib.moe_matmul_i8(h, p, p, 1, p, p, 2, None, None, 1, 1, 1, 4, 0, 0.0, p, F32, None),     # E without offsets
         lib.moe_matmul_i8(h, p, p, 1, p, p, 1025, p, None, 1, 1, 1, 4, 0, 0.0, p, F32, None),
         lib.moe_matmul_i8(h, p, p, 1, p, p, 1, None, None, 1, 2, 1, 4, 0, 0.0, p, F32, None),     # fewer sources than rows
@@ -556,6 +642,18 @@ def test_refusals_of_the_library(blk):
         lib.moe_matmul_i8(h, p, p, 1, p, p, 1, None, None, 1, 1, 2, 4, 1, float("nan"), p, F32, None),
     ]
     assert bad == [mb.MOE_ERR_INVALID_ARG] * len(bad)
+    # more than a launch takes (checked before anything is read; the addresses are never used)
+    far = [p + (i << 44) for i in range(8)]
+    big = [
+        lib.moe_dispatch(h, far[0], F32, far[1], 2 ** 24, 1, 4, 1, far[2], F32, None),
+        lib.moe_combine(h, far[0], F32, 1, far[1], far[2], 2 ** 24, 1, 4, far[3], F32, None),
+        lib.moe_dispatch_grad(h, far[0], F32, 1, far[1], 2 ** 24, 1, 4, far[2], F32, None),
+        lib.moe_combine_grad(h, far[0], F32, far[1], F32, 1, far[2], far[3], 2 ** 21, 64, 4, far[4], far[5], None),
+        lib.moe_quantize_i8(h, far[0], F32, 2 ** 24, 4, far[1], far[2], None),
+        lib.moe_matmul_i8(h, far[0], far[1], 2 ** 30, far[2], far[3], 1, None, None, 1, 2 ** 30, 64, 64, 0, 0.0, far[4], F32, None),
+        lib.moe_matmul_i8(h, far[0], far[1], 2 ** 30, far[2], far[3], 1, None, None, 1, 2 ** 30, 64, 63, 0, 0.0, far[4], F32, None),
+    ]
+    assert big == [mb.MOE_ERR_UNSUPPORTED] * len(big)
     assert b"moe_matmul_i8" in lib.moe_ctx_last_error(h)
     torch.cuda.synchronize()
     assert (buf == 0).all()
