@@ -8,7 +8,6 @@
 
 #include <cmath>
 
-
 static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 // A grid's x dimension holds fewer than 2^32 threads.
@@ -53,8 +52,9 @@ bool launch_dispatch(const void *x, int x_type, const int32_t *inv, int T, int k
       typedef decltype(to) TO;
       constexpr int V = vec_of<TI, TO>();
       const bool nt = (size_t)T * k * H * sizeof(TO) > MOE_STREAM_BYTES;
-      hipLaunchKernelGGL((nt ? k_dispatch<TI, TO, V, true> : k_dispatch<TI, TO, V, false>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
-                         (const TI *)x, inv, k, H, n_rows, (TO *)rows);
+      hipLaunchKernelGGL((nt ? k_dispatch<TI, TO, V, true> : k_dispatch<TI, TO, V, false>),
+                         dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st, (const TI *)x, inv, k, H, n_rows,
+                         (TO *)rows);
     });
   });
   return true;
@@ -69,8 +69,9 @@ bool launch_combine_rows(const void *rows, int rows_type, int n_rows, const floa
       typedef decltype(to) TO;
       constexpr int V = vec_of<TI, TO>();
       const bool nt = (size_t)T * k * H * sizeof(TI) > MOE_STREAM_BYTES;
-      hipLaunchKernelGGL((nt ? k_combine_rows<TI, TO, V, true> : k_combine_rows<TI, TO, V, false>), dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st,
-                         (const TI *)rows, wts, inv, k, H, n_rows, (TO *)out);
+      hipLaunchKernelGGL((nt ? k_combine_rows<TI, TO, V, true> : k_combine_rows<TI, TO, V, false>),
+                         dim3(T, row_splits(T, ceil_div(H, V))), dim3(256), 0, st, (const TI *)rows, wts, inv, k, H, n_rows,
+                         (TO *)out);
     });
   });
   return true;
