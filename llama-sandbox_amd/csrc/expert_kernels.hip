@@ -126,7 +126,46 @@ bool launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, floa
 
 // Tiles of at most BM rows that M rows of E experts can make.
 static long i8_tiles(const i8_mm &a, int BM) {
-  return a.offsets ? a.M / BM + (a.M < a.E ? a.M : a.E) : ((long)a.M + BM - 1) / BM;
+  const long n = a.offsets ? (a.M < a.E ? a.M : a.E) : 1;  // matrices: each rounds up
+  return (a.M + n * (BM - 1)) / BM;
+}
+
+// The launch of a product by one kernel; false: more workgroups than a grid takes.
+typedef bool (*i8_launch)(const i8_mm &, hipStream_t);
+
+template <int M, int C, int U>
+static bool launch_few(const i8_mm &a, hipStream_t st) {
+  const int nt = ceil_div(a.swiglu ? a.N / 2 : a.N, a.swiglu ? C / 2 : C);
+  const long n = i8_tiles(a, M) * nt;
+  if (!fits(n, 64)) return false;
+  hipLaunchKernelGGL((k_mv_i8<M, C, U>), dim3((unsigned)n), dim3(64), 0, st, a, nt);
+  return true;
+}
+
+// The launch of a call whose rows are few enough for k_mv_i8 (else NULL).  More rows a tile read
+// the weights less often, fewer spread them wider.  us, rows x K x N:
+//   rows a tile, channels:   1, 2    1, 4    2, 4    4, 2   staged
+//   1 x 4096 x 4096          5.14    5.40    5.62    5.76    7.29
+//   2 x 2048 x 7168          6.31    5.68    5.47    5.58    6.51
+//   4 x 4096 x 4096          7.36    7.09    6.34    6.01    7.29
+//   4 x 7168 x 7168          29.5    26.2    15.9    14.4    13.5
+//   8 x 7168 x 512           4.46    4.74    5.15    5.41    7.05
+//   8 x 2048 x 1024          4.27    3.71    3.69    3.75    4.48
+//   8 x 7168 x 2048          10.2     8.6     7.0     7.1     7.2
+//   32 x 7168 x 256          5.86    5.61    5.43    5.60    6.97
+//   2 tokens' 8 experts of 2048 x 7168, and 4's:
+//                            51.5    37.4    37.4    52.5    42.8
+//                            98.7    70.4    69.6    98.4    75.5
+// Grouped rows are taken one a tile, up to 16 of them: an expert's weights are then read
+// as often as it has rows (128 rows of 16 tokens, Zipf, 7168 x 4096: 280 us against 165 staged).
+static i8_launch few_rows(const i8_mm &a) {
+  if (a.N > 1 << 22) return nullptr;
+  if (a.offsets) return a.M > 16 ? nullptr : a.K <= 1024 ? launch_few<1, 8, 1> : launch_few<1, 4, 2>;
+  const long n = (long)a.M * a.N;
+  if (a.M == 1 || n <= 4096) return launch_few<1, 2, 4>;
+  if (a.M == 2 || n <= 8192) return launch_few<2, 4, 2>;
+  if (a.M <= 4 && (size_t)a.N * a.K <= (size_t)32 << 20) return launch_few<4, 2, 2>;
+  return nullptr;
 }
 
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
@@ -158,7 +197,7 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
 struct i8_shape {
   int BM, BN, lds;
   float call, tile, k, k_share;
-  bool (*launch)(const i8_mm &, hipStream_t);
+  i8_launch launch;
 };
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 static constexpr i8_shape shape_of(float call, float tile, float k, float k_share) {
@@ -207,7 +246,8 @@ bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
     // weights of more than the caches hold from call to call, each read by one tile: past the caches.  Measured:
     // 939 MB against 16 rows 164 us with plain loads, 146 without (5.75 and 6.5 TB/s)
     a.stream = (size_t)a.N * a.K * (a.M < a.E ? a.M : a.E) > MOE_STREAM_BYTES;
-    return choose_shape(a, n_cu).launch(a, st);
+    const i8_launch few = few_rows(a);
+    return (few ? few : choose_shape(a, n_cu).launch)(a, st);
   }
   const int nt = a.swiglu ? ceil_div(a.N / 2, 32) : ceil_div(a.N, 64);
   const long mt = i8_tiles(a, 64);

@@ -370,6 +370,86 @@ __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
   }
 }
 
+// Few rows: up to M a tile, straight from memory to registers.  A workgroup is one wave
+// and takes C channels (SwiGLU: C / 2 columns, gate and up by turns); lane l multiplies
+// bytes [16 l, +16) of every 1024 of K, U times 1024 in flight for all channels and
+// rows, 4 products an instruction; the lanes' sums meet by DPP.  No LDS and no barrier: where the
+// weights are small the staged tiles spend 4 us on the turns of their loop, and
+// where they are large this streams as well (us, staged / this; rows x K x N):
+// 1 x 7168 x 512 6.8 / 3.4, 1 x 4096 x 4096 7.3 / 5.1, 1 x 7168 x 4096 8.4 / 7.0, 1 x 5120 x 32000 30.1 / 27.3,
+// one token's 8 experts of 7168 x 4096 39.3 / 36.6 (6.4 TB/s).
+template <int M, int C, int U>
+__global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
+  const int lane = threadIdx.x;
+  const i8_tile t = i8_find_tile(a, blockIdx.x / nt, M);
+  if (t.e < 0) return;
+  const int half = a.N / 2, n_end = a.swiglu ? half : a.N, cols = a.swiglu ? C / 2 : C;
+  const int n0 = blockIdx.x % nt * cols;
+  const int8_t *w[C], *x[M];
+#pragma unroll
+  for (int c = 0; c < C; c++) {  // past the end: the last one again
+    const int n = min(n0 + (a.swiglu ? c / 2 : c), n_end - 1);
+    w[c] = a.w + ((size_t)t.e * a.N + (a.swiglu && c % 2 ? half + n : n)) * a.K;
+  }
+  // lane m * cols + o ends up with row m's column o; the scales are asked for first
+  const int m_lane = lane >> (a.swiglu ? __builtin_ctz(C) - 1 : __builtin_ctz(C)), n = n0 + (lane & (cols - 1));
+  const float *ws = a.ws + (size_t)t.e * a.N + min(n, n_end - 1);
+  const float s_n = ws[0], s_up = a.swiglu ? ws[half] : 0.0f;
+  int acc[M][C] = {}, src[M], row = -1;
+#pragma unroll
+  for (int m = 0; m < M; m++) {
+    src[m] = __builtin_amdgcn_readfirstlane(m < t.n ? i8_src(a, t.r0 + m) : -1);
+    x[m] = a.q + (size_t)max(src[m], 0) * a.K;
+    if (m_lane == m) row = src[m];
+  }
+  const float s_row = row >= 0 ? a.qs[row] : 0.0f;
+  auto sums = [&](auto once) __attribute__((always_inline)) {
+    for (int k0 = 0; k0 < a.K; k0 += 1024 * U) {
+      v4i wv[C][U], xv[M][U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {  // past K: the last 16 bytes, against zeros
+        const int at = min(k0 + 1024 * u + 16 * lane, a.K - 16);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const v4i *p = reinterpret_cast<const v4i *>(w[c] + at);
+          wv[c][u] = decltype(once)::value ? __builtin_nontemporal_load(p) : *p;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int k = k0 + 1024 * u + 16 * lane;
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+          const v4i v = *reinterpret_cast<const v4i *>(x[m] + min(k, a.K - 16));
+#pragma unroll
+          for (int i = 0; i < 4; i++) xv[m][u][i] = k < a.K ? v[i] : 0;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+          for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[m][c] = __builtin_amdgcn_sdot4(wv[c][u][i], xv[m][u][i], acc[m][c], false);
+    }
+  };
+  if (a.stream && t.only) sums(std::true_type{});
+  else sums(std::false_type{});
+  int s0 = 0, s1 = 0;
+#pragma unroll
+  for (int m = 0; m < M; m++)
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const int s = src[m] < 0 ? 0 : __builtin_amdgcn_readlane(wave_scan(acc[m][c]), 63);
+      if (lane == m * cols + (a.swiglu ? c / 2 : c)) (a.swiglu && c % 2 ? s1 : s0) = s;
+    }
+  if (m_lane >= t.n || m_lane >= M || n >= n_end) return;
+  const float y = (float)s0 * s_row * s_n;
+  i8_store(a, t.r0 + m_lane, n, a.swiglu ? i8_swiglu(y, (float)s1 * s_row * s_up, a.clamp) : y);
+}
+
 // ---- staged tiles -------------------------------------------------------------------
 //
 // K % 16 == 0 and 16-byte aligned rows.  A workgroup multiplies BM rows with BN

@@ -335,6 +335,32 @@ def test_grouped_product(blk, T, k, E, N, K, dropped, skew, out, sw, gather):
             check_product(got[lo:hi], q[at], s[at], w[e], ws[e], sw, 2.0, TYPES[out])
 
 
+# rows that are few: of one wave's channels to many, K of one lane to several times a
+# wave's, weights past the caches; and as many rows more, on narrow tiles
+FEW = [(1, 1, 16), (1, 2, 16), (1, 7, 1008), (1, 130, 1024), (1, 258, 1040), (1, 66, 9232), (1, 6, 131056), (2, 2, 16),
+       (2, 1030, 64), (2, 4100, 2064), (3, 30, 48), (3, 2730, 272), (4, 2050, 1040), (4, 3000, 4112), (5, 818, 128),
+       (5, 820, 528), (8, 1024, 2048), (9, 14, 272), (16, 512, 512), (4096, 2, 32), (3000, 1, 48), (1, 8192, 12304),
+       (2, 8190, 12304), (4, 8200, 4096), (5, 4098, 272), (16, 1030, 1040), (7, 7168, 64)]
+
+
+@pytest.mark.parametrize("M, N, K", FEW)
+@pytest.mark.parametrize("out, sw, L", [("f32", False, 0.0), ("bf16", True, 1.5)])
+def test_dense_product_of_few_rows(blk, M, N, K, out, sw, L):
+    test_dense_product(blk, M, N, K, out, sw, L)
+
+
+FEW_GROUPED = [  # T, k, E, N, K, dropped, skew
+    (1, 8, 64, 130, 1024, 0.0, False), (1, 8, 256, 34, 1040, 0.0, False), (2, 8, 300, 50, 2064, 0.0, False),
+    (16, 1, 3, 258, 768, 0.0, True), (16, 1, 1, 66, 1040, 0.0, False), (8, 2, 1024, 18, 16, 0.4, False),
+    (1, 8, 16, 2048, 8192, 0.0, False), (17, 1, 3, 66, 768, 0.0, True)]
+
+
+@pytest.mark.parametrize("T, k, E, N, K, dropped, skew", FEW_GROUPED)
+@pytest.mark.parametrize("out, sw, gather", [("f32", False, False), ("bf16", True, True), ("f16", False, True)])
+def test_grouped_product_of_few_rows(blk, T, k, E, N, K, dropped, skew, out, sw, gather):
+    test_grouped_product(blk, T, k, E, N, K, dropped, skew, out, sw, gather)
+
+
 def test_row_map_entries_outside_the_sources_are_zero_rows(blk):
     say("row map entries outside the sources")
     rng = np.random.default_rng(8)
