@@ -471,7 +471,7 @@ __global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
 //     of short tiles (13 thousand cycles before the first MFMA, 21 of K, 16 of output).
 //     A workgroup that takes tile after tile, the next one's loads behind the output,
 //     was slower in every shape (the stores delay the waits for those loads).
-//   one row x 4096 x 7168: 8.6 us, latency: 16x16 tiles, K over 4 waves.
+//   16 rows x 7168 x 4096: 8.6 us, latency: 16x16 tiles, K over 4 waves.
 #define MOE_I8_OOB 0xffffff00u  // a lane offset past any buffer: the load returns 0
 #define MOE_I8_RSRC 0x00020000  // raw buffer, 32-bit dwords, no swizzle
 

@@ -10,6 +10,7 @@ back to ggml-cpu at that point, moe-serv/src/moe_backend.cpp:436-445).
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 import numpy as np
@@ -352,16 +353,31 @@ def check_tensor(t, name: str, dtype: str, shape=None, device: bool = True):
 
 
 _row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled by the first context
-_f32 = _i32 = _i8 = _raw_stream = None
+_raw_stream = _torch_calls = None
 
 
 def _know_torch():
-    global _f32, _i32, _i8, _raw_stream
+    global _raw_stream, _torch_calls
     if not _row_types:
         import torch
-        _f32, _i32, _i8 = torch.float32, torch.int32, torch.int8
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
+        # csrc/moe_torch.cpp, built against one torch; without it the same calls go through ctypes
+        try:
+            spec = importlib.util.spec_from_file_location("moe_torch", os.path.join(_HERE, "moe_torch.so"))
+            calls = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(calls)
+        except ImportError:
+            return
+        if calls.torch_version == torch.__version__.partition("+")[0] and _raw_stream is not None:
+            calls.set_current_stream(_raw_stream)
+            _torch_calls = calls
+
+
+class _Entries(ctypes.Structure):
+    """The entry points that moe_torch calls, by address."""
+    _fields_ = [(n, _vp) for n in ("moe_dispatch", "moe_dispatch_grad", "moe_combine", "moe_combine_grad",
+                                   "moe_quantize_i8", "moe_matmul_i8")]
 
 
 def _row_type(t, name: str) -> int:
@@ -398,10 +414,6 @@ def check_pairs(inv, T: int) -> int:
     if n // T > 64:
         raise ValueError(f"inv: k = {n // T}, at most 64")
     return n // T
-
-
-# What a check that compares without naming may raise for an argument that is no such tensor
-_NOT_FINE = (AttributeError, KeyError, TypeError, ValueError)
 
 
 def check_forward_args(desc, x, ids, wts, out, flags: int = 0):
@@ -486,6 +498,8 @@ class Graph:
 class MoeBlock:
     """One device context: resident layers plus per-call scratch."""
 
+    _calls = None  # moe_torch's argument: the address of this context's library's entry points
+
     def __init__(self, device: int = 0, budget_bytes: int = 2 ** 64 - 1, lib_path: str | None = None):
         self.lib = load_library(lib_path)
         h = _vp()
@@ -495,6 +509,9 @@ class MoeBlock:
         self.h = h.value
         self.device = int(device)
         _know_torch()
+        if _torch_calls is not None:
+            self._entries = _Entries(*(ctypes.cast(getattr(self.lib, n), _vp).value for n, _ in _Entries._fields_))
+            self._calls = ctypes.addressof(self._entries)
         self.descs: dict[int, LayerDesc] = {}
 
     # -- lifecycle --------------------------------------------------------
@@ -628,99 +645,68 @@ class MoeBlock:
                                                _stream(stream)), "moe_route_forward")
 
     # -- around the expert products (torch device tensors) ------------------------
-    # Each call first compares its tensors with what it needs (a fifth of the
-    # cost of the checks that name what is wrong, which run only then: the
-    # smallest calls take a few microseconds on the device).  Buffers that
-    # overlap are refused by the library.
+    # moe_torch compares a call's tensors with what it needs and makes it; the checks
+    # that name what is wrong run only where it returns None.  Buffers that overlap are
+    # refused by the library.
     def _on_device(self, *named):
         for t, name in named:
             if t is not None and t.get_device() != self.device:
                 raise ValueError(f"{name}: on {t.device}, expected this context's ROCm device (cuda:{self.device})")
+            if t is not None and max(t.shape) > 2 ** 31 - 1:
+                raise ValueError(f"{name}: shape {tuple(t.shape)}, at most 2^31 - 1 along each")
 
     def dispatch(self, x, inv, rows, stream=None):
         """rows[inv[t*k+s]] = x[t]: tokens' rows [T, H] to expert order
         [n_rows, H]; inv from group(); rows no pair names stay as they were."""
-        try:
-            xt, rt = _row_types[x.dtype], _row_types[rows.dtype]
-            (T, H), (R, Hr), n, d = x.shape, rows.shape, inv.numel(), self.device
-            k = n // T
-            fine = (inv.dtype is _i32 and H == Hr and inv.dim() == 1 and R and 0 < k <= 64 and k * T == n and H
-                    and x.is_contiguous() and rows.is_contiguous() and inv.is_contiguous()
-                    and x.get_device() == d == rows.get_device() == inv.get_device())
-        except (*_NOT_FINE, ZeroDivisionError):
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.dispatch(self._calls, self.h, self.device, x, inv, rows, stream)
+        if st is None:
             xt = check_rows("x", x)
             T, H = x.shape
             rt = check_rows("rows", rows, None, H)
             k, R = check_pairs(inv, T), rows.shape[0]
             self._on_device((x, "x"), (inv, "inv"), (rows, "rows"))
-        st = self.lib.moe_dispatch(self.h, x.data_ptr(), xt, inv.data_ptr(), T, k, H, R, rows.data_ptr(), rt,
-                                   _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_dispatch(self.h, x.data_ptr(), xt, inv.data_ptr(), T, k, H, R, rows.data_ptr(), rt,
+                                       _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_dispatch")
 
     def dispatch_grad(self, drows, inv, dx, stream=None):
         """dx[t] = sum over s of drows[inv[t*k+s]]."""
-        try:
-            xt, rt = _row_types[dx.dtype], _row_types[drows.dtype]
-            (T, H), (R, Hr), n, d = dx.shape, drows.shape, inv.numel(), self.device
-            k = n // T
-            fine = (inv.dtype is _i32 and H == Hr and inv.dim() == 1 and R and 0 < k <= 64 and k * T == n and H
-                    and dx.is_contiguous() and drows.is_contiguous() and inv.is_contiguous()
-                    and dx.get_device() == d == drows.get_device() == inv.get_device())
-        except (*_NOT_FINE, ZeroDivisionError):
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.dispatch_grad(self._calls, self.h, self.device, drows, inv, dx, stream)
+        if st is None:
             xt = check_rows("dx", dx)
             T, H = dx.shape
             rt = check_rows("drows", drows, None, H)
             k, R = check_pairs(inv, T), drows.shape[0]
             self._on_device((drows, "drows"), (inv, "inv"), (dx, "dx"))
-        st = self.lib.moe_dispatch_grad(self.h, drows.data_ptr(), rt, R, inv.data_ptr(), T, k, H, dx.data_ptr(), xt,
-                                        _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_dispatch_grad(self.h, drows.data_ptr(), rt, R, inv.data_ptr(), T, k, H, dx.data_ptr(), xt,
+                                            _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_dispatch_grad")
 
     def combine(self, rows, wts, inv, out, stream=None):
         """out[t] = sum over s of wts[t, s] * rows[inv[t*k+s]]: expert rows
         [n_rows, H] back in token order [T, H], weighted."""
-        try:
-            ot, rt = _row_types[out.dtype], _row_types[rows.dtype]
-            (T, H), (R, Hr), (Tw, k), d = out.shape, rows.shape, wts.shape, self.device
-            fine = (inv.dtype is _i32 and wts.dtype is _f32 and H == Hr and Tw == T and inv.dim() == 1
-                    and inv.numel() == k * T and T and H and R and 0 < k <= 64 and out.is_contiguous()
-                    and rows.is_contiguous() and wts.is_contiguous() and inv.is_contiguous()
-                    and out.get_device() == d == rows.get_device() == wts.get_device() == inv.get_device())
-        except _NOT_FINE:
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.combine(self._calls, self.h, self.device, rows, wts, inv, out, stream)
+        if st is None:
             ot = check_rows("out", out)
             T, H = out.shape
             rt = check_rows("rows", rows, None, H)
             k, R = check_pairs(inv, T), rows.shape[0]
             check_tensor(wts, "wts", "float32", (T, k), device=False)
             self._on_device((rows, "rows"), (wts, "wts"), (inv, "inv"), (out, "out"))
-        st = self.lib.moe_combine(self.h, rows.data_ptr(), rt, R, wts.data_ptr(), inv.data_ptr(), T, k, H, out.data_ptr(),
-                                  ot, _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_combine(self.h, rows.data_ptr(), rt, R, wts.data_ptr(), inv.data_ptr(), T, k, H,
+                                      out.data_ptr(), ot,
+                                      _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_combine")
 
     def combine_grad(self, dout, rows, wts, inv, drows, dwts, stream=None):
         """combine's gradient: drows[inv[t*k+s]] = wts[t, s] * dout[t] and
         dwts[t, s] = <dout[t], rows[inv[t*k+s]]> (0 for a dropped pair)."""
-        try:
-            dt, rt = _row_types[dout.dtype], _row_types[rows.dtype]
-            (T, H), (R, Hr), (Tw, k), d = dout.shape, rows.shape, wts.shape, self.device
-            fine = (inv.dtype is _i32 and wts.dtype is _f32 and dwts.dtype is _f32 and drows.dtype is rows.dtype
-                    and drows.shape == rows.shape and dwts.shape == wts.shape and H == Hr and Tw == T and inv.dim() == 1
-                    and inv.numel() == k * T and T and H and R and 0 < k <= 64 and dout.is_contiguous()
-                    and rows.is_contiguous() and wts.is_contiguous() and inv.is_contiguous() and drows.is_contiguous()
-                    and dwts.is_contiguous() and dout.get_device() == d == rows.get_device() == wts.get_device()
-                    and inv.get_device() == d == drows.get_device() == dwts.get_device())
-        except _NOT_FINE:
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.combine_grad(self._calls, self.h, self.device, dout, rows, wts, inv, drows, dwts,
+                                                       stream)
+        if st is None:
             dt = check_rows("dout", dout)
             T, H = dout.shape
             rt = check_rows("rows", rows, None, H)
@@ -731,31 +717,24 @@ class MoeBlock:
             check_tensor(wts, "wts", "float32", (T, k), device=False)
             check_tensor(dwts, "dwts", "float32", (T, k), device=False)
             self._on_device((dout, "dout"), (rows, "rows"), (wts, "wts"), (inv, "inv"), (drows, "drows"), (dwts, "dwts"))
-        st = self.lib.moe_combine_grad(self.h, dout.data_ptr(), dt, rows.data_ptr(), rt, R, wts.data_ptr(), inv.data_ptr(),
-                                       T, k, H, drows.data_ptr(), dwts.data_ptr(),
-                                       _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_combine_grad(self.h, dout.data_ptr(), dt, rows.data_ptr(), rt, R, wts.data_ptr(),
+                                           inv.data_ptr(), T, k, H, drows.data_ptr(), dwts.data_ptr(),
+                                           _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_combine_grad")
 
     def quantize_i8(self, x, q, scale, stream=None):
         """Rows x [M, K] in 8 bits: scale [M] = amax / 127, q [M, K] int8 = x /
         scale to the nearest whole number."""
-        try:
-            xt = _row_types[x.dtype]
-            (M, K), d = x.shape, self.device
-            fine = (q.dtype is _i8 and scale.dtype is _f32 and q.shape == (M, K) and scale.shape == (M,) and M and K
-                    and x.is_contiguous() and q.is_contiguous() and scale.is_contiguous()
-                    and x.get_device() == d == q.get_device() == scale.get_device())
-        except _NOT_FINE:
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.quantize_i8(self._calls, self.h, self.device, x, q, scale, stream)
+        if st is None:
             xt = check_rows("x", x)
             M, K = x.shape
             check_tensor(q, "q", "int8", (M, K), device=False)
             check_tensor(scale, "scale", "float32", (M,), device=False)
             self._on_device((x, "x"), (q, "q"), (scale, "scale"))
-        st = self.lib.moe_quantize_i8(self.h, x.data_ptr(), xt, M, K, q.data_ptr(), scale.data_ptr(),
-                                      _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_quantize_i8(self.h, x.data_ptr(), xt, M, K, q.data_ptr(), scale.data_ptr(),
+                                          _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_quantize_i8")
 
@@ -767,28 +746,9 @@ class MoeBlock:
         group(): row r's codes are those of token perm[r] // k; without perm, of
         row r).  swiglu: the channels are N/2 of gate and N/2 of up, and out
         [M, N/2] is silu(gate) * up, clamped as LayerDesc.clamp says."""
-        try:
-            ot = _row_types[out.dtype]
-            (S, K), (M, No), d, E = q.shape, out.shape, self.device, 1
-            if offsets is None:
-                N = w.shape[0]
-                fine = w.shape == (N, K) and w_scale.shape == (N,)
-            else:
-                E, N = w_scale.shape
-                fine = (w.shape == (E, N, K) and offsets.dtype is _i32 and offsets.shape == (E + 1,)
-                        and offsets.is_contiguous() and offsets.get_device() == d)
-            if perm is None:
-                fine = fine and k == 1 and S == M
-            else:
-                fine = fine and perm.dtype is _i32 and perm.shape == (M,) and perm.is_contiguous() and perm.get_device() == d
-            fine = (fine and q.dtype is _i8 and w.dtype is _i8 and scale.dtype is _f32 and w_scale.dtype is _f32
-                    and scale.shape == (S,) and No == (N // 2 if swiglu else N) and not (swiglu and N % 2) and M and N and K
-                    and q.is_contiguous() and w.is_contiguous() and scale.is_contiguous() and w_scale.is_contiguous()
-                    and out.is_contiguous() and q.get_device() == d == w.get_device() == scale.get_device()
-                    and w_scale.get_device() == d == out.get_device())
-        except _NOT_FINE:
-            fine = False
-        if not fine:
+        st = self._calls and _torch_calls.matmul_i8(self._calls, self.h, self.device, q, scale, w, w_scale, out, offsets,
+                                                    perm, k, swiglu, clamp, stream)
+        if st is None:
             grouped = offsets is not None
             check_tensor(q, "q", "int8", (None, None), device=False)
             S, K = q.shape
@@ -810,10 +770,11 @@ class MoeBlock:
                 raise ValueError(f"out: {M} rows for {S} rows of q without perm (k = {k})")
             self._on_device((q, "q"), (scale, "scale"), (w, "w"), (w_scale, "w_scale"), (out, "out"),
                             (offsets, "offsets"), (perm, "perm"))
-        st = self.lib.moe_matmul_i8(self.h, q.data_ptr(), scale.data_ptr(), S, w.data_ptr(), w_scale.data_ptr(), E,
-                                    None if offsets is None else offsets.data_ptr(),
-                                    None if perm is None else perm.data_ptr(), int(k), M, N, K, 1 if swiglu else 0, clamp,
-                                    out.data_ptr(), ot, _device_stream(self.device) if stream is None else int(stream))
+            st = self.lib.moe_matmul_i8(self.h, q.data_ptr(), scale.data_ptr(), S, w.data_ptr(), w_scale.data_ptr(), E,
+                                        None if offsets is None else offsets.data_ptr(),
+                                        None if perm is None else perm.data_ptr(), int(k), M, N, K, 1 if swiglu else 0,
+                                        clamp, out.data_ptr(), ot,
+                                        _device_stream(self.device) if stream is None else int(stream))
         if st:
             self._check(st, "moe_matmul_i8")
 

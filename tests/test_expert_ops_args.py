@@ -114,3 +114,46 @@ def test_null_context_is_refused_by_every_entry_point():
     assert lib.moe_combine_grad(None, p, F32, p, F32, 1, p, p, 1, 1, 4, p, p, None) == mb.MOE_ERR_INVALID_ARG
     assert lib.moe_quantize_i8(None, p, F32, 1, 4, p, p, None) == mb.MOE_ERR_INVALID_ARG
     assert lib.moe_matmul_i8(None, p, p, 1, p, p, 1, None, None, 1, 1, 1, 4, 0, 0.0, p, F32, None) == mb.MOE_ERR_INVALID_ARG
+
+
+def torch_calls():
+    mb._know_torch()
+    if mb._torch_calls is None:
+        pytest.skip("moe_torch.so was not built for this torch")
+    return mb._torch_calls
+
+
+ENTRIES = ctypes.create_string_buffer(8 * 6)  # no entry points: nothing here may get as far as a call
+
+
+@pytest.mark.parametrize("op", list(GOOD))
+def test_the_compiled_comparison_says_nothing_of_what_is_not_fine(op):
+    calls, at = torch_calls(), ctypes.addressof(ENTRIES)
+    args = list(GOOD[op].values()) + ([None, None, 1, False, 0.0] if op == "matmul_i8" else [])
+    call = getattr(calls, op)
+    assert call(at, 1, 0, *args, 0) is None  # host tensors
+    assert call(at, None, 0, *args, 0) is None and call(at, 1, 0, *args, None) is None
+    assert call() is None and call(at, 1, 0, *args) is None and call(at, 1, 0, *args, 0, 0) is None
+    assert call(at, 2 ** 70, 0, *args, 0) is None and call(at, 1, 0, *args, "stream") is None
+    for i in range(len(args)):
+        for bad in (None, 3, "x", torch.zeros(()), torch.zeros(2, 2).to_sparse(), torch.empty((3, 64), device="meta")):
+            assert call(at, 1, 0, *args[:i], bad, *args[i + 1:], 0) is None
+
+
+def test_dimensions_past_32_bits_are_refused():
+    """meta tensors: shapes without memory, on the context's device as far as the check can see."""
+    class OnDevice:
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def get_device(self):
+            return 0
+
+    n = 2 ** 31 + T
+    x, rows = (OnDevice(torch.empty((m, 1), device="meta")) for m in (n, R))
+    inv = OnDevice(torch.empty((n * K_,), dtype=torch.int32, device="meta"))
+    with pytest.raises(ValueError, match="at most 2"):
+        block().dispatch(x, inv, rows)

@@ -625,6 +625,47 @@ def test_captured_and_replayed(blk):
             assert torch.equal(a, b), i
 
 
+def test_calls_are_the_same_without_the_compiled_comparison(blk):
+    """moe_torch and ctypes: the same results, on torch's current stream and on a given one."""
+    say("calls without the compiled comparison")
+    assert blk._calls, "moe_torch.so was not built for this torch"
+    rng = np.random.default_rng(31)
+    T, k, E, H, N = 37, 4, 8, 144, 96
+    ids = ref.ids_of(rng, T, k, E, 0.2)
+    offsets, perm, inv, kept = ref.grouping(ids, E)
+    x, rows, y = floats(rng, (T, H), "bf16").to(DEV), floats(rng, (T * k, H), "f16").to(DEV), floats(rng, (T, H), "f32").to(DEV)
+    wts = dev(rng.random((T, k)).astype(np.float32))
+    q, w, s, ws = dev(codes(rng, (T, H))), dev(codes(rng, (E, N, H))), dev(scales(rng, T, H)), dev(scales(rng, (E, N), H))
+    offsets, perm, inv = dev(offsets), dev(perm), dev(inv)
+
+    def every(stream):
+        z = lambda shape, t: torch.zeros(shape, dtype=t, device=DEV)  # noqa: E731
+        o = [z((T * k, H), torch.float32), z((T, H), torch.bfloat16), z((T, H), torch.float32), z((T * k, H), torch.float16),
+             z((T, k), torch.float32), z((T, H), torch.int8), z((T,), torch.float32), z((T * k, N // 2), torch.bfloat16),
+             z((T, N), torch.float16)]
+        torch.cuda.synchronize()
+        blk.dispatch(x, inv, o[0], stream=stream)
+        blk.dispatch_grad(rows, inv, o[1], stream=stream)
+        blk.combine(rows, wts, inv, o[2], stream=stream)
+        blk.combine_grad(y, rows, wts, inv, o[3], o[4], stream=stream)
+        blk.quantize_i8(x, o[5], o[6], stream=stream)
+        blk.matmul_i8(q, s, w, ws, o[7], offsets=offsets, perm=perm, k=k, swiglu=True, clamp=1.0, stream=stream)
+        blk.matmul_i8(q, s, w[2], ws[2], o[8], stream=stream)
+        torch.cuda.synchronize()
+        return o
+
+    want = every(None)
+    calls, other = blk._calls, torch.cuda.Stream()
+    got = [every(other.cuda_stream)]
+    try:
+        blk._calls = None
+        got += [every(None), every(other.cuda_stream)]
+    finally:
+        blk._calls = calls
+    for o in got:
+        assert all(torch.equal(a, b) for a, b in zip(want, o))
+
+
 def test_two_streams_at_once(blk):
     say("two streams at once")
     rng = np.random.default_rng(13)
