@@ -96,11 +96,11 @@ bool launch_combine_grad(const void *dout, int dout_type, const void *rows, int 
   return true;
 }
 
-template <typename T, int WPR, int VPT>
+template <typename T, int LANES, int VPT>
 static void launch_quantize(const T *x, int M, int K, int8_t *q, float *scale, hipStream_t st) {
-  constexpr int rows = WPR < 4 ? 4 / WPR : 1;
-  hipLaunchKernelGGL((k_quantize_i8<T, WPR, VPT>), dim3(ceil_div(M, rows)), dim3(WPR < 4 ? 256 : 64 * WPR), 0, st, x, M, K,
-                     q, scale);
+  constexpr int rows = LANES < 256 ? 256 / LANES : 1;
+  hipLaunchKernelGGL((k_quantize_i8<T, LANES, VPT>), dim3(ceil_div(M, rows)), dim3(LANES < 256 ? 256 : LANES), 0, st, x, M,
+                     K, q, scale);
 }
 
 // One vector a thread where the rows are too few to fill the chip (a row is
@@ -110,15 +110,19 @@ bool launch_quantize_i8(const void *x, int x_type, int M, int K, int8_t *q, floa
   with_type(x_type, [&](auto t) {
     typedef decltype(t) T;
     const T *p = (const T *)x;
-    const bool few = M < 2 * n_cu;
-    if (K <= 512) launch_quantize<T, 1, 1>(p, M, K, q, scale, st);
-    else if (K <= 1024 && !few) launch_quantize<T, 1, 2>(p, M, K, q, scale, st);
-    else if (K <= 2048 && few) launch_quantize<T, 4, 1>(p, M, K, q, scale, st);
-    else if (K <= 2048) launch_quantize<T, 1, 4>(p, M, K, q, scale, st);
-    else if (K <= 8192 && few) launch_quantize<T, 16, 1>(p, M, K, q, scale, st);
-    else if (K <= 4096) launch_quantize<T, 4, 2>(p, M, K, q, scale, st);
-    else if (K <= 8192) launch_quantize<T, 4, 4>(p, M, K, q, scale, st);
-    else if (K <= 32768) launch_quantize<T, 16, 4>(p, M, K, q, scale, st);
+    if (M < 2 * n_cu && K > 512 && K <= 8192) {
+      if (K <= 2048) launch_quantize<T, 256, 1>(p, M, K, q, scale, st);
+      else launch_quantize<T, 1024, 1>(p, M, K, q, scale, st);
+    }
+    else if (K <= 256) launch_quantize<T, 32, 1>(p, M, K, q, scale, st);
+    else if (K <= 512) launch_quantize<T, 64, 1>(p, M, K, q, scale, st);
+    else if (K <= 768 && M >= 8 * n_cu) launch_quantize<T, 32, 3>(p, M, K, q, scale, st);
+    else if (K <= 1024) launch_quantize<T, 64, 2>(p, M, K, q, scale, st);
+    else if (K <= 2048) launch_quantize<T, 64, 4>(p, M, K, q, scale, st);
+    else if (K <= 4096) launch_quantize<T, 256, 2>(p, M, K, q, scale, st);
+    else if (K <= 6144) launch_quantize<T, 256, 3>(p, M, K, q, scale, st);
+    else if (K <= 8192) launch_quantize<T, 256, 4>(p, M, K, q, scale, st);
+    else if (K <= 32768) launch_quantize<T, 1024, 4>(p, M, K, q, scale, st);
     else hipLaunchKernelGGL((k_quantize_i8_long<T>), dim3(M), dim3(256), 0, st, p, K, q, scale);
   });
   return true;

@@ -56,6 +56,14 @@ __device__ __forceinline__ int i8_code_in(const i8_row &w, float x) {
   return w.inv > 0.0f ? i8_code(x * w.pre, w.s, w.inv) : 0;
 }
 
+// What the code of x is more than u - 1.5 * 2^23, the whole number at most one off; as
+// above, without branches and for rows that need no pre.
+__device__ __forceinline__ int i8_correction(const i8_row &w, float x, float u) {
+  const float r = fmaf(0x1.8p23f - u, w.s, x), past = fabsf(r) - 0.5f * w.s;
+  const bool odd = __builtin_bit_cast(uint32_t, u) & 1;
+  return (past > 0.0f) | ((past == 0.0f) & odd) ? (r < 0.0f ? -1 : 1) : 0;
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
@@ -68,6 +76,15 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
   const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
   return max(max(a, b), max(c, d));
+}
+
+// Of the 32 lanes that a lane is one of.
+__device__ __forceinline__ uint32_t half_wave_max_u(uint32_t v) {
+  v = dpp_max<0xB1>(v);
+  v = dpp_max<0x4E>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  return max(v, (uint32_t)__shfl_xor((int)v, 16));
 }
 
 // Largest |x| of a vector as it was loaded, as the bits of a float: bits without the
@@ -96,33 +113,36 @@ __device__ __forceinline__ uint32_t abs_bits(const raw_v<T, V> &r) {
   }
 }
 
-// A row's codes in one pass: WPR waves hold it in registers, VPT vectors of 8 a
-// thread (K <= 512 WPR VPT); 256 / (64 WPR) rows a workgroup where WPR < 4.
-// Memory bound (2 to 4 bytes in, 1 out) only while the codes are cheap: a
-// quotient x * inv is within 1.6e-5 of x / s, so it decides all but those next
-// to a tie, and the exact comparison runs only for waves that hold one (about
-// one vector in ten).  x * inv + 1.5 * 2^23 is rounded to a whole number, ties to
-// even, with the code in its low byte.  bf16: 4096 rows of 7168 (88 MB) 19.6 us,
-// 4.5 TB/s; 32764 of 768 (76 MB) 24 us; one row 2.7 us, a launch.  Workgroups that
-// walk rows with the next one's loads in flight took 24 to 29 us for the first.
-template <typename T, int WPR, int VPT>
-__global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void k_quantize_i8(const T *__restrict__ x, int M, int K,
-                                                                          int8_t *__restrict__ q, float *__restrict__ scale) {
-  constexpr int RPW = WPR < 4 ? 4 / WPR : 1;  // rows a workgroup
-  __shared__ uint32_t part[WPR < 4 ? 4 : WPR];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, in_row = tid % (64 * WPR);
-  const long row = (long)blockIdx.x * RPW + wave / WPR;
+// A row's codes in one pass: LANES threads hold it in registers, VPT vectors of 8 each
+// (K <= 8 LANES VPT); 256 / LANES rows a workgroup where that is more than one.
+// Memory bound (2 to 4 bytes in, 1 out) only while the codes are cheap: x * inv, before
+// it is rounded, is within 127 * 2^-24 = 7.6e-6 of x / s, so it decides all but those next
+// to a tie, and only waves that hold one look at the remainders: one vector in a hundred
+// of f32 values, most of 16-bit ones (their quotients have small denominators, and meet ties
+// exactly).  x * inv + 1.5 * 2^23 is rounded once, to a whole number, ties to even,
+// with the code in its low byte.  4096 rows of 7168 bf16 (88 MB) 20.0 us, 4.4 TB/s
+// (22.1 where a tie took the whole quotient again, with branches); 32764 of 768 (76 MB)
+// 17.8, two rows a wave (23.5 with one row and a third of the lanes idle); one row
+// 2.7, a launch.  Workgroups that walk rows with the next one's loads in flight took 24
+// to 29 us for the first.
+template <typename T, int LANES, int VPT>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_quantize_i8(const T *__restrict__ x, int M, int K,
+                                                                           int8_t *__restrict__ q, float *__restrict__ scale) {
+  constexpr int RPW = LANES < 256 ? 256 / LANES : 1, WPR = LANES / 64;  // rows a workgroup, waves a row
+  __shared__ uint32_t part[LANES < 256 ? 4 : WPR];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, in_row = tid % LANES;
+  const long row = (long)blockIdx.x * RPW + tid / LANES;
   const T *xr = x + (row < M ? row : 0) * K;
   raw_v<T, 8> r[VPT];
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
-    const int c = (in_row + v * 64 * WPR) * 8;
+    const int c = (in_row + v * LANES) * 8;
     r[v].load(xr + c, row < M ? K - c : 0);
   }
   uint32_t m = 0;
 #pragma unroll
   for (int v = 0; v < VPT; v++) m = max(m, abs_bits(r[v]));
-  m = wave_max_u(m);
+  m = LANES == 32 ? half_wave_max_u(m) : wave_max_u(m);
   if constexpr (WPR > 1) {
     if (lane == 0) part[wave] = m;
     __syncthreads();
@@ -133,19 +153,22 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void k_quantize_i8(const 
   const i8_row w = i8_row_of(m);
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
-    const int c = (in_row + v * 64 * WPR) * 8;
+    const int c = (in_row + v * LANES) * 8;
     if (c >= K) break;
     uint32_t code[8];
-    float far = w.pre != 1.0f ? 1.0f : 0.0f;  // the largest distance of a quotient from its whole number
+    float far = 0.0f;  // the largest distance of a quotient from its whole number
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float t = (float)r[v].v[i] * w.inv, u = t + 0x1.8p23f;
-      far = fmaxf(far, fabsf(t - (u - 0x1.8p23f)));
+      const float e = (float)r[v].v[i], u = fmaf(e, w.inv, 0x1.8p23f);
+      far = fmaxf(far, fabsf(fmaf(e, w.inv, 0x1.8p23f - u)));
       code[i] = __builtin_bit_cast(uint32_t, u);
     }
-    if (__any(far > 0.4999f)) {
+    if (w.pre != 1.0f) {
 #pragma unroll
       for (int i = 0; i < 8; i++) code[i] = (uint32_t)i8_code_in(w, (float)r[v].v[i]);
+    } else if (__any(far > 0.49999f)) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) code[i] += i8_correction(w, (float)r[v].v[i], __builtin_bit_cast(float, code[i]));
     }
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(1)));
     int8_t *to = q + row * K + c;

@@ -202,6 +202,33 @@ def test_quantize(blk, M, K, kind):
     assert torch.equal(q.cpu(), wq)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M, K", [(2100, 700), (2051, 768), (4099, 513), (2049, 8), (700, 256), (515, 255), (600, 1537), (515, 6144),
+                                  (600, 5003), (513, 7168)])
+def test_quantize_many_rows(blk, M, K, kind):
+    test_quantize(blk, M, K, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M, K", [(1, 768), (2100, 700), (600, 248), (9, 7168), (600, 4104)])
+def test_quantize_between_two_codes(blk, M, K, kind):
+    """Rows whose largest value is 127 units: halves of units are ties, and their neighbours
+    the smallest steps beside one."""
+    say("quantize between two codes", M, K, kind)
+    rng = np.random.default_rng(M + K)
+    unit = torch.from_numpy(2.0 ** rng.integers(-8, 8, (M, 1)))
+    x = torch.from_numpy((rng.integers(-126, 126, (M, K)) + 0.5)).to(TYPES[kind]).double()
+    t = torch.finfo(TYPES[kind])
+    step = torch.from_numpy(rng.integers(-1, 2, (M, K))) * t.eps * 2.0 ** torch.floor(torch.log2(x.abs()))
+    x = (x + step).clamp(-127, 127)
+    x[:, K // 3] = 127.0
+    x = (x * unit).to(TYPES[kind])
+    q, scale = torch.full((M, K), 99, dtype=torch.int8, device=DEV), torch.full((M,), 7.0, device=DEV)
+    blk.quantize_i8(x.to(DEV), q, scale)
+    assert torch.equal(scale.cpu().double(), unit[:, 0])
+    assert torch.equal(q.cpu().double(), torch.round(x.double() / unit))
+
+
 @pytest.mark.parametrize("K", [24, 1024, 8192, 33])
 def test_quantize_ties_and_extremes(blk, K):
     say("quantize ties and extremes", K)
