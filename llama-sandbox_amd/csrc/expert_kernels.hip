@@ -177,8 +177,8 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
   const int nt = ceil_div(a.N, BN);
   const long n = i8_tiles(a, BM) * nt;
   if (!fits(n, 64 * WM * WN * WK)) return false;
-  hipLaunchKernelGGL((k_mm_i8<BM, BN, WM, WN, WK, NBUF>), dim3((unsigned)n), dim3(64 * WM * WN * WK),
-                     (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>()), st, a, nt);
+  hipLaunchKernelGGL((a.stream ? k_mm_i8<BM, BN, WM, WN, WK, NBUF, true> : k_mm_i8<BM, BN, WM, WN, WK, NBUF, false>),
+                     dim3((unsigned)n), dim3(64 * WM * WN * WK), (i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>()), st, a, nt);
   return true;
 }
 
@@ -196,6 +196,9 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
 //                     512:     231    136     84   64.2    51.3    40.7     37.2     51.7     96
 //                    1024:     453    265    162    121      93      82       71     55.9     98
 //                    4096:    1788   1036    619    461     331     283      247      215    199
+// (measured before the present order of LDS reads: 256x256 now takes 187 at 4096 rows, 76
+// at 1024; the smaller tiles gained little).  A last round that is partly filled costs less than
+// a whole one, once there are several: its tiles have the memory to themselves.
 // 128x128 stands twice: 3 stages for one workgroup a CU, 2 for two.  Eight waves a
 // workgroup in all but the smallest: with 4 the same tiles took up to a third longer.
 struct i8_shape {
@@ -216,9 +219,9 @@ static const i8_shape i8_shapes[] = {
     shape_of<64, 128, 2, 4, 1, 3>(1.57f, 2.41f, 0.134f, 0.253f),
     shape_of<128, 128, 4, 2, 1, 3>(0.0f, 4.09f, 0.504f, 0.0f),
     shape_of<128, 128, 2, 4, 1, 2>(0.0f, 2.95f, 0.509f, 0.264f),
-    shape_of<128, 256, 2, 4, 1, 3>(0.0f, 5.61f, 0.810f, 0.0f),
+    shape_of<128, 256, 2, 4, 1, 3>(0.0f, 5.55f, 0.775f, 0.0f),
     shape_of<256, 128, 4, 2, 1, 3>(0.0f, 5.59f, 0.779f, 0.0f),
-    shape_of<256, 256, 4, 2, 1, 2>(0.0f, 5.95f, 1.544f, 0.0f),
+    shape_of<256, 256, 2, 4, 1, 2>(0.0f, 5.95f, 1.544f, 0.0f),
 };
 
 static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
@@ -231,7 +234,7 @@ static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
     const float tiles = matrices * row_tiles * (float)ceil_div(a.N, s.BN);
     const int fit = (160 << 10) / s.lds, occ = fit < 4 ? fit : 4;
     const float each = tiles / (float)(n_cu * occ), per_cu = ceilf(tiles / (float)n_cu);
-    const float rounds = each <= 3.0f ? ceilf(each) : each + 0.5f;
+    const float rounds = each <= 3.0f ? ceilf(each) : fminf(ceilf(each), each + 0.5f);
     const float cost = s.call + rounds * (s.tile + a.K / 128.0f * (s.k + s.k_share * (per_cu < occ ? per_cu : occ)));
     if (!best || cost < least) {
       best = &s;

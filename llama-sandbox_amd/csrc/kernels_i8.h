@@ -484,13 +484,14 @@ __global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
 // 16x16x64 MFMA, channels as A and rows as B: D lane l holds row l % 16 of its
 // row tile and channels 4 (l / 16) + i of its channel tile.
 // Bound by, and measured (kernel alone):
-//   4096 x 7168 x 7168, 256x256: 196 us, 2.15 PO/s.  The MFMA pipes are busy half
-//     of the time; the rest is a tile's start and end (a tenth) and loads of
-//     both operands that all CUs ask for at once.  16x16x64 from registers alone
-//     reaches 3.8 PO/s here, 32x32x32 3.3.
+//   4096 x 7168 x 7168, 256x256: 187 us, 2.25 PO/s; 8192 x 8192 x 8192 421 us, 2.61.  A
+//     tile's start and end are a tenth; in the loop the MFMA pipes share the time with the LDS
+//     reads (three quarters of LDS's rate).  Waves of 128 rows x 64 channels 187 us, of
+//     64 x 128 191; a non-temporal choice at every load, which cut the loop into blocks, 204.
+//     16x16x64 from registers alone reaches 3.8 PO/s here, 32x32x32 3.3.
 //   16 or 4096 rows over the experts, 64x128: the weights' stream from HBM, 6.2 to
 //     6.5 TB/s (32x128 to 128x64 within a few percent).
-//   32764 x 768 x 2048 to f32, 256x256: 120 us, the output's 262 MB and the start
+//   32764 x 768 x 2048 to f32, 256x256: 116 us, the output's 262 MB and the start
 //     of short tiles (13 thousand cycles before the first MFMA, 21 of K, 16 of output).
 //     A workgroup that takes tile after tile, the next one's loads behind the output,
 //     was slower in every shape (the stores delay the waits for those loads).
@@ -507,24 +508,32 @@ __device__ __forceinline__ void i8_wait_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// 64 lanes' 16 bytes at base + vo + so into the 1 KiB at buf.  once: read by no other workgroup (non-temporal).
-__device__ __forceinline__ void i8_dma(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so, bool once) {
+// 64 lanes' 16 bytes at base + vo + so into the 1 KiB at buf; _once: read by no other
+// workgroup (non-temporal).
+__device__ __forceinline__ void i8_dma(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so) {
   typedef __attribute__((address_space(3))) void *lds_t;
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, MOE_I8_RSRC);
-  if (once) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 2);
-  else __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 0);
+}
+__device__ __forceinline__ void i8_dma_once(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so) {
+  typedef __attribute__((address_space(3))) void *lds_t;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, MOE_I8_RSRC);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 2);
 }
 
 // Load i of this wave's share (loads wave, wave + NW, ...) of the N_LOAD 1 KiB loads
 // of a stage from K byte k0 on, R rows a block of 128 bytes.  vo: lane offsets at
 // K 0.  Lanes past K, and every lane of a stage past the end, are out of range:
 // they read 0, and the waits can count on the loads.
-template <int R, int N_LOAD, int NW>
+template <int R, int N_LOAD, int NW, bool ONCE>
 __device__ __forceinline__ void i8_load(int i, const int8_t *base, uint32_t bytes, uint32_t vo, v4i *buf, int wave, int k0,
-                                        int k_lane, int K, bool once) {
+                                        int k_lane, int K) {
   const int u = wave + NW * i;
-  if (N_LOAD % NW == 0 || u < N_LOAD)  // uniform over the wave
-    i8_dma(base, bytes, buf + u * 64, k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB, k0 < K ? k0 : 0, once);
+  const uint32_t at = k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB;
+  if (N_LOAD % NW == 0 || u < N_LOAD) {  // uniform over the wave
+    if constexpr (ONCE) i8_dma_once(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
+    else i8_dma(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
+  }
 }
 
 // A wave's rows on their way out: 16 rows of up to 128 bytes, and 16 between them.
@@ -602,15 +611,14 @@ __device__ __forceinline__ void i8_rows_out(T *out, int8_t *reg, int lane, size_
   }
 }
 
-template <int BM, int BN, int WM, int WN, int WK, int NBUF>
-__global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
+// The rest of k_mm_i8 for one tile; ONCE: no other workgroup reads its weights.
+template <int BM, int BN, int WM, int WN, int WK, int NBUF, bool ONCE>
+__device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const i8_tile &t, v4i *lds) {
   constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
   constexpr int STAGE = (BM + BN) * WK * 8;          // 16-byte chunks of a stage
   constexpr int XI = BM * WK / 8, WI = BN * WK / 8;  // 1 KiB loads of a stage
   constexpr int NX = (XI + NW - 1) / NW, NWI = (WI + NW - 1) / NW;
   constexpr int CX = XI / NW, CNT = CX + WI / NW;    // loads of every wave, at least
-  // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
-  extern __shared__ v4i lds[];
   constexpr int LDS = i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>();
   float *scales = reinterpret_cast<float *>(lds + LDS / 16) - (BM + BN);  // rows, channels
   static_assert(NI == 1 || NI % 4 == 0 || NI == 2, "output tiles in pairs, or one");
@@ -621,11 +629,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   const uint32_t xbytes = (uint32_t)a.n_src * (uint32_t)a.K, wbytes = (uint32_t)a.N * (uint32_t)a.K;
   const int stages = (a.K + 128 * WK - 1) / (128 * WK);
 
-  const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
-  if (t.e < 0) return;
   const int c0 = blockIdx.x % nt * WN * cols;  // the workgroup's first column
   const int8_t *wbase = a.w + (size_t)t.e * a.N * a.K;
-  const bool once = a.stream && t.only;
   // weight row of channel row j of the tile; past the end where its column does not exist
   auto channel = [&](int j) __attribute__((always_inline)) {
     const int jt = j % TN / 16, c = c0 + j / TN * cols + i8_column<NI>(a.swiglu, jt, j % 16);
@@ -641,10 +646,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   }
   // loads l of this wave's of stage s, into buffer b: the rows' WK blocks of BM x 128 bytes, then the channels'
   auto load_x = [&](int l, int s, int b) __attribute__((always_inline)) {
-    i8_load<BM, XI, NW>(l, a.q, xbytes, vx[l], lds + b * STAGE, wave, s * 128 * WK, lc * 16, a.K, false);
+    i8_load<BM, XI, NW, false>(l, a.q, xbytes, vx[l], lds + b * STAGE, wave, s * 128 * WK, lc * 16, a.K);
   };
   auto load_w = [&](int l, int s, int b) __attribute__((always_inline)) {
-    i8_load<BN, WI, NW>(l, wbase, wbytes, vw[l], lds + b * STAGE + BM * WK * 8, wave, s * 128 * WK, lc * 16, a.K, once);
+    i8_load<BN, WI, NW, ONCE>(l, wbase, wbytes, vw[l], lds + b * STAGE + BM * WK * 8, wave, s * 128 * WK, lc * 16, a.K);
   };
   // the weights go out before the rows are known (a load and a division away)
 #pragma unroll
@@ -706,6 +711,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
         read(i, kk ^ 1, kk ? next : cur, kk ^ 1);
 #pragma unroll
         for (int j = 0; j < NI; j++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[kk][j], B[kk][i], acc[j][i], 0, 0, 0);
+        // this order, where the compiler would gather a step's LDS reads before the barrier and wait for them there
+        __builtin_amdgcn_sched_group_barrier(0x100, 1 + NI / MI, 0);  // LDS reads
+        __builtin_amdgcn_sched_group_barrier(0x008, NI, 0);           // MFMA
         // spread between the MFMAs: a wave that waits to issue a load issues nothing else
         if (kk == 1) {
 #pragma unroll
@@ -784,4 +792,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
     else if (a.out_type == MOE_GGML_F16) to((_Float16)0.0f);
     else to((bf16_t)0.0f);
   }
+}
+
+// STREAM: the weights are more than the caches hold from call to call, and tiles that alone read
+// their weights read them past the caches.  A kernel of its own: a choice at every
+// load would cut the loop into blocks that the compiler schedules one by one.
+template <int BM, int BN, int WM, int WN, int WK, int NBUF, bool STREAM>
+__global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
+  // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
+  extern __shared__ v4i lds[];
+  const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
+  if (t.e < 0) return;
+  if (STREAM && t.only) i8_multiply<BM, BN, WM, WN, WK, NBUF, true>(a, nt, t, lds);
+  else i8_multiply<BM, BN, WM, WN, WK, NBUF, false>(a, nt, t, lds);
 }
