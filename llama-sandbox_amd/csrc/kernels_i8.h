@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t abs_bits(const raw_v<T, V> &r) {
 // with the code in its low byte.  4096 rows of 7168 bf16 (88 MB) 20.0 us, 4.4 TB/s
 // (22.1 where a tie took the whole quotient again, with branches); 32764 of 768 (76 MB)
 // 17.8, two rows a wave (23.5 with one row and a third of the lanes idle); one row
-// 2.7, a launch.  Workgroups that walk rows with the next one's loads in flight took 24
+// 2.3, a launch.  Workgroups that walk rows with the next one's loads in flight took 24
 // to 29 us for the first.
 template <typename T, int LANES, int VPT>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_quantize_i8(const T *__restrict__ x, int M, int K,
