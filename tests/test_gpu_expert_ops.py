@@ -282,7 +282,10 @@ def scales(rng, shape, K):
 
 
 def check_product(got, q, s, w, ws, sw, L, dtype):
-    y = ref.product(q, s, w, ws)
+    check_against(got, ref.product(q, s, w, ws), sw, L, dtype)
+
+
+def check_against(got, y, sw, L, dtype):
     if sw:
         h, g = ref.swiglu(y, L)
         close(got, h, ref.rounded(ref.swiglu_bound(h, g), h, dtype))
@@ -388,6 +391,49 @@ def test_grouped_product_of_few_rows(blk, T, k, E, N, K, dropped, skew, out, sw,
     test_grouped_product(blk, T, k, E, N, K, dropped, skew, out, sw, gather)
 
 
+# every tile shape that the cost rule knows, at sizes that cut the last tiles
+TILES = [(130, 130, 272), (257, 514, 1040), (257, 514, 272), (257, 1794, 272), (130, 6146, 272), (130, 6146, 528), (257, 6146, 528),
+         (770, 2562, 1040), (5001, 770, 2064), (4001, 2562, 272), (4097, 1794, 2064)]
+
+
+@pytest.mark.parametrize("M, N, K", TILES)
+@pytest.mark.parametrize("out, sw", [("f32", False), ("bf16", True), ("f16", False)])
+def test_dense_product_of_every_tile(blk, M, N, K, out, sw):
+    say("dense product of every tile", M, N, K, out, sw)
+    rng = np.random.default_rng(M + N + K)
+    q, w, s, ws = (dev(t) for t in (codes(rng, (M, K)), codes(rng, (N, K)), scales(rng, M, K), scales(rng, N, K)))
+    got = torch.full((M, N // 2 if sw else N), float("nan"), dtype=TYPES[out], device=DEV)
+    blk.matmul_i8(q, s, w, ws, got, swiglu=sw, clamp=2.0)
+    check_against(got, ref.product(q, s, w, ws).cpu(), sw, 2.0, TYPES[out])
+
+
+# rows, E, N, K; the second half with weights past the caches: experts with one tile and with more
+GROUPED_TILES = [(130, 2, 1026, 272), (130, 2, 1026, 1040), (40, 40, 258, 272), (130, 130, 130, 528), (4001, 2, 258, 528),
+                 (130, 130, 130, 272), (4001, 2, 514, 1040), (4001, 2, 1026, 2064), (4001, 2, 2050, 272),
+                 (130, 130, 514, 2064), (130, 130, 130, 7184), (4001, 130, 130, 7184), (8003, 130, 130, 7184),
+                 (4001, 40, 4098, 1040), (4001, 40, 514, 7184), (4001, 40, 2050, 2064), (8003, 40, 4098, 1040)]
+
+
+@pytest.mark.parametrize("M, E, N, K", GROUPED_TILES)
+@pytest.mark.parametrize("out, sw, gather", [("f32", False, False), ("bf16", True, True)])
+def test_grouped_product_of_every_tile(blk, M, E, N, K, out, sw, gather):
+    say("grouped product of every tile", M, E, N, K, out, sw, gather)
+    rng = np.random.default_rng(M + E + N + K)
+    ids = ref.ids_of(rng, M, 1, E, 0.05, M > E)
+    offsets, perm, inv, kept = ref.grouping(ids, E)
+    g = torch.Generator(device=DEV).manual_seed(M + E)
+    w = torch.randint(-128, 128, (E, N, K), dtype=torch.int8, device=DEV, generator=g)
+    q, s, ws = dev(codes(rng, (M, K))), dev(scales(rng, M, K)), dev(scales(rng, (E, N), K))
+    got = torch.full((M, N // 2 if sw else N), 7.0, dtype=TYPES[out], device=DEV)
+    blk.matmul_i8(q, s, w, ws, got, offsets=dev(offsets), perm=dev(perm) if gather else None, swiglu=sw, clamp=2.0)
+    assert (got[kept:] == 7.0).all()
+    for e in range(E):
+        lo, hi = offsets[e], offsets[e + 1]
+        if lo < hi:
+            at = dev(perm[lo:hi].astype(np.int64)) if gather else torch.arange(lo, hi, device=DEV)
+            check_against(got[lo:hi], ref.product(q[at], s[at], w[e], ws[e]).cpu(), sw, 2.0, TYPES[out])
+
+
 def test_row_map_entries_outside_the_sources_are_zero_rows(blk):
     say("row map entries outside the sources")
     rng = np.random.default_rng(8)
@@ -415,6 +461,24 @@ def test_dense_product_through_a_row_map(blk, K, sw):
     blk.matmul_i8(dev(q), dev(s), dev(w), dev(ws), got, perm=dev(perm), k=3, swiglu=sw)
     at = torch.from_numpy(perm.astype(np.int64) // 3)
     check_product(got, q[at], s[at], w, ws, sw, 0.0, torch.float32)
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 72, 192), (12, 72, 192), (40, 200, 192), (4, 4098, 208)])
+@pytest.mark.parametrize("sw", [False, True])
+def test_dense_product_of_few_rows_through_a_row_map(blk, M, N, K, sw):
+    say("dense product of few rows through a row map", M, N, K, sw)
+    rng = np.random.default_rng(M + N)
+    S = 9
+    perm = rng.integers(0, S * 3, M).astype(np.int32)
+    q, w, s, ws = codes(rng, (S, K)), codes(rng, (N, K)), scales(rng, S, K), scales(rng, N, K)
+    at = torch.from_numpy(perm.astype(np.int64) // 3)
+    y = ref.product(q[at], s[at], w, ws)
+    if M > 1:  # a row from outside the sources
+        perm[M // 2] = S * 3
+        y[M // 2] = 0.0
+    got = torch.full((M, N // 2 if sw else N), float("nan"), device=DEV)
+    blk.matmul_i8(dev(q), dev(s), dev(w), dev(ws), got, perm=dev(perm), k=3, swiglu=sw)
+    check_against(got, y, sw, 0.0, torch.float32)
 
 
 def test_offsets_past_32_bits(blk):
