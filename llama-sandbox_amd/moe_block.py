@@ -10,6 +10,7 @@ back to ggml-cpu at that point, moe-serv/src/moe_backend.cpp:436-445).
 from __future__ import annotations
 
 import ctypes
+import functools
 import importlib.util
 import os
 
@@ -330,7 +331,7 @@ def _is_fine(t, dtype: str, shape, device: bool) -> bool:
             want = _dtypes[dtype] = getattr(torch, dtype)
         return (t.dtype is want and (shape is None or t.shape == shape) and t.is_contiguous()
                 and (not device or t.is_cuda))
-    except AttributeError:
+    except (AttributeError, ImportError):  # without torch nothing is a tensor
         return False
 
 
@@ -352,26 +353,31 @@ def check_tensor(t, name: str, dtype: str, shape=None, device: bool = True):
         raise ValueError(f"{name}: on {t.device}, expected a ROCm device tensor")
 
 
-_row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled by the first context
+_row_types: dict = {}  # torch dtype -> ggml type of a row operand, filled by the first call that takes one
 _raw_stream = _torch_calls = None
 
 
 def _know_torch():
+    """What the operators on torch tensors need of torch; nothing where it is not installed."""
     global _raw_stream, _torch_calls
     if not _row_types:
-        import torch
+        try:
+            import torch
+        except ImportError:
+            return
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
         # csrc/moe_torch.cpp, built against one torch; without it the same calls go through ctypes
         try:
             spec = importlib.util.spec_from_file_location("moe_torch", os.path.join(_HERE, "moe_torch.so"))
             calls = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(calls)
+            if calls.torch_version == torch.__version__.partition("+")[0] and _raw_stream is not None:
+                calls.set_current_stream(_raw_stream)
+                _torch_calls = calls
         except ImportError:
-            return
-        if calls.torch_version == torch.__version__.partition("+")[0] and _raw_stream is not None:
-            calls.set_current_stream(_raw_stream)
-            _torch_calls = calls
+            pass
+        # last: another thread that finds the types finds the rest too
+        _row_types.update({torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16})
 
 
 class _Entries(ctypes.Structure):
@@ -498,8 +504,6 @@ class Graph:
 class MoeBlock:
     """One device context: resident layers plus per-call scratch."""
 
-    _calls = None  # moe_torch's argument: the address of this context's library's entry points
-
     def __init__(self, device: int = 0, budget_bytes: int = 2 ** 64 - 1, lib_path: str | None = None):
         self.lib = load_library(lib_path)
         h = _vp()
@@ -508,11 +512,19 @@ class MoeBlock:
             raise MoeError(st, f"moe_ctx_create: {self.lib.moe_status_str(st).decode()}")
         self.h = h.value
         self.device = int(device)
-        _know_torch()
-        if _torch_calls is not None:
-            self._entries = _Entries(*(ctypes.cast(getattr(self.lib, n), _vp).value for n, _ in _Entries._fields_))
-            self._calls = ctypes.addressof(self._entries)
         self.descs: dict[int, LayerDesc] = {}
+
+    @functools.cached_property
+    def _calls(self):
+        """moe_torch's argument, the address of this context's library's entry points; None: calls go
+        through ctypes.  Found at the first call: a context on host arrays needs no torch."""
+        if not self.h:
+            return None
+        _know_torch()
+        if _torch_calls is None:
+            return None
+        self._entries = _Entries(*(ctypes.cast(getattr(self.lib, n), _vp).value for n, _ in _Entries._fields_))
+        return ctypes.addressof(self._entries)
 
     # -- lifecycle --------------------------------------------------------
     def close(self):
