@@ -513,8 +513,8 @@ void moe_graph_destroy(moe_graph *g);
 /* ---- profiling ----------------------------------------------------------- */
 
 /* Per-kernel GPU time, from a HIP event pair recorded on the launch stream
- * around every kernel the context launches while profiling is on (not under
- * graph capture).  The reference keeps per-split phase timings the same way
+ * around every kernel the context launches while profiling is on (not on a
+ * stream under graph capture, this library's or the caller's own).  The reference keeps per-split phase timings the same way
  * (moe-serv/src/moe_prof.h:36-137, MOESERV_PROFILE) and GPU timestamps
  * around its dispatches (moe-serv/src/moe_probe_custom.cpp:411-475). */
 typedef struct {

@@ -136,7 +136,8 @@ struct moe_ctx {
 };
 
 // HIP-event pair around one kernel launch while profiling is on (never
-// under graph capture: a captured launch is timed by its replays instead).
+// under graph capture, whoever captures: an event recorded there becomes a node
+// of the graph, and moe_prof_read could not read it).
 struct prof_scope {
   moe_ctx *c;
   int kid;
@@ -153,7 +154,13 @@ struct prof_scope {
     return e;
   }
   prof_scope(moe_ctx *ctx, int k, hipStream_t s, bool timed) : c(ctx), kid(k), st(s) {
-    if (!timed || !c->prof.on || c->capturing) return;
+    if (!timed || !c->prof.on) return;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cap) != hipSuccess) {
+      (void)hipGetLastError();  // of this question, not of the launch
+      return;
+    }
+    if (cap != hipStreamCaptureStatusNone) return;
     a = take(c->prof);
     b = a ? take(c->prof) : nullptr;
     if (a && b && hipEventRecord(a, st) != hipSuccess) {

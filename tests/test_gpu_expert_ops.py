@@ -847,3 +847,47 @@ def test_profiler_counts_the_operators(blk):
     got = blk.prof_read()
     blk.prof_enable(False)
     assert got["quantize_i8"][0] == 1
+
+
+def test_a_callers_capture_is_not_timed(blk):
+    """With the profiler on, calls that a caller captures record no events into the graph: every replay is right, and
+    the profiler still reads and counts the eager calls, and only those."""
+    say("a caller's capture with the profiler on")
+    T, k, E, H, N = 12, 2, 8, 64, 48
+    rng = np.random.default_rng(41)
+    x, ids = dev(floats(rng, (T, H), "f32")), dev(ref.ids_of(rng, T, k, E))
+    w, ws = dev(codes(rng, (N, H))), dev(scales(rng, N, H))
+    n = lambda m: torch.empty(m, dtype=torch.int32, device=DEV)  # noqa: E731
+    counts, offsets, perm, inv = n(E), n(E + 1), n(T * k), n(T * k)
+    q, s = torch.empty((T, H), dtype=torch.int8, device=DEV), torch.empty(T, device=DEV)
+    out, rows = torch.empty((T, N), device=DEV), torch.zeros((T * k, H), device=DEV)
+
+    def step():
+        blk.group(ids, E, counts, offsets, perm, inv)
+        blk.dispatch(x, inv, rows)
+        blk.quantize_i8(x, q, s)
+        blk.matmul_i8(q, s, w, ws, out)
+
+    step()
+    torch.cuda.synchronize()
+    blk.prof_enable(True)
+    try:
+        blk.prof_read(reset=True)
+        step()  # the profiler holds events of its own by now
+        names = ("group", "dispatch", "quantize_i8", "matmul_i8")
+        assert {m: c for m, (c, _) in blk.prof_read(reset=True).items()} == {m: 1 for m in names}
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        assert blk.prof_read(reset=True) == {}
+        for i in range(3):
+            x.copy_(floats(rng, (T, H), "f32"))
+            g.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in (rows, q, s, out)]
+            step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, (rows, q, s, out))), i
+        assert {m: c for m, (c, _) in blk.prof_read(reset=True).items()} == {m: 3 for m in names}
+    finally:
+        blk.prof_enable(False)
