@@ -21,8 +21,8 @@
  *    element j+16 is qs[j] >> 4; value = kvalue(nibble) * 2^(e-128) with
  *    kvalues = {0,1,2,3,4,6,8,12,-0,-1,-2,-3,-4,-6,-8,-12}
  *    (moe-serv/src/moe_tp.h:229-233, hip-moe/src/main.hip:44-57).
- *  - One context owns one GPU.  Calls on one context are not thread-safe
- *    (the reference's backend state is process-global singletons,
+ *  - One context owns one GPU.  Calls on one context are not thread-safe,
+ *    but for those that say so (the reference's backend state is process-global singletons,
  *    moe_backend.cpp:58-62, driven by one scheduler thread).
  */
 #ifndef MOE_BLOCK_H
@@ -87,6 +87,8 @@ typedef struct {
  * Replaces moe_tp_init (moe-serv/src/moe_tp.h:392-491). */
 moe_status moe_ctx_create(int device, uint64_t budget_bytes, moe_ctx **out);
 void moe_ctx_destroy(moe_ctx *ctx);
+/* The context's last message, whichever thread's call left it; the text stays until the
+ * calling thread asks again. */
 const char *moe_ctx_last_error(const moe_ctx *ctx);
 const char *moe_status_str(moe_status s);
 uint64_t moe_ctx_budget_left(const moe_ctx *ctx);
@@ -431,7 +433,9 @@ moe_status moe_route_forward(moe_ctx *ctx, int layer, const float *x_dev,
  * H <= 2^30; more tokens than a launch takes (2^24, or 2^26 pairs in
  * moe_combine_grad): MOE_ERR_UNSUPPORTED.  These calls, and the 8-bit ones
  * below, allocate nothing and share no scratch: they may overlap on several
- * streams and be captured, and leave the caller's current device as it was. */
+ * streams, be captured, and be made by several threads at once (with each other and
+ * with moe_prof_read and moe_ctx_last_error; not with the rest of the context's
+ * calls), and they leave the caller's current device as it was. */
 
 /* rows[inv[t*k+s]] = x[t].  x [T][H], rows [n_rows][H]; rows that no pair
  * names are left as they were.  (ggml's mul_mat_id gathers the same rows on

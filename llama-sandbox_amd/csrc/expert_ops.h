@@ -2,9 +2,10 @@
 // gradients, rows quantised to 8 bits and 8-bit products (host code, included
 // by moe_block.hip after what it uses).
 //
-// Nothing here allocates, keeps state or synchronises: a call is one launch
-// on the caller's stream, so calls may overlap on several streams, threads
-// and captured graphs as long as their buffers do not.
+// Nothing here allocates device memory, keeps a call's data or synchronises: a call
+// is one launch on the caller's stream, so calls may overlap on several streams,
+// threads and captured graphs as long as their buffers do not.  What they
+// change in the context, its last message and the profiler's lists, is under moe_ctx::mu.
 #pragma once
 
 // The context's device for one call; the caller's current device afterwards.

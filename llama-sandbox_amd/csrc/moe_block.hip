@@ -21,6 +21,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <chrono>
 #include <cstdarg>
 #include <cstdio>
@@ -31,6 +32,7 @@
 #include <mutex>
 #include <set>
 #include <string>
+#include <thread>
 #include <vector>
 
 namespace {
@@ -88,8 +90,9 @@ static const char *const kernel_names[K_COUNT] = {
     "route", "group", "gate_up_decode", "down_decode", "gate_up_grouped",
     "down_grouped", "combine", "dispatch", "combine_rows", "combine_grad", "quantize_i8", "matmul_i8"};
 
+// What calls of several threads share (moe_ctx::mu guards it).
 struct prof_state {
-  bool on = false;
+  std::atomic<bool> on{false};
   struct rec { int kid; hipEvent_t a, b; };
   std::vector<hipEvent_t> pool;  // idle events
   std::vector<rec> pending;      // recorded, not yet read
@@ -112,7 +115,10 @@ struct moe_ctx {
   uint64_t budget = 0, used = 0;
   std::map<int, dev_layer> layers;
   work_bufs sc;
+  // err, err_read and prof's lists: all that the operators of expert_ops.h change in a context
+  mutable std::mutex mu;
   std::string err;
+  mutable std::map<std::thread::id, std::string> err_read;  // what moe_ctx_last_error gave each thread
   int inject = 0;  // bit 0: forward fails, bit 1: budget forced to 0
   bool capturing = false;
   bool taps = false;  // keep the SwiGLU output h in sc.htap (moe_debug_set_taps)
@@ -143,15 +149,24 @@ struct prof_scope {
   int kid;
   hipStream_t st;
   hipEvent_t a = nullptr, b = nullptr;
-  static hipEvent_t take(prof_state &p) {
-    hipEvent_t e = nullptr;
-    if (!p.pool.empty()) {
-      e = p.pool.back();
-      p.pool.pop_back();
-    } else if (hipEventCreateWithFlags(&e, hipEventDisableSystemFence) != hipSuccess) {  // timing only: no cache flush
-      e = nullptr;
+  static hipEvent_t take(moe_ctx *c) {
+    {
+      std::lock_guard<std::mutex> lk(c->mu);
+      if (!c->prof.pool.empty()) {
+        const hipEvent_t e = c->prof.pool.back();
+        c->prof.pool.pop_back();
+        return e;
+      }
     }
+    hipEvent_t e = nullptr;
+    if (hipEventCreateWithFlags(&e, hipEventDisableSystemFence) != hipSuccess) e = nullptr;  // timing only: no cache flush
     return e;
+  }
+  void put_back() {
+    std::lock_guard<std::mutex> lk(c->mu);
+    if (a) c->prof.pool.push_back(a);
+    if (b) c->prof.pool.push_back(b);
+    a = b = nullptr;
   }
   prof_scope(moe_ctx *ctx, int k, hipStream_t s, bool timed) : c(ctx), kid(k), st(s) {
     if (!timed || !c->prof.on) return;
@@ -161,24 +176,17 @@ struct prof_scope {
       return;
     }
     if (cap != hipStreamCaptureStatusNone) return;
-    a = take(c->prof);
-    b = a ? take(c->prof) : nullptr;
-    if (a && b && hipEventRecord(a, st) != hipSuccess) {
-      c->prof.pool.push_back(a);
-      c->prof.pool.push_back(b);
-      a = b = nullptr;
-    } else if (a && !b) {
-      c->prof.pool.push_back(a);
-      a = nullptr;
-    }
+    a = take(c);
+    b = a ? take(c) : nullptr;
+    if (!b || hipEventRecord(a, st) != hipSuccess) put_back();
   }
   ~prof_scope() {
     if (!a) return;
     if (hipEventRecord(b, st) == hipSuccess) {
+      std::lock_guard<std::mutex> lk(c->mu);
       c->prof.pending.push_back({kid, a, b});
     } else {
-      c->prof.pool.push_back(a);
-      c->prof.pool.push_back(b);
+      put_back();
     }
   }
 };
@@ -214,6 +222,7 @@ static moe_status fail(moe_ctx *c, moe_status s, const char *fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
+    std::lock_guard<std::mutex> lk(c->mu);
     c->err = buf;
   }
   return s;
@@ -443,7 +452,13 @@ extern "C" void moe_ctx_destroy(moe_ctx *c) {
   delete c;
 }
 
-extern "C" const char *moe_ctx_last_error(const moe_ctx *c) { return c ? c->err.c_str() : ""; }
+extern "C" const char *moe_ctx_last_error(const moe_ctx *c) {
+  if (!c) return "";
+  std::lock_guard<std::mutex> lk(c->mu);
+  std::string &mine = c->err_read[std::this_thread::get_id()];  // no other thread's error moves it
+  mine = c->err;
+  return mine.c_str();
+}
 
 extern "C" const char *moe_status_str(moe_status s) {
   switch (s) {
@@ -1227,18 +1242,31 @@ extern "C" moe_status moe_prof_read(moe_ctx *c, moe_kernel_stat *stats, int cap,
   HIPC(c, hipSetDevice(c->device));
   prof_state &p = c->prof;
   moe_status st = MOE_OK;
-  for (auto &r : p.pending) {
+  std::vector<prof_state::rec> recs;
+  {
+    std::lock_guard<std::mutex> lk(c->mu);
+    recs.swap(p.pending);
+  }
+  uint64_t launches[K_COUNT] = {};
+  double total_us[K_COUNT] = {};
+  for (auto &r : recs) {  // waited for without the lock: launches of other threads go on
     float ms = 0.0f;
     if (st == MOE_OK && (hipEventSynchronize(r.b) != hipSuccess || hipEventElapsedTime(&ms, r.a, r.b) != hipSuccess))
       st = fail(c, MOE_ERR_HIP, "moe_prof_read: event query failed");
     if (st == MOE_OK) {
-      p.launches[r.kid] += 1;
-      p.total_us[r.kid] += 1000.0 * (double)ms;
+      launches[r.kid] += 1;
+      total_us[r.kid] += 1000.0 * (double)ms;
     }
+  }
+  std::lock_guard<std::mutex> lk(c->mu);
+  for (auto &r : recs) {
     p.pool.push_back(r.a);
     p.pool.push_back(r.b);
   }
-  p.pending.clear();
+  for (int k = 0; k < K_COUNT; k++) {
+    p.launches[k] += launches[k];
+    p.total_us[k] += total_us[k];
+  }
   int m = 0;
   for (int k = 0; k < K_COUNT; k++) {
     if (!p.launches[k]) continue;

@@ -2,6 +2,7 @@
 the GPU, against 64-bit statements of them (expert_ref.py) with the error
 bounds that f32 sums and the output's rounding allow."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -891,3 +892,55 @@ def test_a_callers_capture_is_not_timed(blk):
         assert {m: c for m, (c, _) in blk.prof_read(reset=True).items()} == {m: 3 for m in names}
     finally:
         blk.prof_enable(False)
+
+
+def test_two_threads_on_one_context(blk):
+    """Each on a stream of its own, with the profiler on, good calls between refused ones: every result is right,
+    every refusal has one of the messages whole, and every launch is counted once."""
+    say("two threads on one context")
+    rng = np.random.default_rng(42)
+    M, N, K, n, wrong = 24, 80, 208, 150, []
+    w, ws = codes(rng, (N, K)), scales(rng, N, K)
+    wd, wsd = dev(w), dev(ws)
+    sets = [(codes(rng, (M, K)), scales(rng, M, K)) for _ in range(2)]
+    put = [(dev(a), dev(b)) for a, b in sets]
+    outs = [torch.zeros((n, M, N), device=DEV) for _ in range(2)]
+    x = torch.zeros((4, 32), device=DEV)
+    inv, clash = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros((4, 32), device=DEV)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    go = threading.Barrier(2)
+
+    def work(i):
+        try:
+            st = streams[i].cuda_stream
+            go.wait(60)
+            for j in range(n):
+                blk.matmul_i8(*put[i], wd, wsd, outs[i][j], stream=st)
+                with pytest.raises(mb.MoeError, match="moe_dispatch: rows overlaps another buffer|"
+                                                      "moe_quantize_i8: an output overlaps another buffer"):
+                    if i:
+                        blk.dispatch(x, inv, x, stream=st)
+                    else:
+                        blk.quantize_i8(clash, clash.view(-1)[:32].view(torch.int8).view(4, 32), ws4, stream=st)
+        except BaseException as e:  # noqa: BLE001 -- a thread's failure is the test's
+            wrong.append(e)
+
+    ws4 = torch.zeros(4, device=DEV)
+    blk.prof_enable(True)
+    try:
+        blk.prof_read(reset=True)
+        both = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in both:
+            t.start()
+        for t in both:
+            t.join()
+        torch.cuda.synchronize()
+        stats = blk.prof_read(reset=True)
+    finally:
+        blk.prof_enable(False)
+    assert not wrong, wrong
+    assert {m: c for m, (c, _) in stats.items()} == {"matmul_i8": 2 * n}
+    for (a, b), o in zip(sets, outs):
+        assert (o == o[:1]).all()
+        check_product(o[0], a, b, w, ws, False, 0.0, torch.float32)
