@@ -430,8 +430,8 @@ moe_status moe_route_forward(moe_ctx *ctx, int layer, const float *x_dev,
  * any H; buffers must not overlap.  Sums are f32, in slot order; a result is
  * rounded once, to its type.  An entry of inv outside [0, n_rows) is taken as
  * dropped.  A valid inv names no row twice (moe_group's does not).  k <= 64,
- * H <= 2^30; more tokens than a launch takes (2^24, or 2^26 pairs in
- * moe_combine_grad): MOE_ERR_UNSUPPORTED.  These calls, and the 8-bit ones
+ * H <= 2^30; T < 2^24, and T*k <= 2^26 - 8 in place of it in moe_combine_grad,
+ * else MOE_ERR_UNSUPPORTED.  These calls, and the 8-bit ones
  * below, allocate nothing and share no scratch: they may overlap on several
  * streams, be captured, and be made by several threads at once (with each other and
  * with moe_prof_read and moe_ctx_last_error; not with the rest of the context's
@@ -462,7 +462,8 @@ moe_status moe_combine_grad(moe_ctx *ctx, const void *dout_dev, int dout_type, c
  * scale[r] to the nearest whole number, ties to even, in [-127, 127]; a row
  * of zeros, or whose scale rounds to 0, has codes 0.  A row with a NaN or an
  * infinity has a NaN scale and codes 0, so that every product of it is NaN.
- * Any K and alignment, M < 2^22.  Also how weights are quantised, a scale for
+ * Any K <= 2^30 and alignment; M < 2^24, from K = 8193 on M < 2^22, else
+ * MOE_ERR_UNSUPPORTED.  Also how weights are quantised, a scale for
  * each channel. */
 moe_status moe_quantize_i8(moe_ctx *ctx, const void *x_dev, int x_type, int M, int K, int8_t *q_dev, float *scale_dev,
                            void *stream);
@@ -480,8 +481,8 @@ moe_status moe_quantize_i8(moe_ctx *ctx, const void *x_dev, int x_type, int M, i
  * on are left as they were.  perm NULL: src(r) = r, k = 1; else
  * src(r) = perm[r] / k (moe_group's perm: the row's token), and a row whose
  * perm is outside [0, n_src*k) is computed from zeros.
- * The sum is exact in 32 bits: K <= 131071, else MOE_ERR_UNSUPPORTED (as are
- * more rows than a launch takes: 2^22).  Any N, K and alignment; the fast path
+ * The sum is exact in 32 bits: K <= 131071, else MOE_ERR_UNSUPPORTED; so are
+ * M >= 2^30 rows.  Any N <= 2^30 - 64, K and alignment; the fast path
  * takes K % 16 == 0, 16-byte aligned q and w, and q and each w[e] below 4 GiB. */
 moe_status moe_matmul_i8(moe_ctx *ctx, const int8_t *q_dev, const float *q_scale_dev, int n_src, const int8_t *w_dev,
                          const float *w_scale_dev, int E, const int32_t *offsets_dev, const int32_t *perm_dev, int k,

@@ -6,7 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#define MOE_I8_MAX_K 131071  // K * 128 * 128 < 2^31: sums are exact in int32
+#define MOE_I8_MAX_K 131071          // K * 128 * 128 < 2^31: sums are exact in int32
+#define MOE_I8_MAX_M ((1 << 30) - 1) // rows of a product: a tile's first row and last stay in 32 bits
 
 // One call of moe_matmul_i8.  Grouped: offsets [E+1] cut the M rows by expert;
 // perm: row r's codes are those of source row perm[r] / k (NULL: row r itself).

@@ -202,13 +202,13 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
 // 128x128 stands twice: 3 stages for one workgroup a CU, 2 for two.  Eight waves a
 // workgroup in all but the smallest: with 4 the same tiles took up to a third longer.
 struct i8_shape {
-  int BM, BN, lds;
+  int BM, BN, threads, lds;
   float call, tile, k, k_share;
   i8_launch launch;
 };
 template <int BM, int BN, int WM, int WN, int WK, int NBUF>
 static constexpr i8_shape shape_of(float call, float tile, float k, float k_share) {
-  return {BM, BN, i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
+  return {BM, BN, 64 * WM * WN * WK, i8_lds_bytes<BM, BN, WM, WN, WK, NBUF>(), call, tile, k, k_share, launch_tiles<BM, BN, WM, WN, WK, NBUF>};
 }
 static const i8_shape i8_shapes[] = {
     shape_of<16, 16, 1, 1, 4, 4>(2.11f, 1.81f, 0.031f, 0.039f),
@@ -224,12 +224,15 @@ static const i8_shape i8_shapes[] = {
     shape_of<256, 256, 2, 4, 1, 2>(0.0f, 5.95f, 1.544f, 0.0f),
 };
 
-static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
+// The launch of the least cost, of the shapes whose tiles a grid takes (NULL: none; the largest
+// take every product whose output fits the memory).
+static i8_launch choose_shape(const i8_mm &a, int n_cu) {
   const i8_shape *best = nullptr;
   float least = 0.0f;
   // experts: as many as can have rows, of the same number each
   const float matrices = a.offsets ? (float)(a.M < a.E ? a.M : a.E) : 1.0f, rows = a.M / matrices;
   for (const i8_shape &s : i8_shapes) {
+    if (!fits(i8_tiles(a, s.BM) * ceil_div(a.N, s.BN), s.threads)) continue;
     const float row_tiles = !a.offsets ? (float)ceil_div(a.M, s.BM) : rows <= s.BM ? 1.0f : rows / s.BM + 0.5f;
     const float tiles = matrices * row_tiles * (float)ceil_div(a.N, s.BN);
     const int fit = (160 << 10) / s.lds, occ = fit < 4 ? fit : 4;
@@ -241,8 +244,10 @@ static const i8_shape &choose_shape(const i8_mm &a, int n_cu) {
       least = cost;
     }
   }
-  return *best;
+  return best ? best->launch : nullptr;
 }
+
+static constexpr long MOE_GRID_Y = 65535;  // most blocks along a grid's y and z dimensions
 
 bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
   i8_mm a = args;
@@ -253,12 +258,13 @@ bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
     // weights of more than the caches hold from call to call, each read by one tile: past the caches.  Measured:
     // 939 MB against 16 rows 164 us with plain loads, 146 without (5.75 and 6.5 TB/s)
     a.stream = (size_t)a.N * a.K * (a.M < a.E ? a.M : a.E) > MOE_STREAM_BYTES;
-    const i8_launch few = few_rows(a);
-    return (few ? few : choose_shape(a, n_cu).launch)(a, st);
+    const i8_launch few = few_rows(a), launch = few ? few : choose_shape(a, n_cu);
+    return launch && launch(a, st);
   }
   const int nt = a.swiglu ? ceil_div(a.N / 2, 32) : ceil_div(a.N, 64);
-  const long mt = i8_tiles(a, 64);
-  if (mt > 65535 || !fits(nt, 256)) return false;
-  hipLaunchKernelGGL(k_mm_i8_any, dim3(nt, (unsigned)mt), dim3(256), 0, st, a);
+  if (!fits(nt, 256)) return false;
+  // tiles of rows along y, and along z as often as they do not fit there
+  const long mt = i8_tiles(a, 64), y = mt < MOE_GRID_Y ? mt : MOE_GRID_Y;
+  hipLaunchKernelGGL(k_mm_i8_any, dim3(nt, (unsigned)y, (unsigned)ceil_div(mt, y)), dim3(256), 0, st, a);
   return true;
 }

@@ -158,13 +158,14 @@ extern "C" moe_status moe_matmul_i8(moe_ctx *c, const int8_t *q, const float *q_
   if (K > MOE_I8_MAX_K)
     return fail(c, MOE_ERR_UNSUPPORTED, "moe_matmul_i8: K = %d: sums of more than %d products can pass 32 bits", K,
                 MOE_I8_MAX_K);
+  if (M > MOE_I8_MAX_M) return fail(c, MOE_ERR_UNSUPPORTED, "moe_matmul_i8: M = %d rows, at most %d", M, MOE_I8_MAX_M);
   const i8_mm a = {q, q_scale, w, w_scale, offsets, perm, out, n_src, E, k, M, N, K, swiglu, out_type, clamp};
   device_scope ds(c->device);
   HIPC(c, ds.err);
   {
     prof_scope ps(c, K_MM_I8, (hipStream_t)stream, true);
     if (!launch_matmul_i8(a, c->n_cu, (hipStream_t)stream))
-      return fail(c, MOE_ERR_UNSUPPORTED, "moe_matmul_i8: M = %d rows", M);
+      return fail(c, MOE_ERR_UNSUPPORTED, "moe_matmul_i8: M = %d rows of N = %d channels", M, N);
   }
   HIPC(c, hipGetLastError());
   return MOE_OK;

@@ -944,3 +944,48 @@ def test_two_threads_on_one_context(blk):
     for (a, b), o in zip(sets, outs):
         assert (o == o[:1]).all()
         check_product(o[0], a, b, w, ws, False, 0.0, torch.float32)
+
+
+def whole_numbers(rng, shape, m):
+    return torch.from_numpy(rng.integers(-m, m + 1, shape, dtype=np.int64).astype(np.int8))
+
+
+@pytest.mark.parametrize("E", [0, 1024])
+@pytest.mark.parametrize("K", [3, 16])
+@pytest.mark.parametrize("M", [65535 * 64 + 1, 2 ** 22 + 65])
+def test_rows_past_one_dimension_of_a_grid(blk, M, K, E):
+    """More tiles of rows than one grid dimension may hold, by either path: dense, and of 1024 experts.  Scales of 1
+    and sums below 2^24: the products are exact."""
+    say("rows past one dimension of a grid", M, K, E)
+    rng = np.random.default_rng(M + K + E)
+    N = 2
+    q, w = dev(whole_numbers(rng, (M, K), 127)), dev(whole_numbers(rng, (max(E, 1), N, K), 127))
+    one, ones = torch.ones(M, device=DEV), torch.ones((max(E, 1), N), device=DEV)
+    got = torch.full((M + 1, N), 7.0, device=DEV)
+    if E:
+        cuts = np.sort(rng.integers(0, M + 1, E - 1))
+        offsets = dev(np.concatenate([[0], cuts, [M]]).astype(np.int32))
+        blk.matmul_i8(q, one, w, ones, got[:M], offsets=offsets)
+        e = torch.searchsorted(offsets[1:].long(), torch.arange(M, device=DEV), right=True)
+    else:
+        blk.matmul_i8(q, one, w[0], ones[0], got[:M])
+        e = torch.zeros(M, dtype=torch.int64, device=DEV)
+    want = torch.stack([(q.int() * w[:, n].int()[e]).sum(1) for n in range(N)], 1)
+    assert torch.equal(got[:M], want.float()) and (got[M:] == 7.0).all()
+
+
+@pytest.mark.parametrize("K", [5, 16])
+def test_the_most_rows_of_a_product(blk, K):
+    """2^30 - 1 rows of few sources through a row map, by either path (one more is refused, test_refusals_of_the_library)."""
+    say("the most rows of a product", K)
+    rng = np.random.default_rng(K)
+    M, S, N = 2 ** 30 - 1, 61, 1
+    q, w = whole_numbers(rng, (S, K), 8), whole_numbers(rng, (N, K), 1)
+    perm = torch.arange(M, dtype=torch.int32, device=DEV).remainder_(S)
+    got = torch.zeros((M, N), dtype=torch.bfloat16, device=DEV)
+    blk.matmul_i8(dev(q), torch.ones(S, device=DEV), dev(w), torch.ones(N, device=DEV), got, perm=perm)
+    want = dev((q.int() * w.int()).sum(1).to(torch.bfloat16))  # at most 128: exact
+    whole = M // S * S
+    assert (got[:whole, 0].view(-1, S) == want).all() and torch.equal(got[whole:, 0], want[:M - whole])
+    del got, perm
+    torch.cuda.empty_cache()
