@@ -989,3 +989,127 @@ def test_the_most_rows_of_a_product(blk, K):
     assert (got[:whole, 0].view(-1, S) == want).all() and torch.equal(got[whole:, 0], want[:M - whole])
     del got, perm
     torch.cuda.empty_cache()
+
+
+# ---- buffers past the caches -----------------------------------------------------------
+
+STREAM_BYTES = 96 << 20  # what is moved past the caches from here on (MOE_STREAM_BYTES)
+
+
+def close_here(got, want, bound):
+    """close(), on the device."""
+    off = (got.double() - want).abs()
+    assert torch.isfinite(got).all() and (off <= bound).all(), f"off by {(off / bound.clamp(min=1e-300)).max().item():.3g} of the bound"
+
+
+def setup_here(T, k, H, dropped, seed):
+    """setup(), with the map on the device too: [T, k] rows, and which pairs have one."""
+    rng, ids, E, inv, kept = setup(T, k, H, dropped, seed)
+    at = dev(inv.astype(np.int64)).view(T, k)
+    return rng, dev(inv), at, at >= 0, kept
+
+
+def floats_here(g, shape, kind):
+    return torch.randn(shape, generator=g, device=DEV).to(TYPES[kind])
+
+
+# tokens, slots (up to 8 of them in flight, and more), type read, type written, dropped
+PAST = [(1500, 8, "f32", "f32", 0.2), (1501, 8, "bf16", "bf16", 0.0), (401, 17, "f32", "f16", 0.3), (400, 17, "bf16", "f32", 0.1),
+        (9000, 1, "f16", "f16", 0.0), (5003, 3, "f16", "bf16", 0.25), (36, 9, "bf16", "bf16", 0.2)]
+
+
+def odd_width(pairs, kind, part=1):
+    """The smallest odd H with which so many rows pass STREAM_BYTES / part."""
+    size = 4 if kind == "f32" else 2
+    return (STREAM_BYTES // part // (pairs * size) + 1) | 1
+
+
+@pytest.mark.parametrize("T, k, a, b, dropped", PAST)
+def test_dispatch_past_the_caches(blk, T, k, a, b, dropped):
+    H = odd_width(T * k, b)
+    say("dispatch past the caches", T, k, H, a, b, dropped)
+    rng, inv, at, there, kept = setup_here(T, k, H, dropped, T + k)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = floats_here(g, (T, H), a)
+    got = torch.full((T * k + 1, H), 7.0, dtype=TYPES[b], device=DEV)
+    blk.dispatch(x, inv, got)
+    want = torch.full_like(got, 7.0)
+    t, s = torch.nonzero(there, as_tuple=True)
+    want[at[t, s]] = x[t].to(TYPES[b])
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T, k, a, b, dropped", PAST)
+def test_combine_and_dispatch_grad_past_the_caches(blk, T, k, a, b, dropped):
+    H = odd_width(T * k, a)
+    say("combine past the caches", T, k, H, a, b, dropped)
+    rng, inv, at, there, kept = setup_here(T, k, H, dropped, 2 * T + k)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    rows, wts = floats_here(g, (kept, H), a), floats_here(g, (T, k), "f32")
+    for w in (wts, None):
+        out = torch.full((T, H), float("nan"), dtype=TYPES[b], device=DEV)
+        if w is None:
+            blk.dispatch_grad(rows, inv, out)
+        else:
+            blk.combine(rows, w, inv, out)
+        want = torch.zeros((T, H), dtype=torch.float64, device=DEV)
+        mag = torch.zeros_like(want)
+        for s in range(k):
+            t = torch.nonzero(there[:, s]).view(-1)
+            y = rows[at[t, s]].double() * (1.0 if w is None else w[t, s, None].double())
+            want[t] += y
+            mag[t] += y.abs()
+        close_here(out, want, ref.rounded((k + 1) * U * mag, want, TYPES[b]))  # as test_combine_and_dispatch_grad
+
+
+@pytest.mark.parametrize("T, k, a, b, dropped", PAST)
+def test_combine_grad_past_the_caches(blk, T, k, a, b, dropped):
+    H = odd_width(T * k, b, 2)
+    say("combine_grad past the caches", T, k, H, a, b, dropped)
+    rng, inv, at, there, kept = setup_here(T, k, H, dropped, 3 * T + k)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    R = kept + 1
+    dout, rows, wts = floats_here(g, (T, H), a), floats_here(g, (R, H), b), floats_here(g, (T, k), "f32")
+    drows = torch.full((R, H), 7.0, dtype=TYPES[b], device=DEV)
+    dwts = torch.full((T, k), float("nan"), device=DEV)
+    blk.combine_grad(dout, rows, wts, inv, drows, dwts)
+    want = torch.full((R, H), 7.0, dtype=torch.float64, device=DEV)
+    dw, mag = (torch.zeros((T, k), dtype=torch.float64, device=DEV) for _ in range(2))
+    for s in range(k):
+        t = torch.nonzero(there[:, s]).view(-1)
+        want[at[t, s]] = dout[t].double() * wts[t, s, None].double()
+        prod = dout[t].double() * rows[at[t, s]].double()
+        dw[t, s], mag[t, s] = prod.sum(1), prod.abs().sum(1)
+    close_here(drows, want, ref.rounded(U * want.abs(), want, TYPES[b]))
+    close_here(dwts, dw, (H / 64 + 8 + 9) * U * mag + 1e-40)  # as test_combine_grad
+
+
+# rows, N, K: weights past the caches against few rows and many, on every tile shape that the cost rule takes for them
+WIDE = [(16, 65538, 7184), (16, 12290, 8208), (16, 24578, 4112), (65, 12290, 8208), (65, 24578, 4112), (65, 65538, 2064),
+        (65, 102402, 1040), (130, 102402, 1040), (130, 12290, 8208), (130, 24578, 4112), (130, 65538, 2064),
+        (257, 102402, 1040), (770, 12290, 8208), (4001, 12290, 8208)]
+
+
+@pytest.mark.parametrize("M, N, K", WIDE)
+@pytest.mark.parametrize("out, sw", [("f32", False), ("bf16", True)])
+def test_dense_product_with_weights_past_the_caches(blk, M, N, K, out, sw):
+    say("dense product with weights past the caches", M, N, K, out, sw)
+    rng = np.random.default_rng(M + N + K)
+    g = torch.Generator(device=DEV).manual_seed(M + N)
+    q, w = (torch.randint(-128, 128, s, dtype=torch.int8, device=DEV, generator=g) for s in ((M, K), (N, K)))
+    s, ws = dev(scales(rng, M, K)), dev(scales(rng, N, K))
+    got = torch.full((M, N // 2 if sw else N), float("nan"), dtype=TYPES[out], device=DEV)
+    blk.matmul_i8(q, s, w, ws, got, swiglu=sw, clamp=2.0)
+    y = ref.product(q, s, w, ws)
+    if sw:
+        h, gate = ref.swiglu(y, 2.0)
+        close_here(got, h, ref.rounded(ref.swiglu_bound(h, gate), h, TYPES[out]))
+    else:
+        close_here(got, y, ref.rounded(ref.product_bound(y), y, TYPES[out]))
+
+
+# rows, E, N, K: the shapes that GROUPED_TILES leaves out
+@pytest.mark.parametrize("M, E, N, K", [(16001, 16, 258, 2064), (130, 3, 2050, 16400), (16001, 130, 130, 7184), (4001, 16, 8194, 1040)])
+@pytest.mark.parametrize("out, sw, gather", [("f32", False, False), ("bf16", True, True)])
+def test_grouped_product_of_the_other_tiles(blk, M, E, N, K, out, sw, gather):
+    test_grouped_product_of_every_tile(blk, M, E, N, K, out, sw, gather)
