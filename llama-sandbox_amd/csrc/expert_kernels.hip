@@ -161,10 +161,21 @@ static bool launch_few(const i8_mm &a, hipStream_t st) {
 //                            51.5    37.4    37.4    52.5    42.8
 //                            98.7    70.4    69.6    98.4    75.5
 // Grouped rows are taken one a tile, up to 16 of them: an expert's weights are then read
-// as often as it has rows (128 rows of 16 tokens, Zipf, 7168 x 4096: 280 us against 165 staged).
+// as often as it has rows (128 rows of 16 tokens, Zipf, 7168 x 4096: 280 us against 165 staged).  So
+// where an expert has 2 rows or more on average, only matrices that the second read finds in L2, and
+// up to 4 rows.  us, one a tile / staged, random experts, weights from HBM where they are more than the caches hold:
+//   rows, experts:       16, 1       16, 2       16, 4        16, 8        16, 12       16, 16       4, 2
+//   7168 x 7168      88.5 / 13.6  90.0 / 19.9  95.1 / 34.1  98.2 / 57.1  101.7 / 79.1  104 / 82  27.2 / 19.8
+//   7168 x 2048           -       13.5 / 7.7   20.0 / 13.7  20.2 / 19.6   24.0 / 30.9  26.2 / 31.5  7.2 / 7.7
+//   2048 x 4096           -       10.0 / 6.4   11.0 / 9.2   14.0 / 12.7   15.4 / 16.3  16.8 / 18.5  5.9 / 6.5
+//   1024 x 4096           -        6.8 / 5.0    7.1 / 6.7    7.8 / 7.8     9.5 / 10.8   9.7 / 11.1  4.7 / 5.1
+//   7168 x 512            -        5.5 / 6.1    5.9 / 6.3    6.7 / 7.1     8.3 / 10.0   8.8 / 10.8  4.7 / 6.1
 static i8_launch few_rows(const i8_mm &a) {
   if (a.N > 1 << 22) return nullptr;
-  if (a.offsets) return a.M > 16 ? nullptr : a.K <= 1024 ? launch_few<1, 8, 1> : launch_few<1, 4, 2>;
+  if (a.offsets) {
+    const bool again = a.M >= 2 * a.E && (a.M > 4 * a.E || (size_t)a.N * a.K > (size_t)4 << 20);
+    return a.M > 16 || again ? nullptr : a.K <= 1024 ? launch_few<1, 8, 1> : launch_few<1, 4, 2>;
+  }
   const long n = (long)a.M * a.N;
   if (a.M == 1 || n <= 4096) return launch_few<1, 2, 4>;
   if (a.M == 2 || n <= 8192) return launch_few<2, 4, 2>;

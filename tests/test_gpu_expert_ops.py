@@ -1113,3 +1113,45 @@ def test_dense_product_with_weights_past_the_caches(blk, M, N, K, out, sw):
 @pytest.mark.parametrize("out, sw, gather", [("f32", False, False), ("bf16", True, True)])
 def test_grouped_product_of_the_other_tiles(blk, M, E, N, K, out, sw, gather):
     test_grouped_product_of_every_tile(blk, M, E, N, K, out, sw, gather)
+
+
+def microseconds(call, n=20):
+    for _ in range(5):
+        call()
+    best = []
+    for _ in range(5):
+        a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(n):
+            call()
+        z.record()
+        z.synchronize()
+        best.append(a.elapsed_time(z) * 1000 / n)
+    return sorted(best)[2]
+
+
+@pytest.mark.parametrize("M", [2, 8, 16])
+def test_rows_of_one_expert_are_the_dense_product(blk, M):
+    """The same bits, and about its time (1 to 1.1 times it): the expert's weights are not read again for every row,
+    which takes 8 times as long for 16 of them."""
+    say("rows of one expert", M)
+    rng = np.random.default_rng(M)
+    g = torch.Generator(device=DEV).manual_seed(M)
+    K = N = 7168
+    w = torch.randint(-128, 128, (1, N, K), dtype=torch.int8, device=DEV, generator=g)
+    q, s, ws = dev(codes(rng, (M, K))), dev(scales(rng, M, K)), dev(scales(rng, (1, N), K))
+    offsets = dev(np.array([0, M], np.int32))
+    dense, grouped = (torch.full((M, N), float("nan"), device=DEV) for _ in range(2))
+    t_dense = microseconds(lambda: blk.matmul_i8(q, s, w[0], ws[0], dense))
+    t_grouped = microseconds(lambda: blk.matmul_i8(q, s, w, ws, grouped, offsets=offsets))
+    say(f"dense {t_dense:.1f} us, grouped {t_grouped:.1f} us")
+    assert torch.equal(dense, grouped)
+    assert t_grouped <= 2 * t_dense
+
+
+# T, k, E, N, K: experts with one row each and with several, matrices on both sides of the limit of 4 MiB
+@pytest.mark.parametrize("T, k, E, N, K", [(16, 1, 4, 258, 768), (8, 2, 4, 130, 1040), (8, 1, 4, 34, 2064), (2, 1, 1, 66, 528),
+                                           (4, 1, 2, 4098, 1040), (16, 1, 5, 130, 1024), (16, 1, 3, 2050, 2064), (16, 1, 9, 2050, 2064)])
+@pytest.mark.parametrize("out, sw, gather", [("f32", False, False), ("bf16", True, True)])
+def test_grouped_product_of_few_rows_and_experts(blk, T, k, E, N, K, out, sw, gather):
+    test_grouped_product(blk, T, k, E, N, K, 0.0, False, out, sw, gather)
