@@ -197,20 +197,21 @@ static bool launch_tiles(const i8_mm &a, hipStream_t st) {
 // on a CU takes about
 //   call + rounds * (tile + K / 128 * (k + k_share * tiles that share the CU))  us,
 // fitted to 83 dense products of 1 to 8192 rows, K and N from 640 to 7168, on each of
-// 25 shapes.  The shape of the least cost is on average 0.6% slower than the
-// fastest of the 25 there (at most 12%), and 2.8% (24%) over 72 grouped calls of 4 to
-// 32764 rows, where the rows of each expert are not known here.
-//   rows x 7168 x 7168, us:  16x16  32x32  64x32  64x64  128x64  64x128  128x128  256x128  256x256
-//                      16:    15.7   14.0   15.8   18.7    22.5    29.2     31.4     41.9     83
-//                      64:    35.9   23.6   17.0   21.8    23.6    31.6     33.5     45.1     87
-//                     256:     118     71     49   38.3    27.3    31.9     37.3     52.9     99
-//                     512:     231    136     84   64.2    51.3    40.7     37.2     51.7     96
-//                    1024:     453    265    162    121      93      82       71     55.9     98
-//                    4096:    1788   1036    619    461     331     283      247      215    199
-// (measured before the present order of LDS reads: 256x256 now takes 187 at 4096 rows, 76
-// at 1024; the smaller tiles gained little).  A last round that is partly filled costs less than
+// 25 shapes, before the present order of LDS reads: then the shape of the least cost was on average 0.6% slower
+// than the fastest of the 25 (at most 12%), and 2.8% (24%) over 72 grouped calls of 4 to
+// 32764 rows, where the rows of each expert are not known here.  It serves to choose, not to predict: with
+// weights from HBM a call takes 10 to 35% more than it says (256x256 less).  The present kernels, weights from
+// HBM, the chosen one marked (its bracket: the weights of the call before, from the cache):
+//   rows x 7168 x 7168, us:  16x16  32x32  64x32  64x64  128x64  64x128  128x128  128x256  256x128  256x256
+//                      16:   13.5*   12.8   13.6   18.0    20.8    28.9     30.3     43.9     41.8     75.0  (10.8)
+//                      64:    33.4   22.2   16.6*  21.7    22.3    31.7     32.8     50.1     43.7     78.9  (12.4)
+//                     256:     118   69.1   46.1   34.6    26.3*   31.0     36.4     53.8     53.1     95.1  (20.3)
+//                     512:     231    132   77.7   59.4    45.3    41.3     36.4*    52.8     52.1     89.6  (29.1)
+//                    1024:     457    258    149    102    84.6    79.2     59.6     55.4*    55.0     87.6  (50.8)
+//                    4096:    1803   1009    580    386     299     271      212      207      201      173* (164)
+// A last round that is partly filled costs less than
 // a whole one, once there are several: its tiles have the memory to themselves.
-// 128x128 stands twice: 3 stages for one workgroup a CU, 2 for two.  Eight waves a
+// 128x128 stands twice (the table: the faster one): 3 stages for one workgroup a CU, 2 for two.  Eight waves a
 // workgroup in all but the smallest: with 4 the same tiles took up to a third longer.
 struct i8_shape {
   int BM, BN, threads, lds;

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void k_combine_rows(const TI *__restrict__ row
 // WPP waves per pair, 8 waves a workgroup (a token's pairs next to each other:
 // dout comes from L2 after the first), 4 vectors of each row in flight.  Bound
 // by memory: drows and the dot product share one pass over dout and rows.
-// 4096 tokens of 8 slots, 7168 bf16 (999 MB) 200 us, 5.0 TB/s; 301 of 4, 2048
+// 4096 tokens of 8 slots, 7168 bf16 (999 MB) 196 us, 5.1 TB/s; 301 of 4, 2048
 // f32 (17 MB) 5.2 us, most of it latency.
 template <typename TD, typename TR, int V, int WPP, bool NT>
 __global__ __launch_bounds__(512) void k_combine_grad(const TD *__restrict__ dout, const TR *__restrict__ rows,

@@ -120,9 +120,9 @@ __device__ __forceinline__ uint32_t abs_bits(const raw_v<T, V> &r) {
 // to a tie, and only waves that hold one look at the remainders: one vector in a hundred
 // of f32 values, most of 16-bit ones (their quotients have small denominators, and meet ties
 // exactly).  x * inv + 1.5 * 2^23 is rounded once, to a whole number, ties to even,
-// with the code in its low byte.  4096 rows of 7168 bf16 (88 MB) 20.0 us, 4.4 TB/s
+// with the code in its low byte.  4096 rows of 7168 bf16 (88 MB) 18.8 to 20.0 us, 4.4 to 4.7 TB/s
 // (22.1 where a tie took the whole quotient again, with branches); 32764 of 768 (76 MB)
-// 17.8, two rows a wave (23.5 with one row and a third of the lanes idle); one row
+// 17.8, between products 21.5, two rows a wave (23.5 with one row and a third of the lanes idle); one row
 // 2.3, a launch.  Workgroups that walk rows with the next one's loads in flight took 24
 // to 29 us for the first.
 template <typename T, int LANES, int VPT>
@@ -320,8 +320,8 @@ __device__ __forceinline__ v4i i8_bytes(const int8_t *row, int k, int K) {
 // 16x16x64 MFMA, channels as A, rows as B: lane l holds K bytes [16 (l/16), +16)
 // of A row (B column) l % 16; D lane l holds column l % 16, rows 4 (l/16) + i.
 // Bound by the loads' latency where the tiles are few, by the small tile's traffic
-// where they are many: K = 1765 against K = 1776 on the staged tiles, 4096 channels:
-// 1 row 12.6 and 4.7 us, 300 rows 22 and 12.7, 4096 rows 134 and 39.
+// where they are many: K = 1765 against K = 1776 on the other kernels, 4096 channels, weights from the
+// caches: 1 row 11.7 and 3.2 us, 300 rows 19 and 8.0, 4096 rows 126 and 34.
 // (nt along x and row tiles along y and z, not one index that is divided: 20000 x 101 x 300 17.5 us, 20.3 with a division.)
 __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
   __shared__ v4i xs[64][9], wsh[64][9];  // 8 chunks of 16 bytes a row, and one of padding
@@ -485,9 +485,10 @@ __global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
 // 16x16x64 MFMA, channels as A and rows as B: D lane l holds row l % 16 of its
 // row tile and channels 4 (l / 16) + i of its channel tile.
 // Bound by, and measured (kernel alone):
-//   4096 x 7168 x 7168, 256x256: 187 us, 2.25 PO/s; 8192 x 8192 x 8192 421 us, 2.61.  A
-//     tile's start and end are a tenth; in the loop the MFMA pipes share the time with the LDS
-//     reads (three quarters of LDS's rate).  Waves of 128 rows x 64 channels 187 us, of
+//   4096 x 7168 x 7168, 256x256: 171 to 187 us, 2.46 to 2.25 PO/s; 8192 x 8192 x 8192 421 us, 2.61.  A
+//     tile's start and end are a tenth; of the launch's cycles the MFMA pipes are busy for 57% (65%
+//     of those in which a CU has one of its 1.75 tiles), the LDS reads for 23%; waves wait for LDS in 4% of
+//     theirs: the rest is mostly the wait at each stage's barrier.  Waves of 128 rows x 64 channels 187 us, of
 //     64 x 128 191; a non-temporal choice at every load, which cut the loop into blocks, 204.
 //     16x16x64 from registers alone reaches 3.8 PO/s here, 32x32x32 3.3.
 //   16 or 4096 rows over the experts, 64x128: the weights' stream from HBM, 6.2 to
