@@ -22,8 +22,9 @@
  *    kvalues = {0,1,2,3,4,6,8,12,-0,-1,-2,-3,-4,-6,-8,-12}
  *    (moe-serv/src/moe_tp.h:229-233, hip-moe/src/main.hip:44-57).
  *  - One context owns one GPU.  Calls on one context are not thread-safe,
- *    but for those that say so (the reference's backend state is process-global singletons,
- *    moe_backend.cpp:58-62, driven by one scheduler thread).
+ *    but for those that say so (the reference's backend state is
+ *    process-global singletons, moe_backend.cpp:58-62, driven by one
+ *    scheduler thread).
  */
 #ifndef MOE_BLOCK_H
 #define MOE_BLOCK_H
@@ -519,7 +520,8 @@ void moe_graph_destroy(moe_graph *g);
 
 /* Per-kernel GPU time, from a HIP event pair recorded on the launch stream
  * around every kernel the context launches while profiling is on (not on a
- * stream under graph capture, this library's or the caller's own).  The reference keeps per-split phase timings the same way
+ * stream under graph capture, this library's or the caller's own).  The
+ * reference keeps per-split phase timings the same way
  * (moe-serv/src/moe_prof.h:36-137, MOESERV_PROFILE) and GPU timestamps
  * around its dispatches (moe-serv/src/moe_probe_custom.cpp:411-475). */
 typedef struct {

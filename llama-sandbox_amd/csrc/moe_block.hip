@@ -30,6 +30,7 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
+#include <new>
 #include <set>
 #include <string>
 #include <thread>
@@ -454,10 +455,14 @@ extern "C" void moe_ctx_destroy(moe_ctx *c) {
 
 extern "C" const char *moe_ctx_last_error(const moe_ctx *c) {
   if (!c) return "";
-  std::lock_guard<std::mutex> lk(c->mu);
-  std::string &mine = c->err_read[std::this_thread::get_id()];  // no other thread's error moves it
-  mine = c->err;
-  return mine.c_str();
+  try {
+    std::lock_guard<std::mutex> lk(c->mu);
+    std::string &mine = c->err_read[std::this_thread::get_id()];  // no other thread's error moves it
+    mine = c->err;
+    return mine.c_str();
+  } catch (const std::bad_alloc &) {
+    return "out of host memory";
+  }
 }
 
 extern "C" const char *moe_status_str(moe_status s) {
