@@ -489,6 +489,77 @@ moe_status moe_matmul_i8(moe_ctx *ctx, const int8_t *q_dev, const float *q_scale
                          const float *w_scale_dev, int E, const int32_t *offsets_dev, const int32_t *perm_dev, int k,
                          int M, int N, int K, uint32_t flags, float clamp, void *out_dev, int out_type, void *stream);
 
+/* ---- on the way into the experts and beside them ------------------------- */
+
+/* These calls keep the rules of the ones above: row types MOE_GGML_F32,
+ * MOE_GGML_F16 or MOE_GGML_BF16; any sizes and alignment within the stated
+ * limits; buffers that are written overlap no other but where it says so; no
+ * allocation, no shared scratch (a workspace is the caller's: calls that
+ * overlap in time need one each), and the caller's current device stays.  T <
+ * 2^24 rows, else MOE_ERR_UNSUPPORTED. */
+
+/* Norm of rows x [T][H], w [H]: y = h * r * w, r = (mean h^2 + eps)^-1/2, eps a
+ * positive normal float.  residual NULL: h = x.  Else h = x + residual,
+ * rounded to res_type and written to total; total may be residual.  The
+ * mean is held in 64 bits.  Outputs: y (y_type, rounded once), or q and scale,
+ * or both; q, scale: y, before that rounding, in 8 bits as moe_quantize_i8 writes
+ * rows (decided in 64 bits).  rstd (may be NULL): r, for the gradient.  A
+ * row with a NaN or an infinity has a NaN scale and codes 0 (its y is what the
+ * formula gives: with an infinity r is 0). */
+moe_status moe_rms_norm(moe_ctx *ctx, const void *x_dev, int x_type, const void *residual_dev, void *total_dev, int res_type,
+                        const void *w_dev, int w_type, float eps, int T, int H, void *y_dev, int y_type, int8_t *q_dev,
+                        float *scale_dev, float *rstd_dev, void *stream);
+
+/* Its gradient.  h [T][H] is what was normalised (total, or x), rstd its r.  With
+ * u = h * r and g = dy * w:
+ *   dx = r * (g - u * mean(g * u)) + dres,  dw = sum over the rows of dy * u
+ * dx is the gradient of x and of residual; dres (may be NULL, dx_type): that
+ * of total from its other readers; it may be dx.  dw [H] f32, sums in f32 in a
+ * fixed order.  part: a workspace of moe_rms_norm_grad_scratch floats (0 for sizes
+ * that the call refuses). */
+size_t moe_rms_norm_grad_scratch(const moe_ctx *ctx, int T, int H);
+moe_status moe_rms_norm_grad(moe_ctx *ctx, const void *dy_dev, int dy_type, const void *h_dev, int h_type, const void *w_dev,
+                             int w_type, const float *rstd_dev, const void *dres_dev, int T, int H, void *dx_dev,
+                             int dx_type, float *dw_dev, float *part_dev, size_t part_floats, void *stream);
+
+/* moe_route with groups of experts, for logits [T][E] of any row type, E <= 1024.
+ * An expert whose logit is -inf is masked: its score is 0 and it is never
+ * picked.  With c = score + bias, group g (experts [g*E/n_group, (g+1)*E/n_group),
+ * n_group <= 64) scores the sum of its `top` (1 or 2) largest c, of fewer
+ * where the mask leaves fewer; the `keep` groups of the highest stay, and the k
+ * largest c of their experts are picked, in that order; ties go to the lowest
+ * index, NaN comes after every number.  k <= 64 and k <= keep * E/n_group.
+ * A slot that finds no expert has id -1, which moe_group drops, and weight 0.
+ * c is compared in 64 bits (moe_route: in 32); without a bias, and with n_group
+ * = 1 or top = 1, the logits themselves are.  Weights as moe_route's.
+ * scores (may be NULL): [T][E] f32. */
+moe_status moe_route_groups(moe_ctx *ctx, const void *logits_dev, int logits_type, const float *bias_dev, int T, int E,
+                            int k, int mode, int n_group, int keep, int top, int norm, float scale, int32_t *ids_dev,
+                            float *wts_dev, float *scores_dev, void *stream);
+
+/* The logits' gradient, from dwts [T][k] of the weights (moe_combine_grad's) and
+ * dscores [T][E] of the scores (NULL: 0).  The picks are constants.  A slot
+ * whose id is outside [0, E) takes no part.  Masked experts get 0. */
+moe_status moe_route_grad(moe_ctx *ctx, const void *logits_dev, int logits_type, const int32_t *ids_dev,
+                          const float *dwts_dev, const float *dscores_dev, int T, int E, int k, int mode, int norm,
+                          float scale, void *dlogits_dev, int dlogits_type, void *stream);
+
+/* Low-rank adapters of many requests, beside a projection of the same rows:
+ *   out[r] = base[r] + scale[a] * B[a] (A[a] x[r]),  a the adapter of row r
+ * x [M][K], A [n][R][K], B [n][N][R] of one type; base, out [M][N] of out_type
+ * (out may be base); scale [n] f32 (NULL: 1).  The rows are grouped by adapter
+ * as the experts' rows are: moe_group of the rows' adapters with k = 1 (-1: the row
+ * has none) gives offsets [n+1] and perm [M]; rows of out without an adapter are
+ * left as they were.  An entry of perm outside [0, M) is skipped; a valid perm names
+ * no row twice.  Adapters of lower rank are padded with zeros.  Sums are f32.
+ * n <= 1024, R <= 1024, K and N <= 2^30.  mid: a workspace of
+ * moe_adapters_scratch floats (0 for sizes that the call refuses). */
+size_t moe_adapters_scratch(const moe_ctx *ctx, int M, int K, int R);
+moe_status moe_adapters(moe_ctx *ctx, const void *x_dev, const void *a_dev, const void *b_dev, int type,
+                        const float *scale_dev, int n, const int32_t *offsets_dev, const int32_t *perm_dev, int M, int K,
+                        int R, int N, const void *base_dev, void *out_dev, int out_type, float *mid_dev, size_t mid_floats,
+                        void *stream);
+
 /* ---- hipGraph of a decode step ------------------------------------------- */
 
 /* Capture n_layers consecutive moe_forward calls (layer ids layers[i],

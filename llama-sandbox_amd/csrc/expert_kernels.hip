@@ -5,21 +5,9 @@
 #include "../../include/moe_block.h"
 #include "kernels_dispatch.h"
 #include "kernels_i8.h"
+#include "launch_common.h"
 
 #include <cmath>
-
-static int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
-
-// A grid's x dimension holds fewer than 2^32 threads.
-static bool fits(long blocks, int threads) { return blocks * threads < (1L << 32); }
-
-// f(T{}) for the element type t.
-template <typename F>
-static void with_type(int t, F f) {
-  if (t == MOE_GGML_F32) f(float{});
-  else if (t == MOE_GGML_F16) f(_Float16{});
-  else f(bf16_t{});
-}
 
 // Elements a thread takes at once: 16 bytes, or 8 elements where a side has 16 bits.
 template <typename A, typename B>

@@ -10,7 +10,8 @@
 
 #include "expert_kernels.h"
 #include "../../include/moe_block.h"
-#include "kernels_dispatch.h"
+#include "group_tiles.h"
+#include "row_vec.h"
 
 #include <type_traits>
 
@@ -210,69 +211,12 @@ __global__ __launch_bounds__(256) void k_quantize_i8_long(const T *__restrict__ 
 
 // ---- products --------------------------------------------------------------------
 
-// The rows of one tile: expert e (-1: none left), rows [r0, r0 + n); only: the expert has no others.
-struct i8_tile {
-  int e, r0, n, only;
-};
-
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int wave_scan(int v) {
-  v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);  // row_bcast15: the last lane of rows 0 and 2 to rows 1 and 3
-  v = dpp_add<0x143, 0xC>(v);  // row_bcast31: lane 31 to rows 2 and 3
-  return v;
-}
-
-// Tile `item` of the grouped rows cut into tiles of at most BM: expert e has
-// ceil(c_e / BM) of them, in expert order.  Every wave finds it for itself: lane
-// l counts the tiles of E / 64 experts side by side (all offsets are asked for
-// at once), a scan over the lanes finds the lane that holds the item.  Offsets are
-// held to [0, M].  PER: experts a lane, at least E / 64.
-template <int PER>
-__device__ __forceinline__ i8_tile i8_search(const i8_mm &a, int item, int BM) {
-  const int lane = threadIdx.x & 63;
-  int o[PER + 1];
-#pragma unroll
-  for (int i = 0; i <= PER; i++) o[i] = a.offsets[min(PER * lane + i, a.E)];  // (past the end: equal, no rows)
-  int c[PER], sum = 0;
-#pragma unroll
-  for (int i = 0; i <= PER; i++) o[i] = min(max(o[i], 0), a.M);
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    c[i] = o[i + 1] > o[i] ? (o[i + 1] - o[i] - 1) / BM + 1 : 0;
-    sum += c[i];
-  }
-  int at = wave_scan(sum) - sum;
-  const uint64_t here = __ballot(at <= item && item < at + sum);
-  if (!here) return {-1, 0, 0, 0};
-  i8_tile t = {-1, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    if (at <= item && item < at + c[i]) {
-      const int r0 = o[i] + (item - at) * BM;
-      t = {PER * lane + i, r0, o[i + 1] - r0 < BM ? o[i + 1] - r0 : BM, c[i] == 1};
-    }
-    at += c[i];
-  }
-  const int owner = __ffsll((unsigned long long)here) - 1;
-  return {__builtin_amdgcn_readlane(t.e, owner), __builtin_amdgcn_readlane(t.r0, owner), __builtin_amdgcn_readlane(t.n, owner),
-          __builtin_amdgcn_readlane(t.only, owner)};
-}
-__device__ __forceinline__ i8_tile i8_find_tile(const i8_mm &a, int item, int BM) {
+__device__ __forceinline__ row_tile i8_find_tile(const i8_mm &a, int item, int BM) {
   if (!a.offsets) {
     const int r0 = item * BM;
     return {r0 < a.M ? 0 : -1, r0, a.M - r0 < BM ? a.M - r0 : BM, a.M <= BM};
   }
-  if (a.E <= 64) return i8_search<1>(a, item, BM);
-  if (a.E <= 256) return i8_search<4>(a, item, BM);
-  return i8_search<16>(a, item, BM);
+  return find_row_tile(a.offsets, a.E, a.M, item, BM);
 }
 
 // Source row of grouped row r (-1 where perm points outside).
@@ -325,7 +269,7 @@ __device__ __forceinline__ v4i i8_bytes(const int8_t *row, int k, int K) {
 // (nt along x and row tiles along y and z, not one index that is divided: 20000 x 101 x 300 17.5 us, 20.3 with a division.)
 __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
   __shared__ v4i xs[64][9], wsh[64][9];  // 8 chunks of 16 bytes a row, and one of padding
-  const i8_tile t = i8_find_tile(a, blockIdx.z * gridDim.y + blockIdx.y, 64);
+  const row_tile t = i8_find_tile(a, blockIdx.z * gridDim.y + blockIdx.y, 64);
   if (t.e < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int half = a.swiglu ? a.N / 2 : 32, per = a.swiglu ? 32 : 64;  // channels a workgroup: per of each half
@@ -405,7 +349,7 @@ __global__ __launch_bounds__(256) void k_mm_i8_any(i8_mm a) {
 template <int M, int C, int U>
 __global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
   const int lane = threadIdx.x;
-  const i8_tile t = i8_find_tile(a, blockIdx.x / nt, M);
+  const row_tile t = i8_find_tile(a, blockIdx.x / nt, M);
   if (t.e < 0) return;
   const int half = a.N / 2, n_end = a.swiglu ? half : a.N, cols = a.swiglu ? C / 2 : C;
   const int n0 = blockIdx.x % nt * cols;
@@ -615,7 +559,7 @@ __device__ __forceinline__ void i8_rows_out(T *out, int8_t *reg, int lane, size_
 
 // The rest of k_mm_i8 for one tile; ONCE: no other workgroup reads its weights.
 template <int BM, int BN, int WM, int WN, int WK, int NBUF, bool ONCE>
-__device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const i8_tile &t, v4i *lds) {
+__device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_tile &t, v4i *lds) {
   constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
   constexpr int STAGE = (BM + BN) * WK * 8;          // 16-byte chunks of a stage
   constexpr int XI = BM * WK / 8, WI = BN * WK / 8;  // 1 KiB loads of a stage
@@ -803,7 +747,7 @@ template <int BM, int BN, int WM, int WN, int WK, int NBUF, bool STREAM>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_mm_i8(i8_mm a, int nt) {
   // one dynamic array: for a static one the compiler would make every LDS read wait for every load in flight
   extern __shared__ v4i lds[];
-  const i8_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
+  const row_tile t = i8_find_tile(a, blockIdx.x / nt, BM);
   if (t.e < 0) return;
   if (STREAM && t.only) i8_multiply<BM, BN, WM, WN, WK, NBUF, true>(a, nt, t, lds);
   else i8_multiply<BM, BN, WM, WN, WK, NBUF, false>(a, nt, t, lds);

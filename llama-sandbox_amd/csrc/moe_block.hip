@@ -18,10 +18,12 @@
 #include "kernels_stacked.h"
 
 #include "kernels_weights.h"
+#include "layer_kernels.h"
 
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cfloat>
 #include <chrono>
 #include <cstdarg>
 #include <cstdio>
@@ -86,10 +88,12 @@ struct work_bufs {
 // Kernel classes timed by the profiler (moe_prof_*), in the order of
 // kernel_names[].
 enum { K_ROUTE = 0, K_GROUP, K_GU_DECODE, K_DOWN_DECODE, K_GU_GROUPED, K_DOWN_GROUPED,
-       K_COMBINE, K_DISPATCH, K_COMBINE_ROWS, K_COMBINE_GRAD, K_QUANT_I8, K_MM_I8, K_COUNT };
+       K_COMBINE, K_DISPATCH, K_COMBINE_ROWS, K_COMBINE_GRAD, K_QUANT_I8, K_MM_I8,
+       K_RMS_NORM, K_RMS_NORM_GRAD, K_ROUTE_GROUPS, K_ROUTE_GRAD, K_ADAPTERS, K_COUNT };
 static const char *const kernel_names[K_COUNT] = {
     "route", "group", "gate_up_decode", "down_decode", "gate_up_grouped",
-    "down_grouped", "combine", "dispatch", "combine_rows", "combine_grad", "quantize_i8", "matmul_i8"};
+    "down_grouped", "combine", "dispatch", "combine_rows", "combine_grad", "quantize_i8", "matmul_i8",
+    "rms_norm", "rms_norm_grad", "route_groups", "route_grad", "adapters"};
 
 // What calls of several threads share (moe_ctx::mu guards it).
 struct prof_state {
@@ -1358,5 +1362,6 @@ extern "C" moe_status moe_debug_last_h(moe_ctx *c, float *h, size_t cap, size_t 
 }
 
 #include "expert_ops.h"
+#include "layer_ops.h"
 #include "moe_server.h"
 #include "graph_split.h"

@@ -20,6 +20,11 @@ struct entries {
   decltype(&moe_combine_grad) combine_grad;
   decltype(&moe_quantize_i8) quantize_i8;
   decltype(&moe_matmul_i8) matmul_i8;
+  decltype(&moe_rms_norm) rms_norm;
+  decltype(&moe_rms_norm_grad) rms_norm_grad;
+  decltype(&moe_route_groups) route_groups;
+  decltype(&moe_route_grad) route_grad;
+  decltype(&moe_adapters) adapters;
 };
 
 static PyObject *current_stream;  // a function: device -> handle of torch's current stream
@@ -67,13 +72,35 @@ struct call {
     return t;
   }
   // ... of rows; *type: the ggml type of their elements
-  const at::Tensor *rows(PyObject *o, int *type) {
+  const at::Tensor *rows(PyObject *o, int *type, int dim = 2) {
     const at::Tensor *t = tensor(o);
     if (!t) return t;
     const at::ScalarType s = t->scalar_type();
     *type = s == at::kFloat ? MOE_GGML_F32 : s == at::kHalf ? MOE_GGML_F16 : MOE_GGML_BF16;
-    fine = t->dim() == 2 && (s == at::kFloat || s == at::kHalf || s == at::kBFloat16);
+    fine = t->dim() == dim && (s == at::kFloat || s == at::kHalf || s == at::kBFloat16);
     return t;
+  }
+  // ... of this shape
+  const at::Tensor *rows_of(PyObject *o, int *type, at::IntArrayRef shape) {
+    const at::Tensor *t = rows(o, type, (int)shape.size());
+    if (t && fine) fine = t->sizes() == shape;
+    return t;
+  }
+  // ... of a size that the library checks
+  const at::Tensor *workspace(PyObject *o) {
+    const at::Tensor *t = tensor(o);
+    if (t) fine = t->scalar_type() == at::kFloat && t->dim() == 1;
+    return t;
+  }
+  // a whole number and a float of the arguments
+  int whole(PyObject *o) {
+    const long v = fine && PyLong_Check(o) ? PyLong_AsLong(o) : (fine = false, 0);
+    if (PyErr_Occurred() || v < INT_MIN || v > INT_MAX) fine = false;
+    return (int)v;
+  }
+  float real(PyObject *o) {
+    if (!fine || !PyFloat_Check(o)) return fine = false, 0.0f;
+    return (float)PyFloat_AS_DOUBLE(o);
   }
   // ... a pair map of T tokens; *k: its slots
   const at::Tensor *pairs(PyObject *o, int64_t T, int *k) {
@@ -250,9 +277,133 @@ static PyObject *matmul_i8(PyObject *, args_t a, Py_ssize_t n) {
   });
 }
 
+static void *data(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
+template <typename T>
+static const T *read(const at::Tensor *t) { return t ? (const T *)t->const_data_ptr() : nullptr; }
+
+// (entries, ctx, device, x, w, eps, residual, total, y, q, scale, rstd, stream); from residual on None: absent
+static PyObject *rms_norm(PyObject *, args_t a, Py_ssize_t n) {
+  return try_call([&]() -> PyObject * {
+    call c(a, n, 13);
+    int xt = 0, wt = 0, rt = 0, tt = 0, yt = 0;
+    const at::Tensor *x = c.fine ? c.rows(a[3], &xt) : nullptr;
+    if (!c.fine) return nullptr;
+    const int64_t T = x->size(0), H = x->size(1);
+    const at::Tensor *w = c.rows_of(a[4], &wt, {H});
+    const float eps = c.real(a[5]);
+    auto rows = [&](PyObject *o, int *type) { return !c.fine || o == Py_None ? nullptr : c.rows_of(o, type, {T, H}); };
+    auto column = [&](PyObject *o) { return !c.fine || o == Py_None ? nullptr : c.array(o, at::kFloat, {T}); };
+    const at::Tensor *res = rows(a[6], &rt), *total = rows(a[7], &tt), *y = rows(a[8], &yt);
+    const at::Tensor *q = !c.fine || a[9] == Py_None ? nullptr : c.array(a[9], at::kChar, {T, H});
+    const at::Tensor *scale = column(a[10]), *rstd = column(a[11]);
+    if (!c.fine || !res != !total || rt != tt || !q != !scale || (!y && !q)) return nullptr;
+    return c.make([&](void *stream) {
+      return c.lib->rms_norm(c.ctx, x->const_data_ptr(), xt, read<void>(res), data(total), rt, w->const_data_ptr(), wt, eps,
+                             (int)T, (int)H, data(y), yt, (int8_t *)data(q), (float *)data(scale), (float *)data(rstd), stream);
+    });
+  });
+}
+
+// (entries, ctx, device, dy, h, w, rstd, dx, dw, part, dres or None, stream)
+static PyObject *rms_norm_grad(PyObject *, args_t a, Py_ssize_t n) {
+  return try_call([&]() -> PyObject * {
+    call c(a, n, 12);
+    int dt = 0, ht = 0, wt = 0, xt = 0, rt = 0;
+    const at::Tensor *dy = c.fine ? c.rows(a[3], &dt) : nullptr;
+    if (!c.fine) return nullptr;
+    const int64_t T = dy->size(0), H = dy->size(1);
+    const at::Tensor *h = c.rows_of(a[4], &ht, {T, H});
+    const at::Tensor *w = c.fine ? c.rows_of(a[5], &wt, {H}) : nullptr;
+    const at::Tensor *rstd = c.fine ? c.array(a[6], at::kFloat, {T}) : nullptr;
+    const at::Tensor *dx = c.fine ? c.rows_of(a[7], &xt, {T, H}) : nullptr;
+    const at::Tensor *dw = c.fine ? c.array(a[8], at::kFloat, {H}) : nullptr;
+    const at::Tensor *part = c.fine ? c.workspace(a[9]) : nullptr;
+    const at::Tensor *dres = !c.fine || a[10] == Py_None ? nullptr : c.rows_of(a[10], &rt, {T, H});
+    if (!c.fine || (dres && rt != xt)) return nullptr;
+    return c.make([&](void *stream) {
+      return c.lib->rms_norm_grad(c.ctx, dy->const_data_ptr(), dt, h->const_data_ptr(), ht, w->const_data_ptr(), wt,
+                                  read<float>(rstd), read<void>(dres), (int)T, (int)H, dx->data_ptr(), xt, (float *)data(dw),
+                                  (float *)data(part), (size_t)part->numel(), stream);
+    });
+  });
+}
+
+// (entries, ctx, device, logits, k, mode, norm, scale, ids, wts, bias or None, n_group, keep, top, scores or None, stream)
+static PyObject *route_groups(PyObject *, args_t a, Py_ssize_t n) {
+  return try_call([&]() -> PyObject * {
+    call c(a, n, 16);
+    int lt = 0;
+    const at::Tensor *l = c.fine ? c.rows(a[3], &lt) : nullptr;
+    if (!c.fine) return nullptr;
+    const int64_t T = l->size(0), E = l->size(1);
+    const int k = c.whole(a[4]), mode = c.whole(a[5]), norm = PyObject_IsTrue(a[6]);
+    const float scale = c.real(a[7]);
+    const at::Tensor *ids = c.fine ? c.array(a[8], at::kInt, {T, k}) : nullptr;
+    const at::Tensor *wts = c.fine ? c.array(a[9], at::kFloat, {T, k}) : nullptr;
+    const at::Tensor *bias = !c.fine || a[10] == Py_None ? nullptr : c.array(a[10], at::kFloat, {E});
+    const int n_group = c.whole(a[11]), keep = c.whole(a[12]), top = c.whole(a[13]);
+    const at::Tensor *scores = !c.fine || a[14] == Py_None ? nullptr : c.array(a[14], at::kFloat, {T, E});
+    if (!c.fine || norm < 0) return nullptr;
+    return c.make([&](void *stream) {
+      return c.lib->route_groups(c.ctx, l->const_data_ptr(), lt, read<float>(bias), (int)T, (int)E, k, mode, n_group, keep, top,
+                                 norm, scale, (int32_t *)data(ids), (float *)data(wts), (float *)data(scores), stream);
+    });
+  });
+}
+
+// (entries, ctx, device, logits, ids, dwts, mode, norm, scale, dlogits, dscores or None, stream)
+static PyObject *route_grad(PyObject *, args_t a, Py_ssize_t n) {
+  return try_call([&]() -> PyObject * {
+    call c(a, n, 12);
+    int lt = 0, dt = 0;
+    const at::Tensor *l = c.fine ? c.rows(a[3], &lt) : nullptr;
+    if (!c.fine) return nullptr;
+    const int64_t T = l->size(0), E = l->size(1);
+    const at::Tensor *ids = c.tensor(a[4]);
+    if (!c.fine || ids->scalar_type() != at::kInt || ids->dim() != 2 || ids->size(0) != T) return nullptr;
+    const int64_t k = ids->size(1);
+    const at::Tensor *dwts = c.array(a[5], at::kFloat, {T, k});
+    const int mode = c.whole(a[6]), norm = PyObject_IsTrue(a[7]);
+    const float scale = c.real(a[8]);
+    const at::Tensor *dl = c.fine ? c.rows_of(a[9], &dt, {T, E}) : nullptr;
+    const at::Tensor *ds = !c.fine || a[10] == Py_None ? nullptr : c.array(a[10], at::kFloat, {T, E});
+    if (!c.fine || norm < 0) return nullptr;
+    return c.make([&](void *stream) {
+      return c.lib->route_grad(c.ctx, l->const_data_ptr(), lt, read<int32_t>(ids), read<float>(dwts), read<float>(ds), (int)T,
+                               (int)E, (int)k, mode, norm, scale, dl->data_ptr(), dt, stream);
+    });
+  });
+}
+
+// (entries, ctx, device, x, a, b, scale or None, offsets, perm, base, out, mid, stream)
+static PyObject *adapters(PyObject *, args_t a, Py_ssize_t n) {
+  return try_call([&]() -> PyObject * {
+    call c(a, n, 13);
+    int xt = 0, at_ = 0, bt = 0, st = 0, ot = 0;
+    const at::Tensor *x = c.fine ? c.rows(a[3], &xt) : nullptr, *A = c.fine ? c.rows(a[4], &at_, 3) : nullptr;
+    const at::Tensor *B = c.fine ? c.rows(a[5], &bt, 3) : nullptr;
+    if (!c.fine || at_ != xt || bt != xt) return nullptr;
+    const int64_t M = x->size(0), K = x->size(1), na = A->size(0), R = A->size(1), N = B->size(1);
+    if (A->size(2) != K || B->size(0) != na || B->size(2) != R) return nullptr;
+    const at::Tensor *scale = a[6] == Py_None ? nullptr : c.array(a[6], at::kFloat, {na});
+    const at::Tensor *offsets = c.fine ? c.array(a[7], at::kInt, {na + 1}) : nullptr;
+    const at::Tensor *perm = c.fine ? c.array(a[8], at::kInt, {M}) : nullptr;
+    const at::Tensor *base = c.fine ? c.rows_of(a[9], &st, {M, N}) : nullptr;
+    const at::Tensor *out = c.fine ? c.rows_of(a[10], &ot, {M, N}) : nullptr;
+    const at::Tensor *mid = c.fine ? c.workspace(a[11]) : nullptr;
+    if (!c.fine || st != ot) return nullptr;
+    return c.make([&](void *stream) {
+      return c.lib->adapters(c.ctx, x->const_data_ptr(), A->const_data_ptr(), B->const_data_ptr(), xt, read<float>(scale),
+                             (int)na, read<int32_t>(offsets), read<int32_t>(perm), (int)M, (int)K, (int)R, (int)N,
+                             base->const_data_ptr(), out->data_ptr(), ot, (float *)data(mid), (size_t)mid->numel(), stream);
+    });
+  });
+}
+
 #define METHOD(f) {#f, (PyCFunction)(void (*)())f, METH_FASTCALL, nullptr}
 static PyMethodDef methods[] = {METHOD(dispatch),     METHOD(dispatch_grad), METHOD(combine), METHOD(combine_grad),
-                                METHOD(quantize_i8), METHOD(matmul_i8),
+                                METHOD(quantize_i8),  METHOD(matmul_i8),     METHOD(rms_norm), METHOD(rms_norm_grad),
+                                METHOD(route_groups), METHOD(route_grad),    METHOD(adapters),
                                 {"set_current_stream", set_current_stream, METH_O, nullptr},
                                 {nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "moe_torch", nullptr, -1, methods};

@@ -51,6 +51,8 @@ EXPORTS = (
     "moe_server_open", "moe_server_close", "moe_server_last_error", "moe_server_handle", "moe_server_listen",
     "moe_server_serve", "moe_router_logits", "moe_node_claimed", "moe_split_parse", "moe_split_compute",
     "moe_dispatch", "moe_dispatch_grad", "moe_combine", "moe_combine_grad", "moe_quantize_i8", "moe_matmul_i8",
+    "moe_rms_norm", "moe_rms_norm_grad", "moe_rms_norm_grad_scratch", "moe_route_groups", "moe_route_grad",
+    "moe_adapters", "moe_adapters_scratch",
 )
 
 # graph nodes of the ggml backend's split (include/moe_block.h, moe_node)
@@ -263,6 +265,21 @@ def load_library(path: str | None = None):
     L.moe_matmul_i8.restype = st
     L.moe_matmul_i8.argtypes = [_vp, _vp, _vp, ci, _vp, _vp, ci, _vp, _vp, ci, ci, ci, ci, ctypes.c_uint32,
                                 ctypes.c_float, _vp, ci, _vp]
+    cf, sz = ctypes.c_float, ctypes.c_size_t
+    L.moe_rms_norm.restype = st
+    L.moe_rms_norm.argtypes = [_vp, _vp, ci, _vp, _vp, ci, _vp, ci, cf, ci, ci, _vp, ci, _vp, _vp, _vp, _vp]
+    L.moe_rms_norm_grad_scratch.restype = sz
+    L.moe_rms_norm_grad_scratch.argtypes = [_vp, ci, ci]
+    L.moe_rms_norm_grad.restype = st
+    L.moe_rms_norm_grad.argtypes = [_vp, _vp, ci, _vp, ci, _vp, ci, _vp, _vp, ci, ci, _vp, ci, _vp, _vp, sz, _vp]
+    L.moe_route_groups.restype = st
+    L.moe_route_groups.argtypes = [_vp, _vp, ci, _vp, ci, ci, ci, ci, ci, ci, ci, ci, cf, _vp, _vp, _vp, _vp]
+    L.moe_route_grad.restype = st
+    L.moe_route_grad.argtypes = [_vp, _vp, ci, _vp, _vp, _vp, ci, ci, ci, ci, ci, cf, _vp, ci, _vp]
+    L.moe_adapters_scratch.restype = sz
+    L.moe_adapters_scratch.argtypes = [_vp, ci, ci, ci]
+    L.moe_adapters.restype = st
+    L.moe_adapters.argtypes = [_vp, _vp, _vp, _vp, ci, _vp, ci, _vp, _vp, ci, ci, ci, ci, _vp, _vp, ci, _vp, sz, _vp]
     if path is None:
         _lib = L
     return L
@@ -383,7 +400,8 @@ def _know_torch():
 class _Entries(ctypes.Structure):
     """The entry points that moe_torch calls, by address."""
     _fields_ = [(n, _vp) for n in ("moe_dispatch", "moe_dispatch_grad", "moe_combine", "moe_combine_grad",
-                                   "moe_quantize_i8", "moe_matmul_i8")]
+                                   "moe_quantize_i8", "moe_matmul_i8", "moe_rms_norm", "moe_rms_norm_grad",
+                                   "moe_route_groups", "moe_route_grad", "moe_adapters")]
 
 
 def _row_type(t, name: str) -> int:
@@ -408,6 +426,16 @@ def check_rows(name: str, t, rows=None, cols=None) -> int:
         raise ValueError(f"{name}: empty")
     if not t.is_contiguous():
         raise ValueError(f"{name}: not contiguous")
+    return ty
+
+
+def check_gain(w, H: int) -> int:
+    """w: a contiguous [H] operand of a row type; its ggml type."""
+    ty = _row_type(w, "w")
+    if w.dim() != 1 or w.shape[0] != H:
+        raise ValueError(f"w: shape {tuple(w.shape)}, expected ({H},)")
+    if not w.is_contiguous():
+        raise ValueError("w: not contiguous")
     return ty
 
 
@@ -790,6 +818,161 @@ class MoeBlock:
         if st:
             self._check(st, "moe_matmul_i8")
 
+    # -- on the way into the experts and beside them (torch device tensors) -------
+    def rms_norm(self, x, w, eps: float, residual=None, total=None, y=None, q=None, scale=None, rstd=None, stream=None):
+        """Norm of rows x [T, H]: y = h * r * w with r = (mean h^2 + eps)^-1/2, w
+        [H].  With residual [T, H], h = x + residual, rounded to its type and
+        written to total (of that type; residual itself: in place), else h = x.
+        q, scale: y in 8 bits as quantize_i8 writes rows (y, q and scale, or
+        both); rstd [T] float32 takes r, for the gradient."""
+        st = self._calls and _torch_calls.rms_norm(self._calls, self.h, self.device, x, w, eps, residual, total, y, q, scale,
+                                                   rstd, stream)
+        if st is None:
+            xt = check_rows("x", x)
+            T, H = x.shape
+            wt = check_gain(w, H)
+            if (residual is None) != (total is None):
+                raise ValueError("residual and total: both or neither")
+            if (q is None) != (scale is None):
+                raise ValueError("q and scale: both or neither")
+            if y is None and q is None:
+                raise ValueError("y, or q and scale: at least one output")
+            rt = yt = 0
+            if residual is not None:
+                rt = check_rows("residual", residual, T, H)
+                if check_rows("total", total, T, H) != rt:
+                    raise ValueError(f"total: dtype {total.dtype}, expected residual's {residual.dtype}")
+            if y is not None:
+                yt = check_rows("y", y, T, H)
+            if q is not None:
+                check_tensor(q, "q", "int8", (T, H), device=False)
+                check_tensor(scale, "scale", "float32", (T,), device=False)
+            if rstd is not None:
+                check_tensor(rstd, "rstd", "float32", (T,), device=False)
+            self._on_device((x, "x"), (w, "w"), (residual, "residual"), (total, "total"), (y, "y"), (q, "q"),
+                            (scale, "scale"), (rstd, "rstd"))
+            st = self.lib.moe_rms_norm(self.h, _ptr(x), xt, _ptr(residual), _ptr(total), rt, _ptr(w), wt, eps, T, H,
+                                       _ptr(y), yt, _ptr(q), _ptr(scale), _ptr(rstd),
+                                       _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_rms_norm")
+
+    def rms_norm_grad_scratch(self, T: int, H: int) -> int:
+        """Floats that rms_norm_grad's part needs for T rows of H."""
+        return int(self.lib.moe_rms_norm_grad_scratch(self.h, T, H))
+
+    def rms_norm_grad(self, dy, h, w, rstd, dx, dw, part, dres=None, stream=None):
+        """rms_norm's gradient, h what was normalised (total, or x) and rstd its r:
+        with u = h * r and g = dy * w, dx = r * (g - u * mean(g * u)) + dres (the
+        gradient of x and of residual; dres, of dx's type, may be dx itself)
+        and dw [H] float32 = sum over the rows of dy * u.  part: float32, a
+        workspace of rms_norm_grad_scratch(T, H) values."""
+        st = self._calls and _torch_calls.rms_norm_grad(self._calls, self.h, self.device, dy, h, w, rstd, dx, dw, part, dres,
+                                                        stream)
+        if st is None:
+            dt = check_rows("dy", dy)
+            T, H = dy.shape
+            ht, wt, xt = check_rows("h", h, T, H), check_gain(w, H), check_rows("dx", dx, T, H)
+            check_tensor(rstd, "rstd", "float32", (T,), device=False)
+            check_tensor(dw, "dw", "float32", (H,), device=False)
+            check_tensor(part, "part", "float32", (None,), device=False)
+            if dres is not None and check_rows("dres", dres, T, H) != xt:
+                raise ValueError(f"dres: dtype {dres.dtype}, expected dx's {dx.dtype}")
+            self._on_device((dy, "dy"), (h, "h"), (w, "w"), (rstd, "rstd"), (dx, "dx"), (dw, "dw"), (part, "part"),
+                            (dres, "dres"))
+            st = self.lib.moe_rms_norm_grad(self.h, _ptr(dy), dt, _ptr(h), ht, _ptr(w), wt, _ptr(rstd), _ptr(dres), T, H,
+                                            _ptr(dx), xt, _ptr(dw), _ptr(part), part.numel(),
+                                            _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_rms_norm_grad")
+
+    def route_groups(self, logits, k: int, mode: int, norm: bool, scale: float, ids, wts, bias=None, n_group: int = 1,
+                     keep: int = 1, top: int = 2, scores=None, stream=None):
+        """route() for logits [T, E] of any row type, with groups: the experts
+        stand in n_group groups of E / n_group, the keep groups stay whose top
+        (1 or 2) best experts sum to most, and the k best of theirs are picked.  An
+        expert whose logit is -inf is masked: a slot that finds no other
+        has id -1 (group() drops the pair) and weight 0.  scores [T, E]
+        float32: the scores as well."""
+        st = self._calls and _torch_calls.route_groups(self._calls, self.h, self.device, logits, k, mode, norm, scale, ids,
+                                                       wts, bias, n_group, keep, top, scores, stream)
+        if st is None:
+            lt = check_rows("logits", logits)
+            T, E = logits.shape
+            check_tensor(ids, "ids", "int32", (T, k), device=False)
+            check_tensor(wts, "wts", "float32", (T, k), device=False)
+            if bias is not None:
+                check_tensor(bias, "bias", "float32", (E,), device=False)
+            if scores is not None:
+                check_tensor(scores, "scores", "float32", (T, E), device=False)
+            self._on_device((logits, "logits"), (ids, "ids"), (wts, "wts"), (bias, "bias"), (scores, "scores"))
+            st = self.lib.moe_route_groups(self.h, _ptr(logits), lt, _ptr(bias), T, E, int(k), mode, n_group, keep, top,
+                                           int(norm), scale, _ptr(ids), _ptr(wts), _ptr(scores),
+                                           _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_route_groups")
+
+    def route_grad(self, logits, ids, dwts, mode: int, norm: bool, scale: float, dlogits, dscores=None, stream=None):
+        """The logits' gradient dlogits [T, E] of route_groups, from dwts [T, k] (of
+        the weights of the experts ids; a slot outside [0, E) takes no part) and
+        dscores [T, E] (of the scores; None: 0), both float32."""
+        st = self._calls and _torch_calls.route_grad(self._calls, self.h, self.device, logits, ids, dwts, mode, norm, scale,
+                                                     dlogits, dscores, stream)
+        if st is None:
+            lt = check_rows("logits", logits)
+            T, E = logits.shape
+            dt = check_rows("dlogits", dlogits, T, E)
+            check_tensor(ids, "ids", "int32", (T, None), device=False)
+            k = ids.shape[1]
+            check_tensor(dwts, "dwts", "float32", (T, k), device=False)
+            if dscores is not None:
+                check_tensor(dscores, "dscores", "float32", (T, E), device=False)
+            self._on_device((logits, "logits"), (ids, "ids"), (dwts, "dwts"), (dlogits, "dlogits"), (dscores, "dscores"))
+            st = self.lib.moe_route_grad(self.h, _ptr(logits), lt, _ptr(ids), _ptr(dwts), _ptr(dscores), T, E, k, mode,
+                                         int(norm), scale, _ptr(dlogits), dt,
+                                         _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_route_grad")
+
+    def adapters_scratch(self, M: int, K: int, R: int) -> int:
+        """Floats that adapters' mid needs for M rows of K and rank R."""
+        return int(self.lib.moe_adapters_scratch(self.h, M, K, R))
+
+    def adapters(self, x, a, b, scale, offsets, perm, base, out, mid, stream=None):
+        """out[r] = base[r] + scale[i] * b[i] (a[i] x[r]) for the rows r of adapter i:
+        x [M, K], a [n, R, K] and b [n, N, R] of one row type, base and out [M, N] of one
+        (out may be base), scale [n] float32 or None (1).  offsets [n + 1] and perm [M]
+        group the rows by adapter, from group() with the rows' adapters as [M, 1] ids
+        (-1: none; such a row of out stays as it was).  mid: float32, a workspace
+        of adapters_scratch(M, K, R) values."""
+        st = self._calls and _torch_calls.adapters(self._calls, self.h, self.device, x, a, b, scale, offsets, perm, base, out,
+                                                   mid, stream)
+        if st is None:
+            xt = check_rows("x", x)
+            M, K = x.shape
+            dt = str(x.dtype).replace("torch.", "")
+            check_tensor(a, "a", dt, (None, None, K), device=False)
+            n, R = a.shape[0], a.shape[1]
+            check_tensor(b, "b", dt, (n, None, R), device=False)
+            N = b.shape[1]
+            if n * R * N == 0:
+                raise ValueError(f"a, b: shapes {tuple(a.shape)}, {tuple(b.shape)}: empty")
+            ot = check_rows("out", out, M, N)
+            if check_rows("base", base, M, N) != ot:
+                raise ValueError(f"base: dtype {base.dtype}, expected out's {out.dtype}")
+            if scale is not None:
+                check_tensor(scale, "scale", "float32", (n,), device=False)
+            check_tensor(offsets, "offsets", "int32", (n + 1,), device=False)
+            check_tensor(perm, "perm", "int32", (M,), device=False)
+            check_tensor(mid, "mid", "float32", (None,), device=False)
+            self._on_device((x, "x"), (a, "a"), (b, "b"), (scale, "scale"), (offsets, "offsets"), (perm, "perm"),
+                            (base, "base"), (out, "out"), (mid, "mid"))
+            st = self.lib.moe_adapters(self.h, _ptr(x), _ptr(a), _ptr(b), xt, _ptr(scale), n, _ptr(offsets), _ptr(perm),
+                                       M, K, R, N, _ptr(base), _ptr(out), ot, _ptr(mid), mid.numel(),
+                                       _device_stream(self.device) if stream is None else int(stream))
+        if st:
+            self._check(st, "moe_adapters")
+
     def split_compute(self, nodes):
         """Compute a parsed split (moe_split_compute) into its MUL node's host data."""
         self._check(self.lib.moe_split_compute(self.h, node_list(nodes), len(nodes)), "moe_split_compute")
@@ -829,7 +1012,7 @@ class MoeBlock:
 
     def prof_read(self, reset: bool = True) -> dict:
         """{kernel class: (launches, total_us)} since the last reset."""
-        cap = 16
+        cap = 32
         arr = (KernelStat * cap)()
         n = ctypes.c_int()
         self._check(self.lib.moe_prof_read(self.h, arr, cap, ctypes.byref(n), int(reset)), "moe_prof_read")
