@@ -14,6 +14,8 @@
 #include "row_vec.h"
 #include "../../include/moe_block.h"
 
+#include <type_traits>
+
 // Element i of a row operand whose type is the same for a whole call: a uniform branch.
 __device__ __forceinline__ float load_any(const void *p, int type, size_t i) {
   if (type == MOE_GGML_F32) return reinterpret_cast<const float *>(p)[i];
@@ -31,41 +33,219 @@ __device__ __forceinline__ float round_any(int type, float v) {
   return v;
 }
 
-template <typename F>
-__device__ __forceinline__ double wave_reduce_d(double v, F f) {
+// 8 elements of a row of S bytes each, as they were loaded.  The kernels are made for sizes, and take
+// the type at their conversions (a uniform branch): three types of four operands would be 81
+// of each.
+template <int S>
+struct raw8 {
+  typedef typename std::conditional<S == 4, float, uint16_t>::type elem;
+  raw_v<elem, 8> r;
+  __device__ __forceinline__ void load(const void *p, size_t i, int left) { r.load(reinterpret_cast<const elem *>(p) + i, left); }
+  __device__ __forceinline__ void get(int type, float (&f)[8]) const {
+    if constexpr (S == 4) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = f(v, __shfl_xor(v, off));
-  return v;
+      for (int i = 0; i < 8; i++) f[i] = r.v[i];
+    } else if (type == MOE_GGML_F16) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint16_t e = r.v[i];
+        f[i] = (float)__builtin_bit_cast(_Float16, e);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) f[i] = __builtin_bit_cast(float, (uint32_t)r.v[i] << 16);
+    }
+  }
+};
+// ... of any type: the gain, read by every row and found in the caches.
+__device__ __forceinline__ void load8_any(const void *p, int type, size_t i, int left, float (&f)[8]) {
+  if (type == MOE_GGML_F32) {
+    raw8<4> r;
+    r.load(p, i, left);
+    r.get(type, f);
+  } else {
+    raw8<2> r;
+    r.load(p, i, left);
+    r.get(type, f);
+  }
+}
+__device__ __forceinline__ void store8_any(void *p, int type, size_t i, int left, const float (&f)[8]) {
+  if (type == MOE_GGML_F32) store_v<float, 8>(reinterpret_cast<float *>(p) + i, left, f);
+  else if (type == MOE_GGML_F16) store_v<_Float16, 8>(reinterpret_cast<_Float16 *>(p) + i, left, f);
+  else store_v<bf16_t, 8>(reinterpret_cast<bf16_t *>(p) + i, left, f);
 }
 
-// Over a workgroup of WAVES waves; every thread gets it.  part: WAVES doubles, read before the
-// next use only after a barrier of the caller's.
-template <int WAVES, typename F>
-__device__ __forceinline__ double block_reduce_d(double v, double *part, F f) {
-  v = wave_reduce_d(v, f);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = part[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; i++) v = f(v, part[i]);
-  return v;
-}
-
+__device__ __forceinline__ double add_d(double a, double b) { return a + b; }
 // NaN wins: a row that holds one has no largest value.
 __device__ __forceinline__ double max_nan(double a, double b) { return a > b || a != a ? a : b; }
+
+__device__ __forceinline__ double readlane_d(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Over the LANES lanes (16, 32 or 64) that a lane is one of; every one gets it.
+template <int LANES, typename F>
+__device__ __forceinline__ double lanes_reduce_d(double v, F f) {
+  v = f(v, dpp_d<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = f(v, dpp_d<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = f(v, dpp_d<0x141>(v));  // row_half_mirror
+  v = f(v, dpp_d<0x140>(v));  // row_mirror: every lane holds its row of 16's
+  if constexpr (LANES == 32) v = f(v, __shfl_xor(v, 16));
+  if constexpr (LANES == 64) v = f(f(readlane_d(v, 0), readlane_d(v, 16)), f(readlane_d(v, 32), readlane_d(v, 48)));
+  return v;
+}
+
+// Over the LANES threads of a row.  part: a double for each wave of the workgroup, not used
+// again before a barrier of the caller's.
+template <int LANES, typename F>
+__device__ __forceinline__ double row_reduce_d(double v, double *part, F f) {
+  v = lanes_reduce_d<(LANES < 64 ? LANES : 64)>(v, f);
+  if constexpr (LANES > 64) {
+    constexpr int W = LANES / 64;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) part[wave] = v;
+    __syncthreads();
+    v = part[wave / W * W];
+#pragma unroll
+    for (int i = 1; i < W; i++) v = f(v, part[wave / W * W + i]);
+  }
+  return v;
+}
 
 // A row's 8-bit scale from its largest |y|; what has none (NaN, infinity) gets NaN.
 __device__ __forceinline__ float norm_scale(double amax) {
   const float s = (float)(amax / 127.0);
   return s < INFINITY ? s : __builtin_nanf("");
 }
-__device__ __forceinline__ int8_t norm_code(double y, float s) {
-  if (!(s > 0.0f)) return 0;
-  return (int8_t)fmin(fmax(__builtin_rint(y / (double)s), -127.0), 127.0);
+
+// A row in one pass: LANES threads hold it in registers, VPT vectors of 8 each (H <= 8 LANES
+// VPT); 256 / LANES rows a workgroup where that is more than one.  SX, SR: bytes of an element of x and of the residual
+// (0: none).
+template <int SX, int SR, int LANES, int VPT>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_call a) {
+  constexpr int NT = LANES < 256 ? 256 : LANES;
+  __shared__ double part[2][NT / 64];
+  const int in_row = threadIdx.x % LANES;
+  const long row = (long)blockIdx.x * (NT / LANES) + threadIdx.x / LANES;
+  const bool there = row < a.T;
+  const size_t at = (size_t)(there ? row : 0) * a.H;
+  raw8<SX> x[VPT];
+  raw8<(SR ? SR : 2)> res[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    const int i = (in_row + v * LANES) * 8, left = there ? a.H - i : 0;
+    x[v].load(a.x, at + i, left);
+    if constexpr (SR != 0) res[v].load(a.res, at + i, left);
+  }
+  // asked for before the barrier; the longest rows have no registers for it, and read it where it is used
+  constexpr bool EARLY = LANES * VPT <= 2048;
+  float w_early[EARLY ? VPT : 1][8];
+  auto load_w = [&](int v, float(&f)[8]) {
+    const int i = (in_row + v * LANES) * 8;
+    load8_any(a.w, a.w_type, i, a.H - i, f);
+  };
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int v = 0; v < VPT; v++) load_w(v, w_early[v]);
+  }
+  auto gain = [&](int v, float(&f)[8]) {
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) f[j] = w_early[v][j];
+    } else {
+      load_w(v, f);
+    }
+  };
+  float h[VPT][8];
+  double sum = 0.0;
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    const int i = (in_row + v * LANES) * 8;
+    x[v].get(a.x_type, h[v]);
+    if constexpr (SR != 0) {
+      float e[8];
+      res[v].get(a.res_type, e);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[v][j] += e[j];
+      if (SR == 2) {
+        if (a.res_type == MOE_GGML_F16) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) h[v][j] = (float)(_Float16)h[v][j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) h[v][j] = (float)(bf16_t)h[v][j];
+        }
+      }
+      if (there && i < a.H) store8_any(a.total, a.res_type, at + i, a.H - i, h[v]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum = fma((double)h[v][j], (double)h[v][j], sum);  // (past the end: 0)
+  }
+  sum = row_reduce_d<LANES>(sum, part[0], add_d);
+  const double r = 1.0 / sqrt(sum / a.H + (double)a.eps);
+  if (a.rstd && there && in_row == 0) a.rstd[row] = (float)r;
+  if (a.y && there) {
+    const float r32 = (float)r;
+#pragma unroll
+    for (int v = 0; v < VPT; v++) {
+      const int i = (in_row + v * LANES) * 8;
+      if (i >= a.H) break;
+      float y[8], w[8];
+      gain(v, w);
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = h[v][j] * r32 * w[j];
+      store8_any(a.y, a.y_type, at + i, a.H - i, y);
+    }
+  }
+  if (!a.q) return;
+  double m = 0.0;
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    float w[8];
+    gain(v, w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max_nan(m, fabs((double)h[v][j] * (double)w[j]));
+  }
+  m = row_reduce_d<LANES>(m, part[1], max_nan);
+  if (!there) return;
+  const float s = norm_scale(m * r);
+  if (in_row == 0) a.scale[row] = s;
+  const double g = s > 0.0f ? r / (double)s : 0.0;
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    const int i = (in_row + v * LANES) * 8;
+    if (i >= a.H) break;
+    float w[8];
+    gain(v, w);
+    uint32_t code[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      code[j] = (uint32_t)(int)fmin(fmax(__builtin_rint((double)h[v][j] * (double)w[j] * g), -127.0), 127.0);
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+    int8_t *to = a.q + at + i;
+    if (!(s > 0.0f)) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) code[j] = 0;
+    }
+    if (i + 8 <= a.H) {
+      u32x2 o;
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        o[k] = (code[4 * k] & 255) | (code[4 * k + 1] & 255) << 8 | (code[4 * k + 2] & 255) << 16 | code[4 * k + 3] << 24;
+      *reinterpret_cast<u32x2 *>(to) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (i + j < a.H) to[j] = (int8_t)code[j];
+    }
+  }
 }
 
-// One workgroup a row, three passes over it.
-__global__ __launch_bounds__(256) void k_rms_norm_any(norm_call a) {
+// Rows too long for registers: one workgroup a row, three passes over it.
+__global__ __launch_bounds__(256) void k_rms_norm_long(norm_call a) {
   __shared__ double part[2][4];
   const size_t at = (size_t)blockIdx.x * a.H;
   const int tid = threadIdx.x;
@@ -80,7 +260,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(norm_call a) {
     }
     sum = fma((double)h, (double)h, sum);
   }
-  sum = block_reduce_d<4>(sum, part[0], [](double p, double q) { return p + q; });
+  sum = row_reduce_d<256>(sum, part[0], add_d);
   const double r = 1.0 / sqrt(sum / a.H + (double)a.eps);
   if (a.rstd && tid == 0) a.rstd[blockIdx.x] = (float)r;
   if (a.y)
@@ -89,15 +269,18 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(norm_call a) {
   if (!a.q) return;
   double m = 0.0;
   for (int i = tid; i < a.H; i += 256) m = max_nan(m, fabs((double)load_any(hp, ht, at + i) * (double)load_any(a.w, a.w_type, i)));
-  m = block_reduce_d<4>(m, part[1], max_nan);
+  m = row_reduce_d<256>(m, part[1], max_nan);
   const float s = norm_scale(m * r);
   if (tid == 0) a.scale[blockIdx.x] = s;
-  for (int i = tid; i < a.H; i += 256)
-    a.q[at + i] = norm_code((double)load_any(hp, ht, at + i) * (double)load_any(a.w, a.w_type, i) * r, s);
+  const double g = s > 0.0f ? r / (double)s : 0.0;
+  for (int i = tid; i < a.H; i += 256) {
+    const double y = (double)load_any(hp, ht, at + i) * (double)load_any(a.w, a.w_type, i) * g;
+    a.q[at + i] = s > 0.0f ? (int8_t)fmin(fmax(__builtin_rint(y), -127.0), 127.0) : (int8_t)0;
+  }
 }
 
-// dx of one row a workgroup.
-__global__ __launch_bounds__(256) void k_rms_norm_dx_any(norm_grad_call a) {
+// The gradient of rows too long for registers: dx of one row a workgroup.
+__global__ __launch_bounds__(256) void k_rms_norm_dx_long(norm_grad_call a) {
   __shared__ double part[4];
   const size_t at = (size_t)blockIdx.x * a.H;
   const int tid = threadIdx.x;
@@ -107,7 +290,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_dx_any(norm_grad_call a) {
     const float g = load_any(a.dy, a.dy_type, at + i) * load_any(a.w, a.w_type, i);
     sum = fma((double)g, (double)(load_any(a.h, a.h_type, at + i) * r), sum);
   }
-  sum = block_reduce_d<4>(sum, part, [](double p, double q) { return p + q; });
+  sum = row_reduce_d<256>(sum, part, add_d);
   const float c = (float)(sum / a.H);
   for (int i = tid; i < a.H; i += 256) {
     const float g = load_any(a.dy, a.dy_type, at + i) * load_any(a.w, a.w_type, i);
@@ -118,7 +301,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_dx_any(norm_grad_call a) {
 }
 
 // dw of 64 columns a workgroup: wave v takes rows v, v + 4, ...
-__global__ __launch_bounds__(256) void k_rms_norm_dw_any(norm_grad_call a) {
+__global__ __launch_bounds__(256) void k_rms_norm_dw_long(norm_grad_call a) {
   __shared__ float part[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
   float sum = 0.0f;

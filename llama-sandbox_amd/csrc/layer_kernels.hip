@@ -8,9 +8,49 @@
 #include "kernels_route.h"
 #include "launch_common.h"
 
+#include <type_traits>
+
+// f(integral_constant) for the bytes of an element of type t.
+template <typename F>
+static void with_size(int t, F f) {
+  if (t == MOE_GGML_F32) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 2>{});
+}
+
+template <int SX, int SR, int LANES, int VPT>
+static void launch_norm(const norm_call &a, hipStream_t st) {
+  constexpr int NT = LANES < 256 ? 256 : LANES;
+  hipLaunchKernelGGL((k_rms_norm<SX, SR, LANES, VPT>), dim3(ceil_div(a.T, NT / LANES)), dim3(NT), 0, st, a);
+}
+
+template <int SX, int SR>
+static void launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
+  const int H = a.H;
+  if (a.T < 2 * n_cu && H > 512 && H <= 8192) {
+    if (H <= 2048) launch_norm<SX, SR, 256, 1>(a, st);
+    else launch_norm<SX, SR, 1024, 1>(a, st);
+  }
+  else if (H <= 128) launch_norm<SX, SR, 16, 1>(a, st);
+  else if (H <= 512) launch_norm<SX, SR, 64, 1>(a, st);
+  else if (H <= 1024) launch_norm<SX, SR, 64, 2>(a, st);
+  else if (H <= 2048) launch_norm<SX, SR, 64, 4>(a, st);
+  else if (H <= 4096) launch_norm<SX, SR, 256, 2>(a, st);
+  else if (H <= 6144) launch_norm<SX, SR, 256, 3>(a, st);
+  else if (H <= 8192) launch_norm<SX, SR, 256, 4>(a, st);
+  else if (H <= 16384) launch_norm<SX, SR, 1024, 2>(a, st);
+  else launch_norm<SX, SR, 1024, 4>(a, st);
+}
+
 bool launch_rms_norm(const norm_call &a, int n_cu, hipStream_t st) {
-  if (!fits(a.T, 256)) return false;
-  hipLaunchKernelGGL(k_rms_norm_any, dim3(a.T), dim3(256), 0, st, a);
+  if (!fits(a.T, 1024)) return false;
+  if (a.H > 32768) {
+    hipLaunchKernelGGL(k_rms_norm_long, dim3(a.T), dim3(256), 0, st, a);
+    return true;
+  }
+  with_size(a.x_type, [&](auto sx) {
+    if (!a.res) launch_norm<sx, 0>(a, n_cu, st);
+    else with_size(a.res_type, [&](auto sr) { launch_norm<sx, sr>(a, n_cu, st); });
+  });
   return true;
 }
 
@@ -18,8 +58,8 @@ size_t norm_grad_scratch(int T, int H, int n_cu) { return 1; }
 
 bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st) {
   if (!fits(a.T, 256)) return false;
-  hipLaunchKernelGGL(k_rms_norm_dx_any, dim3(a.T), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(k_rms_norm_dw_any, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_rms_norm_dx_long, dim3(a.T), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_rms_norm_dw_long, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
   return true;
 }
 
