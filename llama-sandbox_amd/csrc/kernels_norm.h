@@ -279,6 +279,143 @@ __global__ __launch_bounds__(256) void k_rms_norm_long(norm_call a) {
   }
 }
 
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = row16_sum(v);
+  if constexpr (LANES == 32) v += __shfl_xor(v, 16);
+  if constexpr (LANES == 64) v = (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
+  return v;
+}
+
+// The gradient in one pass over the rows: LANES threads hold one, G of them a workgroup, which walks
+// rows in steps of the grid, with the next row's loads in flight while it sums this one's, and keeps
+// its share of dw in registers; k_rms_norm_dw adds the shares up (part: one of H values a workgroup;
+// a single workgroup writes dw itself).  SD, SH, SX: bytes of an element of dy, h, dx and dres.
+template <int SD, int SH, int SX, int LANES, int VPT, int G>
+__global__ __launch_bounds__(LANES *G) void k_rms_norm_grad(norm_grad_call a) {
+  constexpr int NT = LANES * G, W = LANES > 64 ? LANES / 64 : 1;
+  __shared__ float sums[2][NT / 64];
+  __shared__ float share[G > 1 ? G : 1][G > 1 ? LANES * 8 + 4 : 1];  // of dw, of the groups
+  const int in_row = threadIdx.x % LANES, group = threadIdx.x / LANES, wave = threadIdx.x >> 6;
+  const int step = gridDim.x * G;
+  // rows of several vectors a thread leave no registers for the gain and the next row
+  constexpr bool AHEAD = VPT == 1;
+  float w[AHEAD ? VPT : 1][8], acc[VPT][8] = {};
+  auto load_w = [&](int v, float(&f)[8]) {
+    const int i = (in_row + v * LANES) * 8;
+    load8_any(a.w, a.w_type, i, a.H - i, f);
+  };
+  if constexpr (AHEAD) load_w(0, w[0]);
+  raw8<SD> d[VPT];
+  raw8<SH> h[VPT];
+  raw8<SX> s[VPT];
+  float r = 0.0f;
+  auto load = [&](long row) {
+    const bool there = row < a.T;
+    const size_t at = (size_t)(there ? row : 0) * a.H;
+    r = there ? a.rstd[row] : 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; v++) {
+      const int i = (in_row + v * LANES) * 8, left = there ? a.H - i : 0;
+      d[v].load(a.dy, at + i, left);
+      h[v].load(a.h, at + i, left);
+      if (a.dres) s[v].load(a.dres, at + i, left);
+    }
+  };
+  long row = (long)blockIdx.x * G + group;
+  if constexpr (AHEAD) load(row);
+  int turn = 0;
+  for (long first = (long)blockIdx.x * G; first < a.T; first += step, row += step, turn ^= 1) {
+    float g[VPT][8], u[VPT][8], res[VPT][8], dot = 0.0f;
+    if constexpr (!AHEAD) load(row);
+    const float rr = r;
+#pragma unroll
+    for (int v = 0; v < VPT; v++) {
+      if constexpr (!AHEAD) load_w(v, w[0]);
+      d[v].get(a.dy_type, g[v]);
+      h[v].get(a.h_type, u[v]);
+      if (a.dres) s[v].get(a.dx_type, res[v]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        u[v][j] *= rr;
+        acc[v][j] = fmaf(g[v][j], u[v][j], acc[v][j]);
+        g[v][j] *= w[0][j];
+        dot = fmaf(g[v][j], u[v][j], dot);
+      }
+    }
+    if constexpr (AHEAD) load(row + step);
+    dot = lanes_sum<(LANES < 64 ? LANES : 64)>(dot);
+    if constexpr (W > 1) {
+      if ((threadIdx.x & 63) == 0) sums[turn][wave] = dot;
+      __syncthreads();
+      dot = sums[turn][wave / W * W];
+#pragma unroll
+      for (int i = 1; i < W; i++) dot += sums[turn][wave / W * W + i];
+    }
+    const float c = dot / (float)a.H;
+    if (row < a.T) {
+#pragma unroll
+      for (int v = 0; v < VPT; v++) {
+        const int i = (in_row + v * LANES) * 8;
+        if (i >= a.H) break;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          o[j] = rr * fmaf(-u[v][j], c, g[v][j]);
+          if (a.dres) o[j] += res[v][j];
+        }
+        store8_any(a.dx, a.dx_type, (size_t)row * a.H + i, a.H - i, o);
+      }
+    }
+  }
+  float *to = gridDim.x > 1 ? a.part + (size_t)blockIdx.x * a.H : a.dw;
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    const int first = v * LANES * 8;
+    if constexpr (G == 1) {
+      const int i = first + in_row * 8;
+      if (i < a.H) store_v<float, 8>(to + i, a.H - i, acc[v]);
+    } else {
+      if (v > 0) __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; j++) share[group][in_row * 8 + j] = acc[v][j];
+      __syncthreads();
+      for (int i = threadIdx.x; i < LANES * 8 && first + i < a.H; i += NT) {
+        float sum = share[0][i];
+        for (int q = 1; q < G; q++) sum += share[q][i];
+        to[first + i] = sum;
+      }
+    }
+  }
+}
+
+// dw from the n workgroups' shares: 64 columns a workgroup, each of its 16 waves adds 4 shares at once,
+// 16 lanes with 4 columns each.
+__global__ __launch_bounds__(1024) void k_rms_norm_dw(const float *__restrict__ part, int n, int H, float *__restrict__ dw) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane % 16 * 4;
+  float sum[4] = {};
+#pragma unroll 4
+  for (int p = wave * 4 + lane / 16; p < n; p += 64) {
+    float f[4];
+    load_v<float, 4>(part + (size_t)p * H + i, H - i, f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum[j] += f[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    sum[j] += __shfl_xor(sum[j], 16);
+    sum[j] += __shfl_xor(sum[j], 32);
+    if (lane < 16) sums[wave][lane * 4 + j] = sum[j];
+  }
+  __syncthreads();
+  if (wave || blockIdx.x * 64 + lane >= H) return;
+  float s = sums[0][lane];
+#pragma unroll
+  for (int q = 1; q < 16; q++) s += sums[q][lane];
+  dw[blockIdx.x * 64 + lane] = s;
+}
+
 // The gradient of rows too long for registers: dx of one row a workgroup.
 __global__ __launch_bounds__(256) void k_rms_norm_dx_long(norm_grad_call a) {
   __shared__ double part[4];

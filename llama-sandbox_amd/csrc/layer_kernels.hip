@@ -54,12 +54,44 @@ bool launch_rms_norm(const norm_call &a, int n_cu, hipStream_t st) {
   return true;
 }
 
-size_t norm_grad_scratch(int T, int H, int n_cu) { return 1; }
+// The gradient's workgroups walk rows, G of them at once, one workgroup a CU: each has a share of dw.
+static int grad_groups(int H) { return H <= 128 ? 64 : H <= 512 ? 16 : H <= 1024 ? 8 : H <= 2048 ? 4 : H <= 4096 ? 2 : 1; }
+static int grad_blocks(int T, int H, int n_cu) {
+  const int most = ceil_div(T, grad_groups(H));
+  return most < n_cu ? most : n_cu;
+}
+
+size_t norm_grad_scratch(int T, int H, int n_cu) { return H > 16384 ? 1 : (size_t)grad_blocks(T, H, n_cu) * H; }
+
+template <int SD, int SH, int SX, int LANES, int VPT, int G>
+static void launch_grad(const norm_grad_call &a, int n, hipStream_t st) {
+  hipLaunchKernelGGL((k_rms_norm_grad<SD, SH, SX, LANES, VPT, G>), dim3(n), dim3(LANES * G), 0, st, a);
+}
+
+template <int SD, int SH, int SX>
+static void launch_grad(const norm_grad_call &a, int n, hipStream_t st) {
+  const int H = a.H;
+  if (H <= 128) launch_grad<SD, SH, SX, 16, 1, 64>(a, n, st);
+  else if (H <= 512) launch_grad<SD, SH, SX, 64, 1, 16>(a, n, st);
+  else if (H <= 1024) launch_grad<SD, SH, SX, 128, 1, 8>(a, n, st);
+  else if (H <= 2048) launch_grad<SD, SH, SX, 256, 1, 4>(a, n, st);
+  else if (H <= 4096) launch_grad<SD, SH, SX, 512, 1, 2>(a, n, st);
+  else if (H <= 8192) launch_grad<SD, SH, SX, 1024, 1, 1>(a, n, st);
+  else launch_grad<SD, SH, SX, 512, 4, 1>(a, n, st);
+}
 
 bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st) {
-  if (!fits(a.T, 256)) return false;
-  hipLaunchKernelGGL(k_rms_norm_dx_long, dim3(a.T), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(k_rms_norm_dw_long, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
+  if (!fits(a.T, 1024)) return false;
+  if (a.H > 16384) {
+    hipLaunchKernelGGL(k_rms_norm_dx_long, dim3(a.T), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_rms_norm_dw_long, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
+    return true;
+  }
+  const int n = grad_blocks(a.T, a.H, n_cu);
+  with_size(a.dy_type, [&](auto sd) {
+    with_size(a.h_type, [&](auto sh) { with_size(a.dx_type, [&](auto sx) { launch_grad<sd, sh, sx>(a, n, st); }); });
+  });
+  if (n > 1) hipLaunchKernelGGL(k_rms_norm_dw, dim3(ceil_div(a.H, 64)), dim3(1024), 0, st, a.part, n, a.H, a.dw);
   return true;
 }
 
