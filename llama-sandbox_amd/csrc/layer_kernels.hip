@@ -95,12 +95,25 @@ bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st) {
   return true;
 }
 
+template <typename K, int NJ>
+static bool launch_route(const route_call &a, hipStream_t st) {
+  if (a.T >= 1024) hipLaunchKernelGGL((k_route_groups<K, NJ, 4>), dim3(ceil_div(a.T, 4)), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_route_groups<K, NJ, 1>), dim3(a.T), dim3(64), 0, st, a);
+  return true;
+}
+template <typename K>
+static bool launch_route(const route_call &a, hipStream_t st) {
+  return a.E <= 64    ? launch_route<K, 1>(a, st)
+         : a.E <= 128 ? launch_route<K, 2>(a, st)
+         : a.E <= 256 ? launch_route<K, 4>(a, st)
+         : a.E <= 512 ? launch_route<K, 8>(a, st)
+                      : launch_route<K, 16>(a, st);
+}
+
+// Selection scores in 64 bits, but where their order is the logits'.
 bool launch_route_groups(const route_call &a, hipStream_t st) {
   if (!fits(a.T, 64)) return false;
-  with_type(a.type, [&](auto t) {
-    hipLaunchKernelGGL((k_route_groups<decltype(t)>), dim3(a.T), dim3(64), 0, st, a);
-  });
-  return true;
+  return !a.bias && (a.n_group == 1 || a.top == 1) ? launch_route<float>(a, st) : launch_route<double>(a, st);
 }
 
 bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
