@@ -3,12 +3,12 @@
 //
 // s = softmax(l), sigmoid(l) or sqrt(softplus(l)); an expert with l = -inf is masked: its score is 0 and it is
 // not picked.  c = s + bias.  Group score: the sum of the `top` largest c of the group's
-// unmasked experts (-inf without any); the `keep` best groups stay, and the k largest c
-// of their experts are picked; ties go to the lowest index, NaN comes after every number.
+// experts (numbers of unmasked ones; a group without any comes last); the `keep` best groups stay, and the k
+// largest c of their experts are picked; ties go to the lowest index, NaN comes after every number.
 // w = scale * s / max(sum of the picked s, 2^-14).
 //
-// Which experts are picked hangs on the order of scores that may be close: they are
-// compared in 64 bits, or by their logits where that is the same order (no bias, and no sum of two).
+// Which experts are picked hangs on the order of scores that may be close: they are compared as
+// 64-bit numbers would be, experts without a bias by their logits (the scores rise with them).
 // With p = s at the picked, S their sum, D = max(S, 2^-14):
 //   dp_i = scale / D (dw_i - [S >= 2^-14] sum_j dw_j p_j / D),  ds = dscores + dp at the picked
 //   softmax dl = s (ds - sum s ds), sigmoid dl = ds s (1 - s), sqrt softplus dl = ds sigmoid(l) / (2 s)
@@ -25,43 +25,42 @@
 __device__ __forceinline__ double route_score_d(double l, int mode) {
   return mode == MOE_ROUTE_SIGMOID ? 1.0 / (1.0 + exp(-l)) : sqrt(l > 40.0 ? l : log1p(exp(l)));
 }
+// (v_rcp_f32 is off by a step at most; what it takes to 0 is below 2^-126)
 __device__ __forceinline__ float route_score_f(float l, int mode) {
-  if (mode == MOE_ROUTE_SIGMOID) return __fdiv_rn(1.0f, 1.0f + expf(-l));
+  if (mode == MOE_ROUTE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + expf(-l));
   return l < -15.0f ? expf(0.5f * l) : sqrtf(fmaxf(l, 0.0f) + log1pf(expf(-fabsf(l))));  // (softplus: exp(l) up to exp(l) / 2)
 }
 
-__device__ __forceinline__ float wave_max_k(float v) { return wave_max(v); }
-__device__ __forceinline__ double wave_max_k(double v) {
-  v = fmax(v, dpp_d<0xB1>(v));
-  v = fmax(v, dpp_d<0x4E>(v));
-  v = fmax(v, dpp_d<0x141>(v));
-  v = fmax(v, dpp_d<0x140>(v));
-  return fmax(fmax(readlane_d(v, 0), readlane_d(v, 16)), fmax(readlane_d(v, 32), readlane_d(v, 48)));
-}
-__device__ __forceinline__ float readlane_k(float v, int lane) { return readlane_f(v, lane); }
-__device__ __forceinline__ double readlane_k(double v, int lane) { return readlane_d(v, lane); }
 __device__ __forceinline__ double wave_sum_d(double v) { return lanes_reduce_d<64>(v, add_d); }
-
-// What a selection score is compared as: a NaN is -inf, what is -inf the lowest finite value above it.
-template <typename K>
-__device__ __forceinline__ K route_key(K c) {
-  const K low = sizeof(K) == 8 ? (K)-1.7976931348623157e308 : (K)-3.4028234663852886e38f;
-  return c != c ? (K)-INFINITY : c < low ? low : c;
-}
-template <typename K>
-__device__ __forceinline__ K route_unkey(K k) {
-  const K low = sizeof(K) == 8 ? (K)-1.7976931348623157e308 : (K)-3.4028234663852886e38f;
-  return k <= low ? (K)-INFINITY : k;
+__device__ __forceinline__ double wave_max_d(double v) {
+  return lanes_reduce_d<64>(v, [](double a, double b) { return fmax(a, b); });
 }
 
-// The two largest of two pairs in order.
-template <typename K>
-__device__ __forceinline__ void route_merge(K &a1, K &a2, K b1, K b2) {
-  a2 = fmax(fmin(a1, b1), fmax(a2, b2));
-  a1 = fmax(a1, b1);
+// A score as a whole number that orders as it does, NaN below every number; 0: no candidate.
+__device__ __forceinline__ uint32_t route_key(float c) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, c);
+  return c != c ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// For 64 bits: a NaN is -inf, what is -inf the lowest finite value above it.
+#define MOE_ROUTE_LOW (-1.7976931348623157e308)
+#define MOE_ROUTE_LOW_F (-3.4028234663852886e38f)
+__device__ __forceinline__ double route_key_d(double c) { return c != c ? -INFINITY : c < MOE_ROUTE_LOW ? MOE_ROUTE_LOW : c; }
 
-// Logits [at, at + n) of a token as f32, -inf from `left` on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
+// The largest over the wave, as a scalar: five steps towards lane 63, one read.
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = dpp_max_u<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
+  v = dpp_max_u<0x112, 0xF>(v);
+  v = dpp_max_u<0x114, 0xF>(v);
+  v = dpp_max_u<0x118, 0xF>(v);
+  v = dpp_max_u<0x142, 0xA>(v);  // row_bcast15: the last lane of rows 0 and 2 to rows 1 and 3
+  v = dpp_max_u<0x143, 0xC>(v);  // row_bcast31: lane 31 to rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Logits [at, at + N) of a token as f32, -inf from `left` on.
 template <int N>
 __device__ __forceinline__ void route_load(const void *logits, int type, size_t at, int left, float (&l)[N]) {
   auto get = [&](auto t) {
@@ -82,107 +81,279 @@ __device__ __forceinline__ void route_load(const void *logits, int type, size_t 
   else get(bf16_t{});
 }
 
+__device__ __forceinline__ float readlane_k(float v, int lane) { return readlane_f(v, lane); }
+__device__ __forceinline__ double readlane_k(double v, int lane) { return readlane_d(v, lane); }
+template <int CTRL>
+__device__ __forceinline__ float dpp_k(float v) { return dpp_f<CTRL>(v); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_k(double v) { return dpp_d<CTRL>(v); }
+
+// Does the group of this lane stay?  width lanes side by side are a group's, the first n_group * width have one;
+// v1, v2: the two largest scores that this lane holds of it, -inf: none, what is -inf itself: the lowest
+// finite value.  near: how close two groups in 32 bits may be in another order than in 64; close: set
+// where the last that stays and the first that does not are.
+template <typename K>
+__device__ __forceinline__ bool route_stay(const route_call &a, K v1, K v2, int width, K near, bool &close) {
+  const K none = (K)-INFINITY, low = sizeof(K) == 8 ? (K)MOE_ROUTE_LOW : (K)MOE_ROUTE_LOW_F;
+  const int lane = threadIdx.x & 63, g = lane / width;
+  auto merge = [&](K b1, K b2) {
+    v2 = fmax(fmin(v1, b1), fmax(v2, b2));
+    v1 = fmax(v1, b1);
+  };
+  if (width > 1) merge(dpp_k<0xB1>(v1), dpp_k<0xB1>(v2));    // quad_perm [1,0,3,2]
+  if (width > 2) merge(dpp_k<0x4E>(v1), dpp_k<0x4E>(v2));    // quad_perm [2,3,0,1]
+  if (width > 4) merge(dpp_k<0x141>(v1), dpp_k<0x141>(v2));  // row_half_mirror
+  if (width > 8) merge(dpp_k<0x140>(v1), dpp_k<0x140>(v2));  // row_mirror
+  K score = v1;
+  if (a.top == 2 && v2 > none) {
+    const K sum = v1 <= low || v2 <= low ? none : v1 + v2;
+    score = sum > low ? sum : low;
+  }
+  int before = 0;  // groups that come before this lane's
+  for (int o = 0; o < a.n_group; o++) {
+    const K s = readlane_k(score, o * width);
+    before += s > score || (s == score && o < g);
+  }
+  const bool in = before < a.keep;
+  if (sizeof(K) == 4 && near > (K)0 && a.keep < a.n_group) {
+    const float first_out = wave_max(in || g >= a.n_group ? -INFINITY : (float)score);
+    const float last_in = -wave_max(in && g < a.n_group ? -(float)score : -INFINITY);
+    close = last_in > -INFINITY && !(last_in - first_out > (float)near);
+  }
+  return in;
+}
+
+// The same for any groups: c holds the experts' scores by index.  The ballot of the lanes whose groups stay.
+template <typename K>
+__device__ __forceinline__ uint64_t route_stay_any(const route_call &a, const K *c, K near, bool &close) {
+  const int lane = threadIdx.x & 63, g = lane / a.width;
+  K v1 = (K)-INFINITY, v2 = (K)-INFINITY;
+  if (g < a.n_group)
+    for (int e = g * a.per + lane % a.width; e < (g + 1) * a.per; e += a.width) {
+      v2 = fmax(v2, fmin(v1, c[e]));
+      v1 = fmax(v1, c[e]);
+    }
+  return __ballot(route_stay(a, v1, v2, a.width, near, close));
+}
+
 // One wave a token, WAVES tokens a workgroup.  Lane i holds experts [NJ i, NJ i + NJ) (E <= 64 NJ), so that of equal
-// keys the lowest lane has the lowest index, and a pick is a maximum over the wave and a ballot.  K: the type
-// that selection scores are compared in: float where they are the logits.
-template <typename K, int NJ, int WAVES>
+// keys the lowest lane has the lowest index, and a pick is a maximum over the wave and a ballot.
+// Scores with a bias are compared in 32 bits: that decides unless two that stand next to each other in the
+// order come closer than both may be off.  Then those that may be picked are placed by their scores in 64 bits,
+// and where it is two groups (or more experts than a wave has lanes) the token is done again in 64 bits.
+template <int NJ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
-  __shared__ K keys[WAVES][64 * NJ];  // for the groups' scores
+  // for the groups' scores
+  __shared__ float c32[WAVES][64 * NJ];
+  __shared__ double c64[WAVES][64 * NJ];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = a.E, e0 = lane * NJ;
   const long t = (long)blockIdx.x * WAVES + wave;
   if (t >= a.T) return;  // whole waves; no barrier below
   const size_t at = (size_t)t * E;
-  const bool soft = a.mode == MOE_ROUTE_SOFTMAX;
-  float l[NJ];
+  const bool soft = a.mode == MOE_ROUTE_SOFTMAX, sums = a.n_group > 1 && a.top == 2;
+  float l[NJ], b[NJ], p[NJ];
   route_load<NJ>(a.logits, a.type, at + e0, E - e0, l);
-  float b[NJ];
 #pragma unroll
-  for (int j = 0; j < NJ; j++) b[j] = sizeof(K) == 8 && a.bias && e0 + j < E ? a.bias[e0 + j] : 0.0f;
+  for (int j = 0; j < NJ; j++) b[j] = a.bias && e0 + j < E ? a.bias[e0 + j] : 0.0f;
   float top = 0.0f, sum = 1.0f;
-  double sum_d = 1.0;
   if (soft) {
     top = l[0];
 #pragma unroll
     for (int j = 1; j < NJ; j++) top = fmaxf(top, l[j]);
     top = wave_max(top);
     if (top == -INFINITY) top = 0.0f;
-    if constexpr (sizeof(K) == 8) {
-      sum_d = 0.0;
+    float some = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NJ; j++) sum_d += exp((double)l[j] - (double)top);
-      sum_d = wave_sum_d(sum_d);
-      sum = (float)sum_d;
-    } else {
-      sum = 0.0f;
+    for (int j = 0; j < NJ; j++) some += p[j] = expf(l[j] - top);
+    some = wave_sum(some);
+    sum = some != 0.0f ? some : 1.0f;  // (0: every expert is masked)
+  }
+  const float inv_sum = __fdiv_rn(1.0f, sum);
+  if (a.bias || a.scores || sums) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++) sum += expf(l[j] - top);
-      sum = wave_sum(sum);
-    }
+    for (int j = 0; j < NJ; j++) p[j] = l[j] == -INFINITY ? 0.0f : soft ? p[j] * inv_sum : route_score_f(l[j], a.mode);
   }
   if (a.scores) {
 #pragma unroll
     for (int j = 0; j < NJ; j++)
-      if (e0 + j < E)
-        a.scores[at + e0 + j] = l[j] == -INFINITY ? 0.0f : soft ? __fdiv_rn(expf(l[j] - top), sum) : route_score_f(l[j], a.mode);
+      if (e0 + j < E) a.scores[at + e0 + j] = p[j];
   }
-  K key[NJ];
-  uint32_t left = 0;  // bit j: expert e0 + j may be picked
+  // how close two scores in 32 bits may be in another order than in 64: each is off by 7 half steps of f32 (2^-24) of
+  // p, softmax's by 33 and twice the size of the exponent, and one of c; those next to 0 by steps of the smallest values
+  float near = 0.0f;
+  if (a.bias || sums) {
+    float big = 0.0f, each = 7.0f;
+    if (soft) {
+      float low = 0.0f;
 #pragma unroll
-  for (int j = 0; j < NJ; j++) {
-    if constexpr (sizeof(K) == 8)
-      key[j] = route_key((soft ? exp((double)l[j] - (double)top) / sum_d : route_score_d((double)l[j], a.mode)) + (double)b[j]);
-    else
-      key[j] = route_key(l[j]);
-    if (l[j] != -INFINITY) left |= 1u << j;
+      for (int j = 0; j < NJ; j++)
+        if (l[j] != -INFINITY) low = fmaxf(low, top - l[j]);
+      each = 33.0f + 2.0f * fminf(wave_max(low), 100.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const float size = fmaf(each, p[j], fabsf(p[j] + b[j]));
+      big = l[j] != -INFINITY && size < INFINITY ? fmaxf(big, size) : big;  // (infinities are what they are in 64 bits)
+    }
+    near = wave_max(big) * 0x1p-23f + 0x1p-120f;
   }
+  uint32_t key[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) key[j] = l[j] == -INFINITY ? 0 : route_key(a.bias ? p[j] + b[j] : l[j]);
+  const float inv_per = 1.0f / (float)a.per;
+  bool again = false;
+  auto drop = [&](uint64_t stay, auto f) {  // f(j) of the experts whose groups do not stay
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int g = (int)(((float)(e0 + j) + 0.5f) * inv_per);  // (e0 + j) / per: a half is more than the product is off
+      if (e0 + j < E && !((stay >> g * a.width) & 1)) f(j);
+    }
+  };
   if (a.n_group > 1) {
-    // lanes g * width .. of group g scan it
-    const int per = E / a.n_group, width = a.n_group <= 4 ? 16 : 64 >> (32 - __builtin_clz(a.n_group - 1));
-    K v1 = (K)-INFINITY, v2 = (K)-INFINITY;
+    float c[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) keys[wave][e0 + j] = (left >> j) & 1 ? key[j] : (K)-INFINITY;
-    __builtin_amdgcn_wave_barrier();
-    const int g = lane / width;
-    if (g < a.n_group)
-      for (int e = g * per + lane % width; e < (g + 1) * per; e += width) route_merge(v1, v2, keys[wave][e], (K)-INFINITY);
-    for (int off = 1; off < width; off <<= 1) {
-      const K o1 = __shfl_xor(v1, off), o2 = __shfl_xor(v2, off);
-      route_merge(v1, v2, o1, o2);
+    for (int j = 0; j < NJ; j++) {
+      const float v = a.bias ? p[j] + b[j] : sums ? p[j] : l[j];
+      c[j] = l[j] == -INFINITY || v != v ? -INFINITY : fmaxf(v, MOE_ROUTE_LOW_F);
     }
-    // a group without a number: -inf; of one number, that one
-    const K score = a.top == 2 && v2 > (K)-INFINITY ? route_unkey(v1) + route_unkey(v2) : route_unkey(v1);
-    int before = 0;  // groups that come before this lane's
-    for (int o = 0; o < a.n_group; o++) {
-      const K s = readlane_k(score, o * width);
-      before += s > score || (s == score && o < g);
-    }
-    const uint64_t stay = __ballot(before < a.keep);
+    if (a.lanes) {  // whole lanes are a group's
+      float v1 = c[0], v2 = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NJ; j++)
-      if (e0 + j < E && !((stay >> ((e0 + j) / per * width)) & 1)) left &= ~(1u << j);
-  }
-  int my_id = -1;  // lane s: the expert of slot s
-  for (int s = 0; s < a.k; s++) {
-    K best = (K)-INFINITY;
-    int bj = -1;
-#pragma unroll
-    for (int j = 0; j < NJ; j++)
-      if (((left >> j) & 1u) && (bj < 0 || key[j] > best)) {
-        best = key[j];
-        bj = j;
+      for (int j = 1; j < NJ; j++) {
+        v2 = fmaxf(v2, fminf(v1, c[j]));
+        v1 = fmaxf(v1, c[j]);
       }
-    const K mx = wave_max_k(best);
-    const uint64_t m = __ballot(bj >= 0 && best == mx);
-    if (!m) break;
-    const int src = __ffsll((unsigned long long)m) - 1, id = src * NJ + __builtin_amdgcn_readlane(bj, src);
-    if (lane == src) left &= ~(1u << bj);
-    if (lane == s) my_id = id;
+      const bool in = route_stay<float>(a, v1, v2, a.lanes, 2.0f * near, again);
+#pragma unroll
+      for (int j = 0; j < NJ; j++) key[j] = in ? key[j] : 0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) c32[wave][e0 + j] = c[j];
+      __builtin_amdgcn_wave_barrier();
+      drop(route_stay_any<float>(a, c32[wave], 2.0f * near, again), [&](int j) { key[j] = 0; });
+    }
+  }
+  // lane s: the expert of slot s, and its key
+  int my_id = -1;
+  uint32_t my_key = 0;
+  if (!again) {
+    // a lane's keys in order, of equal ones the lower index first: its best left is key[0], and a pick moves the others up
+    uint32_t idx[NJ];
+    auto either = [](uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); };  // (one v_bfi)
+#pragma unroll
+    for (int j = 0; j < NJ; j++) idx[j] = e0 + j;
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+#pragma unroll
+      for (int j = i & 1; j + 1 < NJ; j += 2) {
+        const uint32_t k0 = key[j], k1 = key[j + 1], swap = k1 > k0 ? ~0u : 0u, i0 = idx[j], i1 = idx[j + 1];
+        key[j] = max(k0, k1);
+        key[j + 1] = min(k0, k1);
+        idx[j] = either(swap, i1, i0);
+        idx[j + 1] = either(swap, i0, i1);
+      }
+    // with a bias, as many more as may belong before the last of the k
+    auto value = [](uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k); };
+    float floor = INFINITY;
+    int n = 0;
+    for (; n < 64; n++) {
+      const uint32_t mx = wave_max_u(key[0]);
+      if (mx == 0) break;
+      if (n >= a.k - 1) {
+        if (n == a.k - 1) floor = mx > 1 && a.bias ? value(mx) - near : INFINITY;
+        else if (mx == 1 || !(value(mx) >= floor)) break;
+      }
+      const int src = __ffsll((unsigned long long)__ballot(key[0] == mx)) - 1;
+      const int id = __builtin_amdgcn_readlane((int)idx[0], src);
+      if (lane == n) {
+        my_id = id;
+        my_key = mx;
+      }
+      const uint32_t win = lane == src ? ~0u : 0u;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        key[j] = either(win, j + 1 < NJ ? key[j + 1] : 0u, key[j]);
+        if (j + 1 < NJ) idx[j] = either(win, idx[j + 1], idx[j]);
+      }
+    }
+    if (a.bias) {
+      // two that follow each other, both numbers
+      const uint32_t after = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)my_key, 0x130, 0xF, 0xF, false);  // wave_shl 1
+      if (__ballot(my_key > 1 && after > 1 && !(value(my_key) - value(after) > near))) {
+        again = n == 64;
+        if (!again) {  // those picked and those that may belong among them, by their place in 64 bits
+          double sum_d = 1.0, c = -INFINITY;
+          if (soft) {
+            sum_d = 0.0;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) sum_d += exp((double)l[j] - (double)top);
+            sum_d = wave_sum_d(sum_d);
+          }
+          if (my_id >= 0) {
+            float one[1];
+            route_load<1>(a.logits, a.type, at + my_id, 1, one);
+            c = route_key_d((soft ? exp((double)one[0] - (double)top) / sum_d : route_score_d((double)one[0], a.mode)) +
+                            (double)a.bias[my_id]);
+          }
+          int place = 0;
+          for (int o = 0; o < n; o++) {
+            const double other = readlane_d(c, o);
+            const int other_id = __builtin_amdgcn_readlane(my_id, o);
+            place += other > c || (other == c && other_id < my_id);
+          }
+          my_id = __builtin_amdgcn_ds_permute(4 * (lane < n ? place : lane), my_id);
+        }
+      }
+    }
+    if (lane >= a.k) my_id = -1;
+  }
+  if (again) {
+    double kd[NJ], sum_d = 1.0;
+    uint32_t left = 0;  // bit j: expert e0 + j may be picked
+    if (soft) {
+      sum_d = 0.0;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) sum_d += exp((double)l[j] - (double)top);
+      sum_d = wave_sum_d(sum_d);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      kd[j] = route_key_d((soft ? exp((double)l[j] - (double)top) / sum_d : route_score_d((double)l[j], a.mode)) + (double)b[j]);
+      if (l[j] != -INFINITY) left |= 1u << j;
+    }
+    if (a.n_group > 1) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) c64[wave][e0 + j] = (left >> j) & 1 ? kd[j] : -INFINITY;
+      __builtin_amdgcn_wave_barrier();
+      drop(route_stay_any<double>(a, c64[wave], 0.0, again), [&](int j) { left &= ~(1u << j); });
+    }
+    if (!a.bias) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) kd[j] = route_key_d((double)l[j]);
+    }
+    my_id = -1;
+    for (int s = 0; s < a.k; s++) {
+      double best = -INFINITY;
+      int bj = -1;
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        if (((left >> j) & 1u) && (bj < 0 || kd[j] > best)) {
+          best = kd[j];
+          bj = j;
+        }
+      const double mx = wave_max_d(best);
+      const uint64_t m = __ballot(bj >= 0 && best == mx);
+      if (!m) break;
+      const int src = __ffsll((unsigned long long)m) - 1, id = src * NJ + __builtin_amdgcn_readlane(bj, src);
+      if (lane == src) left &= ~(1u << bj);
+      if (lane == s) my_id = id;
+    }
   }
   float w = 0.0f;
   if (my_id >= 0) {
     float one[1];
     route_load<1>(a.logits, a.type, at + my_id, 1, one);
-    w = soft ? __fdiv_rn(expf(one[0] - top), sum) : route_score_f(one[0], a.mode);
+    w = soft ? expf(one[0] - top) * inv_sum : route_score_f(one[0], a.mode);
   }
   if (a.norm) {
     const float total = wave_sum(w);

@@ -37,6 +37,8 @@ struct route_call {
   float *wts, *scores;
   int type, T, E, k, mode, n_group, keep, top, norm;
   float scale;
+  // set by the launch: experts a group; lanes a group where each takes some; lanes that hold a whole one (0: none do)
+  int per = 0, width = 0, lanes = 0;
 };
 bool launch_route_groups(const route_call &a, hipStream_t st);
 

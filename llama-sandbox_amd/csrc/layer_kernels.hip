@@ -95,25 +95,25 @@ bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st) {
   return true;
 }
 
-template <typename K, int NJ>
-static bool launch_route(const route_call &a, hipStream_t st) {
-  if (a.T >= 1024) hipLaunchKernelGGL((k_route_groups<K, NJ, 4>), dim3(ceil_div(a.T, 4)), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_route_groups<K, NJ, 1>), dim3(a.T), dim3(64), 0, st, a);
-  return true;
-}
-template <typename K>
-static bool launch_route(const route_call &a, hipStream_t st) {
-  return a.E <= 64    ? launch_route<K, 1>(a, st)
-         : a.E <= 128 ? launch_route<K, 2>(a, st)
-         : a.E <= 256 ? launch_route<K, 4>(a, st)
-         : a.E <= 512 ? launch_route<K, 8>(a, st)
-                      : launch_route<K, 16>(a, st);
+template <int NJ>
+static void launch_route(route_call a, hipStream_t st) {
+  const int n = a.per / NJ;
+  if (a.per % NJ == 0 && n <= 16 && (n & (n - 1)) == 0) a.lanes = n;
+  if (a.T >= 1024) hipLaunchKernelGGL((k_route_groups<NJ, 4>), dim3(ceil_div(a.T, 4)), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_route_groups<NJ, 1>), dim3(a.T), dim3(64), 0, st, a);
 }
 
-// Selection scores in 64 bits, but where their order is the logits'.
-bool launch_route_groups(const route_call &a, hipStream_t st) {
-  if (!fits(a.T, 64)) return false;
-  return !a.bias && (a.n_group == 1 || a.top == 1) ? launch_route<float>(a, st) : launch_route<double>(a, st);
+bool launch_route_groups(const route_call &args, hipStream_t st) {
+  if (!fits(args.T, 64)) return false;
+  route_call a = args;
+  a.per = a.E / a.n_group;
+  for (a.width = 16; a.width * a.n_group > 64;) a.width >>= 1;
+  if (a.E <= 64) launch_route<1>(a, st);
+  else if (a.E <= 128) launch_route<2>(a, st);
+  else if (a.E <= 256) launch_route<4>(a, st);
+  else if (a.E <= 512) launch_route<8>(a, st);
+  else launch_route<16>(a, st);
+  return true;
 }
 
 bool launch_route_grad(const route_grad_call &a, hipStream_t st) {

@@ -90,21 +90,21 @@ def route(l, bias, k, mode, n_group, keep, top, norm, scale):
     l = l.astype(np.float64)
     T, E = l.shape
     p = scores(l, mode)
-    by_logit = bias is None and (n_group == 1 or top == 1)
-    c = l if by_logit else p if bias is None else p + bias.astype(np.float64)
+    c = p if bias is None else p + bias.astype(np.float64)
+    key = l if bias is None else c  # without a bias the scores are in the logits' order
+    group_key = key if top == 1 else c
     per = E // n_group
     ids, wts = np.full((T, k), -1, np.int32), np.zeros((T, k))
     for t in range(T):
         there = [e for e in range(E) if l[t, e] != -np.inf]
         if n_group > 1:
-            g_score = np.full(n_group, -np.inf)
+            order = []
             for g in range(n_group):
-                best = _order(c[t], [e for e in there if e // per == g])[:top]
-                if best:
-                    g_score[g] = sum(c[t, best])
-            stay = set(_order(g_score, range(n_group))[:keep])
+                best = _order(group_key[t], [e for e in there if e // per == g and not np.isnan(group_key[t, e])])[:top]
+                order.append((not best, -sum(group_key[t, best]) if best else 0.0, g))
+            stay = {g for _, _, g in sorted(order)[:keep]}
             there = [e for e in there if e // per in stay]
-        pick = _order(c[t], there)[:k]
+        pick = _order(key[t], there)[:k]
         ids[t, :len(pick)], wts[t, :len(pick)] = pick, p[t, pick]
     if norm:
         wts = wts / np.maximum(wts.sum(1, keepdims=True), FLOOR)
