@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
 
 // s and its slope of one logit, element-wise score functions.
 __device__ __forceinline__ void route_slope(float l, int mode, float &s, float &slope) {
-  const float z = expf(-fabsf(l)), big = __fdiv_rn(1.0f, 1.0f + z), sig = l >= 0.0f ? big : z * big;
+  const float z = expf(-fabsf(l)), big = __builtin_amdgcn_rcpf(1.0f + z), sig = l >= 0.0f ? big : z * big;
   if (mode == MOE_ROUTE_SIGMOID) {
     s = sig;
     slope = big * (z * big);
@@ -381,55 +381,72 @@ __device__ __forceinline__ void route_slope(float l, int mode, float &s, float &
   }
 }
 
-// One wave a token.
-template <typename T>
-__global__ __launch_bounds__(64) void k_route_grad(route_grad_call a) {
-  __shared__ float s[MOE_ROUTE_GROUPS_MAX_E], ds[MOE_ROUTE_GROUPS_MAX_E];
-  const int t = blockIdx.x, lane = threadIdx.x, E = a.E;
-  const T *l = reinterpret_cast<const T *>(a.logits) + (size_t)t * E;
-  const float *from = a.dscores ? a.dscores + (size_t)t * E : nullptr;
+// One wave a token, WAVES a workgroup, lane i with experts [NJ i, NJ i + NJ) in registers.  The picked
+// experts' gradients go to their lanes slot by slot, which adds an expert that is named twice in slot order.
+template <int NJ, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_route_grad(route_grad_call a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = a.E, e0 = lane * NJ;
+  const long t = (long)blockIdx.x * WAVES + wave;
+  if (t >= a.T) return;  // whole waves
+  const size_t at = (size_t)t * E;
   const bool soft = a.mode == MOE_ROUTE_SOFTMAX;
-  float top = -INFINITY, sum = 0.0f, unused;
-  if (soft) {
-    for (int e = lane; e < E; e += 64) top = fmaxf(top, (float)l[e]);
-    top = wave_max(top);
-    if (top == -INFINITY) top = 0.0f;
-    for (int e = lane; e < E; e += 64) sum += s[e] = expf((float)l[e] - top);
-    sum = wave_sum(sum);
+  float l[NJ], ds[NJ], p[NJ], slope[NJ];
+  route_load<NJ>(a.logits, a.type, at + e0, E - e0, l);
+  if (a.dscores) {
+    load_v<float, NJ>(a.dscores + at + e0, E - e0, ds);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) ds[j] = 0.0f;
   }
-  for (int e = lane; e < E; e += 64) {
-    const float v = (float)l[e];
-    if (v == -INFINITY) s[e] = 0.0f;
-    else if (soft) s[e] = __fdiv_rn(s[e], sum);
-    else route_slope(v, a.mode, s[e], unused);
-    ds[e] = from ? from[e] : 0.0f;
-  }
-  __syncthreads();
+  // lane s: slot s
   const int id = lane < a.k ? a.ids[(size_t)t * a.k + lane] : -1;
   const bool there = id >= 0 && id < E;
-  float dw = there ? a.dwts[(size_t)t * a.k + lane] : 0.0f;
+  float dw = there ? a.dwts[(size_t)t * a.k + lane] : 0.0f, mine[1] = {-INFINITY};
+  if (there) route_load<1>(a.logits, a.type, at + id, 1, mine);
+  float top = 0.0f, inv_sum = 1.0f, own, unused;
+  if (soft) {
+    top = l[0];
+#pragma unroll
+    for (int j = 1; j < NJ; j++) top = fmaxf(top, l[j]);
+    top = wave_max(top);
+    if (top == -INFINITY) top = 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) sum += p[j] = expf(l[j] - top);
+    sum = wave_sum(sum);
+    inv_sum = __fdiv_rn(1.0f, sum != 0.0f ? sum : 1.0f);  // (0: every expert is masked)
+#pragma unroll
+    for (int j = 0; j < NJ; j++) p[j] *= inv_sum;
+    own = expf(mine[0] - top) * inv_sum;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) route_slope(l[j], a.mode, p[j], slope[j]);
+    route_slope(mine[0], a.mode, own, unused);
+  }
+  if (mine[0] == -INFINITY) own = 0.0f;
   if (a.scale != 0.0f) dw *= a.scale;
   if (a.norm) {
-    const float p = there ? s[id] : 0.0f, S = wave_sum(p), D = fmaxf(S, MOE_ROUTE_FLOOR), in = wave_sum(dw * p);
+    const float S = wave_sum(own), in = wave_sum(dw * own), D = fmaxf(S, MOE_ROUTE_FLOOR);
     dw = __fdiv_rn(dw - (S >= MOE_ROUTE_FLOOR ? __fdiv_rn(in, D) : 0.0f), D);
   }
-  for (int j = 0; j < a.k; j++) {
-    if (lane == j && there) ds[id] += dw;  // in slot order, also where an expert is named twice
-    __syncthreads();
+  if (!there) dw = 0.0f;
+  for (int s = 0; s < a.k; s++) {
+    const int e = __builtin_amdgcn_readlane(id, s);
+    const float d = readlane_f(dw, s);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) ds[j] += e0 + j == e ? d : 0.0f;
   }
   float in = 0.0f;
-  if (soft)
-    for (int e = lane; e < E; e += 64) in = s[e] != 0.0f ? fmaf(s[e], ds[e], in) : in;
-  in = wave_sum(in);
-  for (int e = lane; e < E; e += 64) {
-    const float v = (float)l[e];
-    float slope = s[e], d;
-    if (!soft) route_slope(v, a.mode, unused, slope);
-    d = soft ? s[e] * (ds[e] - in) : ds[e] * slope;
-    if (v == -INFINITY) d = 0.0f;
-    const size_t at = (size_t)t * E + e;
-    if (a.out_type == MOE_GGML_F32) reinterpret_cast<float *>(a.dlogits)[at] = d;
-    else if (a.out_type == MOE_GGML_F16) reinterpret_cast<_Float16 *>(a.dlogits)[at] = (_Float16)d;
-    else reinterpret_cast<bf16_t *>(a.dlogits)[at] = (bf16_t)d;
+  if (soft) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) in = p[j] != 0.0f ? fmaf(p[j], ds[j], in) : in;
+    in = wave_sum(in);
   }
+  float d[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) d[j] = l[j] == -INFINITY ? 0.0f : soft ? p[j] * (ds[j] - in) : ds[j] * slope[j];
+  if (e0 >= E) return;
+  if (a.out_type == MOE_GGML_F32) store_v<float, NJ>(reinterpret_cast<float *>(a.dlogits) + at + e0, E - e0, d);
+  else if (a.out_type == MOE_GGML_F16) store_v<_Float16, NJ>(reinterpret_cast<_Float16 *>(a.dlogits) + at + e0, E - e0, d);
+  else store_v<bf16_t, NJ>(reinterpret_cast<bf16_t *>(a.dlogits) + at + e0, E - e0, d);
 }

@@ -116,11 +116,19 @@ bool launch_route_groups(const route_call &args, hipStream_t st) {
   return true;
 }
 
+template <int NJ>
+static void launch_grad(const route_grad_call &a, hipStream_t st) {
+  if (a.T >= 1024) hipLaunchKernelGGL((k_route_grad<NJ, 4>), dim3(ceil_div(a.T, 4)), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_route_grad<NJ, 1>), dim3(a.T), dim3(64), 0, st, a);
+}
+
 bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
   if (!fits(a.T, 64)) return false;
-  with_type(a.type, [&](auto t) {
-    hipLaunchKernelGGL((k_route_grad<decltype(t)>), dim3(a.T), dim3(64), 0, st, a);
-  });
+  if (a.E <= 64) launch_grad<1>(a, st);
+  else if (a.E <= 128) launch_grad<2>(a, st);
+  else if (a.E <= 256) launch_grad<4>(a, st);
+  else if (a.E <= 512) launch_grad<8>(a, st);
+  else launch_grad<16>(a, st);
   return true;
 }
 

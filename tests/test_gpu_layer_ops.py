@@ -294,6 +294,50 @@ def test_route_ties_go_to_the_lowest_index(blk, mode, n_group, keep, top):
             check_route(run_route(blk, l, bias, *args), l, bias, *args)
 
 
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("n_group, keep, top", [(1, 1, 1), (8, 3, 2), (8, 3, 1), (5, 2, 2)])
+@pytest.mark.parametrize("alike", [2, 5, 20, 160])
+def test_route_of_scores_closer_than_32_bits_tell(blk, mode, n_group, keep, top, alike):
+    """Biases that bring some experts' scores within a rounding of each other: the order in 32 bits is another than
+    in 64 for some tokens (which the test checks of its inputs), and the one in 64 holds."""
+    say("route close", mode, n_group, keep, top, alike)
+    rng = np.random.default_rng(alike + mode)
+    E, args = 160, (8, mode, n_group, keep, top, True, 1.0)
+    other = 0
+    for _ in range(6):
+        l = rng.standard_normal((1, E)).astype(np.float32)
+        p = ref.scores(l.astype(np.float64), mode)[0]
+        bias = (0.1 * rng.standard_normal(E)).astype(np.float32)
+        some = rng.permutation(E)[:alike]
+        bias[some] = (2.0 - p[some]).astype(np.float32)
+        check_route(run_route(blk, torch.from_numpy(l), bias, *args), torch.from_numpy(l), bias, *args)
+        c32 = p[some].astype(np.float32) + bias[some]
+        other += (np.argsort(-c32, kind="stable") != np.argsort(-(p[some] + bias[some].astype(np.float64)), kind="stable")).any()
+    assert other
+
+
+def test_route_of_groups_closer_than_32_bits_tell(blk):
+    """Groups whose two best scores sum to within a rounding of the same."""
+    say("route groups close")
+    rng = np.random.default_rng(11)
+    E, G, args = 64, 8, (4, 1, 8, 3, 2, True, 1.0)
+    other = 0
+    for _ in range(12):
+        l = rng.standard_normal((1, E)).astype(np.float32)
+        p = ref.scores(l.astype(np.float64), 1)[0]
+        bias = np.full(E, -1.0, np.float32)
+        for g in range(G):
+            a, b = g * 8 + rng.permutation(8)[:2]
+            bias[a] = 0.25 + 0.1 * g
+            bias[b] = np.float32(3.0 - p[b] - p[a] - np.float64(bias[a]))
+        check_route(run_route(blk, torch.from_numpy(l), bias, *args), torch.from_numpy(l), bias, *args)
+        c = p + bias.astype(np.float64)
+        two = np.sort(c.reshape(G, 8), 1)[:, -2:].sum(1)
+        two32 = np.sort((p.astype(np.float32) + bias).reshape(G, 8), 1)[:, -2:].sum(1)
+        other += set(np.argsort(-two, kind="stable")[:3]) != set(np.argsort(-two32, kind="stable")[:3])
+    assert other
+
+
 def test_route_of_extreme_logits(blk):
     """The type's lowest and highest values, saturated scores, infinities and NaN."""
     say("route extremes")
