@@ -132,15 +132,48 @@ bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
   return true;
 }
 
-size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)M * R; }
+// Rows of an adapter a workgroup.
+static int adapters_tile(int M) { return M <= 64 ? 16 : 32; }
 
-bool launch_adapters(const adapters_call &a, int n_cu, hipStream_t st) {
-  if (a.M > 65535) return false;
+// Pieces of K that the product with A is cut into: workgroups for the chip (four a CU where every tile is full), each
+// with eight steps at least.
+static int adapters_splits(int M, int K, int n_cu) {
+  const int most = ceil_div(K, 256), want = ceil_div(4L * n_cu, ceil_div(M, adapters_tile(M)));
+  return most < want ? most : want;
+}
+
+size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, n_cu) * M * R; }
+
+template <typename T, int MT>
+static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
+  const unsigned x = (unsigned)(tiles * a.splits);
+  if (a.R <= 16) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 1>), dim3(x), dim3(256), 0, st, a);
+  else if (a.R <= 32) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 2>), dim3(x), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_adapters_shrink<T, MT, 4>), dim3(x, ceil_div(a.R, 64)), dim3(256), 0, st, a);
+}
+
+template <typename T, typename TO, int MT>
+static void launch_expand(const adapters_call &a, long tiles, hipStream_t st) {
+  // parts of mid: see k_adapters_expand
+  constexpr int PARTS = sizeof(T) == 4 ? 1 : std::is_same<T, bf16_t>::value && sizeof(TO) == 2 ? 2 : 3;
+  hipLaunchKernelGGL((k_adapters_expand<T, TO, MT, PARTS>), dim3((unsigned)(tiles * a.col_blocks)), dim3(256), 0, st, a);
+}
+
+bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
+  adapters_call a = args;
+  const int BM = adapters_tile(a.M);
+  a.splits = adapters_splits(a.M, a.K, n_cu);
+  a.piece = ceil_div(ceil_div(a.K, a.splits), 32) * 32;
+  a.col_blocks = ceil_div(a.N, 256);
+  const long tiles = (a.M + (long)(a.M < a.n ? a.M : a.n) * (BM - 1)) / BM;
+  if (!fits(tiles * a.splits, 256) || !fits(tiles * a.col_blocks, 256)) return false;
   with_type(a.type, [&](auto t) {
     typedef decltype(t) T;
-    hipLaunchKernelGGL((k_adapters_shrink<T>), dim3(ceil_div(a.R, 4), a.M), dim3(256), 0, st, a);
+    if (BM == 16) launch_shrink<T, 1>(a, tiles, st);
+    else launch_shrink<T, 2>(a, tiles, st);
     with_type(a.out_type, [&](auto to) {
-      hipLaunchKernelGGL((k_adapters_expand<T, decltype(to)>), dim3(ceil_div(a.N, 256), a.M), dim3(256), 0, st, a);
+      if (BM == 16) launch_expand<T, decltype(to), 1>(a, tiles, st);
+      else launch_expand<T, decltype(to), 2>(a, tiles, st);
     });
   });
   return true;
