@@ -56,13 +56,13 @@ __device__ __forceinline__ int adapters_row(const adapters_call &a, const row_ti
 }
 
 // mid, as a.splits shares of it, [split][grouped row][R].  grid (tiles * splits, ceil(R / (16 RT))): a workgroup has the share
-// of one piece of K of 16 MT grouped rows and 16 RT rows of A; its 4 waves take every fourth step of K and meet in LDS.
+// of one piece of K of 16 MT grouped rows and 16 RT rows of A; its waves take pieces of U steps in turn and meet in LDS.
 // Absent rows read another's (their columns are not written).
-template <typename T, int MT, int RT>
-__global__ __launch_bounds__(256) void k_adapters_shrink(adapters_call a) {
+template <typename T, int MT, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a) {
   typedef frag<T> F;
-  constexpr int U = MT + RT > 4 ? 2 : 4;  // steps in flight
-  __shared__ f32x4_t part[3][MT * RT][64];
+  constexpr int U = MT + RT > 4 ? 2 : 4;  // steps in flight, next to each other in memory
+  __shared__ f32x4_t part[WAVES][MT * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, split = blockIdx.x % a.splits;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.splits, 16 * MT);
   if (t.e < 0) return;
@@ -77,17 +77,26 @@ __global__ __launch_bounds__(256) void k_adapters_shrink(adapters_call a) {
   for (int r = 0; r < RT; r++)
     w[r] = reinterpret_cast<const T *>(a.a) + ((size_t)t.e * a.R + min(r0 + r * 16 + lane % 16, a.R - 1)) * a.K + k0;
   f32x4_t acc[MT][RT] = {};
-  const int begin = split * a.piece + wave * F::STEP, end = min(a.K, (split + 1) * a.piece);
-  int k = begin;
-  // whole steps, U at once
-  for (; k + ((U - 1) * 4 + 1) * F::STEP <= end; k += U * 4 * F::STEP) {
+  const int end = min(a.K, (split + 1) * a.piece);
+  for (int k = split * a.piece + wave * U * F::STEP; k < end; k += WAVES * U * F::STEP) {
     F fx[U][MT], fw[U][RT];
+    if (k + U * F::STEP <= end) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+      for (int u = 0; u < U; u++) {
 #pragma unroll
-      for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * 4 * F::STEP);
+        for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * F::STEP);
 #pragma unroll
-      for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * 4 * F::STEP);
+        for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * F::STEP);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int left = end - k - u * F::STEP - k0;
+#pragma unroll
+        for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * F::STEP, left);
+#pragma unroll
+        for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * F::STEP, left);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -96,37 +105,18 @@ __global__ __launch_bounds__(256) void k_adapters_shrink(adapters_call a) {
 #pragma unroll
         for (int r = 0; r < RT; r++) acc[m][r] = mfma16(fw[u][r], fx[u][m], acc[m][r]);
   }
-  for (; k < end; k += 4 * F::STEP) {
-    F fx[MT], fw[RT];
 #pragma unroll
-    for (int m = 0; m < MT; m++) fx[m].load(x[m] + k, end - k - k0);
+  for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int r = 0; r < RT; r++) fw[r].load(w[r] + k, end - k - k0);
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int r = 0; r < RT; r++) acc[m][r] = mfma16(fw[r], fx[m], acc[m][r]);
-  }
-  if (wave) {
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int r = 0; r < RT; r++) part[wave - 1][m * RT + r][lane] = acc[m][r];
-  }
+    for (int r = 0; r < RT; r++) part[wave][m * RT + r][lane] = acc[m][r];
   __syncthreads();
-  if (wave) return;
+  for (int q = wave; q < MT * RT; q += WAVES) {
+    f32x4_t sum = part[0][q][lane];
 #pragma unroll
-  for (int m = 0; m < MT; m++) {
-    const int i = m * 16 + lane % 16;
-    if (i >= t.n) continue;
-    float *to = a.mid + ((size_t)split * a.M + t.r0 + i) * a.R;
-#pragma unroll
-    for (int r = 0; r < RT; r++) {
-      const f32x4_t sum = (acc[m][r] + part[0][m * RT + r][lane]) + (part[1][m * RT + r][lane] + part[2][m * RT + r][lane]);
-      const float f[4] = {sum[0], sum[1], sum[2], sum[3]};
-      const int at = r0 + r * 16 + lane / 16 * 4;
-      if (at < a.R) store_v<float, 4>(to + at, a.R - at, f);
-    }
+    for (int v = 1; v < WAVES; v++) sum += part[v][q][lane];
+    const int i = q / RT * 16 + lane % 16, at = r0 + q % RT * 16 + lane / 16 * 4;
+    const float f[4] = {sum[0], sum[1], sum[2], sum[3]};
+    if (i < t.n && at < a.R) store_v<float, 4>(a.mid + ((size_t)split * a.M + t.r0 + i) * a.R + at, a.R - at, f);
   }
 }
 
@@ -153,89 +143,125 @@ __device__ __forceinline__ void weight_parts(const frag<_Float16> &w, frag<bf16_
   }
 }
 
-// out.  grid (tiles * column blocks): 16 MT grouped rows by 256 columns of out a workgroup, 64 a wave; mid's shares
-// are added up and cut into parts in LDS, 64 of R at a time.
+// out.  grid (tiles * column blocks): 16 MT grouped rows by a.col_groups times 256 columns of out a workgroup, 64 a wave;
+// mid's shares are added up and cut into parts in LDS, 64 of R at a time.
 template <typename T, typename TO, int MT, int PARTS>
 __global__ __launch_bounds__(256) void k_adapters_expand(adapters_call a) {
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
   constexpr int RC = 64, STEPS = RC / F::STEP, WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
-  constexpr int ROW = RC + F::V;  // a piece more, so that rows lie in different banks
+  constexpr int ROW = RC + F::V;            // a piece more, so that rows lie in different banks
+  constexpr int SLOTS = 16 * MT * RC / 1024;  // of 4 values of mid that a thread cuts
   __shared__ __attribute__((aligned(16))) TE mid[PARTS][16 * MT][ROW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % 16, kg = lane / 16;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.col_blocks, 16 * MT);
   if (t.e < 0) return;
-  const int n0 = blockIdx.x % a.col_blocks * 256 + wave * 64;
   const T *b = reinterpret_cast<const T *>(a.b) + (size_t)t.e * a.N * a.R;
-  // lane's 8 columns n0 + 32 q + 8 kg + .. of the pairs q of weight tiles, of rows m * 16 + col
+  const float scale = a.scale ? a.scale[t.e] : 1.0f;
   int row[MT];
-  raw_v<TO, 8> base[MT][2];
 #pragma unroll
-  for (int m = 0; m < MT; m++) {
-    row[m] = adapters_row(a, t, m * 16 + col);
+  for (int m = 0; m < MT; m++) row[m] = adapters_row(a, t, m * 16 + col);
+
+  auto stage = [&](int rc) {
+    float f[SLOTS][4] = {};
+    for (int s = 0; s < a.splits; s += 4) {
+      float g[SLOTS][4][4];
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-      const int n = n0 + q * 32 + kg * 8;
-      base[m][q].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[m] < 0 ? 0 : row[m]) * a.N + n,
-                      row[m] < 0 ? 0 : a.N - n);
-    }
-  }
-  f32x4_t acc[MT][4] = {};
-  for (int rc = 0; rc < a.R; rc += RC) {
-    if (rc) __syncthreads();
-    for (int i = threadIdx.x; i < 16 * MT * RC; i += 256) {
-      const int m = i / RC, r = rc + i % RC;
-      float f = 0.0f;
-      if (m < t.n && r < a.R) {
-        const float *from = a.mid + (size_t)(t.r0 + m) * a.R + r;
-#pragma unroll 8
-        for (int s = 0; s < a.splits; s++) f += from[(size_t)s * a.M * a.R];
+      for (int q = 0; q < SLOTS; q++) {
+        const int i = threadIdx.x + q * 256, m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
+        const float *from = a.mid + ((size_t)s * a.M + t.r0 + m) * a.R + r;
+#pragma unroll
+        for (int v = 0; v < 4; v++) load_v<float, 4>(from + (size_t)v * a.M * a.R, s + v < a.splits && m < t.n ? a.R - r : 0, g[q][v]);
       }
+#pragma unroll
+      for (int q = 0; q < SLOTS; q++)
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) f[q][j] += g[q][v][j];
+    }
+#pragma unroll
+    for (int q = 0; q < SLOTS; q++) {
+      const int i = threadIdx.x + q * 256;
+      typedef TE vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int p = 0; p < PARTS; p++) {
-        const TE part = (TE)f;
-        mid[p][m][i % RC] = part;
-        f -= (float)part;
+        vec4 o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          o[j] = (TE)f[q][j];
+          f[q][j] -= (float)o[j];
+        }
+        *reinterpret_cast<vec4 *>(&mid[p][i / (RC / 4)][i % (RC / 4) * 4]) = o;
       }
     }
-    __syncthreads();
+  };
+
+  const int first = (blockIdx.x % a.col_blocks * a.col_groups) * 256 + wave * 64;
+  // a lane's 8 columns n0 + 32 q + 8 kg + .. of the pairs q of weight tiles, of rows m * 16 + col
+  raw_v<TO, 8> base[MT][2];
+  auto load_base = [&](int n0) {
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-      const int r = s * F::STEP + kg * F::V;
-      if (rc + s * F::STEP >= a.R) break;
-      F fm[MT][PARTS];
+    for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int q = 0; q < 2; q++) {
+        const int n = n0 + q * 32 + kg * 8;
+        base[m][q].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[m] < 0 ? 0 : row[m]) * a.N + n,
+                        row[m] < 0 ? 0 : a.N - n);
+      }
+  };
+  load_base(first);
+  for (int g = 0; g < a.col_groups; g++) {
+    const int n0 = first + g * 256;
+    f32x4_t acc[MT][4] = {};
+    for (int rc = 0; rc < a.R; rc += RC) {
+      if (g == 0 || a.R > RC) {
+        if (g || rc) __syncthreads();
+        stage(rc);
+        __syncthreads();
+      }
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) fm[m][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][m * 16 + col][r]);
+      for (int s = 0; s < STEPS; s++) {
+        const int r = s * F::STEP + kg * F::V;
+        if (rc + s * F::STEP >= a.R) break;
+        frag<T> w[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int n = min(n0 + j / 2 * 32 + col / 4 * 8 + j % 2 * 4 + col % 4, a.N - 1);
-        frag<T> w;
-        F wp[WP];
-        w.load(b + (size_t)n * a.R + rc + r, a.R - rc - r);
-        weight_parts(w, wp);
+        for (int j = 0; j < 4; j++) {
+          const int n = min(n0 + j / 2 * 32 + col / 4 * 8 + j % 2 * 4 + col % 4, a.N - 1);
+          w[j].load(b + (size_t)n * a.R + rc + r, a.R - rc - r);
+        }
+        F fm[MT][PARTS];
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int p = 0; p < PARTS; p++)
+          for (int p = 0; p < PARTS; p++) fm[m][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][m * 16 + col][r]);
 #pragma unroll
-            for (int q = 0; q < WP; q++) acc[m][j] = mfma16(wp[q], fm[m][p], acc[m][j]);
+        for (int j = 0; j < 4; j++) {
+          F wp[WP];
+          weight_parts(w[j], wp);
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+              for (int q = 0; q < WP; q++) acc[m][j] = mfma16(wp[q], fm[m][p], acc[m][j]);
+        }
       }
     }
-  }
-  const float scale = a.scale ? a.scale[t.e] : 1.0f;
+    float out[MT][2][8];
 #pragma unroll
-  for (int m = 0; m < MT; m++) {
-    if (row[m] < 0) continue;
+    for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-      const int n = n0 + q * 32 + kg * 8;
-      if (n >= a.N) continue;
-      float f[8];
+      for (int q = 0; q < 2; q++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = fmaf(scale, acc[m][2 * q + i / 4][i % 4], (float)base[m][q].v[i]);
-      store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, f);
-    }
+        for (int i = 0; i < 8; i++) out[m][q][i] = fmaf(scale, acc[m][2 * q + i / 4][i % 4], (float)base[m][q].v[i]);
+    if (g + 1 < a.col_groups) load_base(n0 + 256);
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int q = 0; q < 2; q++) {
+        const int n = n0 + q * 32 + kg * 8;
+        if (row[m] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, out[m][q]);
+      }
   }
 }

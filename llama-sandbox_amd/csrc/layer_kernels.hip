@@ -132,24 +132,24 @@ bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
   return true;
 }
 
-// Rows of an adapter a workgroup.
+// Rows of an adapter a workgroup, and the waves of one that multiplies with A: 64 KB of results meet in LDS.
 static int adapters_tile(int M) { return M <= 64 ? 16 : 32; }
+static int shrink_waves(int M, int R) { return (adapters_tile(M) == 16 ? 1 : 2) * (R <= 16 ? 1 : R <= 32 ? 2 : 4) <= 2 ? 16 : 8; }
 
-// Pieces of K that the product with A is cut into: workgroups for the chip (four a CU where every tile is full), each
-// with eight steps at least.
-static int adapters_splits(int M, int K, int n_cu) {
-  const int most = ceil_div(K, 256), want = ceil_div(4L * n_cu, ceil_div(M, adapters_tile(M)));
+// Pieces of K that the product with A is cut into: 16 waves a CU where every tile is full, two steps a wave at least.
+static int adapters_splits(int M, int K, int R, int n_cu) {
+  const int w = shrink_waves(M, R), most = ceil_div(K, 64 * w), want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
   return most < want ? most : want;
 }
 
-size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, n_cu) * M * R; }
+size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, R, n_cu) * M * R; }
 
 template <typename T, int MT>
 static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
   const unsigned x = (unsigned)(tiles * a.splits);
-  if (a.R <= 16) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 1>), dim3(x), dim3(256), 0, st, a);
-  else if (a.R <= 32) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 2>), dim3(x), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_adapters_shrink<T, MT, 4>), dim3(x, ceil_div(a.R, 64)), dim3(256), 0, st, a);
+  if (a.R <= 16) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 1, 16>), dim3(x), dim3(1024), 0, st, a);
+  else if (a.R <= 32) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 2, MT == 1 ? 16 : 8>), dim3(x), dim3(MT == 1 ? 1024 : 512), 0, st, a);
+  else hipLaunchKernelGGL((k_adapters_shrink<T, MT, 4, 8>), dim3(x, ceil_div(a.R, 64)), dim3(512), 0, st, a);
 }
 
 template <typename T, typename TO, int MT>
@@ -161,12 +161,15 @@ static void launch_expand(const adapters_call &a, long tiles, hipStream_t st) {
 
 bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   adapters_call a = args;
-  const int BM = adapters_tile(a.M);
-  a.splits = adapters_splits(a.M, a.K, n_cu);
+  const int BM = adapters_tile(a.M), groups = ceil_div(a.N, 256);
+  a.splits = adapters_splits(a.M, a.K, a.R, n_cu);
   a.piece = ceil_div(ceil_div(a.K, a.splits), 32) * 32;
-  a.col_blocks = ceil_div(a.N, 256);
+  // several groups of columns for one reading of mid, as long as there are four workgroups a CU
+  const long each = (long)ceil_div(a.M, BM) * groups / (4 * n_cu);
+  a.col_groups = each < 1 ? 1 : each < groups ? (int)each : groups;
+  a.col_blocks = ceil_div(groups, a.col_groups);
   const long tiles = (a.M + (long)(a.M < a.n ? a.M : a.n) * (BM - 1)) / BM;
-  if (!fits(tiles * a.splits, 256) || !fits(tiles * a.col_blocks, 256)) return false;
+  if (!fits(tiles * a.splits, 1024) || !fits(tiles * a.col_blocks, 256)) return false;
   with_type(a.type, [&](auto t) {
     typedef decltype(t) T;
     if (BM == 16) launch_shrink<T, 1>(a, tiles, st);
