@@ -27,12 +27,16 @@ struct frag {
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
   vec v;
   __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const vec *>(p); }
-  __device__ __forceinline__ void load(const T *p, int left) {  // 0 from `left` on
+  // 0 from `left` on; whole: the same for a wave, pieces are there as a whole or not at all
+  __device__ __forceinline__ void load(const T *p, int left, bool whole) {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = (T)0.0f;
     if (left >= V) {
       load(p);
-    } else {
+    } else if (!whole) {
 #pragma unroll
-      for (int i = 0; i < V; i++) v[i] = i < left ? p[i] : (T)0.0f;
+      for (int i = 0; i < V; i++)
+        if (i < left) v[i] = p[i];
     }
   }
 };
@@ -93,9 +97,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a)
       for (int u = 0; u < U; u++) {
         const int left = end - k - u * F::STEP - k0;
 #pragma unroll
-        for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * F::STEP, left);
+        for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * F::STEP, left, a.K % F::V == 0);
 #pragma unroll
-        for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * F::STEP, left);
+        for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * F::STEP, left, a.K % F::V == 0);
       }
     }
 #pragma unroll
@@ -143,77 +147,82 @@ __device__ __forceinline__ void weight_parts(const frag<_Float16> &w, frag<bf16_
   }
 }
 
-// out.  grid (tiles * column blocks): 16 MT grouped rows by a.col_groups times 256 columns of out a workgroup, 64 a wave;
-// mid's shares are added up and cut into parts in LDS, 64 of R at a time.
+// out.  grid (tiles * column blocks): 16 MT grouped rows by a.col_groups times 128 columns of out a workgroup, 32 a wave,
+// with the next group's loads in flight; mid's shares are added up and cut into parts in LDS, 64 of R at a time.
 template <typename T, typename TO, int MT, int PARTS>
-__global__ __launch_bounds__(256) void k_adapters_expand(adapters_call a) {
+__global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
   constexpr int RC = 64, STEPS = RC / F::STEP, WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
-  constexpr int ROW = RC + F::V;            // a piece more, so that rows lie in different banks
-  constexpr int SLOTS = 16 * MT * RC / 1024;  // of 4 values of mid that a thread cuts
+  constexpr int ROW = RC + F::V;  // a piece more, so that rows lie in different banks
   __shared__ __attribute__((aligned(16))) TE mid[PARTS][16 * MT][ROW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % 16, kg = lane / 16;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.col_blocks, 16 * MT);
   if (t.e < 0) return;
   const T *b = reinterpret_cast<const T *>(a.b) + (size_t)t.e * a.N * a.R;
-  const float scale = a.scale ? a.scale[t.e] : 1.0f;
   int row[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) row[m] = adapters_row(a, t, m * 16 + col);
 
   auto stage = [&](int rc) {
-    float f[SLOTS][4] = {};
-    for (int s = 0; s < a.splits; s += 4) {
-      float g[SLOTS][4][4];
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 16 * MT * RC / 4; i += 256) {
+      const int m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
+      const float *from = a.mid + ((size_t)t.r0 + m) * a.R + r;
+      const size_t share = (size_t)a.M * a.R;
+      const int left = m < t.n ? a.R - r : 0;
+      float f[4] = {};
+      for (int s = 0; s < a.splits; s += 4, from += 4 * share) {
+        frag<float> g[4];
 #pragma unroll
-      for (int q = 0; q < SLOTS; q++) {
-        const int i = threadIdx.x + q * 256, m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
-        const float *from = a.mid + ((size_t)s * a.M + t.r0 + m) * a.R + r;
-#pragma unroll
-        for (int v = 0; v < 4; v++) load_v<float, 4>(from + (size_t)v * a.M * a.R, s + v < a.splits && m < t.n ? a.R - r : 0, g[q][v]);
-      }
-#pragma unroll
-      for (int q = 0; q < SLOTS; q++)
+        for (int v = 0; v < 4; v++) g[v].load(from + v * share, s + v < a.splits ? left : 0, a.R % 4 == 0);
 #pragma unroll
         for (int v = 0; v < 4; v++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) f[q][j] += g[q][v][j];
-    }
-#pragma unroll
-    for (int q = 0; q < SLOTS; q++) {
-      const int i = threadIdx.x + q * 256;
+          for (int j = 0; j < 4; j++) f[j] += g[v].v[j];
+      }
       typedef TE vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int p = 0; p < PARTS; p++) {
         vec4 o;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          o[j] = (TE)f[q][j];
-          f[q][j] -= (float)o[j];
+          o[j] = (TE)f[j];
+          f[j] -= (float)o[j];
         }
-        *reinterpret_cast<vec4 *>(&mid[p][i / (RC / 4)][i % (RC / 4) * 4]) = o;
+        *reinterpret_cast<vec4 *>(&mid[p][m][i % (RC / 4) * 4]) = o;
       }
     }
   };
 
-  const int first = (blockIdx.x % a.col_blocks * a.col_groups) * 256 + wave * 64;
-  // a lane's 8 columns n0 + 32 q + 8 kg + .. of the pairs q of weight tiles, of rows m * 16 + col
-  raw_v<TO, 8> base[MT][2];
+  const int first = (blockIdx.x % a.col_blocks * a.col_groups) * 128 + wave * 32;
+  // a lane's 8 columns n0 + 8 kg + .. of rows m * 16 + col; absent rows read the first
+  raw_v<TO, 8> base[MT];
   auto load_base = [&](int n0) {
+    const int n = n0 + kg * 8;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int q = 0; q < 2; q++) {
-        const int n = n0 + q * 32 + kg * 8;
-        base[m][q].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[m] < 0 ? 0 : row[m]) * a.N + n,
-                        row[m] < 0 ? 0 : a.N - n);
-      }
+    for (int m = 0; m < MT; m++) {
+      const TO *p = reinterpret_cast<const TO *>(a.base) + (size_t)(row[m] < 0 ? 0 : row[m]) * a.N + n;
+      if (n0 + 32 <= a.N) base[m].v = *reinterpret_cast<const typename raw_v<TO, 8>::vec_t *>(p);
+      else base[m].load(p, a.N - n);
+    }
   };
+  // the pieces of B of one step: 32 rows, dealt to the two tiles four and four
+  frag<T> w[2];
+  auto load_b = [&](int n0, int r) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const T *p = b + (size_t)min(n0 + col / 4 * 8 + j * 4 + col % 4, a.N - 1) * a.R + r + kg * F::V;
+      if (r + F::STEP <= a.R) w[j].load(p);
+      else w[j].load(p, a.R - r - kg * F::V, a.R % F::V == 0);
+    }
+  };
+  load_b(first, 0);
   load_base(first);
+  const float scale = a.scale ? a.scale[t.e] : 1.0f;
   for (int g = 0; g < a.col_groups; g++) {
-    const int n0 = first + g * 256;
-    f32x4_t acc[MT][4] = {};
+    const int n0 = first + g * 128;
+    f32x4_t acc[MT][2] = {};
     for (int rc = 0; rc < a.R; rc += RC) {
       if (g == 0 || a.R > RC) {
         if (g || rc) __syncthreads();
@@ -222,46 +231,37 @@ __global__ __launch_bounds__(256) void k_adapters_expand(adapters_call a) {
       }
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
-        const int r = s * F::STEP + kg * F::V;
-        if (rc + s * F::STEP >= a.R) break;
-        frag<T> w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int n = min(n0 + j / 2 * 32 + col / 4 * 8 + j % 2 * 4 + col % 4, a.N - 1);
-          w[j].load(b + (size_t)n * a.R + rc + r, a.R - rc - r);
-        }
-        F fm[MT][PARTS];
+        const int r = rc + s * F::STEP, next = r + F::STEP;
+        if (r >= a.R) break;
+        F fm[MT][PARTS], wp[2][WP];
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int p = 0; p < PARTS; p++) fm[m][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][m * 16 + col][r]);
+          for (int p = 0; p < PARTS; p++)
+            fm[m][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][m * 16 + col][s * F::STEP + kg * F::V]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          F wp[WP];
-          weight_parts(w[j], wp);
+        for (int j = 0; j < 2; j++) weight_parts(w[j], wp[j]);
+        if (next < a.R) load_b(n0, next);
+        else if (g + 1 < a.col_groups) load_b(n0 + 128, 0);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
 #pragma unroll
           for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int p = 0; p < PARTS; p++)
 #pragma unroll
-              for (int q = 0; q < WP; q++) acc[m][j] = mfma16(wp[q], fm[m][p], acc[m][j]);
-        }
+              for (int q = 0; q < WP; q++) acc[m][j] = mfma16(wp[j][q], fm[m][p], acc[m][j]);
       }
     }
-    float out[MT][2][8];
+    const int n = n0 + kg * 8;
+    float out[MT][8];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int q = 0; q < 2; q++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) out[m][q][i] = fmaf(scale, acc[m][2 * q + i / 4][i % 4], (float)base[m][q].v[i]);
-    if (g + 1 < a.col_groups) load_base(n0 + 256);
+      for (int i = 0; i < 8; i++) out[m][i] = fmaf(scale, acc[m][i / 4][i % 4], (float)base[m].v[i]);
+    if (g + 1 < a.col_groups) load_base(n0 + 128);
 #pragma unroll
     for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int q = 0; q < 2; q++) {
-        const int n = n0 + q * 32 + kg * 8;
-        if (row[m] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, out[m][q]);
-      }
+      if (row[m] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, out[m]);
   }
 }

@@ -62,7 +62,7 @@ struct adapters_call {
   void *out;
   float *mid;
   int type, out_type, n, M, K, R, N;
-  // set by the launch: shares of mid, elements of K of each, blocks of out's columns, groups of 256 columns in a block
+  // set by the launch: shares of mid, elements of K of each, blocks of out's columns, groups of 128 columns in a block
   int splits = 1, piece = 0, col_blocks = 0, col_groups = 1;
 };
 size_t adapters_scratch(int M, int K, int R, int n_cu);

@@ -134,22 +134,27 @@ bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
 
 // Rows of an adapter a workgroup, and the waves of one that multiplies with A: 64 KB of results meet in LDS.
 static int adapters_tile(int M) { return M <= 64 ? 16 : 32; }
-static int shrink_waves(int M, int R) { return (adapters_tile(M) == 16 ? 1 : 2) * (R <= 16 ? 1 : R <= 32 ? 2 : 4) <= 2 ? 16 : 8; }
+static constexpr int shrink_waves(int MT, int RT) { return MT * RT <= 2 ? 16 : 8; }
 
 // Pieces of K that the product with A is cut into: 16 waves a CU where every tile is full, two steps a wave at least.
 static int adapters_splits(int M, int K, int R, int n_cu) {
-  const int w = shrink_waves(M, R), most = ceil_div(K, 64 * w), want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
+  const int w = shrink_waves(adapters_tile(M) / 16, R <= 16 ? 1 : R <= 32 ? 2 : 4), most = ceil_div(K, 64 * w), want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
   return most < want ? most : want;
 }
 
 size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, R, n_cu) * M * R; }
 
+template <typename T, int MT, int RT>
+static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
+  constexpr int W = shrink_waves(MT, RT);
+  hipLaunchKernelGGL((k_adapters_shrink<T, MT, RT, W>), dim3((unsigned)(tiles * a.splits), ceil_div(a.R, 16 * RT)), dim3(64 * W), 0,
+                     st, a);
+}
 template <typename T, int MT>
 static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
-  const unsigned x = (unsigned)(tiles * a.splits);
-  if (a.R <= 16) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 1, 16>), dim3(x), dim3(1024), 0, st, a);
-  else if (a.R <= 32) hipLaunchKernelGGL((k_adapters_shrink<T, MT, 2, MT == 1 ? 16 : 8>), dim3(x), dim3(MT == 1 ? 1024 : 512), 0, st, a);
-  else hipLaunchKernelGGL((k_adapters_shrink<T, MT, 4, 8>), dim3(x, ceil_div(a.R, 64)), dim3(512), 0, st, a);
+  if (a.R <= 16) launch_shrink<T, MT, 1>(a, tiles, st);
+  else if (a.R <= 32) launch_shrink<T, MT, 2>(a, tiles, st);
+  else launch_shrink<T, MT, 4>(a, tiles, st);
 }
 
 template <typename T, typename TO, int MT>
@@ -161,7 +166,8 @@ static void launch_expand(const adapters_call &a, long tiles, hipStream_t st) {
 
 bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   adapters_call a = args;
-  const int BM = adapters_tile(a.M), groups = ceil_div(a.N, 256);
+  // no larger a tile than the adapters' rows fill
+  const int BM = a.M / (a.M < a.n ? a.M : a.n) <= 16 ? 16 : adapters_tile(a.M), groups = ceil_div(a.N, 128);
   a.splits = adapters_splits(a.M, a.K, a.R, n_cu);
   a.piece = ceil_div(ceil_div(a.K, a.splits), 32) * 32;
   // several groups of columns for one reading of mid, as long as there are four workgroups a CU
