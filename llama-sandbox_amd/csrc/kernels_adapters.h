@@ -84,14 +84,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a)
   const int end = min(a.K, (split + 1) * a.piece);
   for (int k = split * a.piece + wave * U * F::STEP; k < end; k += WAVES * U * F::STEP) {
     F fx[U][MT], fw[U][RT];
+    // a row's steps one after the other: two share a cache line, and rows of many lengths share sets of the cache
     if (k + U * F::STEP <= end) {
 #pragma unroll
-      for (int u = 0; u < U; u++) {
+      for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int m = 0; m < MT; m++) fx[u][m].load(x[m] + k + u * F::STEP);
+        for (int u = 0; u < U; u++) fx[u][m].load(x[m] + k + u * F::STEP);
 #pragma unroll
-        for (int r = 0; r < RT; r++) fw[u][r].load(w[r] + k + u * F::STEP);
-      }
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int u = 0; u < U; u++) fw[u][r].load(w[r] + k + u * F::STEP);
     } else {
 #pragma unroll
       for (int u = 0; u < U; u++) {
