@@ -253,7 +253,7 @@ bool launch_matmul_i8(const i8_mm &args, int n_cu, hipStream_t st) {
   i8_mm a = args;
   // the tiles: 16-byte loads at 32-bit offsets (a smaller row count is a uniform matter of the operands)
   const bool aligned = a.K % 16 == 0 && ((uintptr_t)a.q | (uintptr_t)a.w) % 16 == 0;
-  const bool offsets32 = (uint64_t)a.n_src * a.K < MOE_I8_OOB && (uint64_t)a.N * a.K < MOE_I8_OOB;
+  const bool offsets32 = (uint64_t)a.n_src * a.K < MOE_LDS_OOB && (uint64_t)a.N * a.K < MOE_LDS_OOB;
   if (aligned && offsets32) {
     // weights of more than the caches hold from call to call, each read by one tile: past the caches.  Measured:
     // 939 MB against 16 rows 164 us with plain loads, 146 without (5.75 and 6.5 TB/s)

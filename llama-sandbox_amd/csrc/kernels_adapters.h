@@ -11,6 +11,7 @@
 
 #include "group_tiles.h"
 #include "layer_kernels.h"
+#include "lds_dma.h"
 #include "row_vec.h"
 #include "../../include/moe_block.h"
 
@@ -126,6 +127,88 @@ __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a)
   }
 }
 
+// The same for adapters of many rows: 64 of them a workgroup, 16 a wave.  Loads that give neighbouring lanes
+// other rows take a cycle a lane (above: 59 accesses a load); here rows come as runs of 128 bytes, straight to LDS,
+// NBUF - 1 stages ahead, and are read from there as operands (chunk c of row r lies at c ^ (r & 7)).  Rows and A of
+// whole 16 bytes, below 4 GiB.
+template <typename T, int RT, int NBUF>
+__global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a) {
+  typedef frag<T> F;
+  typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
+  constexpr int RB = 16 * RT, STAGE = (64 + RB) * 8;                   // rows of A, chunks of a stage
+  constexpr int CX = 2, NWI = (RB / 8 + 3) / 4, CNT = CX + RB / 32;        // 1 KiB loads a wave: of x, of A; both, at least
+  __shared__ chunk_t lds[NBUF * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), split = blockIdx.x % a.splits;
+  const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.splits, 64);
+  if (t.e < 0) return;
+  const int r0 = blockIdx.y * RB, rows_a = min(RB, a.R - r0);
+  const uint32_t row_bytes = (uint32_t)a.K * sizeof(T), xbytes = (uint32_t)a.M * row_bytes, wbytes = (uint32_t)rows_a * row_bytes;
+  const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)t.e * a.R + r0) * a.K;
+  const uint32_t begin = (uint32_t)(split * a.piece) * sizeof(T);
+  const uint32_t end = min(row_bytes, begin + (uint32_t)a.piece * (uint32_t)sizeof(T));
+  const int stages = begin < end ? (int)((end - begin + 127) / 128) : 0;
+  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) * 16;
+  uint32_t vx[CX], vw[NWI];
+#pragma unroll
+  for (int i = 0; i < NWI; i++) {
+    const int row = 8 * (wave + 4 * i) + lr;
+    vw[i] = row < rows_a ? (uint32_t)row * row_bytes + lc : MOE_LDS_OOB;
+  }
+  // stage s of this wave's loads into its buffer; past the end they read 0, so that the waits can count on them
+  auto load_w = [&](int s) __attribute__((always_inline)) {
+    const uint32_t at = begin + s * 128;
+    const bool there = s < stages && at + lc < end;
+#pragma unroll
+    for (int i = 0; i < NWI; i++)
+      if (RB / 8 % 4 == 0 || wave + 4 * i < RB / 8)
+        lds_dma(w, wbytes, lds + s % NBUF * STAGE + (64 / 8 + wave + 4 * i) * 64, there ? vw[i] : MOE_LDS_OOB, s < stages ? at : 0);
+  };
+  auto load_x = [&](int s) __attribute__((always_inline)) {
+    const uint32_t at = begin + s * 128;
+    const bool there = s < stages && at + lc < end;
+#pragma unroll
+    for (int i = 0; i < CX; i++)
+      lds_dma(a.x, xbytes, lds + s % NBUF * STAGE + (wave + 4 * i) * 64, there ? vx[i] : MOE_LDS_OOB, s < stages ? at : 0);
+  };
+  // A goes out before the rows are known
+#pragma unroll
+  for (int s = 0; s < NBUF - 1; s++) load_w(s);
+#pragma unroll
+  for (int i = 0; i < CX; i++) {
+    const int row = adapters_row(a, t, 8 * (wave + 4 * i) + lr);
+    vx[i] = row >= 0 ? (uint32_t)row * row_bytes + lc : MOE_LDS_OOB;
+  }
+#pragma unroll
+  for (int s = 0; s < NBUF - 1; s++) load_x(s);
+  f32x4_t acc[RT] = {};
+  const int fr = lane & 15, fg = lane >> 4;
+  for (int s = 0; s < stages; s++) {
+    // this stage has landed, and every wave is done with the one before, whose buffer the next loads take
+    if (s < NBUF - 2) lds_wait_barrier<(NBUF - 2) * CX>();
+    else lds_wait_barrier<(NBUF - 2) * CNT>();
+    load_w(s + NBUF - 1);
+    load_x(s + NBUF - 1);
+    const chunk_t *x = lds + s % NBUF * STAGE + (wave * 16 + fr) * 8, *wl = lds + s % NBUF * STAGE + (64 + fr) * 8;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int c = (k * 4 + fg) ^ (fr & 7);
+      const F fx = {__builtin_bit_cast(typename F::vec, x[c])};
+#pragma unroll
+      for (int r = 0; r < RT; r++) acc[r] = mfma16(F{__builtin_bit_cast(typename F::vec, wl[r * 128 + c])}, fx, acc[r]);
+    }
+  }
+  lds_wait_barrier<0>();  // what is on its way has landed
+  const int i = wave * 16 + fr;
+  if (i >= t.n) return;
+  float *to = a.mid + ((size_t)split * a.M + t.r0 + i) * a.R;
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const int at = r0 + r * 16 + fg * 4;
+    const float f[4] = {acc[r][0], acc[r][1], acc[r][2], acc[r][3]};
+    if (at < a.R) store_v<float, 4>(to + at, a.R - at, f);
+  }
+}
+
 // A 16-byte piece of mid as the operands that multiply a piece of B: f32 as it is; else as PARTS bf16 parts, each what
 // the ones before leave (2: 2^-16 of it is lost, where the output is rounded to 2^-8 of its; 3: 2^-24).
 // A piece of f16 weights is two bf16 pieces, which hold it exactly, at bf16's range: mid may be past f16's.
@@ -149,6 +232,40 @@ __device__ __forceinline__ void weight_parts(const frag<_Float16> &w, frag<bf16_
   }
 }
 
+// mid of ROWS grouped rows of a tile from rc on, its shares added up, cut into parts in LDS: 64 of R.  256 threads.
+template <typename TE, int PARTS, int ROWS, int ROW>
+__device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile &t, int rc, TE (&mid)[PARTS][ROWS][ROW]) {
+  constexpr int RC = 64;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < ROWS * RC / 4; i += 256) {
+    const int m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
+    const float *from = a.mid + ((size_t)t.r0 + m) * a.R + r;
+    const size_t share = (size_t)a.M * a.R;
+    const int left = m < t.n ? a.R - r : 0;
+    float f[4] = {};
+    for (int s = 0; s < a.splits; s += 4, from += 4 * share) {
+      frag<float> g[4];
+#pragma unroll
+      for (int v = 0; v < 4; v++) g[v].load(from + v * share, s + v < a.splits ? left : 0, a.R % 4 == 0);
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[j] += g[v].v[j];
+    }
+    typedef TE vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) {
+      vec4 o;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        o[j] = (TE)f[j];
+        f[j] -= (float)o[j];
+      }
+      *reinterpret_cast<vec4 *>(&mid[p][m][i % (RC / 4) * 4]) = o;
+    }
+  }
+}
+
 // out.  grid (tiles * column blocks): 16 MT grouped rows by a.col_groups times 128 columns of out a workgroup, 32 a wave,
 // with the next group's loads in flight; mid's shares are added up and cut into parts in LDS, 64 of R at a time.
 template <typename T, typename TO, int MT, int PARTS>
@@ -165,37 +282,6 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
   int row[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) row[m] = adapters_row(a, t, m * 16 + col);
-
-  auto stage = [&](int rc) {
-#pragma unroll 1
-    for (int i = threadIdx.x; i < 16 * MT * RC / 4; i += 256) {
-      const int m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
-      const float *from = a.mid + ((size_t)t.r0 + m) * a.R + r;
-      const size_t share = (size_t)a.M * a.R;
-      const int left = m < t.n ? a.R - r : 0;
-      float f[4] = {};
-      for (int s = 0; s < a.splits; s += 4, from += 4 * share) {
-        frag<float> g[4];
-#pragma unroll
-        for (int v = 0; v < 4; v++) g[v].load(from + v * share, s + v < a.splits ? left : 0, a.R % 4 == 0);
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) f[j] += g[v].v[j];
-      }
-      typedef TE vec4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-      for (int p = 0; p < PARTS; p++) {
-        vec4 o;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          o[j] = (TE)f[j];
-          f[j] -= (float)o[j];
-        }
-        *reinterpret_cast<vec4 *>(&mid[p][m][i % (RC / 4) * 4]) = o;
-      }
-    }
-  };
 
   const int first = (blockIdx.x % a.col_blocks * a.col_groups) * 128 + wave * 32;
   // a lane's 8 columns n0 + 8 kg + .. of rows m * 16 + col; absent rows read the first
@@ -228,7 +314,7 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
     for (int rc = 0; rc < a.R; rc += RC) {
       if (g == 0 || a.R > RC) {
         if (g || rc) __syncthreads();
-        stage(rc);
+        stage_mid<TE, PARTS, 16 * MT, ROW>(a, t, rc, mid);
         __syncthreads();
       }
 #pragma unroll
@@ -265,5 +351,78 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
 #pragma unroll
     for (int m = 0; m < MT; m++)
       if (row[m] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, out[m]);
+  }
+}
+
+// out for adapters of many rows and R <= 64: 64 grouped rows, 16 a wave, by 256 columns a workgroup.  B's rows come to LDS
+// as runs, all at once, and tokens are the rows of the result: tile j of a group of 128 columns has the columns
+// 8 l + j, so that a lane holds 8 next to each other and 16 lanes a run of 128 columns of base and out.
+// LDS row 16 j + l of a group is row 8 l + j of B.  B's rows are whole 16 bytes, an adapter's below 4 GiB.
+template <typename T, typename TO, int PARTS>
+__global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a) {
+  typedef typename expand_of<T>::type TE;
+  typedef frag<TE> F;
+  typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
+  constexpr int RC = 64, STEPS = RC / F::STEP, WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1, ROW = RC + F::V;
+  constexpr int BLOCKS = RC * (int)sizeof(T) / 128;  // of 128 bytes of B's rows
+  __shared__ chunk_t lds[BLOCKS * 256 * 8];
+  __shared__ __attribute__((aligned(16))) TE mid[PARTS][64][ROW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
+  const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.col_blocks, 64);
+  if (t.e < 0) return;
+  const int first = blockIdx.x % a.col_blocks * 256;
+  const uint32_t row_bytes = (uint32_t)a.R * sizeof(T), bbytes = (uint32_t)a.N * row_bytes;
+  const T *b = reinterpret_cast<const T *>(a.b) + (size_t)t.e * a.N * a.R;
+  const int lr = lane >> 3, lc = ((lane & 7) ^ lr) * 16;
+#pragma unroll
+  for (int k = 0; k < BLOCKS; k++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int row = 8 * (wave + 4 * i) + lr, n = first + row / 128 * 128 + row % 16 * 8 + row % 128 / 16;
+      const uint32_t at = k * 128 + lc;
+      lds_dma(b, bbytes, lds + (k * 32 + wave + 4 * i) * 64, n < a.N && at < row_bytes ? (uint32_t)n * row_bytes + at : MOE_LDS_OOB, 0);
+    }
+  int row[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) row[i] = adapters_row(a, t, wave * 16 + fg * 4 + i);
+  const float scale = a.scale ? a.scale[t.e] : 1.0f;
+  stage_mid<TE, PARTS, 64, ROW>(a, t, 0, mid);
+  lds_wait_barrier<0>();
+  F fm[STEPS][PARTS];
+#pragma unroll
+  for (int s = 0; s < STEPS; s++)
+#pragma unroll
+    for (int p = 0; p < PARTS; p++)
+      fm[s][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][wave * 16 + fr][s * F::STEP + fg * F::V]);
+#pragma unroll 1
+  for (int g = 0; g < 2; g++) {
+    const int n = first + g * 128 + fr * 8;
+    if (first + g * 128 >= a.N) break;
+    raw_v<TO, 8> base[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      base[i].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[i] < 0 ? 0 : row[i]) * a.N + n, row[i] < 0 ? 0 : a.N - n);
+    f32x4_t acc[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        if (s * F::STEP >= a.R) break;
+        const int c = s * 4 + fg;  // chunk of the row
+        const frag<T> w = {__builtin_bit_cast(typename frag<T>::vec, lds[((c / 8 * 256) + g * 128 + j * 16 + fr) * 8 + ((c & 7) ^ (fr & 7))])};
+        F wp[WP];
+        weight_parts(w, wp);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+          for (int q = 0; q < WP; q++) acc[j] = mfma16(fm[s][p], wp[q], acc[j]);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) f[j] = fmaf(scale, acc[j][i], (float)base[i].v[j]);
+      if (row[i] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[i] * a.N + n, a.N - n, f);
+    }
   }
 }

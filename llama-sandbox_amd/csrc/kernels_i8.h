@@ -11,6 +11,7 @@
 #include "expert_kernels.h"
 #include "../../include/moe_block.h"
 #include "group_tiles.h"
+#include "lds_dma.h"
 #include "row_vec.h"
 
 #include <type_traits>
@@ -442,31 +443,6 @@ __global__ __launch_bounds__(64) void k_mv_i8(i8_mm a, int nt) {
 //     A workgroup that takes tile after tile, the next one's loads behind the output,
 //     was slower in every shape (the stores delay the waits for those loads).
 //   16 rows x 7168 x 4096: 8.6 us, latency: 16x16 tiles, K over 4 waves.
-#define MOE_I8_OOB 0xffffff00u  // a lane offset past any buffer: the load returns 0
-#define MOE_I8_RSRC 0x00020000  // raw buffer, 32-bit dwords, no swizzle
-
-// Waits for vmcnt <= n only (gfx9 encoding), then for this wave's LDS reads, then for every wave.
-template <int N>
-__device__ __forceinline__ void i8_wait_barrier() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70 | 0xF00);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// 64 lanes' 16 bytes at base + vo + so into the 1 KiB at buf; _once: read by no other
-// workgroup (non-temporal).
-__device__ __forceinline__ void i8_dma(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so) {
-  typedef __attribute__((address_space(3))) void *lds_t;
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, MOE_I8_RSRC);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 0);
-}
-__device__ __forceinline__ void i8_dma_once(const int8_t *base, uint32_t bytes, v4i *buf, uint32_t vo, uint32_t so) {
-  typedef __attribute__((address_space(3))) void *lds_t;
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, MOE_I8_RSRC);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)buf, 16, vo, so, 0, 2);
-}
-
 // Load i of this wave's share (loads wave, wave + NW, ...) of the N_LOAD 1 KiB loads
 // of a stage from K byte k0 on, R rows a block of 128 bytes.  vo: lane offsets at
 // K 0.  Lanes past K, and every lane of a stage past the end, are out of range:
@@ -475,10 +451,10 @@ template <int R, int N_LOAD, int NW, bool ONCE>
 __device__ __forceinline__ void i8_load(int i, const int8_t *base, uint32_t bytes, uint32_t vo, v4i *buf, int wave, int k0,
                                         int k_lane, int K) {
   const int u = wave + NW * i;
-  const uint32_t at = k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_I8_OOB;
+  const uint32_t at = k0 + 8 * u / R * 128 + k_lane < K ? vo : MOE_LDS_OOB;
   if (N_LOAD % NW == 0 || u < N_LOAD) {  // uniform over the wave
-    if constexpr (ONCE) i8_dma_once(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
-    else i8_dma(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
+    if constexpr (ONCE) lds_dma_once(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
+    else lds_dma(base, bytes, buf + u * 64, at, k0 < K ? k0 : 0);
   }
 }
 
@@ -588,7 +564,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
 #pragma unroll
   for (int i = 0; i < NWI; i++) {
     const int rr = 8 * (wave + NW * i), w = channel(rr % BN + lr);
-    vw[i] = w < a.N ? (uint32_t)w * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_I8_OOB;
+    vw[i] = w < a.N ? (uint32_t)w * (uint32_t)a.K + rr / BN * 128 + lc * 16 : MOE_LDS_OOB;
   }
   // loads l of this wave's of stage s, into buffer b: the rows' WK blocks of BM x 128 bytes, then the channels'
   auto load_x = [&](int l, int s, int b) __attribute__((always_inline)) {
@@ -606,7 +582,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
 #pragma unroll
   for (int i = 0; i < NX; i++) {
     const int rr = 8 * (wave + NW * i), row = rr % BM + lr, s = row < t.n ? i8_src(a, t.r0 + row) : -1;
-    vx[i] = s >= 0 ? (uint32_t)s * (uint32_t)a.K + rr / BM * 128 + lc * 16 : MOE_I8_OOB;
+    vx[i] = s >= 0 ? (uint32_t)s * (uint32_t)a.K + rr / BM * 128 + lc * 16 : MOE_LDS_OOB;
   }
   const float row_scale = srow >= 0 ? a.qs[srow] : 0.0f;
   const float channel_scale = schannel < a.N ? a.ws[(size_t)t.e * a.N + schannel] : 0.0f;
@@ -632,7 +608,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
     for (int j = 0; j < NI; j++)
       if (j * MI / NI == i) A[set][j] = wb[j * 128 + c];
   };
-  i8_wait_barrier<(NBUF - 1) * CX>();
+  lds_wait_barrier<(NBUF - 1) * CX>();
 #pragma unroll
   for (int i = 0; i < MI; i++) read(i, 0, 0, 0);
 #pragma unroll
@@ -649,8 +625,8 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
       // holds the rest of this one in registers, so its buffer is free.  (The
       // first NBUF stages' weights were all asked for before their rows.)
       if (kk == 1) {
-        if (NBUF > 2 && s < NBUF - 2) i8_wait_barrier<(NBUF - 2) * CX>();
-        else i8_wait_barrier<(NBUF - 2) * CNT>();
+        if (NBUF > 2 && s < NBUF - 2) lds_wait_barrier<(NBUF - 2) * CX>();
+        else lds_wait_barrier<(NBUF - 2) * CNT>();
       }
 #pragma unroll
       for (int i = 0; i < MI; i++) {
@@ -674,7 +650,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
     cur = next;
   }
   if constexpr (WK > 1) {
-    i8_wait_barrier<0>();  // the last loads, out of range as they are, have landed: the stages are free
+    lds_wait_barrier<0>();  // the last loads, out of range as they are, have landed: the stages are free
     v4i *part = lds + ((wm * WN + wn) * MI * NI) * 64 + lane;
     if (wk > 0) {
 #pragma unroll
@@ -682,7 +658,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
 #pragma unroll
         for (int i = 0; i < MI; i++) part[((wk - 1) * WM * WN * MI * NI + j * MI + i) * 64] = acc[j][i];
     }
-    i8_wait_barrier<0>();
+    lds_wait_barrier<0>();
     if (wk > 0) return;
     for (int q = 0; q < WK - 1; q++)
 #pragma unroll
@@ -690,7 +666,7 @@ __device__ __forceinline__ void i8_multiply(const i8_mm &a, int nt, const row_ti
 #pragma unroll
         for (int i = 0; i < MI; i++) acc[j][i] += part[(q * WM * WN * MI * NI + j * MI + i) * 64];
   } else {
-    i8_wait_barrier<0>();
+    lds_wait_barrier<0>();
   }
 
   int8_t *reg = reinterpret_cast<int8_t *>(lds) + (WK - 1) * BM * BN * 4 + (wm * WN + wn) * MOE_I8_OUT_BYTES;

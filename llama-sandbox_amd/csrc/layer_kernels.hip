@@ -157,32 +157,59 @@ static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
   else launch_shrink<T, MT, 4>(a, tiles, st);
 }
 
+template <typename T, int RT>
+static void launch_shrink_staged(const adapters_call &a, long tiles, hipStream_t st) {
+  hipLaunchKernelGGL((k_adapters_shrink_staged<T, RT, 3>), dim3((unsigned)(tiles * a.splits), ceil_div(a.R, 16 * RT)), dim3(256), 0,
+                     st, a);
+}
+template <typename T>
+static void launch_shrink_staged(const adapters_call &a, long tiles, hipStream_t st) {
+  if (a.R <= 16) launch_shrink_staged<T, 1>(a, tiles, st);
+  else if (a.R <= 32) launch_shrink_staged<T, 2>(a, tiles, st);
+  else launch_shrink_staged<T, 4>(a, tiles, st);
+}
+
+// Parts of mid: see k_adapters_expand.
+template <typename T, typename TO>
+static constexpr int expand_parts() { return sizeof(T) == 4 ? 1 : std::is_same<T, bf16_t>::value && sizeof(TO) == 2 ? 2 : 3; }
+
 template <typename T, typename TO, int MT>
 static void launch_expand(const adapters_call &a, long tiles, hipStream_t st) {
-  // parts of mid: see k_adapters_expand
-  constexpr int PARTS = sizeof(T) == 4 ? 1 : std::is_same<T, bf16_t>::value && sizeof(TO) == 2 ? 2 : 3;
-  hipLaunchKernelGGL((k_adapters_expand<T, TO, MT, PARTS>), dim3((unsigned)(tiles * a.col_blocks)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_adapters_expand<T, TO, MT, expand_parts<T, TO>()>), dim3((unsigned)(tiles * a.col_blocks)), dim3(256), 0, st,
+                     a);
 }
 
 bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   adapters_call a = args;
+  const int matrices = a.M < a.n ? a.M : a.n, each = a.M / matrices;  // adapters that can have rows; rows of each
+  const size_t size = a.type == MOE_GGML_F32 ? 4 : 2;
+  const bool staged_a = each >= 32 && a.K * size % 16 == 0 && ((uintptr_t)a.x | (uintptr_t)a.a) % 16 == 0 &&
+                        (uint64_t)a.M * a.K * size < MOE_LDS_OOB && (uint64_t)a.R * a.K * size < MOE_LDS_OOB;
+  const bool staged_b = each >= 32 && a.R <= 64 && a.R * size % 16 == 0 && (uintptr_t)a.b % 16 == 0 &&
+                        (uint64_t)a.N * a.R * size < MOE_LDS_OOB;
   // no larger a tile than the adapters' rows fill
-  const int BM = a.M / (a.M < a.n ? a.M : a.n) <= 16 ? 16 : adapters_tile(a.M), groups = ceil_div(a.N, 128);
+  const int BM = each <= 16 ? 16 : adapters_tile(a.M), groups = ceil_div(a.N, staged_b ? 256 : 128);
+  auto tiles_of = [&](int rows) { return (a.M + (long)matrices * (rows - 1)) / rows; };
+  const long tiles_a = tiles_of(staged_a ? 64 : BM), tiles_b = tiles_of(staged_b ? 64 : BM);
   a.splits = adapters_splits(a.M, a.K, a.R, n_cu);
-  a.piece = ceil_div(ceil_div(a.K, a.splits), 32) * 32;
+  a.piece = ceil_div(ceil_div(a.K, a.splits), 64) * 64;
   // several groups of columns for one reading of mid, as long as there are four workgroups a CU
-  const long each = (long)ceil_div(a.M, BM) * groups / (4 * n_cu);
-  a.col_groups = each < 1 ? 1 : each < groups ? (int)each : groups;
+  const long wide = (long)ceil_div(a.M, BM) * groups / (4 * n_cu);
+  a.col_groups = wide < 1 || staged_b ? 1 : wide < groups ? (int)wide : groups;
   a.col_blocks = ceil_div(groups, a.col_groups);
-  const long tiles = (a.M + (long)(a.M < a.n ? a.M : a.n) * (BM - 1)) / BM;
-  if (!fits(tiles * a.splits, 1024) || !fits(tiles * a.col_blocks, 256)) return false;
+  if (!fits(tiles_a * a.splits, 1024) || !fits(tiles_b * a.col_blocks, 256)) return false;
   with_type(a.type, [&](auto t) {
     typedef decltype(t) T;
-    if (BM == 16) launch_shrink<T, 1>(a, tiles, st);
-    else launch_shrink<T, 2>(a, tiles, st);
+    if (staged_a) launch_shrink_staged<T>(a, tiles_a, st);
+    else if (BM == 16) launch_shrink<T, 1>(a, tiles_a, st);
+    else launch_shrink<T, 2>(a, tiles_a, st);
     with_type(a.out_type, [&](auto to) {
-      if (BM == 16) launch_expand<T, decltype(to), 1>(a, tiles, st);
-      else launch_expand<T, decltype(to), 2>(a, tiles, st);
+      typedef decltype(to) TO;
+      if (staged_b)
+        hipLaunchKernelGGL((k_adapters_expand_staged<T, TO, expand_parts<T, TO>()>), dim3((unsigned)(tiles_b * a.col_blocks)),
+                           dim3(256), 0, st, a);
+      else if (BM == 16) launch_expand<T, TO, 1>(a, tiles_b, st);
+      else launch_expand<T, TO, 2>(a, tiles_b, st);
     });
   });
   return true;
