@@ -137,7 +137,8 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
   typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
   constexpr int RB = 16 * RT, STAGE = (64 + RB) * 8;                   // rows of A, chunks of a stage
   constexpr int CX = 2, NWI = (RB / 8 + 3) / 4, CNT = CX + RB / 32;        // 1 KiB loads a wave: of x, of A; both, at least
-  __shared__ chunk_t lds[NBUF * STAGE];
+  extern __shared__ uint32_t adapters_lds[];  // NBUF * STAGE chunks
+  chunk_t *lds = reinterpret_cast<chunk_t *>(adapters_lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), split = blockIdx.x % a.splits;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.splits, 64);
   if (t.e < 0) return;
@@ -235,33 +236,41 @@ __device__ __forceinline__ void weight_parts(const frag<_Float16> &w, frag<bf16_
 // mid of ROWS grouped rows of a tile from rc on, its shares added up, cut into parts in LDS: 64 of R.  256 threads.
 template <typename TE, int PARTS, int ROWS, int ROW>
 __device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile &t, int rc, TE (&mid)[PARTS][ROWS][ROW]) {
-  constexpr int RC = 64;
+  // pieces of 4 a thread, and shares of each in flight
+  constexpr int RC = 64, PIECES = ROWS * RC / 4 / 256, SHARES = PIECES == 1 ? 4 : 2;
+  const size_t share = (size_t)a.M * a.R;
+  float f[PIECES][4] = {};
 #pragma unroll 1
-  for (int i = threadIdx.x; i < ROWS * RC / 4; i += 256) {
-    const int m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
-    const float *from = a.mid + ((size_t)t.r0 + m) * a.R + r;
-    const size_t share = (size_t)a.M * a.R;
-    const int left = m < t.n ? a.R - r : 0;
-    float f[4] = {};
-    for (int s = 0; s < a.splits; s += 4, from += 4 * share) {
-      frag<float> g[4];
+  for (int s = 0; s < a.splits; s += SHARES) {
+    frag<float> g[PIECES][SHARES];
 #pragma unroll
-      for (int v = 0; v < 4; v++) g[v].load(from + v * share, s + v < a.splits ? left : 0, a.R % 4 == 0);
+    for (int q = 0; q < PIECES; q++) {
+      const int i = threadIdx.x + q * 256, m = i / (RC / 4), r = rc + i % (RC / 4) * 4;
+      const float *from = a.mid + ((size_t)s * a.M + t.r0 + m) * a.R + r;
 #pragma unroll
-      for (int v = 0; v < 4; v++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) f[j] += g[v].v[j];
+      for (int v = 0; v < SHARES; v++)
+        g[q][v].load(from + v * share, s + v < a.splits && m < t.n ? a.R - r : 0, a.R % 4 == 0);
     }
+#pragma unroll
+    for (int q = 0; q < PIECES; q++)
+#pragma unroll
+      for (int v = 0; v < SHARES; v++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[q][j] += g[q][v].v[j];
+  }
+#pragma unroll
+  for (int q = 0; q < PIECES; q++) {
+    const int i = threadIdx.x + q * 256;
     typedef TE vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
       vec4 o;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        o[j] = (TE)f[j];
-        f[j] -= (float)o[j];
+        o[j] = (TE)f[q][j];
+        f[q][j] -= (float)o[j];
       }
-      *reinterpret_cast<vec4 *>(&mid[p][m][i % (RC / 4) * 4]) = o;
+      *reinterpret_cast<vec4 *>(&mid[p][i / (RC / 4)][i % (RC / 4) * 4]) = o;
     }
   }
 }
@@ -385,6 +394,14 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
   int row[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) row[i] = adapters_row(a, t, wave * 16 + fg * 4 + i);
+  raw_v<TO, 8> base[2][4];
+#pragma unroll
+  for (int g = 0; g < 2; g++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int n = first + g * 128 + fr * 8;
+      base[g][i].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[i] < 0 ? 0 : row[i]) * a.N + n, row[i] < 0 ? 0 : a.N - n);
+    }
   const float scale = a.scale ? a.scale[t.e] : 1.0f;
   stage_mid<TE, PARTS, 64, ROW>(a, t, 0, mid);
   lds_wait_barrier<0>();
@@ -394,14 +411,10 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
 #pragma unroll
     for (int p = 0; p < PARTS; p++)
       fm[s][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][wave * 16 + fr][s * F::STEP + fg * F::V]);
-#pragma unroll 1
+#pragma unroll
   for (int g = 0; g < 2; g++) {
     const int n = first + g * 128 + fr * 8;
     if (first + g * 128 >= a.N) break;
-    raw_v<TO, 8> base[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      base[i].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[i] < 0 ? 0 : row[i]) * a.N + n, row[i] < 0 ? 0 : a.N - n);
     f32x4_t acc[8] = {};
 #pragma unroll
     for (int j = 0; j < 8; j++)
@@ -421,7 +434,7 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
     for (int i = 0; i < 4; i++) {
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = fmaf(scale, acc[j][i], (float)base[i].v[j]);
+      for (int j = 0; j < 8; j++) f[j] = fmaf(scale, acc[j][i], (float)base[g][i].v[j]);
       if (row[i] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[i] * a.N + n, a.N - n, f);
     }
   }

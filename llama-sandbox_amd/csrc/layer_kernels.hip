@@ -157,18 +157,6 @@ static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
   else launch_shrink<T, MT, 4>(a, tiles, st);
 }
 
-template <typename T, int RT>
-static void launch_shrink_staged(const adapters_call &a, long tiles, hipStream_t st) {
-  hipLaunchKernelGGL((k_adapters_shrink_staged<T, RT, 3>), dim3((unsigned)(tiles * a.splits), ceil_div(a.R, 16 * RT)), dim3(256), 0,
-                     st, a);
-}
-template <typename T>
-static void launch_shrink_staged(const adapters_call &a, long tiles, hipStream_t st) {
-  if (a.R <= 16) launch_shrink_staged<T, 1>(a, tiles, st);
-  else if (a.R <= 32) launch_shrink_staged<T, 2>(a, tiles, st);
-  else launch_shrink_staged<T, 4>(a, tiles, st);
-}
-
 // Parts of mid: see k_adapters_expand.
 template <typename T, typename TO>
 static constexpr int expand_parts() { return sizeof(T) == 4 ? 1 : std::is_same<T, bf16_t>::value && sizeof(TO) == 2 ? 2 : 3; }
@@ -183,10 +171,17 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   adapters_call a = args;
   const int matrices = a.M < a.n ? a.M : a.n, each = a.M / matrices;  // adapters that can have rows; rows of each
   const size_t size = a.type == MOE_GGML_F32 ? 4 : 2;
-  const bool staged_a = each >= 32 && a.K * size % 16 == 0 && ((uintptr_t)a.x | (uintptr_t)a.a) % 16 == 0 &&
+  // Staged where adapters have rows for its tiles: the product with A from rank 33 on, the one with B where there are
+  // four workgroups a CU.  us, staged / straight to registers (bf16 rows x K x rank x N, adapters; * the rule's):
+  //   with A:  4096 x 7168 x 64 x 7168, 8   59.6* / 63.9   x 32  52.5 / 53.5*   x 16  50.3 / 48.7*
+  //            2048 x 2048 x 64 x 2048, 16 (f32)  37.6* / 40.6    2048 x 768 x 8 x 768, 60 (f32)  16.1 / 13.1*
+  //   with B:  4096 x 7168 x 64 x 7168, 8   59.6* / 67.4   x 16  48.7* / 51.2
+  //            2048 x 2048 x 64 x 2048, 16 (f32)  43.8 / 37.6*    512 x 4096 x 32 x 4096, 16  16.6 / 13.1*
+  //   both at 16 rows an adapter: 517 x 2048 x 8 x 768, 32  15.6 / 9.3*
+  const bool staged_a = each >= 32 && a.R > 32 && a.K * size % 16 == 0 && ((uintptr_t)a.x | (uintptr_t)a.a) % 16 == 0 &&
                         (uint64_t)a.M * a.K * size < MOE_LDS_OOB && (uint64_t)a.R * a.K * size < MOE_LDS_OOB;
-  const bool staged_b = each >= 32 && a.R <= 64 && a.R * size % 16 == 0 && (uintptr_t)a.b % 16 == 0 &&
-                        (uint64_t)a.N * a.R * size < MOE_LDS_OOB;
+  const bool staged_b = each >= 32 && (long)ceil_div(a.M, 64) * ceil_div(a.N, 256) >= 4 * n_cu && a.R <= 64 &&
+                        a.R * size % 16 == 0 && (uintptr_t)a.b % 16 == 0 && (uint64_t)a.N * a.R * size < MOE_LDS_OOB;
   // no larger a tile than the adapters' rows fill
   const int BM = each <= 16 ? 16 : adapters_tile(a.M), groups = ceil_div(a.N, staged_b ? 256 : 128);
   auto tiles_of = [&](int rows) { return (a.M + (long)matrices * (rows - 1)) / rows; };
@@ -200,7 +195,10 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   if (!fits(tiles_a * a.splits, 1024) || !fits(tiles_b * a.col_blocks, 256)) return false;
   with_type(a.type, [&](auto t) {
     typedef decltype(t) T;
-    if (staged_a) launch_shrink_staged<T>(a, tiles_a, st);
+    constexpr int NBUF = 5;
+    if (staged_a)
+      hipLaunchKernelGGL((k_adapters_shrink_staged<T, 4, NBUF>), dim3((unsigned)(tiles_a * a.splits), ceil_div(a.R, 64)), dim3(256),
+                         NBUF * 128 * 128, st, a);
     else if (BM == 16) launch_shrink<T, 1>(a, tiles_a, st);
     else launch_shrink<T, 2>(a, tiles_a, st);
     with_type(a.out_type, [&](auto to) {
