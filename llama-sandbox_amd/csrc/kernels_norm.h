@@ -69,10 +69,16 @@ __device__ __forceinline__ void load8_any(const void *p, int type, size_t i, int
     r.get(type, f);
   }
 }
-__device__ __forceinline__ void store8_any(void *p, int type, size_t i, int left, const float (&f)[8]) {
-  if (type == MOE_GGML_F32) store_v<float, 8>(reinterpret_cast<float *>(p) + i, left, f);
-  else if (type == MOE_GGML_F16) store_v<_Float16, 8>(reinterpret_cast<_Float16 *>(p) + i, left, f);
-  else store_v<bf16_t, 8>(reinterpret_cast<bf16_t *>(p) + i, left, f);
+template <bool NT>
+__device__ __forceinline__ void store8_type(void *p, int type, size_t i, int left, const float (&f)[8]) {
+  if (type == MOE_GGML_F32) store_v<float, 8, NT>(reinterpret_cast<float *>(p) + i, left, f);
+  else if (type == MOE_GGML_F16) store_v<_Float16, 8, NT>(reinterpret_cast<_Float16 *>(p) + i, left, f);
+  else store_v<bf16_t, 8, NT>(reinterpret_cast<bf16_t *>(p) + i, left, f);
+}
+// nt: past the caches, the same for a whole call.
+__device__ __forceinline__ void store8_any(void *p, int type, size_t i, int left, const float (&f)[8], int nt = 0) {
+  if (nt) store8_type<true>(p, type, i, left, f);
+  else store8_type<false>(p, type, i, left, f);
 }
 
 __device__ __forceinline__ double add_d(double a, double b) { return a + b; }
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
           for (int j = 0; j < 8; j++) h[v][j] = (float)(bf16_t)h[v][j];
         }
       }
-      if (there && i < a.H) store8_any(a.total, a.res_type, at + i, a.H - i, h[v]);
+      if (there && i < a.H) store8_any(a.total, a.res_type, at + i, a.H - i, h[v], a.nt);
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) sum = fma((double)h[v][j], (double)h[v][j], sum);  // (past the end: 0)
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
       gain(v, w);
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] = h[v][j] * r32 * w[j];
-      store8_any(a.y, a.y_type, at + i, a.H - i, y);
+      store8_any(a.y, a.y_type, at + i, a.H - i, y, a.nt);
     }
   }
   if (!a.q) return;
@@ -235,7 +241,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
 #pragma unroll
       for (int k = 0; k < 2; k++)
         o[k] = (code[4 * k] & 255) | (code[4 * k + 1] & 255) << 8 | (code[4 * k + 2] & 255) << 16 | code[4 * k + 3] << 24;
-      *reinterpret_cast<u32x2 *>(to) = o;
+      if (a.nt) __builtin_nontemporal_store(o, reinterpret_cast<u32x2 *>(to));
+      else *reinterpret_cast<u32x2 *>(to) = o;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++)

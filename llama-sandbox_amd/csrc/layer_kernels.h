@@ -14,6 +14,7 @@ struct norm_call {
   float *scale, *rstd;
   int x_type, res_type, w_type, y_type, T, H;
   float eps;
+  int nt = 0;  // set by the launch: outputs go past the caches
 };
 bool launch_rms_norm(const norm_call &a, int n_cu, hipStream_t st);
 

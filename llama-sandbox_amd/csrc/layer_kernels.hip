@@ -23,30 +23,39 @@ static void launch_norm(const norm_call &a, hipStream_t st) {
   hipLaunchKernelGGL((k_rms_norm<SX, SR, LANES, VPT>), dim3(ceil_div(a.T, NT / LANES)), dim3(NT), 0, st, a);
 }
 
+// Threads a row and vectors a thread.  A row of 4097 to 8192 in one vector a thread where the rows are too few to fill
+// the chip.  us, with outputs past the caches (4096 rows of 7168 bf16 with residual / to 8 bits; 8191 of 2048; 1024):
+//   threads x vectors:   7168:  1024 x 1  45.6 / 58.0   512 x 2  45.8 / 50.9   256 x 4  48.6 / 47.5   128 x 8  80 / 90
+//                        2048:  256 x 1  25.2   128 x 2  26.4   64 x 4  27.9     1024:  128 x 1  14.8   64 x 2  14.9
 template <int SX, int SR>
 static void launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
   const int H = a.H;
-  if (a.T < 2 * n_cu && H > 512 && H <= 8192) {
-    if (H <= 2048) launch_norm<SX, SR, 256, 1>(a, st);
-    else launch_norm<SX, SR, 1024, 1>(a, st);
-  }
-  else if (H <= 128) launch_norm<SX, SR, 16, 1>(a, st);
+  if (H <= 128) launch_norm<SX, SR, 16, 1>(a, st);
   else if (H <= 512) launch_norm<SX, SR, 64, 1>(a, st);
-  else if (H <= 1024) launch_norm<SX, SR, 64, 2>(a, st);
-  else if (H <= 2048) launch_norm<SX, SR, 64, 4>(a, st);
+  else if (H <= 1024) launch_norm<SX, SR, 128, 1>(a, st);
+  else if (H <= 2048) launch_norm<SX, SR, 256, 1>(a, st);
   else if (H <= 4096) launch_norm<SX, SR, 256, 2>(a, st);
-  else if (H <= 6144) launch_norm<SX, SR, 256, 3>(a, st);
-  else if (H <= 8192) launch_norm<SX, SR, 256, 4>(a, st);
+  else if (H <= 8192 && a.T < 2 * n_cu) launch_norm<SX, SR, 1024, 1>(a, st);
+  else if (H <= 8192) launch_norm<SX, SR, 512, 2>(a, st);
   else if (H <= 16384) launch_norm<SX, SR, 1024, 2>(a, st);
   else launch_norm<SX, SR, 1024, 4>(a, st);
 }
 
-bool launch_rms_norm(const norm_call &a, int n_cu, hipStream_t st) {
+// Outputs of more than this go past the caches: a kernel ends only when the caches have written back what it left
+// there, and the next one reads it from the memory's cache as fast.  us, through them / past them, norm and then
+// moe_quantize_i8 of its y, H = 7168 bf16 with residual:  64 rows (1.8 MB) 7.4 / 7.6, 512 (14.7 MB) 15.6 / 12.9, 1500
+// 30.6 / 29.0, 4096 61.8 / 60.8; 2000 of 2048 (16.4 MB) 17.1 / 14.1, 8191 42.8 / 39.6.
+static constexpr size_t MOE_NORM_STREAM_BYTES = (size_t)4 << 20;
+
+bool launch_rms_norm(const norm_call &args, int n_cu, hipStream_t st) {
+  norm_call a = args;
   if (!fits(a.T, 1024)) return false;
   if (a.H > 32768) {
     hipLaunchKernelGGL(k_rms_norm_long, dim3(a.T), dim3(256), 0, st, a);
     return true;
   }
+  auto size = [](const void *p, int type) { return p ? type == MOE_GGML_F32 ? 4 : 2 : 0; };
+  a.nt = (size_t)a.T * a.H * (size(a.total, a.res_type) + size(a.y, a.y_type) + (a.q ? 1 : 0)) > MOE_NORM_STREAM_BYTES;
   with_size(a.x_type, [&](auto sx) {
     if (!a.res) launch_norm<sx, 0>(a, n_cu, st);
     else with_size(a.res_type, [&](auto sr) { launch_norm<sx, sr>(a, n_cu, st); });
