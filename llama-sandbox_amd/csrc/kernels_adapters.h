@@ -54,6 +54,14 @@ __device__ __forceinline__ f32x4_t mfma16(const frag<float> &a, const frag<float
   return c;
 }
 
+// 8 values of out; nt: past the caches, the same for a whole call.
+template <typename TO>
+__device__ __forceinline__ void store_out(const adapters_call &a, int row, int n, const float (&f)[8]) {
+  TO *to = reinterpret_cast<TO *>(a.out) + (size_t)row * a.N + n;
+  if (a.nt) store_v<TO, 8, true>(to, a.N - n, f);
+  else store_v<TO, 8>(to, a.N - n, f);
+}
+
 // The row of x, base and out that grouped row i is; -1: none.
 __device__ __forceinline__ int adapters_row(const adapters_call &a, const row_tile &t, int i) {
   const int row = i < t.n ? a.perm[t.r0 + i] : -1;
@@ -131,27 +139,27 @@ __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a)
 // other rows take a cycle a lane (above: 59 accesses a load); here rows come as runs of 128 bytes, straight to LDS,
 // NBUF - 1 stages ahead, and are read from there as operands (chunk c of row r lies at c ^ (r & 7)).  Rows and A of
 // whole 16 bytes, below 4 GiB.
-template <typename T, int RT, int NBUF>
+template <typename T, int NBUF>
 __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a) {
   typedef frag<T> F;
   typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
-  constexpr int RB = 16 * RT, STAGE = (64 + RB) * 8;                   // rows of A, chunks of a stage
-  constexpr int CX = 2, NWI = (RB / 8 + 3) / 4, CNT = CX + RB / 32;        // 1 KiB loads a wave: of x, of A; both, at least
+  constexpr int RT = 4, STAGE = (64 + 64) * 8;  // tiles of A's rows; chunks of a stage
+  constexpr int CX = 2, CW = 2;                 // 1 KiB loads a wave: of x, of A
   extern __shared__ uint32_t adapters_lds[];  // NBUF * STAGE chunks
   chunk_t *lds = reinterpret_cast<chunk_t *>(adapters_lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), split = blockIdx.x % a.splits;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.splits, 64);
   if (t.e < 0) return;
-  const int r0 = blockIdx.y * RB, rows_a = min(RB, a.R - r0);
+  const int r0 = blockIdx.y * 64, rows_a = min(64, a.R - r0);
   const uint32_t row_bytes = (uint32_t)a.K * sizeof(T), xbytes = (uint32_t)a.M * row_bytes, wbytes = (uint32_t)rows_a * row_bytes;
   const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)t.e * a.R + r0) * a.K;
   const uint32_t begin = (uint32_t)(split * a.piece) * sizeof(T);
   const uint32_t end = min(row_bytes, begin + (uint32_t)a.piece * (uint32_t)sizeof(T));
   const int stages = begin < end ? (int)((end - begin + 127) / 128) : 0;
   const int lr = lane >> 3, lc = ((lane & 7) ^ lr) * 16;
-  uint32_t vx[CX], vw[NWI];
+  uint32_t vx[CX], vw[CW];
 #pragma unroll
-  for (int i = 0; i < NWI; i++) {
+  for (int i = 0; i < CW; i++) {
     const int row = 8 * (wave + 4 * i) + lr;
     vw[i] = row < rows_a ? (uint32_t)row * row_bytes + lc : MOE_LDS_OOB;
   }
@@ -160,9 +168,8 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
     const uint32_t at = begin + s * 128;
     const bool there = s < stages && at + lc < end;
 #pragma unroll
-    for (int i = 0; i < NWI; i++)
-      if (RB / 8 % 4 == 0 || wave + 4 * i < RB / 8)
-        lds_dma(w, wbytes, lds + s % NBUF * STAGE + (64 / 8 + wave + 4 * i) * 64, there ? vw[i] : MOE_LDS_OOB, s < stages ? at : 0);
+    for (int i = 0; i < CW; i++)
+      lds_dma(w, wbytes, lds + s % NBUF * STAGE + (64 / 8 + wave + 4 * i) * 64, there ? vw[i] : MOE_LDS_OOB, s < stages ? at : 0);
   };
   auto load_x = [&](int s) __attribute__((always_inline)) {
     const uint32_t at = begin + s * 128;
@@ -186,7 +193,7 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
   for (int s = 0; s < stages; s++) {
     // this stage has landed, and every wave is done with the one before, whose buffer the next loads take
     if (s < NBUF - 2) lds_wait_barrier<(NBUF - 2) * CX>();
-    else lds_wait_barrier<(NBUF - 2) * CNT>();
+    else lds_wait_barrier<(NBUF - 2) * (CX + CW)>();
     load_w(s + NBUF - 1);
     load_x(s + NBUF - 1);
     const chunk_t *x = lds + s % NBUF * STAGE + (wave * 16 + fr) * 8, *wl = lds + s % NBUF * STAGE + (64 + fr) * 8;
@@ -359,7 +366,7 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
     if (g + 1 < a.col_groups) load_base(n0 + 128);
 #pragma unroll
     for (int m = 0; m < MT; m++)
-      if (row[m] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[m] * a.N + n, a.N - n, out[m]);
+      if (row[m] >= 0 && n < a.N) store_out<TO>(a, row[m], n, out[m]);
   }
 }
 
@@ -435,7 +442,7 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
       float f[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) f[j] = fmaf(scale, acc[j][i], (float)base[g][i].v[j]);
-      if (row[i] >= 0 && n < a.N) store_v<TO, 8>(reinterpret_cast<TO *>(a.out) + (size_t)row[i] * a.N + n, a.N - n, f);
+      if (row[i] >= 0 && n < a.N) store_out<TO>(a, row[i], n, f);
     }
   }
 }

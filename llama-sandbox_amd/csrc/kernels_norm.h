@@ -371,7 +371,7 @@ __global__ __launch_bounds__(LANES *G) void k_rms_norm_grad(norm_grad_call a) {
           o[j] = rr * fmaf(-u[v][j], c, g[v][j]);
           if (a.dres) o[j] += res[v][j];
         }
-        store8_any(a.dx, a.dx_type, (size_t)row * a.H + i, a.H - i, o);
+        store8_any(a.dx, a.dx_type, (size_t)row * a.H + i, a.H - i, o, a.nt);
       }
     }
   }

@@ -25,6 +25,7 @@ struct norm_grad_call {
   void *dx;
   float *dw, *part;
   int dy_type, h_type, w_type, dx_type, T, H;
+  int nt = 0;  // set by the launch: dx goes past the caches
 };
 // Floats of `part` that a call needs.
 size_t norm_grad_scratch(int T, int H, int n_cu);
@@ -63,8 +64,9 @@ struct adapters_call {
   void *out;
   float *mid;
   int type, out_type, n, M, K, R, N;
-  // set by the launch: shares of mid, elements of K of each, blocks of out's columns, groups of 128 columns in a block
-  int splits = 1, piece = 0, col_blocks = 0, col_groups = 1;
+  // set by the launch: shares of mid, elements of K of each, blocks of out's columns, groups of 128 columns in a block;
+  // out past the caches
+  int splits = 1, piece = 0, col_blocks = 0, col_groups = 1, nt = 0;
 };
 size_t adapters_scratch(int M, int K, int R, int n_cu);
 bool launch_adapters(const adapters_call &a, int n_cu, hipStream_t st);

@@ -10,6 +10,13 @@
 
 #include <type_traits>
 
+// Outputs of more than this go past the caches: a kernel ends only when the caches have written back what it left
+// there, and the next one reads it from the memory's cache as fast.  us, through them / past them, norm and then
+// moe_quantize_i8 of its y, H = 7168 bf16 with residual:  64 rows (1.8 MB) 7.4 / 7.6, 512 (14.7 MB) 15.6 / 12.9, 1500
+// 30.6 / 29.0, 4096 61.8 / 60.8; 2000 of 2048 (16.4 MB) 17.1 / 14.1, 8191 42.8 / 39.6.  The gradient alone, 509 rows of 5120 f32 15.3 /
+// 12.9, 4096 of 7168 bf16 54.9 / 54.2, 2048 of 7168 f32 51.5 / 52.8; adapters, 4096 rows of 7168 bf16 59.2 / 55.4.
+static constexpr size_t MOE_LAYER_STREAM_BYTES = (size_t)4 << 20;
+
 // f(integral_constant) for the bytes of an element of type t.
 template <typename F>
 static void with_size(int t, F f) {
@@ -41,12 +48,6 @@ static void launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
   else launch_norm<SX, SR, 1024, 4>(a, st);
 }
 
-// Outputs of more than this go past the caches: a kernel ends only when the caches have written back what it left
-// there, and the next one reads it from the memory's cache as fast.  us, through them / past them, norm and then
-// moe_quantize_i8 of its y, H = 7168 bf16 with residual:  64 rows (1.8 MB) 7.4 / 7.6, 512 (14.7 MB) 15.6 / 12.9, 1500
-// 30.6 / 29.0, 4096 61.8 / 60.8; 2000 of 2048 (16.4 MB) 17.1 / 14.1, 8191 42.8 / 39.6.
-static constexpr size_t MOE_NORM_STREAM_BYTES = (size_t)4 << 20;
-
 bool launch_rms_norm(const norm_call &args, int n_cu, hipStream_t st) {
   norm_call a = args;
   if (!fits(a.T, 1024)) return false;
@@ -55,7 +56,7 @@ bool launch_rms_norm(const norm_call &args, int n_cu, hipStream_t st) {
     return true;
   }
   auto size = [](const void *p, int type) { return p ? type == MOE_GGML_F32 ? 4 : 2 : 0; };
-  a.nt = (size_t)a.T * a.H * (size(a.total, a.res_type) + size(a.y, a.y_type) + (a.q ? 1 : 0)) > MOE_NORM_STREAM_BYTES;
+  a.nt = (size_t)a.T * a.H * (size(a.total, a.res_type) + size(a.y, a.y_type) + (a.q ? 1 : 0)) > MOE_LAYER_STREAM_BYTES;
   with_size(a.x_type, [&](auto sx) {
     if (!a.res) launch_norm<sx, 0>(a, n_cu, st);
     else with_size(a.res_type, [&](auto sr) { launch_norm<sx, sr>(a, n_cu, st); });
@@ -89,8 +90,10 @@ static void launch_grad(const norm_grad_call &a, int n, hipStream_t st) {
   else launch_grad<SD, SH, SX, 512, 4, 1>(a, n, st);
 }
 
-bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st) {
+bool launch_rms_norm_grad(const norm_grad_call &args, int n_cu, hipStream_t st) {
+  norm_grad_call a = args;
   if (!fits(a.T, 1024)) return false;
+  a.nt = (size_t)a.T * a.H * (a.dx_type == MOE_GGML_F32 ? 4 : 2) > MOE_LAYER_STREAM_BYTES;
   if (a.H > 16384) {
     hipLaunchKernelGGL(k_rms_norm_dx_long, dim3(a.T), dim3(256), 0, st, a);
     hipLaunchKernelGGL(k_rms_norm_dw_long, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
@@ -201,12 +204,13 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   const long wide = (long)ceil_div(a.M, BM) * groups / (4 * n_cu);
   a.col_groups = wide < 1 || staged_b ? 1 : wide < groups ? (int)wide : groups;
   a.col_blocks = ceil_div(groups, a.col_groups);
+  a.nt = (size_t)a.M * a.N * (a.out_type == MOE_GGML_F32 ? 4 : 2) > MOE_LAYER_STREAM_BYTES;
   if (!fits(tiles_a * a.splits, 1024) || !fits(tiles_b * a.col_blocks, 256)) return false;
   with_type(a.type, [&](auto t) {
     typedef decltype(t) T;
     constexpr int NBUF = 5;
     if (staged_a)
-      hipLaunchKernelGGL((k_adapters_shrink_staged<T, 4, NBUF>), dim3((unsigned)(tiles_a * a.splits), ceil_div(a.R, 64)), dim3(256),
+      hipLaunchKernelGGL((k_adapters_shrink_staged<T, NBUF>), dim3((unsigned)(tiles_a * a.splits), ceil_div(a.R, 64)), dim3(256),
                          NBUF * 128 * 128, st, a);
     else if (BM == 16) launch_shrink<T, 1>(a, tiles_a, st);
     else launch_shrink<T, 2>(a, tiles_a, st);

@@ -541,6 +541,52 @@ def test_adapters_keep_a_nan_in_its_row(blk):
         close(got[ok], want, bound)
 
 
+# ---- past 4 GiB ------------------------------------------------------------------------------
+
+
+def test_norm_and_gradient_past_4_gib(blk):
+    """Rows whose elements lie past 2^32 bytes, and 2^31 elements, from the buffers' start."""
+    say("norm past 4 GiB")
+    T, H = 270000, 8192
+    x = torch.empty((T, H), dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    w = torch.ones(H, dtype=torch.bfloat16, device=DEV)
+    y, q, qs, rstd = torch.empty_like(x), torch.empty((T, H), dtype=torch.int8, device=DEV), zeros(T), zeros(T)
+    blk.rms_norm(x, w, EPS, y=y, q=q, scale=qs, rstd=rstd)
+    some = [0, 1, 131071, 131072, 262143, 262144, T - 2, T - 1]
+    check_norm(dict(y=y[some].cpu(), q=q[some].cpu(), scale=qs[some].cpu(), rstd=rstd[some].cpu()), x[some].cpu(), None, w.cpu())
+    dx, dw = torch.empty_like(x), zeros(H)
+    blk.rms_norm_grad(y, x, w, rstd, dx, dw, torch.empty(blk.rms_norm_grad_scratch(T, H), device=DEV))
+    some = torch.tensor(some)
+    ys, xs, rs = y[some.to(DEV)].cpu(), x[some.to(DEV)].cpu(), rstd[some.to(DEV)].cpu()
+    wx, _, ex, _ = ref.norm_grad(ys, xs, w.cpu(), rs, None)
+    close(dx[some.to(DEV)], wx, rounded(ex, wx, torch.bfloat16))
+    want, mag = torch.zeros(H, dtype=torch.float64, device=DEV), torch.zeros(H, dtype=torch.float64, device=DEV)
+    for i in range(0, T, 10000):
+        term = y[i:i + 10000].double() * (x[i:i + 10000].double() * rstd[i:i + 10000].double()[:, None])
+        want += term.sum(0)
+        mag += term.abs().sum(0)
+    # a workgroup's share is a chain of T / 256 rows and more, the shares a dozen steps
+    close(dw, want.cpu(), ((T // 128) * U * mag).cpu())
+
+
+def test_adapters_past_4_gib(blk):
+    say("adapters past 4 GiB")
+    M, K, R, N, n = 70000, 32768, 8, 40, 2
+    x = torch.empty((M, K), dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(2))
+    rng = np.random.default_rng(3)
+    _, _, a, b, scale, _ = adapters_inputs(rng, 4, K, R, N, n, "bf16", "f32", True)
+    of = np.sort(rng.integers(-1, n, M)).astype(np.int32)
+    offsets, perm, _, _ = expert_ref.grouping(of[:, None], n)
+    base, out, mid = zeros(M, N), zeros(M, N), torch.empty(blk.adapters_scratch(M, K, R), device=DEV)
+    blk.adapters(x, dev(a), dev(b), dev(scale), dev(offsets), dev(perm), base, out, mid)
+    some = torch.tensor([0, 1, 30000, 65535, 65536, 66000, M - 2, M - 1])
+    xs = x[some.to(DEV)].cpu()
+    want, bound = ref.adapters(xs, a, b, scale, torch.from_numpy(of)[some], base.cpu()[some], torch.float32)
+    close(out.cpu()[some], want, bound)
+
+
 # ---- refusals of the library -------------------------------------------------------------------
 
 
