@@ -494,9 +494,10 @@ moe_status moe_matmul_i8(moe_ctx *ctx, const int8_t *q_dev, const float *q_scale
 /* These calls keep the rules of the ones above: row types MOE_GGML_F32,
  * MOE_GGML_F16 or MOE_GGML_BF16; any sizes and alignment within the stated
  * limits; buffers that are written overlap no other but where it says so; no
- * allocation, no shared scratch (a workspace is the caller's: calls that
- * overlap in time need one each), and the caller's current device stays.  T <
- * 2^24 rows, else MOE_ERR_UNSUPPORTED. */
+ * allocation, no scratch of the context (a workspace is the caller's: calls that
+ * overlap in time, graphs that may replay at once among them, need one each);
+ * several streams, threads and captures; and the caller's current device stays.
+ * T < 2^22 rows, else MOE_ERR_UNSUPPORTED where a launch does not take them. */
 
 /* Norm of rows x [T][H], w [H]: y = h * r * w, r = (mean h^2 + eps)^-1/2, eps a
  * positive normal float.  residual NULL: h = x.  Else h = x + residual,
@@ -529,7 +530,8 @@ moe_status moe_rms_norm_grad(moe_ctx *ctx, const void *dy_dev, int dy_type, cons
  * where there are fewer numbers; a group without any comes last); the `keep` best groups
  * stay, and the k largest c of their experts are picked, in that order; ties go
  * to the lowest index, NaN comes after every number.  k <= 64 and k <= keep *
- * E/n_group.  A slot that finds no expert has id -1, which moe_group drops, and weight 0.
+ * E/n_group.  A slot that finds no expert has id -1 and weight 0: moe_group drops
+ * such a pair; moe_forward does not take it.
  * The order is that of c in 64 bits (moe_route: in 32), without a bias that of
  * the logits.  Weights as moe_route's.  scores (may be NULL): [T][E] f32. */
 moe_status moe_route_groups(moe_ctx *ctx, const void *logits_dev, int logits_type, const float *bias_dev, int T, int E,
@@ -550,8 +552,9 @@ moe_status moe_route_grad(moe_ctx *ctx, const void *logits_dev, int logits_type,
  * as the experts' rows are: moe_group of the rows' adapters with k = 1 (-1: the row
  * has none) gives offsets [n+1] and perm [M]; rows of out without an adapter are
  * left as they were.  An entry of perm outside [0, M) is skipped; a valid perm names
- * no row twice.  Adapters of lower rank are padded with zeros.  Sums are f32.
- * n <= 1024, R <= 1024, K and N <= 2^30.  mid: a workspace of
+ * no row twice.  Adapters of lower rank are padded with zeros.  Sums are f32; a
+ * value that is not finite makes its row's not finite (an infinity may become
+ * NaN).  n <= 1024, R <= 1024, K and N <= 2^30.  mid: a workspace of
  * moe_adapters_scratch floats (0 for sizes that the call refuses). */
 size_t moe_adapters_scratch(const moe_ctx *ctx, int M, int K, int R);
 moe_status moe_adapters(moe_ctx *ctx, const void *x_dev, const void *a_dev, const void *b_dev, int type,

@@ -129,7 +129,9 @@ __device__ __forceinline__ float norm_scale(double amax) {
 
 // A row in one pass: LANES threads hold it in registers, VPT vectors of 8 each (H <= 8 LANES
 // VPT); 256 / LANES rows a workgroup where that is more than one.  SX, SR: bytes of an element of x and of the residual
-// (0: none).
+// (0: none).  Bound by memory: 4096 rows of 7168 bf16 with residual (235 MB) 45.7 us, 5.1 TB/s, as a large copy; 512
+// rows 7.3; 8191 of 2048 25.6.  To 8 bits the same 4096 rows (205 MB) take 52.5: products, maxima and codes in 64 bits
+// (18 such instructions a value) are then as much as the loads hide.  One row 3.6 us: a launch, the loads, two barriers.
 template <int SX, int SR, int LANES, int VPT>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_call a) {
   constexpr int NT = LANES < 256 ? 256 : LANES;
@@ -298,6 +300,9 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // rows in steps of the grid, with the next row's loads in flight while it sums this one's, and keeps
 // its share of dw in registers; k_rms_norm_dw adds the shares up (part: one of H values a workgroup;
 // a single workgroup writes dw itself).  SD, SH, SX: bytes of an element of dy, h, dx and dres.
+// One workgroup of 1024 threads a CU: two of 512 with two vectors a thread need 148 registers and ran one at a time
+// (4096 rows of 7168 bf16 64 us).  Bound by memory: those rows (235 MB, and 7 of shares written and read) 49.6 us and
+// 4.8 for the shares; 301 of 2048 f32 5.2 and 2.6, latency; 1000 of 12000 (no row ahead) 39.
 template <int SD, int SH, int SX, int LANES, int VPT, int G>
 __global__ __launch_bounds__(LANES *G) void k_rms_norm_grad(norm_grad_call a) {
   constexpr int NT = LANES * G, W = LANES > 64 ? LANES / 64 : 1;

@@ -141,6 +141,9 @@ __device__ __forceinline__ uint64_t route_stay_any(const route_call &a, const K 
 // Scores with a bias are compared in 32 bits: that decides unless two that stand next to each other in the
 // order come closer than both may be off.  Then those that may be picked are placed by their scores in 64 bits,
 // and where it is two groups (or more experts than a wave has lanes) the token is done again in 64 bits.
+// Bound by the instructions of a pick, about 35 one after the other (0.12 us alone), and by latency: 256 experts in 8
+// groups, bias, top-8: one token 4.6 us, 4096 9.7 (everything in 64 bits 13.4; keys not sorted in their lanes
+// 14.3; without bias and groups 5.9).  Lanes hold neighbours, not every 64th expert: a group is then whole lanes.
 template <int NJ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
   // for the groups' scores
@@ -383,6 +386,7 @@ __device__ __forceinline__ void route_slope(float l, int mode, float &s, float &
 
 // One wave a token, WAVES a workgroup, lane i with experts [NJ i, NJ i + NJ) in registers.  The picked
 // experts' gradients go to their lanes slot by slot, which adds an expert that is named twice in slot order.
+// Latency: 4096 tokens of 256 experts with dscores (12.8 MB) 6.6 us (10.9 with the scores in LDS); 301 of 160 3.4.
 template <int NJ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_route_grad(route_grad_call a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = a.E, e0 = lane * NJ;

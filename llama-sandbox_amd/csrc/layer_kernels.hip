@@ -25,9 +25,12 @@ static void with_size(int t, F f) {
 }
 
 template <int SX, int SR, int LANES, int VPT>
-static void launch_norm(const norm_call &a, hipStream_t st) {
+static bool launch_norm(const norm_call &a, hipStream_t st) {
   constexpr int NT = LANES < 256 ? 256 : LANES;
-  hipLaunchKernelGGL((k_rms_norm<SX, SR, LANES, VPT>), dim3(ceil_div(a.T, NT / LANES)), dim3(NT), 0, st, a);
+  const int n = ceil_div(a.T, NT / LANES);
+  if (!fits(n, NT)) return false;
+  hipLaunchKernelGGL((k_rms_norm<SX, SR, LANES, VPT>), dim3(n), dim3(NT), 0, st, a);
+  return true;
 }
 
 // Threads a row and vectors a thread.  A row of 4097 to 8192 in one vector a thread where the rows are too few to fill
@@ -35,33 +38,34 @@ static void launch_norm(const norm_call &a, hipStream_t st) {
 //   threads x vectors:   7168:  1024 x 1  45.6 / 58.0   512 x 2  45.8 / 50.9   256 x 4  48.6 / 47.5   128 x 8  80 / 90
 //                        2048:  256 x 1  25.2   128 x 2  26.4   64 x 4  27.9     1024:  128 x 1  14.8   64 x 2  14.9
 template <int SX, int SR>
-static void launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
+static bool launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
   const int H = a.H;
-  if (H <= 128) launch_norm<SX, SR, 16, 1>(a, st);
-  else if (H <= 512) launch_norm<SX, SR, 64, 1>(a, st);
-  else if (H <= 1024) launch_norm<SX, SR, 128, 1>(a, st);
-  else if (H <= 2048) launch_norm<SX, SR, 256, 1>(a, st);
-  else if (H <= 4096) launch_norm<SX, SR, 256, 2>(a, st);
-  else if (H <= 8192 && a.T < 2 * n_cu) launch_norm<SX, SR, 1024, 1>(a, st);
-  else if (H <= 8192) launch_norm<SX, SR, 512, 2>(a, st);
-  else if (H <= 16384) launch_norm<SX, SR, 1024, 2>(a, st);
-  else launch_norm<SX, SR, 1024, 4>(a, st);
+  if (H <= 128) return launch_norm<SX, SR, 16, 1>(a, st);
+  if (H <= 512) return launch_norm<SX, SR, 64, 1>(a, st);
+  if (H <= 1024) return launch_norm<SX, SR, 128, 1>(a, st);
+  if (H <= 2048) return launch_norm<SX, SR, 256, 1>(a, st);
+  if (H <= 4096) return launch_norm<SX, SR, 256, 2>(a, st);
+  if (H <= 8192 && a.T < 2 * n_cu) return launch_norm<SX, SR, 1024, 1>(a, st);
+  if (H <= 8192) return launch_norm<SX, SR, 512, 2>(a, st);
+  if (H <= 16384) return launch_norm<SX, SR, 1024, 2>(a, st);
+  return launch_norm<SX, SR, 1024, 4>(a, st);
 }
 
 bool launch_rms_norm(const norm_call &args, int n_cu, hipStream_t st) {
   norm_call a = args;
-  if (!fits(a.T, 1024)) return false;
   if (a.H > 32768) {
+    if (!fits(a.T, 256)) return false;
     hipLaunchKernelGGL(k_rms_norm_long, dim3(a.T), dim3(256), 0, st, a);
     return true;
   }
   auto size = [](const void *p, int type) { return p ? type == MOE_GGML_F32 ? 4 : 2 : 0; };
   a.nt = (size_t)a.T * a.H * (size(a.total, a.res_type) + size(a.y, a.y_type) + (a.q ? 1 : 0)) > MOE_LAYER_STREAM_BYTES;
+  bool fine = false;
   with_size(a.x_type, [&](auto sx) {
-    if (!a.res) launch_norm<sx, 0>(a, n_cu, st);
-    else with_size(a.res_type, [&](auto sr) { launch_norm<sx, sr>(a, n_cu, st); });
+    if (!a.res) fine = launch_norm<sx, 0>(a, n_cu, st);
+    else with_size(a.res_type, [&](auto sr) { fine = launch_norm<sx, sr>(a, n_cu, st); });
   });
-  return true;
+  return fine;
 }
 
 // The gradient's workgroups walk rows, G of them at once, one workgroup a CU: each has a share of dw.
@@ -92,9 +96,9 @@ static void launch_grad(const norm_grad_call &a, int n, hipStream_t st) {
 
 bool launch_rms_norm_grad(const norm_grad_call &args, int n_cu, hipStream_t st) {
   norm_grad_call a = args;
-  if (!fits(a.T, 1024)) return false;
   a.nt = (size_t)a.T * a.H * (a.dx_type == MOE_GGML_F32 ? 4 : 2) > MOE_LAYER_STREAM_BYTES;
   if (a.H > 16384) {
+    if (!fits(a.T, 256)) return false;
     hipLaunchKernelGGL(k_rms_norm_dx_long, dim3(a.T), dim3(256), 0, st, a);
     hipLaunchKernelGGL(k_rms_norm_dw_long, dim3(ceil_div(a.H, 64)), dim3(256), 0, st, a);
     return true;
