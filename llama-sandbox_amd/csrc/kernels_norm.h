@@ -130,8 +130,8 @@ __device__ __forceinline__ float norm_scale(double amax) {
 // A row in one pass: LANES threads hold it in registers, VPT vectors of 8 each (H <= 8 LANES
 // VPT); 256 / LANES rows a workgroup where that is more than one.  SX, SR: bytes of an element of x and of the residual
 // (0: none).  Bound by memory: 4096 rows of 7168 bf16 with residual (235 MB) 45.7 us, 5.1 TB/s, as a large copy; 512
-// rows 7.3; 8191 of 2048 25.6.  To 8 bits the same 4096 rows (205 MB) take 52.5: products, maxima and codes in 64 bits
-// (18 such instructions a value) are then as much as the loads hide.  One row 3.6 us: a launch, the loads, two barriers.
+// rows 7.3; 8191 of 2048 25.6.  To 8 bits the same 4096 rows (205 MB) take 48.1, 4.3 TB/s: products, maxima and codes in
+// 64 bits are 14 instructions a value (with 20, 52.5).  One row 3.6 us: a launch, the loads, two barriers.
 template <int SX, int SR, int LANES, int VPT>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_call a) {
   constexpr int NT = LANES < 256 ? 256 : LANES;
@@ -210,14 +210,18 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
   }
   if (!a.q) return;
   double m = 0.0;
+  float odd = 0.0f;  // NaN where the gain has a value that is not finite (one of h shows in r)
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
     float w[8];
     gain(v, w);
 #pragma unroll
-    for (int j = 0; j < 8; j++) m = max_nan(m, fabs((double)h[v][j] * (double)w[j]));
+    for (int j = 0; j < 8; j++) {
+      m = fmax(m, fabs((double)h[v][j] * (double)w[j]));
+      odd = fmaf(w[j], 0.0f, odd);
+    }
   }
-  m = row_reduce_d<LANES>(m, part[1], max_nan);
+  m = row_reduce_d<LANES>(odd == odd ? m : __builtin_nan(""), part[1], max_nan);
   if (!there) return;
   const float s = norm_scale(m * r);
   if (in_row == 0) a.scale[row] = s;
@@ -229,9 +233,12 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
     float w[8];
     gain(v, w);
     uint32_t code[8];
+    // + 1.5 * 2^52 rounds to a whole number, ties to even, with it in the low word; past 127 only by a denormal scale
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      code[j] = (uint32_t)(int)fmin(fmax(__builtin_rint((double)h[v][j] * (double)w[j] * g), -127.0), 127.0);
+    for (int j = 0; j < 8; j++) {
+      const double u = fma((double)h[v][j] * (double)w[j], g, 0x1.8p52);
+      code[j] = (uint32_t)min(max((int)(uint32_t)__builtin_bit_cast(uint64_t, u), -127), 127);
+    }
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(1)));
     int8_t *to = a.q + at + i;
     if (!(s > 0.0f)) {

@@ -122,6 +122,22 @@ def test_norm_of_rows_without_a_norm(blk, H):
         check_norm({k: v[ok] for k, v in got.items()}, x[ok], None, w)
 
 
+@pytest.mark.parametrize("H", [16, 777, 7168, 36000])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+def test_norm_with_a_gain_that_is_not_finite(blk, H, what):
+    """Every row has such a value, so none has a scale."""
+    say("norm gain", H, what)
+    rng = np.random.default_rng(H)
+    x, w = floats(rng, (5, H), "bf16"), floats(rng, (H,), "f32")
+    w[H // 2] = what
+    got = run_norm(blk, x, None, w, "f32", True)
+    assert torch.isnan(got["scale"]).all() and not got["q"].any()
+    ok = [i for i in range(H) if i != H // 2]
+    y, _ = ref.norm(x, w, EPS)
+    close(got["y"][:, ok], y[:, ok], ref.norm_bound(y[:, ok], torch.float32))
+    assert not torch.isfinite(got["y"][:, H // 2]).any()
+
+
 def test_codes_next_to_a_tie(blk):
     """Values whose quotients lie at a half and next to it: decided as in 64 bits."""
     say("ties")
