@@ -36,9 +36,9 @@ __device__ __forceinline__ double wave_max_d(double v) {
   return lanes_reduce_d<64>(v, [](double a, double b) { return fmax(a, b); });
 }
 
-// A score as a whole number that orders as it does, NaN below every number; 0: no candidate.
+// A score as a whole number that orders as it does (-0 as 0), NaN below every number; 0: no candidate.
 __device__ __forceinline__ uint32_t route_key(float c) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, c);
+  const uint32_t u = __builtin_bit_cast(uint32_t, c + 0.0f);
   return c != c ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 // For 64 bits: a NaN is -inf, what is -inf the lowest finite value above it.
@@ -50,7 +50,7 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_max_u(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
 }
-// The largest over the wave, as a scalar: five steps towards lane 63, one read.
+// The largest over the wave, as a scalar: six steps towards lane 63, one read.
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   v = dpp_max_u<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
   v = dpp_max_u<0x112, 0xF>(v);
@@ -60,6 +60,7 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   v = dpp_max_u<0x143, 0xC>(v);  // row_bcast31: lane 31 to rows 2 and 3
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+
 // Logits [at, at + N) of a token as f32, -inf from `left` on.
 template <int N>
 __device__ __forceinline__ void route_load(const void *logits, int type, size_t at, int left, float (&l)[N]) {
@@ -282,30 +283,29 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
     if (a.bias) {
       // two that follow each other, both numbers
       const uint32_t after = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)my_key, 0x130, 0xF, 0xF, false);  // wave_shl 1
-      if (__ballot(my_key > 1 && after > 1 && !(value(my_key) - value(after) > near))) {
-        again = n == 64;
-        if (!again) {  // those picked and those that may belong among them, by their place in 64 bits
-          double sum_d = 1.0, c = -INFINITY;
-          if (soft) {
-            sum_d = 0.0;
+      again = n == 64;  // (there may be more that belong among them)
+      if (!again && __ballot(my_key > 1 && after > 1 && !(value(my_key) - value(after) > near))) {
+        // those picked and those that may belong among them, by their place in 64 bits
+        double sum_d = 1.0, c = -INFINITY;
+        if (soft) {
+          sum_d = 0.0;
 #pragma unroll
-            for (int j = 0; j < NJ; j++) sum_d += exp((double)l[j] - (double)top);
-            sum_d = wave_sum_d(sum_d);
-          }
-          if (my_id >= 0) {
-            float one[1];
-            route_load<1>(a.logits, a.type, at + my_id, 1, one);
-            c = route_key_d((soft ? exp((double)one[0] - (double)top) / sum_d : route_score_d((double)one[0], a.mode)) +
-                            (double)a.bias[my_id]);
-          }
-          int place = 0;
-          for (int o = 0; o < n; o++) {
-            const double other = readlane_d(c, o);
-            const int other_id = __builtin_amdgcn_readlane(my_id, o);
-            place += other > c || (other == c && other_id < my_id);
-          }
-          my_id = __builtin_amdgcn_ds_permute(4 * (lane < n ? place : lane), my_id);
+          for (int j = 0; j < NJ; j++) sum_d += exp((double)l[j] - (double)top);
+          sum_d = wave_sum_d(sum_d);
         }
+        if (my_id >= 0) {
+          float one[1];
+          route_load<1>(a.logits, a.type, at + my_id, 1, one);
+          c = route_key_d((soft ? exp((double)one[0] - (double)top) / sum_d : route_score_d((double)one[0], a.mode)) +
+                          (double)a.bias[my_id]);
+        }
+        int place = 0;
+        for (int o = 0; o < n; o++) {
+          const double other = readlane_d(c, o);
+          const int other_id = __builtin_amdgcn_readlane(my_id, o);
+          place += other > c || (other == c && other_id < my_id);
+        }
+        my_id = __builtin_amdgcn_ds_permute(4 * (lane < n ? place : lane), my_id);
       }
     }
     if (lane >= a.k) my_id = -1;

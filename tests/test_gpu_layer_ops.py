@@ -332,6 +332,37 @@ def test_route_of_scores_closer_than_32_bits_tell(blk, mode, n_group, keep, top,
     assert other
 
 
+def test_route_where_the_last_pick_is_close_to_the_next(blk):
+    """Of 100 experts well apart, the k-th and the next within a rounding; as many picks as a wave has lanes, and fewer."""
+    say("route last pick")
+    rng = np.random.default_rng(21)
+    for k in (1, 5, 63, 64):
+        other = 0
+        for _ in range(12):
+            l = rng.standard_normal((1, 100)).astype(np.float32)
+            p = ref.scores(l.astype(np.float64), 1)[0]
+            place = rng.permutation(100)
+            target = 2.0 - 0.01 * place
+            target[place == k] = target[place == k - 1]  # the expert after the k-th
+            bias = (target - p).astype(np.float32)
+            args = (k, 1, 1, 1, 1, True, 1.0)
+            check_route(run_route(blk, torch.from_numpy(l), bias, *args), torch.from_numpy(l), bias, *args)
+            c = p + bias.astype(np.float64)
+            other += (np.argsort(-c, kind="stable") != np.argsort(-(p.astype(np.float32) + bias), kind="stable")).any()
+        assert other
+
+
+def test_route_takes_the_two_zeros_as_equal(blk):
+    say("route zeros")
+    rng = np.random.default_rng(22)
+    for n_group, keep in ((1, 1), (4, 2)):
+        l = torch.from_numpy(rng.choice([-0.0, 0.0, -1.0], (30, 64)).astype(np.float32))
+        for bias in (None, rng.choice([-0.5, -0.0, 0.0], 64).astype(np.float32)):
+            for mode in (0, 1, 2):
+                args = (6, mode, n_group, keep, 1, False, 1.0)
+                check_route(run_route(blk, l, bias, *args), l, bias, *args)
+
+
 def test_route_of_groups_closer_than_32_bits_tell(blk):
     """Groups whose two best scores sum to within a rounding of the same."""
     say("route groups close")
