@@ -188,15 +188,16 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   const int matrices = a.M < a.n ? a.M : a.n, each = a.M / matrices;  // adapters that can have rows; rows of each
   const size_t size = a.type == MOE_GGML_F32 ? 4 : 2;
   // Staged where adapters have rows for its tiles: the product with A from rank 33 on, the one with B where there are
-  // four workgroups a CU.  us, staged / straight to registers (bf16 rows x K x rank x N, adapters; * the rule's):
+  // three workgroups for two CUs.  us, staged / straight to registers (bf16 rows x K x rank x N, adapters; * the rule's):
   //   with A:  4096 x 7168 x 64 x 7168, 8   59.6* / 63.9   x 32  52.5 / 53.5*   x 16  50.3 / 48.7*
   //            2048 x 2048 x 64 x 2048, 16 (f32)  37.6* / 40.6    2048 x 768 x 8 x 768, 60 (f32)  16.1 / 13.1*
   //   with B:  4096 x 7168 x 64 x 7168, 8   59.6* / 67.4   x 16  48.7* / 51.2
-  //            2048 x 2048 x 64 x 2048, 16 (f32)  43.8 / 37.6*    512 x 4096 x 32 x 4096, 16  16.6 / 13.1*
+  //            2048 x 4096 x 64 x 4096, 16   27.4* / 32.5   x 16  24.1* / 27.4    1024 x 7168 x 64 x 7168, 4  25.4* / 28.4
+  //            2048 x 2048 x 64 x 2048, 16 (f32)  42.8 / 35.4*   (f16)  24.5 / 20.9*    512 x 4096 x 32 x 4096, 16  16.6 / 13.1*
   //   both at 16 rows an adapter: 517 x 2048 x 8 x 768, 32  15.6 / 9.3*
   const bool staged_a = each >= 32 && a.R > 32 && a.K * size % 16 == 0 && ((uintptr_t)a.x | (uintptr_t)a.a) % 16 == 0 &&
                         (uint64_t)a.M * a.K * size < MOE_LDS_OOB && (uint64_t)a.R * a.K * size < MOE_LDS_OOB;
-  const bool staged_b = each >= 32 && (long)ceil_div(a.M, 64) * ceil_div(a.N, 256) >= 4 * n_cu && a.R <= 64 &&
+  const bool staged_b = each >= 32 && 2L * ceil_div(a.M, 64) * ceil_div(a.N, 256) >= 3 * n_cu && a.R <= 64 &&
                         a.R * size % 16 == 0 && (uintptr_t)a.b % 16 == 0 && (uint64_t)a.N * a.R * size < MOE_LDS_OOB;
   // no larger a tile than the adapters' rows fill
   const int BM = each <= 16 ? 16 : adapters_tile(a.M), groups = ceil_div(a.N, staged_b ? 256 : 128);

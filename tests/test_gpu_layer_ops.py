@@ -518,7 +518,7 @@ ADAPTERS = [(1, 64, 8, 64, 1), (1, 7168, 16, 512, 3), (2, 7, 1, 3, 2), (16, 256,
             # rows enough for the staged tiles, of every rank class, over ragged K and N
             (200, 256, 16, 300, 2), (600, 520, 64, 264, 5), (129, 1024, 8, 128, 3), (96, 72, 40, 1000, 1),
             (700, 200, 24, 2056, 4), (150, 64, 128, 136, 2), (2000, 136, 32, 96, 60), (300, 2056, 60, 129, 3),
-            (2100, 64, 24, 7945, 3), (2100, 72, 64, 8000, 2)]
+            (2100, 64, 24, 7945, 3), (2100, 72, 64, 8000, 2), (1000, 64, 8, 7000, 30)]
 
 
 @pytest.mark.parametrize("M, K, R, N, n", ADAPTERS)
