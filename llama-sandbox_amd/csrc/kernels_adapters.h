@@ -5,8 +5,8 @@
 //
 // Two launches on 16x16 MFMA tiles of an adapter's rows.  Lane l of an operand holds row l % 16 and V
 // consecutive elements of K from V (l / 16) on (V = 8 of 16 bits, 4 of f32); of the result column l % 16 and
-// rows 4 (l / 16) + i.  Tokens are the columns in both, so that a lane's four values are next to each other in mid,
-// and, with the weight rows dealt to two tiles four and four, its eight in out.
+// rows 4 (l / 16) + i.  Tokens are the columns, so that a lane's four values are next to each other in mid,
+// and, with the weight rows dealt to two tiles four and four, its eight in out (the last kernel: the other way round).
 #pragma once
 
 #include "group_tiles.h"
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
   typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
   constexpr int RT = 4, STAGE = (64 + 64) * 8;  // tiles of A's rows; chunks of a stage
   constexpr int CX = 2, CW = 2;                 // 1 KiB loads a wave: of x, of A
-  extern __shared__ uint32_t adapters_lds[];  // NBUF * STAGE chunks
+  extern __shared__ __align__(16) uint32_t adapters_lds[];  // NBUF * STAGE chunks
   chunk_t *lds = reinterpret_cast<chunk_t *>(adapters_lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), split = blockIdx.x % a.splits;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.splits, 64);

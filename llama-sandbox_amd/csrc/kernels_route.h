@@ -19,7 +19,6 @@
 #include "row_vec.h"
 #include "../../include/moe_block.h"
 
-#define MOE_ROUTE_GROUPS_MAX_E 1024
 #define MOE_ROUTE_FLOOR 6.103515625e-5f  // 2^-14
 
 __device__ __forceinline__ double route_score_d(double l, int mode) {

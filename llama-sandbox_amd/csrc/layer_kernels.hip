@@ -154,7 +154,8 @@ static constexpr int shrink_waves(int MT, int RT) { return MT * RT <= 2 ? 16 : 8
 
 // Pieces of K that the product with A is cut into: 16 waves a CU where every tile is full, two steps a wave at least.
 static int adapters_splits(int M, int K, int R, int n_cu) {
-  const int w = shrink_waves(adapters_tile(M) / 16, R <= 16 ? 1 : R <= 32 ? 2 : 4), most = ceil_div(K, 64 * w), want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
+  const int w = shrink_waves(adapters_tile(M) / 16, R <= 16 ? 1 : R <= 32 ? 2 : 4), most = ceil_div(K, 64 * w);
+  const int want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
   return most < want ? most : want;
 }
 
