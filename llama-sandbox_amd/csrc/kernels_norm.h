@@ -210,7 +210,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
   }
   if (!a.q) return;
   double m = 0.0;
-  float odd = 0.0f;  // NaN where the gain has a value that is not finite (one of h shows in r)
+  float odd = 0.0f;  // NaN where the gain has a value that is not finite; one of h shows in r, a NaN or, of an infinity, 0
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
     float w[8];
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
       odd = fmaf(w[j], 0.0f, odd);
     }
   }
-  m = row_reduce_d<LANES>(odd == odd ? m : __builtin_nan(""), part[1], max_nan);
+  m = row_reduce_d<LANES>(odd == odd && r > 0.0 ? m : __builtin_nan(""), part[1], max_nan);
   if (!there) return;
   const float s = norm_scale(m * r);
   if (in_row == 0) a.scale[row] = s;
