@@ -182,10 +182,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
       if (e0 + j < E) a.scores[at + e0 + j] = p[j];
   }
   // how close two scores in 32 bits may be in another order than in 64: each is off by 7 half steps of f32 (2^-24) of
-  // p, softmax's by 33 and twice the size of the exponent, and one of c; those next to 0 by steps of the smallest values
+  // p, softmax's by 33 and twice the size of the exponent, and one of c; those next to 0 by steps of the smallest values.
+  // A sum of two is off by what both are and by its own rounding, half a step of |c1 + c2|: as if each c were off by
+  // two.  So two scores are off by `near` together, and two groups' sums of `top` scores by top times as much
   float near = 0.0f;
   if (a.bias || sums) {
     float big = 0.0f, each = 7.0f;
+    const float round_c = sums ? 2.0f : 1.0f;
     if (soft) {
       float low = 0.0f;
 #pragma unroll
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-      const float size = fmaf(each, p[j], fabsf(p[j] + b[j]));
+      const float size = fmaf(each, p[j], round_c * fabsf(p[j] + b[j]));
       big = l[j] != -INFINITY && size < INFINITY ? fmaxf(big, size) : big;  // (infinities are what they are in 64 bits)
     }
     near = wave_max(big) * 0x1p-23f + 0x1p-120f;
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
   uint32_t key[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; j++) key[j] = l[j] == -INFINITY ? 0 : route_key(a.bias ? p[j] + b[j] : l[j]);
-  const float inv_per = 1.0f / (float)a.per;
+  const float inv_per = 1.0f / (float)a.per, near_groups = (float)a.top * near;
   bool again = false;
   auto drop = [&](uint64_t stay, auto f) {  // f(j) of the experts whose groups do not stay
 #pragma unroll
@@ -226,14 +229,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
         v2 = fmaxf(v2, fminf(v1, c[j]));
         v1 = fmaxf(v1, c[j]);
       }
-      const bool in = route_stay<float>(a, v1, v2, a.lanes, 2.0f * near, again);
+      const bool in = route_stay<float>(a, v1, v2, a.lanes, near_groups, again);
 #pragma unroll
       for (int j = 0; j < NJ; j++) key[j] = in ? key[j] : 0;
     } else {
 #pragma unroll
       for (int j = 0; j < NJ; j++) c32[wave][e0 + j] = c[j];
       __builtin_amdgcn_wave_barrier();
-      drop(route_stay_any<float>(a, c32[wave], 2.0f * near, again), [&](int j) { key[j] = 0; });
+      drop(route_stay_any<float>(a, c32[wave], near_groups, again), [&](int j) { key[j] = 0; });
     }
   }
   // lane s: the expert of slot s, and its key
