@@ -517,7 +517,8 @@ moe_status moe_rms_norm(moe_ctx *ctx, const void *x_dev, int x_type, const void 
  * dx is the gradient of x and of residual; dres (may be NULL, dx_type): that
  * of total from its other readers; it may be dx.  dw [H] f32, sums in f32 in a
  * fixed order.  part: a workspace of moe_rms_norm_grad_scratch floats (0 for sizes
- * that the call refuses). */
+ * that the call refuses), which grow with T and H: one for the largest call serves
+ * every smaller one. */
 size_t moe_rms_norm_grad_scratch(const moe_ctx *ctx, int T, int H);
 moe_status moe_rms_norm_grad(moe_ctx *ctx, const void *dy_dev, int dy_type, const void *h_dev, int h_type, const void *w_dev,
                              int w_type, const float *rstd_dev, const void *dres_dev, int T, int H, void *dx_dev,
@@ -555,7 +556,8 @@ moe_status moe_route_grad(moe_ctx *ctx, const void *logits_dev, int logits_type,
  * no row twice.  Adapters of lower rank are padded with zeros.  Sums are f32; a
  * value that is not finite makes its row's not finite (an infinity may become
  * NaN).  n <= 1024, R <= 1024, K and N <= 2^30.  mid: a workspace of
- * moe_adapters_scratch floats (0 for sizes that the call refuses). */
+ * moe_adapters_scratch floats (0 for sizes that the call refuses), which grow with
+ * M, K and R: one for the largest call serves every smaller one. */
 size_t moe_adapters_scratch(const moe_ctx *ctx, int M, int K, int R);
 moe_status moe_adapters(moe_ctx *ctx, const void *x_dev, const void *a_dev, const void *b_dev, int type,
                         const float *scale_dev, int n, const int32_t *offsets_dev, const int32_t *perm_dev, int M, int K,

@@ -27,7 +27,8 @@ struct norm_grad_call {
   int dy_type, h_type, w_type, dx_type, T, H;
   int nt = 0;  // set by the launch: dx goes past the caches
 };
-// Floats of `part` that a call needs.
+// Floats of `part` that a call needs, and that every call of at most these sizes can do with.
+size_t norm_grad_need(int T, int H, int n_cu);
 size_t norm_grad_scratch(int T, int H, int n_cu);
 bool launch_rms_norm_grad(const norm_grad_call &a, int n_cu, hipStream_t st);
 
@@ -68,5 +69,7 @@ struct adapters_call {
   // out past the caches
   int splits = 1, piece = 0, col_blocks = 0, col_groups = 1, nt = 0;
 };
+// As for the gradient: floats of `mid`.
+size_t adapters_need(int M, int K, int R, int n_cu);
 size_t adapters_scratch(int M, int K, int R, int n_cu);
 bool launch_adapters(const adapters_call &a, int n_cu, hipStream_t st);

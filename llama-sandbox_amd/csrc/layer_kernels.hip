@@ -75,7 +75,11 @@ static int grad_blocks(int T, int H, int n_cu) {
   return most < n_cu ? most : n_cu;
 }
 
-size_t norm_grad_scratch(int T, int H, int n_cu) { return H > 16384 ? 1 : (size_t)grad_blocks(T, H, n_cu) * H; }
+size_t norm_grad_need(int T, int H, int n_cu) { return H > 16384 ? 1 : (size_t)grad_blocks(T, H, n_cu) * H; }
+
+// Grows with T and H: a workspace for the largest call serves every smaller one, those of 16384 the longer rows', which have no
+// shares.
+size_t norm_grad_scratch(int T, int H, int n_cu) { return norm_grad_need(T, H < 16384 ? H : 16384, n_cu); }
 
 template <int SD, int SH, int SX, int LANES, int VPT, int G>
 static void launch_grad(const norm_grad_call &a, int n, hipStream_t st) {
@@ -152,14 +156,24 @@ bool launch_route_grad(const route_grad_call &a, hipStream_t st) {
 static int adapters_tile(int M) { return M <= 64 ? 16 : 32; }
 static constexpr int shrink_waves(int MT, int RT) { return MT * RT <= 2 ? 16 : 8; }
 
+static int split_waves(int M, int R) { return shrink_waves(adapters_tile(M) / 16, R <= 16 ? 1 : R <= 32 ? 2 : 4); }
 // Pieces of K that the product with A is cut into: 16 waves a CU where every tile is full, two steps a wave at least.
+static int most_splits(int M, int K, int R) { return ceil_div(K, 64 * split_waves(M, R)); }
 static int adapters_splits(int M, int K, int R, int n_cu) {
-  const int w = shrink_waves(adapters_tile(M) / 16, R <= 16 ? 1 : R <= 32 ? 2 : 4), most = ceil_div(K, 64 * w);
-  const int want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * w);
+  const int most = most_splits(M, K, R), want = ceil_div(16L * n_cu, (long)ceil_div(M, adapters_tile(M)) * split_waves(M, R));
   return most < want ? most : want;
 }
 
-size_t adapters_scratch(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, R, n_cu) * M * R; }
+size_t adapters_need(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, R, n_cu) * M * R; }
+
+// The pieces get fewer as the tiles get more, so what a call needs goes up and down with M.  A bound that grows with M, K and R, so
+// that a workspace for the largest call serves every smaller one: with M rows in t tiles of h <= 32, ceil(16 n_cu / (t w)) pieces
+// of M rows are fewer than 16 n_cu h / w + M rows.  (h / w grows with M and R, from 1 to 4, and the pieces of K, two steps
+// of w waves each, do too.)
+size_t adapters_scratch(int M, int K, int R, int n_cu) {
+  const size_t some = (size_t)16 * n_cu * adapters_tile(M) / split_waves(M, R) + M, all = (size_t)most_splits(M, K, R) * M;
+  return (some < all ? some : all) * R;
+}
 
 template <typename T, int MT, int RT>
 static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {

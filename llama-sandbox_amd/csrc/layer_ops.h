@@ -46,7 +46,7 @@ extern "C" moe_status moe_rms_norm_grad(moe_ctx *c, const void *dy, int dy_type,
       !is_array(rstd, 4) || (dres && !is_array(dres, db)) || !is_array(dx, db) || !is_array(dw, 4) || !is_array(part, 4) ||
       T <= 0 || H <= 0 || H > MOE_ROW_MAX)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_rms_norm_grad: bad arguments");
-  const size_t n = (size_t)T * H, need = norm_grad_scratch(T, H, c->n_cu);
+  const size_t n = (size_t)T * H, need = norm_grad_need(T, H, c->n_cu);
   if (part_floats < need)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_rms_norm_grad: part holds %zu floats, this call needs %zu", part_floats, need);
   if (overlap({{dy, n * type_bytes(dy_type), false}, {h, n * type_bytes(h_type), false}, {w, (size_t)H * type_bytes(w_type), false},
@@ -129,7 +129,7 @@ extern "C" moe_status moe_adapters(moe_ctx *c, const void *x, const void *a, con
       !is_array(perm, 4) || !is_array(base, ob) || !is_array(out, ob) || !is_array(mid, 4) || n <= 0 || n > MOE_ADAPTERS_MAX ||
       !adapters_sizes(M, K, R) || N <= 0 || N > MOE_ROW_MAX)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_adapters: bad arguments");
-  const size_t need = adapters_scratch(M, K, R, c->n_cu), no = (size_t)M * N * ob;
+  const size_t need = adapters_need(M, K, R, c->n_cu), no = (size_t)M * N * ob;
   if (mid_floats < need)
     return fail(c, MOE_ERR_INVALID_ARG, "moe_adapters: mid holds %zu floats, this call needs %zu", mid_floats, need);
   if (overlap({{x, (size_t)M * K * tb, false}, {a, (size_t)n * R * K * tb, false}, {b, (size_t)n * N * R * tb, false},

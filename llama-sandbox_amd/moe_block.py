@@ -858,7 +858,7 @@ class MoeBlock:
             self._check(st, "moe_rms_norm")
 
     def rms_norm_grad_scratch(self, T: int, H: int) -> int:
-        """Floats that rms_norm_grad's part needs for T rows of H."""
+        """Floats of rms_norm_grad's part for T rows of H and for every smaller call."""
         return int(self.lib.moe_rms_norm_grad_scratch(self.h, T, H))
 
     def rms_norm_grad(self, dy, h, w, rstd, dx, dw, part, dres=None, stream=None):
@@ -935,7 +935,7 @@ class MoeBlock:
             self._check(st, "moe_route_grad")
 
     def adapters_scratch(self, M: int, K: int, R: int) -> int:
-        """Floats that adapters' mid needs for M rows of K and rank R."""
+        """Floats of adapters' mid for M rows of K and rank R and for every smaller call."""
         return int(self.lib.moe_adapters_scratch(self.h, M, K, R))
 
     def adapters(self, x, a, b, scale, offsets, perm, base, out, mid, stream=None):

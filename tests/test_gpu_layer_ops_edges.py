@@ -5,9 +5,10 @@ import numpy as np
 import pytest
 import torch
 
+import layer_ref as ref
 from expert_ref import rounded
-from test_gpu_expert_ops import blk, floats, say  # noqa: F401
-from test_gpu_layer_ops import check_norm, run_norm, run_route
+from test_gpu_expert_ops import blk, close, dev, floats, say  # noqa: F401
+from test_gpu_layer_ops import DEV, EPS, check_norm, run_norm, run_route, zeros
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,65 @@ def test_route_of_groups_on_a_tie_of_their_sums(blk):
         clear = np.abs(two[:, 0] - two[:, 1]) > 1e-12
         assert (ids[clear].min(1) // 2 == (two[:, 1] > two[:, 0])[clear]).all()
     assert other
+
+
+def test_a_workspace_serves_every_smaller_call(blk):
+    """What a call needs grows with each size, so that one workspace for the largest of them does for all."""
+    say("workspaces")
+    rng = np.random.default_rng(41)
+    most = blk.adapters_scratch
+    sizes = sorted(set([1, 2, 16, 63, 64, 65, 128, 1000, 4000, 4064, 4095, 4096, 4097, 8160, 8192, 20000]
+                       + rng.integers(1, 20000, 60).tolist()))
+    for K in (64, 1000, 7168, 100000):
+        for R in (1, 8, 16, 17, 32, 33, 64, 65, 1024):
+            need = [most(M, K, R) for M in sizes]
+            assert all(a <= b for a, b in zip(need, need[1:])), (K, R)
+    for M in sizes:
+        need = [most(M, K, 16) for K in (1, 63, 64, 1000, 1024, 1025, 7168, 50000)]
+        assert all(a <= b for a, b in zip(need, need[1:])), M
+        need = [most(M, 7168, R) for R in (1, 15, 16, 17, 32, 33, 64, 65, 128, 1024)]
+        assert all(a <= b for a, b in zip(need, need[1:])), M
+    widths = (1, 64, 128, 129, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 40000, 2 ** 30)
+    for T in (1, 3, 64, 255, 256, 257, 5000, 10 ** 6):
+        need = [blk.rms_norm_grad_scratch(T, H) for H in widths]
+        assert all(a <= b for a, b in zip(need, need[1:])), T
+    for H in widths:
+        need = [blk.rms_norm_grad_scratch(T, H) for T in sizes]
+        assert all(a <= b for a, b in zip(need, need[1:])), H
+
+
+@pytest.mark.parametrize("R", [16, 64])
+def test_adapters_of_a_smaller_batch_in_the_largest_ones_workspace(blk, R):
+    say("adapters, one workspace", R)
+    rng = np.random.default_rng(R)
+    K, N, n, top = 7168, 64, 3, 4096
+    mid = torch.full((blk.adapters_scratch(top, K, R) + 3,), float("nan"), device=DEV)
+    x, base = floats(rng, (top, K), "bf16"), floats(rng, (top, N), "f32")
+    a = (torch.from_numpy(rng.standard_normal((n, R, K)).astype(np.float32)) / K ** 0.5).bfloat16()
+    b = (torch.from_numpy(rng.standard_normal((n, N, R)).astype(np.float32)) / R ** 0.5).bfloat16()
+    xd, ad, bd = dev(x), dev(a), dev(b)
+    for M in (4096, 4064, 2049, 2000, 100, 65, 64, 1):
+        of = np.sort(rng.integers(0, n, M)).astype(np.int32)
+        counts, offsets, perm = zeros(n, dtype=torch.int32), zeros(n + 1, dtype=torch.int32), zeros(M, dtype=torch.int32)
+        blk.group(dev(of[:, None]), n, counts, offsets, perm)
+        out = zeros(M, N)
+        blk.adapters(xd[:M], ad, bd, None, offsets, perm, dev(base[:M]), out, mid[:-3])
+        some = sorted(set([0, M // 3, M // 2, M - 1]))
+        want, bound = ref.adapters(x[some], a, b, None, torch.from_numpy(of)[some], base[some], torch.float32)
+        close(out.cpu()[some], want, bound)
+    assert torch.isnan(mid[-3:]).all()
+
+
+def test_norm_gradients_in_the_largest_ones_workspace(blk):
+    say("norm_grad, one workspace")
+    rng = np.random.default_rng(43)
+    part = torch.full((blk.rms_norm_grad_scratch(300, 20000) + 3,), float("nan"), device=DEV)
+    for T, H in ((300, 20000), (300, 16384), (300, 16385), (299, 8192), (40, 9000), (300, 64), (1, 20000)):
+        dy, h, w = floats(rng, (T, H), "f32"), floats(rng, (T, H), "f32"), floats(rng, (H,), "f32")
+        rstd = ref.norm(h, w, EPS)[1].float()
+        dx, dw = zeros(T, H), zeros(H)
+        blk.rms_norm_grad(dev(dy), dev(h), dev(w), dev(rstd), dx, dw, part[:-3])
+        wx, ww, ex, ew = ref.norm_grad(dy, h, w, rstd, None)
+        close(dx, wx, rounded(ex, wx, torch.float32))
+        close(dw, ww, ew + 1e-40)
+    assert torch.isnan(part[-3:]).all()
