@@ -515,10 +515,10 @@ moe_status moe_rms_norm(moe_ctx *ctx, const void *x_dev, int x_type, const void 
  * u = h * r and g = dy * w:
  *   dx = r * (g - u * mean(g * u)) + dres,  dw = sum over the rows of dy * u
  * dx is the gradient of x and of residual; dres (may be NULL, dx_type): that
- * of total from its other readers; it may be dx.  dw [H] f32, sums in f32 in a
- * fixed order.  part: a workspace of moe_rms_norm_grad_scratch floats (0 for sizes
- * that the call refuses), which grow with T and H: one for the largest call serves
- * every smaller one. */
+ * of total from its other readers; it may be dx.  dw [H] f32, sums in f32 (in 64
+ * bits for rows of more than 16384) in a fixed order.  part: a workspace of
+ * moe_rms_norm_grad_scratch floats (0 for sizes that the call refuses), which
+ * grow with T and H: one for the largest call serves every smaller one. */
 size_t moe_rms_norm_grad_scratch(const moe_ctx *ctx, int T, int H);
 moe_status moe_rms_norm_grad(moe_ctx *ctx, const void *dy_dev, int dy_type, const void *h_dev, int h_type, const void *w_dev,
                              int w_type, const float *rstd_dev, const void *dres_dev, int T, int H, void *dx_dev,

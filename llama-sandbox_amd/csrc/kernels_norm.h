@@ -456,15 +456,18 @@ __global__ __launch_bounds__(256) void k_rms_norm_dx_long(norm_grad_call a) {
   }
 }
 
-// dw of 64 columns a workgroup: wave v takes rows v, v + 4, ...
+// dw of 64 columns a workgroup: wave v takes rows v, v + 4, ..., a quarter of all after each other, so the sums are in 64
+// bits (in 32 they would be off by up to T / 4 half steps, where k_rms_norm_grad's chains are T / 256 and tens).  Rows
+// this long have no fast form: 1000 of 17000 bf16 384 us for dx and dw, as with sums in 32 bits.
 __global__ __launch_bounds__(256) void k_rms_norm_dw_long(norm_grad_call a) {
-  __shared__ float part[4][64];
+  __shared__ double part[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
-  float sum = 0.0f;
+  double sum = 0.0;
   if (i < a.H)
     for (int t = wave; t < a.T; t += 4)
-      sum = fmaf(load_any(a.dy, a.dy_type, (size_t)t * a.H + i), load_any(a.h, a.h_type, (size_t)t * a.H + i) * a.rstd[t], sum);
+      sum = fma((double)load_any(a.dy, a.dy_type, (size_t)t * a.H + i),
+                (double)(load_any(a.h, a.h_type, (size_t)t * a.H + i) * a.rstd[t]), sum);
   part[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && i < a.H) a.dw[i] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+  if (wave == 0 && i < a.H) a.dw[i] = (float)((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
 }

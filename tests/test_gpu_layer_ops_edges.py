@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import layer_ref as ref
-from expert_ref import rounded
+from expert_ref import TYPES, U, rounded
 from test_gpu_expert_ops import blk, close, dev, floats, say  # noqa: F401
 from test_gpu_layer_ops import DEV, EPS, check_norm, run_norm, run_route, zeros
 
@@ -149,3 +149,31 @@ def test_norm_gradients_in_the_largest_ones_workspace(blk):
         close(dx, wx, rounded(ex, wx, torch.float32))
         close(dw, ww, ew + 1e-40)
     assert torch.isnan(part[-3:]).all()
+
+
+def test_gain_gradient_of_long_rows_and_many(blk):
+    """Terms of one sign that f32 rounds the same way at each addition: a sum along all the rows would be off by far
+    more than one of parts."""
+    say("dw of long rows, many rows")
+    T, H = 8000, 16392
+    v = 1.0 + 2.0 ** -14 - 2.0 ** -20
+    dy, h = torch.full((T, H), v, device=DEV), torch.ones((T, H), device=DEV)
+    dx, dw = torch.empty((T, H), device=DEV), zeros(H)
+    blk.rms_norm_grad(dy, h, torch.ones(H, device=DEV), torch.ones(T, device=DEV), dx, dw,
+                      zeros(blk.rms_norm_grad_scratch(T, H)))
+    want = torch.full((H,), T * v, dtype=torch.float64)
+    close(dw, want, (ref.chain(T) + 3) * U * want)
+
+
+@pytest.mark.parametrize("T, H", [(700, 16386), (2500, 17001)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_norm_grad_of_long_rows(blk, T, H, kind):
+    say("norm_grad long", T, H, kind)
+    rng = np.random.default_rng(T)
+    dy, h, w = floats(rng, (T, H), kind), floats(rng, (T, H), kind), floats(rng, (H,), "f32")
+    rstd = ref.norm(h, w, EPS)[1].float()
+    dx, dw = zeros(T, H, dtype=TYPES[kind]), zeros(H)
+    blk.rms_norm_grad(dev(dy), dev(h), dev(w), dev(rstd), dx, dw, zeros(blk.rms_norm_grad_scratch(T, H)))
+    wx, ww, ex, ew = ref.norm_grad(dy, h, w, rstd, None)
+    close(dx, wx, rounded(ex, wx, TYPES[kind]))
+    close(dw, ww, ew + 1e-40)
