@@ -432,8 +432,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_grad(route_grad_call a) {
   if (mine[0] == -INFINITY) own = 0.0f;
   if (a.scale != 0.0f) dw *= a.scale;
   if (a.norm) {
-    const float S = wave_sum(own), in = wave_sum(dw * own), D = fmaxf(S, MOE_ROUTE_FLOOR);
-    dw = __fdiv_rn(dw - (S >= MOE_ROUTE_FLOOR ? __fdiv_rn(in, D) : 0.0f), D);
+    // (a sum that is NaN is no less than its floor: the weights are NaN, and so is their gradient)
+    const float S = wave_sum(own), in = wave_sum(dw * own), D = S < MOE_ROUTE_FLOOR ? MOE_ROUTE_FLOOR : S;
+    dw = __fdiv_rn(dw - (S < MOE_ROUTE_FLOOR ? 0.0f : __fdiv_rn(in, D)), D);
   }
   if (!there) dw = 0.0f;
   for (int s = 0; s < a.k; s++) {

@@ -177,3 +177,28 @@ def test_norm_grad_of_long_rows(blk, T, H, kind):
     wx, ww, ex, ew = ref.norm_grad(dy, h, w, rstd, None)
     close(dx, wx, rounded(ex, wx, TYPES[kind]))
     close(dw, ww, ew + 1e-40)
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_route_grad_of_picks_with_a_score_that_is_no_number(blk, mode, what):
+    """Weights divided by a sum that is NaN (or by an infinite one) have no gradient: neither has the sum's floor."""
+    say("route_grad nan", mode, what)
+    rng = np.random.default_rng(51)
+    T, E, k = 6, 40, 4
+    l, dwts = rng.standard_normal((T, E)).astype(np.float32), rng.standard_normal((T, k)).astype(np.float32)
+    ids = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32)
+    l[2, ids[2, 1]] = what
+    dl = zeros(T, E)
+    blk.route_grad(dev(l), dev(ids), dev(dwts), mode, True, 1.5, dl)
+    got = dl.cpu().double().numpy()
+    with np.errstate(all="ignore"):
+        want, bound = ref.route_grad(l, ids, dwts, None, mode, True, 1.5)
+    ok = [0, 1, 3, 4, 5]
+    close(torch.from_numpy(got[ok]), torch.from_numpy(want[ok]), torch.from_numpy(bound[ok]))
+    rest = np.setdiff1d(np.arange(E), ids[2])
+    assert (got[2, rest] == 0).all()
+    if mode == 1 and what == float("inf"):  # a score of 1
+        close(torch.from_numpy(got[2]), torch.from_numpy(want[2]), torch.from_numpy(bound[2]))
+    else:
+        assert np.isnan(got[2, ids[2]]).all(), got[2, ids[2]]
