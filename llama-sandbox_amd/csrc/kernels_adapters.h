@@ -221,8 +221,10 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
   }
 }
 
-// A 16-byte piece of mid as the operands that multiply a piece of B: f32 as it is; else as PARTS bf16 parts, each what
-// the ones before leave (2: 2^-16 of it is lost, where the output is rounded to 2^-8 of its; 3: 2^-24).
+// mid as the operands that multiply a piece of B: f32 as it is; else as three bf16 parts, each the leading 8 bits of what
+// the ones before leave, so that together they are its 24 bits.  (Two would do for an output of 16 bits, but not where
+// base and update, or the products of B, cancel; 4096 rows x 64 x 7168 bf16 36.6 us with two.)  The parts are cut, not
+// rounded: a value next to the largest stays finite.
 // A piece of f16 weights is two bf16 pieces, which hold it exactly, at bf16's range: mid may be past f16's.
 template <typename T>
 struct expand_of {
@@ -244,7 +246,33 @@ __device__ __forceinline__ void weight_parts(const frag<_Float16> &w, frag<bf16_
   }
 }
 
-// mid of ROWS grouped rows of a tile from rc on, its shares added up, cut into parts in LDS: 64 of R.  256 threads.
+template <typename T>
+constexpr int mid_parts() { return sizeof(T) == 4 ? 1 : 3; }
+
+template <typename TE, int N>
+using vec_of_n = TE __attribute__((ext_vector_type(N)));
+
+template <int N>
+__device__ __forceinline__ void cut_mid(float (&f)[N], vec_of_n<float, N> (&o)[1]) {
+#pragma unroll
+  for (int j = 0; j < N; j++) o[0][j] = f[j];
+}
+template <int N>
+__device__ __forceinline__ void cut_mid(float (&f)[N], vec_of_n<bf16_t, N> (&o)[3]) {
+#pragma unroll
+  for (int p = 0; p < 3; p++) {
+    vec_of_n<uint16_t, N> top;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const uint32_t u = __builtin_bit_cast(uint32_t, f[j]);
+      top[j] = (uint16_t)(u >> 16);
+      f[j] -= __builtin_bit_cast(float, u & 0xffff0000u);
+    }
+    o[p] = __builtin_bit_cast(vec_of_n<bf16_t, N>, top);
+  }
+}
+
+// mid of ROWS grouped rows of a tile from rc on, its shares added up, in LDS as parts of TE: 64 of R.  256 threads.
 template <typename TE, int PARTS, int ROWS, int ROW>
 __device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile &t, int rc, TE (&mid)[PARTS][ROWS][ROW]) {
   // pieces of 4 a thread, and shares of each in flight
@@ -272,17 +300,10 @@ __device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile
 #pragma unroll
   for (int q = 0; q < PIECES; q++) {
     const int i = threadIdx.x + q * 256;
-    typedef TE vec4 __attribute__((ext_vector_type(4)));
+    vec_of_n<TE, 4> o[PARTS];
+    cut_mid(f[q], o);
 #pragma unroll
-    for (int p = 0; p < PARTS; p++) {
-      vec4 o;
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        o[j] = (TE)f[q][j];
-        f[q][j] -= (float)o[j];
-      }
-      *reinterpret_cast<vec4 *>(&mid[p][i / (RC / 4)][i % (RC / 4) * 4]) = o;
-    }
+    for (int p = 0; p < PARTS; p++) *reinterpret_cast<vec_of_n<TE, 4> *>(&mid[p][i / (RC / 4)][i % (RC / 4) * 4]) = o[p];
   }
 }
 
@@ -290,11 +311,11 @@ __device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile
 // with the next group's loads in flight; mid's shares are added up and cut into parts in LDS, 64 of R at a time.
 // Four workgroups a CU (at most 128 registers) or the chains of loads show: 4096 rows x 16 x 7168 45 us with 208
 // registers, 31 with 102.  16 single tokens x 16 x 4096 4.5 us.
-template <typename T, typename TO, int MT, int PARTS>
+template <typename T, typename TO, int MT>
 __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
-  constexpr int RC = 64, STEPS = RC / F::STEP, WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
+  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>(), WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
   constexpr int ROW = RC + F::V;  // a piece more, so that rows lie in different banks
   __shared__ __attribute__((aligned(16))) TE mid[PARTS][16 * MT][ROW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % 16, kg = lane / 16;
@@ -382,15 +403,16 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
 // LDS row 16 j + l of a group is row 8 l + j of B.  B's rows are whole 16 bytes, an adapter's below 4 GiB.  4096 rows of
 // 64 x 7168 bf16 (117 MB of base and out) 36.6 us, x 16 31: workgroups of one phase after another (offsets; B, mid, base;
 // the products; out), three a CU.
-template <typename T, typename TO, int PARTS>
+template <typename T, typename TO>
 __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a) {
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
   typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
-  constexpr int RC = 64, STEPS = RC / F::STEP, WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1, ROW = RC + F::V;
+  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>(), WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
+  constexpr int ROW = RC + 4;                        // a piece more, so that rows lie in different banks
   constexpr int BLOCKS = RC * (int)sizeof(T) / 128;  // of 128 bytes of B's rows
   __shared__ chunk_t lds[BLOCKS * 256 * 8];
-  __shared__ __attribute__((aligned(16))) TE mid[PARTS][64][ROW];
+  __shared__ __attribute__((aligned(16))) float mid[1][64][ROW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
   const row_tile t = find_row_tile(a.offsets, a.n, a.M, blockIdx.x / a.col_blocks, 64);
   if (t.e < 0) return;
@@ -418,14 +440,20 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
       base[g][i].load(reinterpret_cast<const TO *>(a.base) + (size_t)(row[i] < 0 ? 0 : row[i]) * a.N + n, row[i] < 0 ? 0 : a.N - n);
     }
   const float scale = a.scale ? a.scale[t.e] : 1.0f;
-  stage_mid<TE, PARTS, 64, ROW>(a, t, 0, mid);
+  stage_mid<float, 1, 64, ROW>(a, t, 0, mid);
   lds_wait_barrier<0>();
+  // (as f32 in LDS, cut here: a row's parts are one wave's, and three of them in LDS would leave two workgroups a CU)
   F fm[STEPS][PARTS];
 #pragma unroll
-  for (int s = 0; s < STEPS; s++)
+  for (int s = 0; s < STEPS; s++) {
+    float f[F::V];
 #pragma unroll
-    for (int p = 0; p < PARTS; p++)
-      fm[s][p].v = *reinterpret_cast<const typename F::vec *>(&mid[p][wave * 16 + fr][s * F::STEP + fg * F::V]);
+    for (int j = 0; j < F::V; j++) f[j] = mid[0][wave * 16 + fr][s * F::STEP + fg * F::V + j];
+    vec_of_n<TE, F::V> o[PARTS];
+    cut_mid(f, o);
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) fm[s][p].v = o[p];
+  }
 #pragma unroll
   for (int g = 0; g < 2; g++) {
     const int n = first + g * 128 + fr * 8;

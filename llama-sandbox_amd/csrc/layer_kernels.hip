@@ -188,14 +188,9 @@ static void launch_shrink(const adapters_call &a, long tiles, hipStream_t st) {
   else launch_shrink<T, MT, 4>(a, tiles, st);
 }
 
-// Parts of mid: see k_adapters_expand.
-template <typename T, typename TO>
-static constexpr int expand_parts() { return sizeof(T) == 4 ? 1 : std::is_same<T, bf16_t>::value && sizeof(TO) == 2 ? 2 : 3; }
-
 template <typename T, typename TO, int MT>
 static void launch_expand(const adapters_call &a, long tiles, hipStream_t st) {
-  hipLaunchKernelGGL((k_adapters_expand<T, TO, MT, expand_parts<T, TO>()>), dim3((unsigned)(tiles * a.col_blocks)), dim3(256), 0, st,
-                     a);
+  hipLaunchKernelGGL((k_adapters_expand<T, TO, MT>), dim3((unsigned)(tiles * a.col_blocks)), dim3(256), 0, st, a);
 }
 
 bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
@@ -237,8 +232,7 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
     with_type(a.out_type, [&](auto to) {
       typedef decltype(to) TO;
       if (staged_b)
-        hipLaunchKernelGGL((k_adapters_expand_staged<T, TO, expand_parts<T, TO>()>), dim3((unsigned)(tiles_b * a.col_blocks)),
-                           dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_adapters_expand_staged<T, TO>), dim3((unsigned)(tiles_b * a.col_blocks)), dim3(256), 0, st, a);
       else if (BM == 16) launch_expand<T, TO, 1>(a, tiles_b, st);
       else launch_expand<T, TO, 2>(a, tiles_b, st);
     });

@@ -202,3 +202,60 @@ def test_route_grad_of_picks_with_a_score_that_is_no_number(blk, mode, what):
         close(torch.from_numpy(got[2]), torch.from_numpy(want[2]), torch.from_numpy(bound[2]))
     else:
         assert np.isnan(got[2, ids[2]]).all(), got[2, ids[2]]
+
+
+EXACT = [(40, 24, 2, 40, 3), (17, 100, 5, 33, 4), (300, 64, 24, 200, 2), (2100, 64, 8, 7000, 3), (2100, 64, 64, 7000, 3)]
+
+
+@pytest.mark.parametrize("M, K, R, N, n", EXACT)
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("x", ["bf16", "f16"])
+def test_adapters_whose_products_cancel(blk, M, K, R, N, n, out, x):
+    """Pairs of A x that agree to 16 bits and are subtracted by B: what is left is in the last 8 bits of 24.  A x is
+    a + b / 2^8 + c / 2^16 with whole numbers below 2^7, exact in f32 in any order."""
+    say("adapters cancel", M, K, R, N, n, out, x)
+    rng = np.random.default_rng(M + R)
+    t, pairs = TYPES[x], R // 2
+    xs = torch.zeros((M, K))
+    xs[:, 3], xs[:, 9], xs[:, K - 1] = 1.0, 2.0 ** -8, 2.0 ** -16 if x == "bf16" else 2.0 ** -14
+    a = torch.zeros((n, R, K))
+    head = torch.from_numpy(rng.integers(64, 128, (n, pairs, 2)).astype(np.float32))
+    for half in (0, 1):  # rows 0 .. pairs, and pairs .. 2 pairs: the same but for the last numbers
+        at = slice(half * pairs, (half + 1) * pairs)
+        a[:, at, 3], a[:, at, 9] = head[:, :, 0], head[:, :, 1]
+        a[:, at, K - 1] = torch.from_numpy(rng.integers(0, 128, (n, pairs)).astype(np.float32))
+    b = torch.zeros((n, N, R))
+    sign = torch.from_numpy(rng.choice([-1.0, 1.0], (n, N, pairs)).astype(np.float32))
+    b[:, :, :pairs], b[:, :, pairs:2 * pairs] = sign, -sign
+    of = np.sort(rng.integers(0, n, M)).astype(np.int32)
+    base = torch.zeros((M, N), dtype=TYPES[out])
+    counts, offsets, perm = zeros(n, dtype=torch.int32), zeros(n + 1, dtype=torch.int32), zeros(M, dtype=torch.int32)
+    blk.group(dev(of[:, None]), n, counts, offsets, perm)
+    got = zeros(M, N, dtype=TYPES[out])
+    blk.adapters(dev(xs.to(t)), dev(a.to(t)), dev(b.to(t)), None, offsets, perm, dev(base), got,
+                 zeros(blk.adapters_scratch(M, K, R)))
+    which = torch.from_numpy(of).long()
+    mid = torch.stack([a[i].double() @ xs[0].double() for i in range(n)])  # every row of x is the same
+    want = torch.stack([b[i].double() @ mid[i] for i in range(n)])[which]
+    mag = torch.stack([b[i].double().abs() @ mid[i].abs() for i in range(n)])[which]
+    # the sum over R: R + 2 additions
+    close(got, want, rounded((R + 2) * U * mag, want, TYPES[out]))
+
+
+@pytest.mark.parametrize("M, N", [(5, 40), (2100, 7000)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_adapters_with_products_next_to_the_largest_value(blk, M, N, out):
+    """A x within f32 but past the largest value of bf16, times a small B."""
+    say("adapters largest", M, N, out)
+    K, R = 64, 8
+    x, a, b = torch.zeros((M, K)), torch.zeros((1, R, K)), torch.zeros((1, N, R))
+    x[:, 1], x[:, 40] = 2.0 ** 64, 2.0 ** 60
+    a[0, :, 1], a[0, :, 40] = (2 - 2.0 ** -7) * 2.0 ** 63, 1.5 * 2.0 ** 59
+    b[0, :, 5] = 2.0 ** -100
+    offsets, perm = torch.tensor([0, M], dtype=torch.int32), torch.arange(M, dtype=torch.int32)
+    got = zeros(M, N, dtype=TYPES[out])
+    blk.adapters(dev(x.bfloat16()), dev(a.bfloat16()), dev(b.bfloat16()), None, dev(offsets), dev(perm),
+                 torch.zeros((M, N), dtype=TYPES[out], device=DEV), got, zeros(blk.adapters_scratch(M, K, R)))
+    v = ((2 - 2.0 ** -7) * 2.0 ** 127 + 1.5 * 2.0 ** 119) * 2.0 ** -100
+    want = torch.full((M, N), v, dtype=torch.float64)
+    close(got, want, rounded((R + 2) * U * want, want, TYPES[out]))
