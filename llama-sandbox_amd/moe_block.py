@@ -388,7 +388,8 @@ def _know_torch():
             spec = importlib.util.spec_from_file_location("moe_torch", os.path.join(_HERE, "moe_torch.so"))
             calls = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(calls)
-            if calls.torch_version == torch.__version__.partition("+")[0] and _raw_stream is not None:
+            whole = all(hasattr(calls, n[len("moe_"):]) for n, _ in _Entries._fields_)  # (not one of an earlier build)
+            if whole and calls.torch_version == torch.__version__.partition("+")[0] and _raw_stream is not None:
                 calls.set_current_stream(_raw_stream)
                 _torch_calls = calls
         except ImportError:
