@@ -259,3 +259,76 @@ def test_adapters_with_products_next_to_the_largest_value(blk, M, N, out):
     v = ((2 - 2.0 ** -7) * 2.0 ** 127 + 1.5 * 2.0 ** 119) * 2.0 ** -100
     want = torch.full((M, N), v, dtype=torch.float64)
     close(got, want, rounded((R + 2) * U * want, want, TYPES[out]))
+
+
+def same(got, want, bound):
+    """Numbers within the bound; infinities and NaN the same."""
+    got, want = got.double().numpy(), np.asarray(want, np.float64)
+    assert (np.isnan(got) == np.isnan(want)).all() and (np.isinf(got) == np.isinf(want)).all()
+    inf = np.isinf(want)
+    assert (got[inf] == want[inf]).all()
+    ok = np.isfinite(want)
+    assert (np.abs(got - want)[ok] <= np.broadcast_to(bound, want.shape)[ok]).all()
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("n_group, keep, top", [(1, 1, 1), (4, 2, 1), (8, 3, 2), (6, 2, 2)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_of_scores_that_are_no_numbers(blk, mode, n_group, keep, top, biased):
+    """NaN, infinities and the largest values among the logits and the biases: every row's picks, weights and scores."""
+    say("route not finite", mode, n_group, keep, top, biased)
+    rng = np.random.default_rng(61)
+    T, E, k = 24, 48, 5
+    l = rng.standard_normal((T, E)).astype(np.float32)
+    high = np.finfo(np.float32).max
+    l[0, 3], l[1, 9], l[2, 1], l[3, 2], l[4] = np.inf, np.nan, high, -high, np.nan
+    l[5, :46] = -np.inf
+    l[5, 46] = np.nan
+    l[6, ::2] = np.nan
+    l[7, 5:9] = np.inf
+    l[8, 4], l[8, 5] = np.inf, np.nan
+    l[9, ::3] = -np.inf
+    l[10] = -np.inf
+    l[11, 1:] = -high
+    l[12, :44] = np.nan  # fewer numbers than picks
+    bias = None
+    if biased:
+        bias = (0.3 * rng.standard_normal(E)).astype(np.float32)
+        bias[[7, 20, 33]] = np.nan, -np.inf, -np.inf
+        bias[13], bias[40] = np.inf, high
+    with np.errstate(all="ignore"):
+        args = (k, mode, n_group, keep, top, True, 1.5)
+        want_ids, want_w, p = ref.route(l, bias, *args)
+        half = ref.score_half_steps(np.clip(l.astype(np.float64), -200, 200), mode)
+    ids, wts, sc = run_route(blk, torch.from_numpy(l), bias, *args)
+    assert (ids == want_ids).all(), np.nonzero((ids != want_ids).any(1))[0]
+    with np.errstate(all="ignore"):
+        same(sc, p, half * U * np.abs(p) + 1e-37)
+        same(wts, want_w, (2 * half + k + 6) * U * np.abs(want_w) + 1e-37)
+
+
+@pytest.mark.parametrize("M, K, R, N, n", [(40, 512, 16, 64, 3), (300, 520, 64, 264, 2), (2100, 64, 32, 7000, 3)])
+@pytest.mark.parametrize("x, out", [("f16", "f32"), ("bf16", "f32"), ("f16", "bf16"), ("bf16", "f16"), ("f32", "f32")])
+def test_adapters_keep_what_f32_keeps(blk, M, K, R, N, n, x, out):
+    """Rows of very different size, A x past f16's range: no value is off by more than its own f32 sums are."""
+    say("adapters in 24 bits", M, K, R, N, n, x, out)
+    rng = np.random.default_rng(M + K)
+    t = TYPES[x]
+    xs = (floats(rng, (M, K), "f32") * torch.from_numpy(4.0 ** rng.integers(-5, 7, (M, 1))).float()).to(t)
+    a = (64 * torch.from_numpy(rng.standard_normal((n, R, K)).astype(np.float32)) / K ** 0.5).to(t)
+    b = (torch.from_numpy(rng.standard_normal((n, N, R)).astype(np.float32)) / R ** 0.5 / 1024).to(t)
+    of, base = np.sort(rng.integers(0, n, M)).astype(np.int32), floats(rng, (M, N), out)
+    counts, offsets, perm = zeros(n, dtype=torch.int32), zeros(n + 1, dtype=torch.int32), zeros(M, dtype=torch.int32)
+    blk.group(dev(of[:, None]), n, counts, offsets, perm)
+    got = zeros(M, N, dtype=TYPES[out])
+    blk.adapters(dev(xs), dev(a), dev(b), None, offsets, perm, dev(base), got, zeros(blk.adapters_scratch(M, K, R)))
+    # sums over K as in layer_ref.py, over R R + 10 half steps, nothing for a cutting of A x
+    want, bound = base.double(), torch.zeros((M, N), dtype=torch.float64)
+    for i in range(n):
+        r = torch.from_numpy(np.nonzero(of == i)[0])
+        X, A, B = xs[r].double(), a[i].double(), b[i].double()
+        mid, err = X @ A.t(), (K / 16 + 40) * U * (X.abs() @ A.abs().t())
+        want[r] += mid @ B.t()
+        e = err @ B.abs().t() + (R + 10) * U * ((mid.abs() + err) @ B.abs().t())
+        bound[r] = e + U * (want[r].abs() + e)
+    close(got, want, rounded(bound, want, TYPES[out]))
