@@ -92,14 +92,14 @@ __device__ __forceinline__ double readlane_d(double v, int lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Over the LANES lanes (16, 32 or 64) that a lane is one of; every one gets it.
+// Over the LANES lanes (16 or 64) that a lane is one of; every one gets it.
 template <int LANES, typename F>
 __device__ __forceinline__ double lanes_reduce_d(double v, F f) {
+  static_assert(LANES == 16 || LANES == 64, "a row of 16 lanes, or the wave");
   v = f(v, dpp_d<0xB1>(v));   // quad_perm [1,0,3,2]
   v = f(v, dpp_d<0x4E>(v));   // quad_perm [2,3,0,1]
   v = f(v, dpp_d<0x141>(v));  // row_half_mirror
   v = f(v, dpp_d<0x140>(v));  // row_mirror: every lane holds its row of 16's
-  if constexpr (LANES == 32) v = f(v, __shfl_xor(v, 16));
   if constexpr (LANES == 64) v = f(f(readlane_d(v, 0), readlane_d(v, 16)), f(readlane_d(v, 32), readlane_d(v, 48)));
   return v;
 }
@@ -297,10 +297,8 @@ __global__ __launch_bounds__(256) void k_rms_norm_long(norm_call a) {
 
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
-  v = row16_sum(v);
-  if constexpr (LANES == 32) v += __shfl_xor(v, 16);
-  if constexpr (LANES == 64) v = (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
-  return v;
+  static_assert(LANES == 16 || LANES == 64, "a row of 16 lanes, or the wave");
+  return LANES == 16 ? row16_sum(v) : wave_sum(v);
 }
 
 // The gradient in one pass over the rows: LANES threads hold one, G of them a workgroup, which walks
