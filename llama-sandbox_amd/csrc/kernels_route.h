@@ -105,9 +105,11 @@ __device__ __forceinline__ bool route_stay(const route_call &a, K v1, K v2, int 
   if (width > 4) merge(dpp_k<0x141>(v1), dpp_k<0x141>(v2));  // row_half_mirror
   if (width > 8) merge(dpp_k<0x140>(v1), dpp_k<0x140>(v2));  // row_mirror
   K score = v1;
+  bool wide = false;  // 32 bits take -inf and the lowest value for one: the sum with a v1 that counts beside it may be either's
   if (a.top == 2 && v2 > none) {
     const K sum = v1 <= low || v2 <= low ? none : v1 + v2;
     score = sum > low ? sum : low;
+    wide = sizeof(K) == 4 && v2 <= low && v1 > (K)0x1p102f;
   }
   int before = 0;  // groups that come before this lane's
   for (int o = 0; o < a.n_group; o++) {
@@ -116,7 +118,7 @@ __device__ __forceinline__ bool route_stay(const route_call &a, K v1, K v2, int 
   }
   const bool in = before < a.keep;
   if (sizeof(K) == 4 && near > (K)0 && a.keep < a.n_group) {
-    const float first_out = wave_max(in || g >= a.n_group ? -INFINITY : (float)score);
+    const float first_out = wave_max(wide ? INFINITY : in || g >= a.n_group ? -INFINITY : (float)score);
     const float last_in = -wave_max(in && g < a.n_group ? -(float)score : -INFINITY);
     close = last_in > -INFINITY && !(last_in - first_out > (float)near);
   }
@@ -183,25 +185,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_route_groups(route_call a) {
   }
   // how close two scores in 32 bits may be in another order than in 64: each is off by 7 half steps of f32 (2^-24) of
   // p, softmax's by 33 and twice the size of the exponent, and one of c; those next to 0 by steps of the smallest values.
-  // A sum of two is off by what both are and by its own rounding, half a step of |c1 + c2|: as if each c were off by
-  // two.  So two scores are off by `near` together, and two groups' sums of `top` scores by top times as much
+  // A sum of two is off by what both are and by its own rounding, half a step of |c1 + c2|: as if each c were off by two,
+  // which is counted for all.  So two scores are off by `near` together, two groups' sums of `top` by top times as much
   float near = 0.0f;
   if (a.bias || sums) {
-    float big = 0.0f, each = 7.0f;
-    const float round_c = sums ? 2.0f : 1.0f;
+    float big = 0.0f, each = 3.5f;  // in double steps, so that no finite c passes f32
     if (soft) {
       float low = 0.0f;
 #pragma unroll
       for (int j = 0; j < NJ; j++)
         if (l[j] != -INFINITY) low = fmaxf(low, top - l[j]);
-      each = 33.0f + 2.0f * fminf(wave_max(low), 100.0f);
+      each = 16.5f + fminf(wave_max(low), 100.0f);
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-      const float size = fmaf(each, p[j], round_c * fabsf(p[j] + b[j]));
+      const float size = fmaf(each, p[j], fabsf(p[j] + b[j]));
       big = l[j] != -INFINITY && size < INFINITY ? fmaxf(big, size) : big;  // (infinities are what they are in 64 bits)
     }
-    near = wave_max(big) * 0x1p-23f + 0x1p-120f;
+    near = fmaf(wave_max(big), 0x1p-22f, 0x1p-120f);
   }
   uint32_t key[NJ];
 #pragma unroll

@@ -332,3 +332,22 @@ def test_adapters_keep_what_f32_keeps(blk, M, K, R, N, n, x, out):
         e = err @ B.abs().t() + (R + 10) * U * ((mid.abs() + err) @ B.abs().t())
         bound[r] = e + U * (want[r].abs() + e)
     close(got, want, rounded(bound, want, TYPES[out]))
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("keep, k", [(1, 2), (2, 3), (3, 6)])
+def test_route_of_groups_with_the_lowest_value_beside_a_large_one(blk, mode, keep, k):
+    """A bias of f32's lowest value is a number, and a sum with it may be any number, or an infinity."""
+    say("route lowest value", mode, keep, k)
+    rng = np.random.default_rng(71)
+    high = np.finfo(np.float32).max
+    bias = np.array([1, 1, np.inf, -high, 3e38, -high, -1e38, -1e38], np.float32)
+    for order in (range(4), (2, 0, 3, 1), (3, 2, 1, 0)):
+        b = bias.reshape(4, 2)[list(order)].reshape(-1)
+        l = torch.from_numpy(rng.standard_normal((7, 8)).astype(np.float32))
+        args = (k, mode, 4, keep, 2, False, 1.0)
+        ids, wts, _ = run_route(blk, l, b, *args)
+        want_ids, want_w, p = ref.route(l.numpy(), b, *args)
+        assert (ids == want_ids).all()
+        w = torch.from_numpy(want_w)
+        close(wts, w, torch.from_numpy(ref.score_half_steps(l.double().numpy(), mode)) * U * w + 1e-37)
