@@ -528,13 +528,16 @@ moe_status moe_rms_norm_grad(moe_ctx *ctx, const void *dy_dev, int dy_type, cons
  * An expert whose logit is -inf is masked: its score is 0 and it is never
  * picked.  With c = score + bias, group g (experts [g*E/n_group, (g+1)*E/n_group),
  * n_group <= 64) scores the sum of its `top` (1 or 2) largest c (of fewer
- * where there are fewer numbers; a group without any comes last); the `keep` best groups
- * stay, and the k largest c of their experts are picked, in that order; ties go
- * to the lowest index, NaN comes after every number.  k <= 64 and k <= keep *
- * E/n_group.  A slot that finds no expert has id -1 and weight 0: moe_group drops
- * such a pair; moe_forward does not take it.
- * The order is that of c in 64 bits (moe_route: in 32), without a bias that of
- * the logits.  Weights as moe_route's.  scores (may be NULL): [T][E] f32. */
+ * where there are fewer numbers; two infinities of different sign sum to the lower
+ * one; a group without any comes last); the `keep` best groups stay, and the k
+ * largest c of their experts are picked, in that order; ties go to the lowest
+ * index, NaN comes after every number.  k <= 64 and k <= keep * E/n_group.  A slot
+ * that finds no expert has id -1 and weight 0: moe_group drops such a pair;
+ * moe_forward does not take it.
+ * The order is that of c in 64 bits (moe_route: in 32, so that scores within a
+ * rounding of each other may come in another order there), without a bias that
+ * of the logits.  Weights as moe_route's, and scores (may be NULL, [T][E]), are f32
+ * arithmetic. */
 moe_status moe_route_groups(moe_ctx *ctx, const void *logits_dev, int logits_type, const float *bias_dev, int T, int E,
                             int k, int mode, int n_group, int keep, int top, int norm, float scale, int32_t *ids_dev,
                             float *wts_dev, float *scores_dev, void *stream);

@@ -72,7 +72,7 @@ __device__ __forceinline__ int adapters_row(const adapters_call &a, const row_ti
 // of one piece of K of 16 MT grouped rows and 16 RT rows of A; its waves take pieces of U steps in turn and meet in LDS.
 // Absent rows read another's (their columns are not written).
 // 16 single tokens of 16 adapters of 7168 x 16 (3.7 MB): 4.2 us, the chain of offsets, perm, x; 4096 rows of 7168 x
-// 16 16.8, x 64 24.6.  Bound there by the address unit, which takes a lane a cycle for loads whose neighbours are other
+// 16 14.0, x 64 25.  Bound there by the address unit, which takes a lane a cycle for loads whose neighbours are other
 // rows; neither deeper rings nor another order of the loads moved it.
 template <typename T, int MT, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a) {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_adapters_shrink(adapters_call a)
 // The same for adapters of many rows: 64 of them a workgroup, 16 a wave.  Loads that give neighbouring lanes
 // other rows take a cycle a lane (above: 59 accesses a load); here rows come as runs of 128 bytes, straight to LDS,
 // NBUF - 1 stages ahead, and are read from there as operands (chunk c of row r lies at c ^ (r & 7)).  Rows and A of
-// whole 16 bytes, below 4 GiB.  4096 rows of 7168 x 64 bf16 (59 MB of x, 62 of A from L2) 22.6 us; more pieces of K
+// whole 16 bytes, below 4 GiB.  4096 rows of 7168 x 64 bf16 (59 MB of x, 62 of A from L2) 22.7 us; more pieces of K
 // (3 to 8) move time from here to the reading of the shares, another start in K for each tile does nothing.
 template <typename T, int NBUF>
 __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a) {
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
 
 // mid as the operands that multiply a piece of B: f32 as it is; else as three bf16 parts, each the leading 8 bits of what
 // the ones before leave, so that together they are its 24 bits.  (Two would do for an output of 16 bits, but not where
-// base and update, or the products of B, cancel; 4096 rows x 64 x 7168 bf16 36.6 us with two.)  The parts are cut, not
+// base and update, or the products of B, cancel; 4096 rows x 64 x 7168 bf16 36.6 us with two, 37.5 with three.)  The parts are cut, not
 // rounded: a value next to the largest stays finite.
 // A piece of f16 weights is two bf16 pieces, which hold it exactly, at bf16's range: mid may be past f16's.
 template <typename T>
@@ -309,8 +309,8 @@ __device__ __forceinline__ void stage_mid(const adapters_call &a, const row_tile
 
 // out.  grid (tiles * column blocks): 16 MT grouped rows by a.col_groups times 128 columns of out a workgroup, 32 a wave,
 // with the next group's loads in flight; mid's shares are added up and cut into parts in LDS, 64 of R at a time.
-// Four workgroups a CU (at most 128 registers) or the chains of loads show: 4096 rows x 16 x 7168 45 us with 208
-// registers, 31 with 102.  16 single tokens x 16 x 4096 4.5 us.
+// Four workgroups a CU (at most 128 registers) or the chains of loads show: with 208 registers half as slow again.  16
+// single tokens x 16 x 4096 4.8 us; 4096 rows x 16 x 7168, which the staged kernel takes, 43.
 template <typename T, typename TO, int MT>
 __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
   typedef typename expand_of<T>::type TE;
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
 // as runs, all at once, and tokens are the rows of the result: tile j of a group of 128 columns has the columns
 // 8 l + j, so that a lane holds 8 next to each other and 16 lanes a run of 128 columns of base and out.
 // LDS row 16 j + l of a group is row 8 l + j of B.  B's rows are whole 16 bytes, an adapter's below 4 GiB.  4096 rows of
-// 64 x 7168 bf16 (117 MB of base and out) 36.6 us, x 16 31: workgroups of one phase after another (offsets; B, mid, base;
+// 64 x 7168 bf16 (117 MB of base and out) 37.5 us, x 16 30.7: workgroups of one phase after another (offsets; B, mid, base;
 // the products; out), three a CU.
 template <typename T, typename TO>
 __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a) {

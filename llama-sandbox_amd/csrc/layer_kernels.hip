@@ -12,9 +12,9 @@
 
 // Outputs of more than this go past the caches: a kernel ends only when the caches have written back what it left
 // there, and the next one reads it from the memory's cache as fast.  us, through them / past them, norm and then
-// moe_quantize_i8 of its y, H = 7168 bf16 with residual:  64 rows (1.8 MB) 7.4 / 7.6, 512 (14.7 MB) 15.6 / 12.9, 1500
-// 30.6 / 29.0, 4096 61.8 / 60.8; 2000 of 2048 (16.4 MB) 17.1 / 14.1, 8191 42.8 / 39.6.  The gradient alone, 509 rows of 5120 f32 15.3 /
-// 12.9, 4096 of 7168 bf16 54.9 / 54.2, 2048 of 7168 f32 51.5 / 52.8; adapters, 4096 rows of 7168 bf16 59.2 / 55.4.
+// moe_quantize_i8 of its y, H = 7168 bf16 with residual:  64 rows (1.8 MB) 7.5 / 7.6, 512 (14.7 MB) 15.8 / 13.0, 1500
+// 31.0 / 29.5, 4096 62.0 / 60.4; 2000 of 2048 (16.4 MB) 16.1 / 14.2, 8191 36.6 / 36.3.  The gradient alone, with dres: 509 rows of 5120
+// f32 17.8 / 15.7, 4096 of 7168 bf16 54.4 / 54.1, 2048 of 7168 f32 52.1 / 52.3; adapters, 4096 rows of 7168 x 64 x 7168 bf16 60.5 / 56.3.
 static constexpr size_t MOE_LAYER_STREAM_BYTES = (size_t)4 << 20;
 
 // f(integral_constant) for the bytes of an element of type t.
@@ -34,9 +34,19 @@ static bool launch_norm(const norm_call &a, hipStream_t st) {
 }
 
 // Threads a row and vectors a thread.  A row of 4097 to 8192 in one vector a thread where the rows are too few to fill
-// the chip.  us, with outputs past the caches (4096 rows of 7168 bf16 with residual / to 8 bits; 8191 of 2048; 1024):
-//   threads x vectors:   7168:  1024 x 1  45.6 / 58.0   512 x 2  45.8 / 50.9   256 x 4  48.6 / 47.5   128 x 8  80 / 90
-//                        2048:  256 x 1  25.2   128 x 2  26.4   64 x 4  27.9     1024:  128 x 1  14.8   64 x 2  14.9
+// the chip.  us, bf16 with residual, output in values / in 8 bits (* the rule's):
+//   threads x vectors:      1024 x 1         512 x 2          256 x 4          (128 x 8: 4096 rows 80 / 90)
+//   4096 rows of 7168       47.6  / 54.6     45.7* / 48.1*    49.9  / 45.4
+//   600 of 7168             8.4   / 13.0     9.6*  / 12.0*    9.0   / 11.0
+//   500 of 7168             6.9*  / 9.7*     7.1   / 8.9      8.0   / 9.4
+//   509 of 5120             7.4*  / 9.9*     7.7   / 8.9      8.1   / 8.9
+//   one of 7168             3.6*             4.0              5.2
+//                           256 x 1          128 x 2          64 x 4
+//   8191 of 2048            26.8* / 26.4*    27.9  / 22.8     28.9  / 24.0
+//                           128 x 1          64 x 2
+//   8191 of 1024            14.7* / 15.1*    15.4  / 13.6
+// The rule is the one for values at both ends, one row and thousands.  In 8 bits, bound by instructions, half the threads would
+// take up to a seventh off; the rule does not look at the output.
 template <int SX, int SR>
 static bool launch_norm(const norm_call &a, int n_cu, hipStream_t st) {
   const int H = a.H;
@@ -199,12 +209,14 @@ bool launch_adapters(const adapters_call &args, int n_cu, hipStream_t st) {
   const size_t size = a.type == MOE_GGML_F32 ? 4 : 2;
   // Staged where adapters have rows for its tiles: the product with A from rank 33 on, the one with B where there are
   // three workgroups for two CUs.  us, staged / straight to registers (bf16 rows x K x rank x N, adapters; * the rule's):
-  //   with A:  4096 x 7168 x 64 x 7168, 8   59.6* / 63.9   x 32  52.5 / 53.5*   x 16  50.3 / 48.7*
-  //            2048 x 2048 x 64 x 2048, 16 (f32)  37.6* / 40.6    2048 x 768 x 8 x 768, 60 (f32)  16.1 / 13.1*
-  //   with B:  4096 x 7168 x 64 x 7168, 8   59.6* / 67.4   x 16  48.7* / 51.2
-  //            2048 x 4096 x 64 x 4096, 16   27.4* / 32.5   x 16  24.1* / 27.4    1024 x 7168 x 64 x 7168, 4  25.4* / 28.4
-  //            2048 x 2048 x 64 x 2048, 16 (f32)  42.8 / 35.4*   (f16)  24.5 / 20.9*    512 x 4096 x 32 x 4096, 16  16.6 / 13.1*
-  //   both at 16 rows an adapter: 517 x 2048 x 8 x 768, 32  15.6 / 9.3*
+  //   with A:  4096 x 7168 x 64 x 7168, 8   56.8* / 62.7   x 32  49.2 / 50.8*   x 16  54.0 / 45.8*
+  //            2048 x 2048 x 64 x 2048, 16 (f32)  35.5* / 39.0    2048 x 768 x 8 x 768, 60 (f32)  27.0 / 13.7*
+  //   with B:  4096 x 7168 x 64 x 7168, 8   56.4* / 67.8   x 16  45.9* / 56.9
+  //            2048 x 4096 x 64 x 4096, 16   27.9* / 32.8   x 16  24.2* / 27.6    1024 x 7168 x 64 x 7168, 4  25.7* / 28.5
+  //            2048 x 2048 x 64 x 2048, 16 (f32)  42.8 / 35.4*   (f16)  24.4 / 20.6*    512 x 4096 x 32 x 4096, 16  16.5 / 12.8*
+  //   both at 16 rows an adapter: 517 x 2048 x 8 x 768, 32  17.2 / 8.9*
+  // `each` counts adapters that are there, not those with rows, which only the device knows: 4096 rows of four of 256 adapters
+  // take 114 us in 16-row tiles, of four of 64 60.6.
   const bool staged_a = each >= 32 && a.R > 32 && a.K * size % 16 == 0 && ((uintptr_t)a.x | (uintptr_t)a.a) % 16 == 0 &&
                         (uint64_t)a.M * a.K * size < MOE_LDS_OOB && (uint64_t)a.R * a.K * size < MOE_LDS_OOB;
   const bool staged_b = each >= 32 && 2L * ceil_div(a.M, 64) * ceil_div(a.N, 256) >= 3 * n_cu && a.R <= 64 &&
