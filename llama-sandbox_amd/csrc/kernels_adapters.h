@@ -223,8 +223,8 @@ __global__ __launch_bounds__(256) void k_adapters_shrink_staged(adapters_call a)
 
 // mid as the operands that multiply a piece of B: f32 as it is; else as three bf16 parts, each the leading 8 bits of what
 // the ones before leave, so that together they are its 24 bits.  (Two would do for an output of 16 bits, but not where
-// base and update, or the products of B, cancel; 4096 rows x 64 x 7168 bf16 36.6 us with two, 37.5 with three.)  The parts are cut, not
-// rounded: a value next to the largest stays finite.
+// base and update, or the products of B, cancel; 4096 rows x 64 x 7168 bf16 36.6 us with two, 37.5 with three.)  The
+// parts are cut, not rounded: a value next to the largest stays finite.
 // A piece of f16 weights is two bf16 pieces, which hold it exactly, at bf16's range: mid may be past f16's.
 template <typename T>
 struct expand_of {
@@ -315,7 +315,8 @@ template <typename T, typename TO, int MT>
 __global__ __launch_bounds__(256, 4) void k_adapters_expand(adapters_call a) {
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
-  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>(), WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
+  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>();
+  constexpr int WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
   constexpr int ROW = RC + F::V;  // a piece more, so that rows lie in different banks
   __shared__ __attribute__((aligned(16))) TE mid[PARTS][16 * MT][ROW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % 16, kg = lane / 16;
@@ -408,7 +409,8 @@ __global__ __launch_bounds__(256) void k_adapters_expand_staged(adapters_call a)
   typedef typename expand_of<T>::type TE;
   typedef frag<TE> F;
   typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
-  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>(), WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
+  constexpr int RC = 64, STEPS = RC / F::STEP, PARTS = mid_parts<T>();
+  constexpr int WP = sizeof(T) == 2 && !std::is_same<T, TE>::value ? 2 : 1;
   constexpr int ROW = RC + 4;                        // a piece more, so that rows lie in different banks
   constexpr int BLOCKS = RC * (int)sizeof(T) / 128;  // of 128 bytes of B's rows
   __shared__ chunk_t lds[BLOCKS * 256 * 8];

@@ -210,7 +210,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm(norm_cal
   }
   if (!a.q) return;
   double m = 0.0;
-  float odd = 0.0f;  // NaN where the gain has a value that is not finite; one of h shows in r, a NaN or, of an infinity, 0
+  // NaN where the gain has a value that is not finite; one of h shows in r, as a NaN or, of an infinity, as 0
+  float odd = 0.0f;
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
     float w[8];

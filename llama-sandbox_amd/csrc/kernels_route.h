@@ -105,7 +105,8 @@ __device__ __forceinline__ bool route_stay(const route_call &a, K v1, K v2, int 
   if (width > 4) merge(dpp_k<0x141>(v1), dpp_k<0x141>(v2));  // row_half_mirror
   if (width > 8) merge(dpp_k<0x140>(v1), dpp_k<0x140>(v2));  // row_mirror
   K score = v1;
-  bool wide = false;  // 32 bits take -inf and the lowest value for one: the sum with a v1 that counts beside it may be either's
+  // 32 bits take -inf and the lowest value for one: the sum with a v1 that counts beside it may be either's
+  bool wide = false;
   if (a.top == 2 && v2 > none) {
     const K sum = v1 <= low || v2 <= low ? none : v1 + v2;
     score = sum > low ? sum : low;

@@ -87,8 +87,8 @@ static int grad_blocks(int T, int H, int n_cu) {
 
 size_t norm_grad_need(int T, int H, int n_cu) { return H > 16384 ? 1 : (size_t)grad_blocks(T, H, n_cu) * H; }
 
-// Grows with T and H: a workspace for the largest call serves every smaller one, those of 16384 the longer rows', which have no
-// shares.
+// Grows with T and H: a workspace for the largest call serves every smaller one.  (Longer rows have no shares, and the
+// workspace of rows of 16384.)
 size_t norm_grad_scratch(int T, int H, int n_cu) { return norm_grad_need(T, H < 16384 ? H : 16384, n_cu); }
 
 template <int SD, int SH, int SX, int LANES, int VPT, int G>
@@ -176,10 +176,10 @@ static int adapters_splits(int M, int K, int R, int n_cu) {
 
 size_t adapters_need(int M, int K, int R, int n_cu) { return (size_t)adapters_splits(M, K, R, n_cu) * M * R; }
 
-// The pieces get fewer as the tiles get more, so what a call needs goes up and down with M.  A bound that grows with M, K and R, so
-// that a workspace for the largest call serves every smaller one: with M rows in t tiles of h <= 32, ceil(16 n_cu / (t w)) pieces
-// of M rows are fewer than 16 n_cu h / w + M rows.  (h / w grows with M and R, from 1 to 4, and the pieces of K, two steps
-// of w waves each, do too.)
+// The pieces get fewer as the tiles get more, so what a call needs goes up and down with M.  This is a bound that grows
+// with M, K and R, so that a workspace for the largest call serves every smaller one: of M rows in t tiles of h, the
+// ceil(16 n_cu / (t w)) pieces have fewer than 16 n_cu h / w + M rows.  (h / w grows with M and R, from 1 to 4, and so does
+// the most pieces of K, as w falls.)
 size_t adapters_scratch(int M, int K, int R, int n_cu) {
   const size_t some = (size_t)16 * n_cu * adapters_tile(M) / split_waves(M, R) + M, all = (size_t)most_splits(M, K, R) * M;
   return (some < all ? some : all) * R;
